@@ -439,6 +439,118 @@ int prism_import_external_memory(prism_ctx* ctx, int32_t fd, uint64_t size, pris
                                  void** dev_ptr);
 int prism_release_external_memory(prism_ctx* ctx, prism_external_buffer* buf);
 
+/* ---- sequence operators: positions, paged cache, attention along time ---- */
+
+/* What a renderer of video needs next to the window attention of one frame: the
+ * same tokens seeing earlier ones. Each operator stands by itself: it takes
+ * device pointers to 16-bit values (fp16 or bf16, `dtype`), needs no model
+ * loaded, keeps nothing between calls and allocates nothing, so it may be
+ * captured into a graph. Sums, softmax statistics and angles are held in 32
+ * bits or more; outputs are rounded once, to nearest. Pointers to values are
+ * 16-byte aligned and strides are in elements, multiples of 8, not negative
+ * (0 repeats an input; an output's rows must not overlap). head_dim is the
+ * innermost, contiguous dimension. The call runs on the context's device and
+ * leaves the caller's current device as it was. A call without rows does
+ * nothing. The reference has no counterpart: its attention sees one window of
+ * one frame (shaders/split2_qkv_attn_d256.comp.glsl:24-79). */
+#define PRISM_F16  0
+#define PRISM_BF16 1
+
+#define PRISM_ROPE_HALVES      0 /* pair i of n = channels i and i + n      */
+#define PRISM_ROPE_ADJACENT    1 /* pair i = channels 2i and 2i + 1         */
+#define PRISM_ROPE_AXIS_LADDER 0 /* f = base^(-j / pairs[a]), j-th pair of axis a */
+#define PRISM_ROPE_ONE_LADDER  1 /* f = base^(-i / n), i-th pair of all n   */
+
+/* Rotary positions: the first n = sum of pairs[0..n_axes) pairs of channels of
+ * every head turn by phi = position * f, the first pairs[0] of them by the
+ * position on axis 0, and so on; channels from 2n on are copied. Pair (x, y)
+ * becomes (x cos phi - y sin phi, y cos phi + x sin phi); `inverse` turns by
+ * -phi, which is also the gradient's way back. Token t of axis a is at
+ * pos[a * pos_stride + t] (any int32; angles are reduced in 64 bits). head_dim
+ * is a multiple of 8 up to 256; 2n <= head_dim; base > 0. in == out with equal
+ * strides works in place; otherwise the two must not overlap. */
+typedef struct prism_rope_push {
+    int32_t dtype, n_tokens, n_heads, head_dim;
+    int32_t n_axes; /* 1..4 */
+    int32_t pairs[4];
+    int32_t layout, ladder, inverse;
+    double base;
+    int64_t in_token_stride, in_head_stride, out_token_stride, out_head_stride;
+    int64_t pos_stride;
+} prism_rope_push;
+int prism_rope(prism_ctx* ctx, const prism_rope_push* p, const void* in, const int32_t* pos, void* out,
+               void* stream);
+
+/* A paged cache: keys and values each [n_pages][n_kv_heads][page_size]
+ * [head_dim], dense, and a table int32 [n_seqs][table_pages]: token j of
+ * sequence s is slot j % page_size of page table[s][j / page_size]. page_size
+ * is a power of two up to 4096; head_dim 16, 32, 64 or 128. Pages and
+ * the table are the caller's: sequences may share pages that are only read,
+ * and an entry that no call needs may hold anything. */
+typedef struct prism_cache_desc {
+    int32_t dtype, n_kv_heads, head_dim, page_size, n_pages, n_seqs, table_pages;
+} prism_cache_desc;
+
+/* Write n_new tokens' keys and values (rows of k and v) into the cache: row i is
+ * token pos_of[i] of sequence seq_of[i]. A row whose sequence, position or
+ * page is out of range is skipped (give padding rows sequence -1). Two rows for
+ * one slot leave it unspecified which of them it holds. */
+typedef struct prism_append_push {
+    prism_cache_desc cache;
+    int32_t n_new;
+    int64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+} prism_append_push;
+int prism_cache_append(prism_ctx* ctx, const prism_append_push* p, const void* k, const void* v,
+                       const int32_t* seq_of, const int32_t* pos_of, const int32_t* table, void* k_pages,
+                       void* v_pages, void* stream);
+
+/* Attention of one new token per sequence over the cache, which holds the new
+ * token already: with L = lengths[s], query s is at position L - 1 and sees
+ * the `left` keys before it (negative: all), itself, and the first `sinks`
+ * keys. Head h reads key head h / (n_heads / n_kv_heads). out = softmax(scale
+ * q.k) v over the keys seen; a sequence that sees none (L <= 0) gets zeros. A
+ * length past the table's end counts as its end; keys of a page that is not in
+ * the pool are not seen. Values outside the keys seen are never used (they may
+ * be NaN), and pages all of whose keys are out of the window need not exist.
+ * max_len (0 = the table's end) is the longest length that the caller expects:
+ * it decides how the work is split; longer sequences are still right. workspace:
+ * device memory of prism_paged_attn_workspace bytes (16-byte aligned; may be
+ * NULL if that is 0), free to reuse after the call's work; calls that may
+ * overlap need one each. scale is positive and finite. */
+typedef struct prism_paged_attn_push {
+    prism_cache_desc cache;
+    int32_t n_heads;
+    int32_t left, sinks;
+    int32_t max_len;
+    float scale;
+    int64_t q_seq_stride, q_head_stride, out_seq_stride, out_head_stride;
+} prism_paged_attn_push;
+/* Bytes of workspace for calls with this push; negative PRISM_ERR_* for one
+ * that prism_paged_attn refuses. Host only. */
+int64_t prism_paged_attn_workspace(const prism_paged_attn_push* p);
+int prism_paged_attn(prism_ctx* ctx, const prism_paged_attn_push* p, const void* q, const void* k_pages,
+                     const void* v_pages, const int32_t* table, const int32_t* lengths, void* out,
+                     void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Attention along n_seqs sequences that lie one behind the other in n_q rows of
+ * q and out and n_k rows of k and v: sequence s has rows [cu_q[s], cu_q[s+1])
+ * and [cu_k[s], cu_k[s+1]) (int32 device arrays of n_seqs + 1 starts, in order
+ * and within the rows; NULL = equal lengths, n_seqs divides the rows). The last
+ * query stands at the last key: query i of nq, over nk keys, is at p = nk - nq
+ * + i and sees key j if j <= p + right (right < 0: no limit) and j >= p - left
+ * (left < 0: no limit) or j < sinks. Heads, scale and rows without a
+ * key as in prism_paged_attn. Rows of out before the first sequence and behind
+ * the last one stay as they were. head_dim 16, 32, 64 or 128. */
+typedef struct prism_seq_attn_push {
+    int32_t dtype, n_seqs, n_q, n_k, n_heads, n_kv_heads, head_dim;
+    int32_t left, right, sinks;
+    float scale;
+    int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride;
+    int64_t v_token_stride, v_head_stride, out_token_stride, out_head_stride;
+} prism_seq_attn_push;
+int prism_seq_attn(prism_ctx* ctx, const prism_seq_attn_push* p, const void* q, const void* k, const void* v,
+                   const int32_t* cu_q, const int32_t* cu_k, void* out, void* stream);
+
 /* aux arena size in int32 elements that a router + expert pair needs for
  * n_experts experts and batch*n_tokens tokens when laid out as
  * [assignment | counts | perm]. */

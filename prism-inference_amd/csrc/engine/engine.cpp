@@ -124,6 +124,16 @@ extern "C" int prism_create(prism_ctx** out, int32_t device, const char* code_ob
             for (int r = 0; r <= 4; ++r)
                 all.emplace_back(&c->f_attn[di][w8][r], std::string("prism_attn_d") + (di ? "256" : "128") +
                                                             (w8 ? "_w8" : "") + (r ? "_r" + std::to_string(r) : ""));
+    all.emplace_back(&c->f_append, "prism_cache_append");
+    for (int t = 0; t < 2; ++t) {
+        const std::string type = t == PRISM_BF16 ? "bf16" : "f16";
+        all.emplace_back(&c->f_rope[t], "prism_rope_" + type);
+        for (int i = 0; i < 4; ++i) {
+            const std::string shape = type + "_h" + std::to_string(16 << i);
+            all.emplace_back(&c->f_paged[t][i], "prism_paged_attn_" + shape);
+            all.emplace_back(&c->f_seq[t][i], "prism_seq_attn_" + shape);
+        }
+    }
     for (auto& f : all) {
         e = hipModuleGetFunction(f.first, c->module, f.second.c_str());
         if (e != hipSuccess) {

@@ -1,0 +1,135 @@
+/* seq_rules.h - which calls of the sequence operators are refused, and how their
+ * work is split, as functions of the parameters alone (no HIP). Host plain
+ * C++. Every check_* returns PRISM_OK or the error code, and why in a text. */
+#ifndef PRISM_SEQ_RULES_H
+#define PRISM_SEQ_RULES_H
+
+#include <cmath>
+#include <cstdint>
+
+#include "prism.h"
+
+namespace prism {
+
+/* Strides are held to 2^40 elements so that no offset passes 64 bits. */
+constexpr int64_t SEQ_MAX_STRIDE = int64_t(1) << 40;
+
+inline int seq_bad(const char** why, int code, const char* text) {
+    if (why) *why = text;
+    return code;
+}
+
+inline int check_dtype(int32_t dtype, const char** why) {
+    return dtype == PRISM_F16 || dtype == PRISM_BF16 ? PRISM_OK
+                                                     : seq_bad(why, PRISM_ERR_INVALID, "dtype is neither PRISM_F16 nor PRISM_BF16");
+}
+
+inline int check_strides(int64_t token, int64_t head, const char** why) {
+    if (token < 0 || head < 0 || token % 8 || head % 8 || token > SEQ_MAX_STRIDE || head > SEQ_MAX_STRIDE)
+        return seq_bad(why, PRISM_ERR_INVALID, "strides are multiples of 8 from 0 to 2^40");
+    return PRISM_OK;
+}
+
+/* An output's rows must not overlap: either all heads of a row lie before the
+ * next row's, or all rows of a head before the next head's. */
+inline int check_out(int64_t rows, int64_t heads, int64_t head_dim, int64_t token, int64_t head, const char** why) {
+    if (int rc = check_strides(token, head, why)) return rc;
+    const bool rows_apart = (heads == 1 || head >= head_dim) && (rows <= 1 || token >= (heads - 1) * head + head_dim);
+    const bool heads_apart = (rows <= 1 || token >= head_dim) && (heads == 1 || head >= (rows - 1) * token + head_dim);
+    if (!rows_apart && !heads_apart) return seq_bad(why, PRISM_ERR_INVALID, "output rows overlap");
+    return PRISM_OK;
+}
+
+inline bool seq_head_dim(int32_t hd) { return hd == 16 || hd == 32 || hd == 64 || hd == 128; }
+
+inline int check_heads(int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, const char** why) {
+    if (n_kv_heads < 1 || n_heads < 1 || n_heads > 65536 || n_heads % n_kv_heads)
+        return seq_bad(why, PRISM_ERR_INVALID, "n_heads is a multiple of n_kv_heads, from 1 to 65536");
+    if (!seq_head_dim(head_dim))
+        return seq_bad(why, PRISM_ERR_UNSUPPORTED, "head_dim is 16, 32, 64 or 128");
+    return PRISM_OK;
+}
+
+inline int check_scale(float scale, const char** why) {
+    return scale > 0.f && std::isfinite(scale) ? PRISM_OK : seq_bad(why, PRISM_ERR_INVALID, "scale is not positive");
+}
+
+inline int check_rope(const prism_rope_push& p, const char** why) {
+    if (int rc = check_dtype(p.dtype, why)) return rc;
+    if (p.n_tokens < 0 || p.n_heads < 1 || p.n_heads > 65536)
+        return seq_bad(why, PRISM_ERR_INVALID, "n_tokens or n_heads out of range");
+    if (p.head_dim < 8 || p.head_dim > 256 || p.head_dim % 8)
+        return seq_bad(why, PRISM_ERR_UNSUPPORTED, "head_dim is a multiple of 8 up to 256");
+    if (p.n_axes < 1 || p.n_axes > 4) return seq_bad(why, PRISM_ERR_INVALID, "n_axes 1 to 4");
+    int64_t n = 0;
+    for (int a = 0; a < p.n_axes; ++a) {
+        if (p.pairs[a] < 0) return seq_bad(why, PRISM_ERR_INVALID, "negative pairs");
+        n += p.pairs[a];
+    }
+    if (n < 1 || 2 * n > p.head_dim) return seq_bad(why, PRISM_ERR_INVALID, "turned pairs do not fit the head");
+    if ((p.layout != PRISM_ROPE_HALVES && p.layout != PRISM_ROPE_ADJACENT) ||
+        (p.ladder != PRISM_ROPE_AXIS_LADDER && p.ladder != PRISM_ROPE_ONE_LADDER) || (p.inverse != 0 && p.inverse != 1))
+        return seq_bad(why, PRISM_ERR_INVALID, "layout, ladder or inverse");
+    if (!(p.base > 0) || !std::isfinite(p.base)) return seq_bad(why, PRISM_ERR_INVALID, "base is not positive");
+    if (p.pos_stride < 0 || p.pos_stride > SEQ_MAX_STRIDE) return seq_bad(why, PRISM_ERR_INVALID, "pos_stride");
+    if (int rc = check_strides(p.in_token_stride, p.in_head_stride, why)) return rc;
+    return check_out(p.n_tokens, p.n_heads, p.head_dim, p.out_token_stride, p.out_head_stride, why);
+}
+
+inline int check_cache(const prism_cache_desc& d, const char** why) {
+    if (int rc = check_dtype(d.dtype, why)) return rc;
+    if (!seq_head_dim(d.head_dim))
+        return seq_bad(why, PRISM_ERR_UNSUPPORTED, "head_dim is 16, 32, 64 or 128");
+    if (d.page_size < 1 || d.page_size > 4096 || (d.page_size & (d.page_size - 1)))
+        return seq_bad(why, PRISM_ERR_INVALID, "page_size: a power of two up to 4096");
+    if (d.n_kv_heads < 1 || d.n_kv_heads > 65536 || d.n_pages < 0 || d.n_seqs < 0 || d.table_pages < 0)
+        return seq_bad(why, PRISM_ERR_INVALID, "cache sizes out of range");
+    return PRISM_OK;
+}
+
+inline int check_append(const prism_append_push& p, const char** why) {
+    if (int rc = check_cache(p.cache, why)) return rc;
+    if (p.n_new < 0) return seq_bad(why, PRISM_ERR_INVALID, "n_new < 0");
+    if (int rc = check_strides(p.k_token_stride, p.k_head_stride, why)) return rc;
+    return check_strides(p.v_token_stride, p.v_head_stride, why);
+}
+
+inline int check_paged(const prism_paged_attn_push& p, const char** why) {
+    if (int rc = check_cache(p.cache, why)) return rc;
+    if (int rc = check_heads(p.n_heads, p.cache.n_kv_heads, p.cache.head_dim, why)) return rc;
+    if (p.sinks < 0 || p.max_len < 0) return seq_bad(why, PRISM_ERR_INVALID, "sinks or max_len < 0");
+    if (int rc = check_scale(p.scale, why)) return rc;
+    if (int rc = check_strides(p.q_seq_stride, p.q_head_stride, why)) return rc;
+    return check_out(p.cache.n_seqs, p.n_heads, p.cache.head_dim, p.out_seq_stride, p.out_head_stride, why);
+}
+
+inline int check_seq(const prism_seq_attn_push& p, const char** why) {
+    if (int rc = check_dtype(p.dtype, why)) return rc;
+    if (int rc = check_heads(p.n_heads, p.n_kv_heads, p.head_dim, why)) return rc;
+    if (p.n_seqs < 0 || p.n_q < 0 || p.n_k < 0) return seq_bad(why, PRISM_ERR_INVALID, "n_seqs, n_q or n_k < 0");
+    if (p.sinks < 0) return seq_bad(why, PRISM_ERR_INVALID, "sinks < 0");
+    if (int rc = check_scale(p.scale, why)) return rc;
+    if (int rc = check_strides(p.q_token_stride, p.q_head_stride, why)) return rc;
+    if (int rc = check_strides(p.k_token_stride, p.k_head_stride, why)) return rc;
+    if (int rc = check_strides(p.v_token_stride, p.v_head_stride, why)) return rc;
+    return check_out(p.n_q, p.n_heads, p.head_dim, p.out_token_stride, p.out_head_stride, why);
+}
+
+/* The frequency of every turned pair in turns per unit of position, and where
+ * each axis' pairs end; returns the number of pairs. */
+inline int rope_turns(const prism_rope_push& p, int32_t axis_end[4], double* turns) {
+    int n = 0, i = 0;
+    for (int a = 0; a < p.n_axes; ++a) n += p.pairs[a];
+    const double turn = (p.inverse ? -1.0 : 1.0) / 6.283185307179586476925286766559;
+    for (int a = 0; a < 4; ++a) {
+        const int pairs = a < p.n_axes ? p.pairs[a] : 0;
+        for (int j = 0; j < pairs; ++j, ++i)
+            turns[i] = turn * std::pow(p.base, p.ladder == PRISM_ROPE_ONE_LADDER ? -(double)i / n : -(double)j / pairs);
+        axis_end[a] = i;
+    }
+    return n;
+}
+
+}  // namespace prism
+
+#endif

@@ -160,4 +160,60 @@ typedef struct CodecArgs {
 #define CODEC_DEC_ROWS 2
 #define CODEC_DEC_COLS 32
 
+/* ---- sequence operators (rope.hpp, cache.hpp, paged_attn.hpp, seq_attn.hpp) */
+
+#define ROPE_MAX_PAIRS 128
+typedef struct RopeArgs {
+    const uint16_t* in;
+    uint16_t* out;
+    const int32_t* pos;     /* axis a of token t at pos[a * pos_stride + t] */
+    int64_t in_token_stride, in_head_stride, out_token_stride, out_head_stride, pos_stride;
+    int32_t n_tokens, n_heads, head_dim;
+    int32_t n_pairs;        /* turned pairs of channels of a head             */
+    int32_t adjacent;       /* pair i = channels 2i, 2i + 1; else i, i + n_pairs */
+    int32_t axis_end[4];    /* pairs [axis_end[a-1], axis_end[a]) belong to axis a */
+    double turns[ROPE_MAX_PAIRS]; /* turns per unit of position, negative for the inverse */
+} RopeArgs;
+
+typedef struct AppendArgs {
+    const uint16_t* k;
+    const uint16_t* v;
+    uint16_t* k_pages;      /* [n_pages][n_kv_heads][page_size][head_dim] */
+    uint16_t* v_pages;
+    const int32_t* table;   /* [n_seqs][table_pages] */
+    const int32_t* seq_of;  /* [n_new] */
+    const int32_t* pos_of;  /* [n_new] */
+    int64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+    int32_t n_new, n_seqs, n_kv_heads, head_dim;
+    int32_t page_log2, n_pages, table_pages;
+} AppendArgs;
+
+typedef struct PagedAttnArgs {
+    const uint16_t* q;
+    const uint16_t* k_pages;
+    const uint16_t* v_pages;
+    const int32_t* table;
+    const int32_t* lengths; /* [n_seqs] */
+    uint16_t* out;
+    int64_t q_seq_stride, q_head_stride, out_seq_stride, out_head_stride;
+    int32_t n_seqs, n_heads, n_kv_heads;
+    int32_t page_log2, n_pages, table_pages;
+    int32_t left, sinks;
+    float scale_log2;       /* scale * log2(e) */
+} PagedAttnArgs;
+
+typedef struct SeqAttnArgs {
+    const uint16_t* q;
+    const uint16_t* k;
+    const uint16_t* v;
+    uint16_t* out;
+    const int32_t* cu_q;    /* [n_seqs + 1] or NULL */
+    const int32_t* cu_k;
+    int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride;
+    int64_t v_token_stride, v_head_stride, out_token_stride, out_head_stride;
+    int32_t n_seqs, n_q, n_k, n_heads, n_kv_heads;
+    int32_t left, right, sinks;
+    float scale_log2;       /* scale * log2(e) */
+} SeqAttnArgs;
+
 #endif

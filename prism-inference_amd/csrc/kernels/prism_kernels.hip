@@ -14,6 +14,10 @@
  *   prism_codec_enc01, prism_codec_dec21_out       the same, fused in the frame (persistent)
  *   prism_codec_enc{2,3}, prism_codec_dec3         stages and frame alike (persistent)
  *   prism_codec_dec1_out                           dec1 + output conv + PixelShuffle + sigmoid
+ *   prism_rope_{f16,bf16}                          rotary positions with several axes
+ *   prism_cache_append                             new tokens into a paged cache
+ *   prism_paged_attn_{f16,bf16}_h{16,32,64,128}    one new token per sequence over its paged cache
+ *   prism_seq_attn_{f16,bf16}_h{16,32,64,128}      attention along sequences, window and sinks
  *   prism_zero_i32                                 clears routing counters
  */
 #include "attn.hpp"
@@ -23,6 +27,10 @@
 #include "codec.hpp"
 #include "codec_enc.hpp"
 #include "codec_dec.hpp"
+#include "rope.hpp"
+#include "cache.hpp"
+#include "paged_attn.hpp"
+#include "seq_attn.hpp"
 
 /* Routing counters must start at zero; a kernel (not a memset node) keeps
  * the launch safe under stream capture. */

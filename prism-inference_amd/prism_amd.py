@@ -29,6 +29,13 @@ ERR_BLOB = -5
 ERR_NOMEM = -6
 ERR_CODE_OBJECT = -7
 
+F16 = 0
+BF16 = 1
+ROPE_HALVES = 0
+ROPE_ADJACENT = 1
+ROPE_AXIS_LADDER = 0
+ROPE_ONE_LADDER = 1
+
 ROUTE_RANDOM = 0
 ROUTE_UNIFORM = 1
 ROUTE_ZIPF = 2
@@ -105,6 +112,39 @@ class ProjectPush(C.Structure):
                 ("b_offset", C.c_int64), ("input_offset", C.c_int64), ("output_offset", C.c_int64)]
 
 
+class RopePush(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("n_tokens", C.c_int32), ("n_heads", C.c_int32), ("head_dim", C.c_int32),
+                ("n_axes", C.c_int32), ("pairs", C.c_int32 * 4), ("layout", C.c_int32), ("ladder", C.c_int32),
+                ("inverse", C.c_int32), ("base", C.c_double), ("in_token_stride", C.c_int64),
+                ("in_head_stride", C.c_int64), ("out_token_stride", C.c_int64), ("out_head_stride", C.c_int64),
+                ("pos_stride", C.c_int64)]
+
+
+class CacheDesc(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in
+                ("dtype", "n_kv_heads", "head_dim", "page_size", "n_pages", "n_seqs", "table_pages")]
+
+
+class AppendPush(C.Structure):
+    _fields_ = [("cache", CacheDesc), ("n_new", C.c_int32), ("k_token_stride", C.c_int64),
+                ("k_head_stride", C.c_int64), ("v_token_stride", C.c_int64), ("v_head_stride", C.c_int64)]
+
+
+class PagedAttnPush(C.Structure):
+    _fields_ = [("cache", CacheDesc), ("n_heads", C.c_int32), ("left", C.c_int32), ("sinks", C.c_int32),
+                ("max_len", C.c_int32), ("scale", C.c_float), ("q_seq_stride", C.c_int64),
+                ("q_head_stride", C.c_int64), ("out_seq_stride", C.c_int64), ("out_head_stride", C.c_int64)]
+
+
+class SeqAttnPush(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in
+                ("dtype", "n_seqs", "n_q", "n_k", "n_heads", "n_kv_heads", "head_dim", "left", "right", "sinks")] + \
+               [("scale", C.c_float)] + \
+               [(n, C.c_int64) for n in
+                ("q_token_stride", "q_head_stride", "k_token_stride", "k_head_stride",
+                 "v_token_stride", "v_head_stride", "out_token_stride", "out_head_stride")]
+
+
 # Every entry point the header declares: name -> (restype, argtypes)
 _P = C.c_void_p
 SIGNATURES = {
@@ -151,6 +191,11 @@ SIGNATURES = {
     "prism_encode": (C.c_int, [_P, _P, _P, C.c_int32, _P]),
     "prism_decode": (C.c_int, [_P, _P, _P, C.c_int32, _P]),
     "prism_codec_stage": (C.c_int, [_P, C.c_int32, _P, _P, _P, C.c_int32, _P]),
+    "prism_rope": (C.c_int, [_P, C.POINTER(RopePush), _P, _P, _P, _P]),
+    "prism_cache_append": (C.c_int, [_P, C.POINTER(AppendPush), _P, _P, _P, _P, _P, _P, _P, _P]),
+    "prism_paged_attn_workspace": (C.c_int64, [C.POINTER(PagedAttnPush)]),
+    "prism_paged_attn": (C.c_int, [_P, C.POINTER(PagedAttnPush), _P, _P, _P, _P, _P, _P, _P, C.c_int64, _P]),
+    "prism_seq_attn": (C.c_int, [_P, C.POINTER(SeqAttnPush), _P, _P, _P, _P, _P, _P, _P]),
     "prism_forward_e2e": (C.c_int, [_P, _P, _P, C.c_int32, _P]),
     "prism_forward_e2e_graph": (C.c_int, [_P, _P, _P, C.c_int32, _P]),
 }
@@ -608,6 +653,31 @@ class Engine:
     def project_push(self, up: bool, n_tokens: int, in_off: int, out_off: int) -> ProjectPush:
         a = self.aoffs
         return ProjectPush(n_tokens, 0, a.up_w if up else a.down_w, a.up_b if up else a.down_b, in_off, out_off)
+
+    # sequence operators: device pointers, raising on a refused call
+    def rope(self, push: RopePush, x: int, pos: int, y: int, stream: int | None = None):
+        _check(self.L.prism_rope(self.h, C.byref(push), x, pos, y, stream), self.h)
+
+    def cache_append(self, push: AppendPush, k: int, v: int, seq_of: int, pos_of: int, table: int, k_pages: int,
+                     v_pages: int, stream: int | None = None):
+        _check(self.L.prism_cache_append(self.h, C.byref(push), k, v, seq_of, pos_of, table, k_pages, v_pages, stream),
+               self.h)
+
+    def paged_attn_workspace(self, push: PagedAttnPush) -> int:
+        """Bytes of workspace that paged_attn needs for this push."""
+        n = self.L.prism_paged_attn_workspace(C.byref(push))
+        if n < 0:
+            _check(int(n))
+        return n
+
+    def paged_attn(self, push: PagedAttnPush, q: int, k_pages: int, v_pages: int, table: int, lengths: int, out: int,
+                   workspace: int | None, workspace_bytes: int, stream: int | None = None):
+        _check(self.L.prism_paged_attn(self.h, C.byref(push), q, k_pages, v_pages, table, lengths, out, workspace,
+                                       workspace_bytes, stream), self.h)
+
+    def seq_attn(self, push: SeqAttnPush, q: int, k: int, v: int, cu_q: int | None, cu_k: int | None, out: int,
+                 stream: int | None = None):
+        _check(self.L.prism_seq_attn(self.h, C.byref(push), q, k, v, cu_q, cu_k, out, stream), self.h)
 
     def chain_launch_times(self, x: int, y: int, batch: int, stream: int | None = None):
         """prism_chain_launch_times: (attention ms, expert ms, attention grid,

@@ -1,0 +1,26 @@
+/* The sequence operators' checks, splits and index arithmetic
+ * (csrc/engine/seq_rules.h, csrc/seq_index.h) for ctypes. */
+#include "../prism-inference_amd/csrc/engine/seq_rules.h"
+#include "../prism-inference_amd/csrc/seq_index.h"
+
+using namespace prism;
+
+extern "C" {
+int rope_check(const prism_rope_push* p) { const char* w; return check_rope(*p, &w); }
+int append_check(const prism_append_push* p) { const char* w; return check_append(*p, &w); }
+int paged_check(const prism_paged_attn_push* p) { const char* w; return check_paged(*p, &w); }
+int seq_check(const prism_seq_attn_push* p) { const char* w; return check_seq(*p, &w); }
+int turns(const prism_rope_push* p, int32_t* axis_end, double* t) { return rope_turns(*p, axis_end, t); }
+void keys(int32_t p, int32_t n, int32_t left, int32_t right, int32_t sinks, int32_t* out) {
+    const KeyRange r = key_range(p, n, left, right, sinks);
+    out[0] = r.sink;
+    out[1] = r.lo;
+    out[2] = r.hi;
+}
+void rows(const int32_t* cu, int32_t s, int32_t n_seqs, int32_t n, int32_t* out) {
+    const RowRange r = row_range(cu, s, n_seqs, n);
+    out[0] = r.start;
+    out[1] = r.end;
+}
+int page(int32_t entry, int32_t n_pages) { return page_ok(entry, n_pages); }
+}

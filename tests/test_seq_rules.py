@@ -1,0 +1,183 @@
+"""The sequence operators' checks of arguments and index arithmetic, on the CPU (csrc/engine/seq_rules.h,
+csrc/seq_index.h), and the C entries' refusals that need no device."""
+import ctypes as C
+import os
+import subprocess
+
+import numpy as np
+import pytest
+
+import prism_amd as P
+from conftest import ROOT
+from seqlib import visible
+
+MAX = 2 ** 31 - 1
+
+
+@pytest.fixture(scope="module")
+def rules(tmp_path_factory):
+    so = str(tmp_path_factory.mktemp("seq") / "seq_rules.so")
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Wextra", "-fsanitize=undefined", "-fno-sanitize-recover=all",
+                    "-shared", "-fPIC", "-I", os.path.join(ROOT, "include"),
+                    os.path.join(ROOT, "tests", "seq_rules.cpp"), "-o", so], check=True, timeout=120)
+    lib = C.CDLL(so)
+    lib.rows.argtypes = [C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p]
+    lib.turns.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p]
+    return lib
+
+
+def rope(**kw):
+    d = dict(dtype=P.F16, n_tokens=5, n_heads=4, head_dim=32, n_axes=3, pairs=(4, 6, 6, 0), layout=0, ladder=0, inverse=0,
+             base=10000.0, in_token_stride=128, in_head_stride=32, out_token_stride=128, out_head_stride=32, pos_stride=5)
+    return P.RopePush(**{**d, **kw})
+
+
+def cache(**kw):
+    d = dict(dtype=P.F16, n_kv_heads=2, head_dim=32, page_size=16, n_pages=9, n_seqs=3, table_pages=4)
+    return P.CacheDesc(**{**d, **kw})
+
+
+def append(**kw):
+    d = dict(cache=cache(), n_new=5, k_token_stride=64, k_head_stride=32, v_token_stride=64, v_head_stride=32)
+    return P.AppendPush(**{**d, **kw})
+
+
+def paged(**kw):
+    d = dict(cache=cache(), n_heads=4, left=-1, sinks=0, max_len=64, scale=0.2, q_seq_stride=128, q_head_stride=32,
+             out_seq_stride=128, out_head_stride=32)
+    return P.PagedAttnPush(**{**d, **kw})
+
+
+def seq(**kw):
+    d = dict(dtype=P.BF16, n_seqs=2, n_q=10, n_k=20, n_heads=4, n_kv_heads=2, head_dim=64, left=-1, right=0, sinks=0,
+             scale=0.2, q_token_stride=256, q_head_stride=64, k_token_stride=128, k_head_stride=64, v_token_stride=128,
+             v_head_stride=64, out_token_stride=256, out_head_stride=64)
+    return P.SeqAttnPush(**{**d, **kw})
+
+
+nan, inf = float("nan"), float("inf")
+STRIDES = [-8, 4, 2 ** 41]
+
+
+@pytest.mark.parametrize("bad", [
+    dict(dtype=2), dict(dtype=-1), dict(n_tokens=-1), dict(n_heads=0), dict(n_heads=65537), dict(head_dim=12),
+    dict(head_dim=264), dict(head_dim=0), dict(n_axes=0), dict(n_axes=5), dict(pairs=(4, -1, 6, 0)), dict(pairs=(0, 0, 0, 9)),
+    dict(pairs=(5, 6, 6, 0)), dict(pairs=(MAX, MAX, 6, 0)), dict(layout=2), dict(ladder=-1), dict(inverse=2), dict(base=0.0),
+    dict(base=-3.0), dict(base=nan), dict(base=inf), dict(pos_stride=-1), dict(out_token_stride=64),
+    dict(out_head_stride=0), dict(out_head_stride=16), dict(out_token_stride=0),
+] + [{f: s} for f in ("in_token_stride", "in_head_stride", "out_token_stride", "out_head_stride") for s in STRIDES])
+def test_rope_refusals(rules, bad):
+    assert rules.rope_check(C.byref(rope(**bad))) < 0
+
+
+@pytest.mark.parametrize("good", [
+    {}, dict(n_tokens=0), dict(head_dim=8, pairs=(1, 0, 2, 0)), dict(head_dim=256, out_head_stride=256, out_token_stride=1024),
+    dict(in_head_stride=0), dict(in_token_stride=0), dict(out_head_stride=160, out_token_stride=32),  # heads outermost
+    dict(n_axes=1, pairs=(16, 99, 0, 0)), dict(n_axes=4, pairs=(4, 4, 4, 4)), dict(base=1.0), dict(pos_stride=0),
+])
+def test_rope_accepts(rules, good):
+    assert rules.rope_check(C.byref(rope(**good))) == 0
+
+
+CACHES = [dict(dtype=3), dict(n_kv_heads=0), dict(head_dim=48), dict(head_dim=256), dict(page_size=0), dict(page_size=24),
+          dict(page_size=8192), dict(page_size=-16), dict(n_pages=-1), dict(n_seqs=-1), dict(table_pages=-1)]
+
+
+@pytest.mark.parametrize("bad", [dict(cache=cache(**c)) for c in CACHES] + [dict(n_new=-1)] +
+                         [{f: s} for f in ("k_token_stride", "k_head_stride", "v_token_stride", "v_head_stride")
+                          for s in STRIDES])
+def test_append_refusals(rules, bad):
+    assert rules.append_check(C.byref(append(**bad))) < 0
+    assert rules.append_check(C.byref(append())) == 0
+
+
+@pytest.mark.parametrize("bad", [dict(cache=cache(**c)) for c in CACHES] + [
+    dict(n_heads=0), dict(n_heads=5), dict(n_heads=-2), dict(n_heads=65538), dict(sinks=-1), dict(max_len=-1), dict(scale=0.0),
+    dict(scale=-1.0), dict(scale=nan), dict(scale=inf), dict(out_head_stride=16), dict(out_seq_stride=96),
+] + [{f: s} for f in ("q_seq_stride", "q_head_stride", "out_seq_stride", "out_head_stride") for s in STRIDES])
+def test_paged_refusals(rules, bad):
+    assert rules.paged_check(C.byref(paged(**bad))) < 0
+    assert P.lib().prism_paged_attn_workspace(C.byref(paged(**bad))) < 0
+    assert rules.paged_check(C.byref(paged())) == 0
+
+
+@pytest.mark.parametrize("bad", [
+    dict(dtype=9), dict(n_seqs=-1), dict(n_q=-1), dict(n_k=-1), dict(n_heads=3), dict(n_kv_heads=0), dict(head_dim=40),
+    dict(sinks=-2), dict(scale=0.0), dict(scale=nan), dict(out_token_stride=192), dict(out_head_stride=32),
+] + [{f: s} for f in ("q_token_stride", "k_head_stride", "v_token_stride", "out_token_stride") for s in STRIDES])
+def test_seq_refusals(rules, bad):
+    assert rules.seq_check(C.byref(seq(**bad))) < 0
+    assert rules.seq_check(C.byref(seq())) == 0
+
+
+def test_entries_without_a_context():
+    lib = P.lib()
+    assert lib.prism_rope(None, C.byref(rope()), None, None, None, None) == P.ERR_INVALID
+    assert lib.prism_cache_append(None, C.byref(append()), *[None] * 8) == P.ERR_INVALID
+    assert lib.prism_paged_attn(None, C.byref(paged()), *[None] * 7, 0, None) == P.ERR_INVALID
+    assert lib.prism_seq_attn(None, C.byref(seq()), *[None] * 7) == P.ERR_INVALID
+    assert lib.prism_paged_attn_workspace(None) == P.ERR_INVALID
+    assert lib.prism_paged_attn_workspace(C.byref(paged())) >= 0
+
+
+def test_keys_a_query_sees(rules):
+    """Against the definition, for every small position, window and number of sinks."""
+    out = (C.c_int32 * 3)()
+    for n in (0, 1, 2, 5, 9):
+        for p in range(-4, n + 3):
+            for left in (-1, 0, 1, 3, 20):
+                for right in (-1, 0, 2, 20):
+                    for sinks in (0, 1, 4, 30):
+                        rules.keys(p, n, left, right, sinks, out)
+                        sink, lo, hi = out
+                        assert 0 <= sink <= lo <= hi <= n
+                        got = np.zeros(n, bool)
+                        got[:sink] = True
+                        got[lo:hi] = True
+                        assert (got == visible(p, n, left, right, sinks)).all(), (n, p, left, right, sinks)
+
+
+@pytest.mark.parametrize("p,n,left,right,sinks,want", [
+    (MAX - 1, MAX, MAX, MAX, MAX, (0, 0, MAX)), (MAX - 1, MAX, 0, 0, MAX, (MAX - 1, MAX - 1, MAX)),
+    (-MAX, 5, MAX, 0, 4, (0, 0, 0)), (-MAX, 5, MAX, MAX, 4, (0, 0, 1)),
+])
+def test_keys_at_the_ends_of_the_range(rules, p, n, left, right, sinks, want):
+    out = (C.c_int32 * 3)()
+    rules.keys(p, n, left, right, sinks, out)
+    assert tuple(out) == want
+
+
+@pytest.mark.parametrize("cu,n", [([0, 3, 3, 10], 10), ([0, 30, -5, 10], 10), ([-7, -7, MAX, 4], 10), ([9, 8, 7, 6], 10),
+                                  ([0, 0, 0, 0], 0), ([2, 4, 6, 8], 10)])
+def test_rows_stay_in_range(rules, cu, n):
+    a = np.array(cu, np.int32)
+    out = (C.c_int32 * 2)()
+    for s in range(3):
+        rules.rows(a.ctypes.data, s, 3, n, out)
+        assert 0 <= out[0] <= out[1] <= n
+        if 0 <= cu[s] <= cu[s + 1] <= n:
+            assert (out[0], out[1]) == (cu[s], cu[s + 1])
+    rules.rows(None, 2, 3, 12, out)
+    assert tuple(out) == (8, 12)
+
+
+def test_pages_out_of_the_pool(rules):
+    assert [rules.page(e, 4) for e in (-2 ** 31, -1, 0, 3, 4, MAX)] == [0, 0, 1, 1, 0, 0]
+    assert rules.page(0, 0) == 0
+
+
+@pytest.mark.parametrize("kw", [{}, dict(ladder=1), dict(inverse=1), dict(n_axes=1, pairs=(16, 3, 3, 3)),
+                                dict(pairs=(0, 5, 0, 0)), dict(n_axes=4, pairs=(1, 2, 3, 4), ladder=1)])
+def test_frequencies(rules, kw):
+    p = rope(**kw)
+    end, t = (C.c_int32 * 4)(), (C.c_double * 128)()
+    n = rules.turns(C.byref(p), end, t)
+    pairs = list(p.pairs)[:p.n_axes] + [0] * (4 - p.n_axes)
+    assert n == sum(pairs) and list(end) == list(np.cumsum(pairs))
+    i = 0
+    for a in range(4):
+        for j in range(pairs[a]):
+            e = i / n if p.ladder else j / pairs[a]
+            want = (-1 if p.inverse else 1) * 10000.0 ** -e / (2 * np.pi)
+            assert abs(t[i] - want) <= 4e-16 * abs(want)
+            i += 1
