@@ -7,6 +7,7 @@
 #include <cmath>
 #include <cstdint>
 
+#include "../kernel_args.h"
 #include "prism.h"
 
 namespace prism {
@@ -128,6 +129,15 @@ inline int rope_turns(const prism_rope_push& p, int32_t axis_end[4], double* tur
         axis_end[a] = i;
     }
     return n;
+}
+
+/* Tokens per workgroup of a rope launch: as many as the table of angles holds, but
+ * not so many that the launch has fewer than 4 workgroups per CU. */
+inline int rope_tile(int64_t n_tokens, int n_pairs) {
+    const int most = ROPE_TILE_PAIRS / ((n_pairs + 7) & ~7);
+    int tile = 1;
+    while (2 * tile <= most && n_tokens >= (int64_t)2 * tile * 4 * 256) tile *= 2;
+    return tile;
 }
 
 }  // namespace prism

@@ -88,8 +88,9 @@ extern "C" int prism_rope(prism_ctx* c, const prism_rope_push* p, const void* in
     a.head_dim = p->head_dim;
     a.adjacent = p->layout == PRISM_ROPE_ADJACENT;
     a.n_pairs = rope_turns(*p, a.axis_end, a.turns);
-    const int64_t rows = (int64_t)p->n_tokens * p->n_heads;
-    return launch(c, c->f_rope[p->dtype], "rope", (rows + 255) / 256, 256, &a, stream);
+    a.copy = in != out;
+    a.tile = rope_tile(p->n_tokens, a.n_pairs);
+    return launch(c, c->f_rope[p->dtype], "rope", ((int64_t)p->n_tokens + a.tile - 1) / a.tile, 256, &a, stream);
 }
 
 extern "C" int prism_cache_append(prism_ctx* c, const prism_append_push* p, const void* k, const void* v,

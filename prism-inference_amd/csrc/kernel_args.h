@@ -163,6 +163,7 @@ typedef struct CodecArgs {
 /* ---- sequence operators (rope.hpp, cache.hpp, paged_attn.hpp, seq_attn.hpp) */
 
 #define ROPE_MAX_PAIRS 128
+#define ROPE_TILE_PAIRS 1024 /* of a workgroup's tokens together, each token's pairs rounded up to 8 */
 typedef struct RopeArgs {
     const uint16_t* in;
     uint16_t* out;
@@ -170,6 +171,8 @@ typedef struct RopeArgs {
     int64_t in_token_stride, in_head_stride, out_token_stride, out_head_stride, pos_stride;
     int32_t n_tokens, n_heads, head_dim;
     int32_t n_pairs;        /* turned pairs of channels of a head             */
+    int32_t tile;           /* tokens per workgroup                           */
+    int32_t copy;           /* write the channels that do not turn (not in place) */
     int32_t adjacent;       /* pair i = channels 2i, 2i + 1; else i, i + n_pairs */
     int32_t axis_end[4];    /* pairs [axis_end[a-1], axis_end[a]) belong to axis a */
     double turns[ROPE_MAX_PAIRS]; /* turns per unit of position, negative for the inverse */

@@ -10,7 +10,7 @@
 #include <stdint.h>
 
 #ifdef __HIP__
-#define PRISM_HD __host__ __device__ __forceinline__
+#define PRISM_HD __host__ __device__ inline __attribute__((always_inline))
 #else
 #define PRISM_HD inline
 #endif
