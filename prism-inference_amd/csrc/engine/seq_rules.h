@@ -140,6 +140,10 @@ inline int rope_tile(int64_t n_tokens, int n_pairs) {
     return tile;
 }
 
+/* Query tiles of a sequence attention: enough for any lengths (seq_attn.hpp's
+ * seq_of_tile). */
+inline int64_t seq_tiles(int64_t n_q, int64_t n_seqs) { return n_q / SEQ_BM + n_seqs; }
+
 }  // namespace prism
 
 #endif

@@ -207,6 +207,6 @@ extern "C" int prism_seq_attn(prism_ctx* c, const prism_seq_attn_push* p, const 
     a.right = p->right;
     a.sinks = p->sinks;
     a.scale_log2 = p->scale * 1.4426950408889634f;
-    return launch(c, c->f_seq[p->dtype][hd_index(p->head_dim)], "sequence attention", (int64_t)p->n_q * p->n_heads, 64, &a,
-                  stream);
+    return launch(c, c->f_seq[p->dtype][hd_index(p->head_dim)], "sequence attention", seq_tiles(p->n_q, p->n_seqs) * p->n_heads, 256,
+                  &a, stream);
 }

@@ -205,6 +205,7 @@ typedef struct PagedAttnArgs {
     float scale_log2;       /* scale * log2(e) */
 } PagedAttnArgs;
 
+#define SEQ_BM 128 /* queries per workgroup of a sequence attention */
 typedef struct SeqAttnArgs {
     const uint16_t* q;
     const uint16_t* k;

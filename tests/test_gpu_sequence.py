@@ -429,6 +429,48 @@ def test_seq_rising_scores(engine, dev):
         assert not outside(got[i, 0], want, bound), i
 
 
+@pytest.mark.parametrize("dtype,hd", [("fp16", 16), ("bf16", 32), ("fp16", 64), ("bf16", 128)])
+@pytest.mark.parametrize("what", ["v nan", "v inf", "k nan"])
+def test_seq_bad_values_reach_only_who_sees_them(engine, dev, dtype, hd, what):
+    """One key's value is NaN or infinite: the queries that see it get what the formula gives, the others what they
+    would get without it."""
+    rng = np.random.default_rng(hd)
+    n, at, left, sinks = 300, 100, 40, 2
+    q, k, v = (normal(rng, (n, 1, hd), dtype) for _ in range(3))
+    inf = 0x7C00 if dtype == "fp16" else 0x7F80
+    if what == "k nan":
+        k[at, 0, 3] = NAN[dtype]
+    else:
+        v[at, 0, 5] = inf if what == "v inf" else NAN[dtype]
+    out = dev.put(np.full((n, 1, hd), NAN[dtype], np.uint16))
+    st = {f"{x}_{y}_stride": hd for x in ("q", "k", "v", "out") for y in ("token", "head")}
+    engine.seq_attn(P.SeqAttnPush(dtype=TYPES[dtype], n_seqs=1, n_q=n, n_k=n, n_heads=1, n_kv_heads=1, head_dim=hd, left=left,
+                                  right=0, sinks=sinks, scale=0.1, **st), dev.put(q), dev.put(k), dev.put(v), None, None, out)
+    got = values(dev.get(out, (n, hd)), dtype)
+    qv, kv, vv = (values(x[:, 0], dtype) for x in (q, k, v))
+    for i in range(n):
+        seen = visible(i, n, left, 0, sinks)
+        if not seen[at]:
+            want, bound = attention_row(qv[i], kv, vv, seen, 0.1, dtype)
+            assert not outside(got[i], want, bound), i
+        elif what == "k nan":
+            assert np.isnan(got[i]).all(), i
+        else:
+            want, bound = attention_row(qv[i], kv, np.where(np.isfinite(vv), vv, 0), seen, 0.1, dtype)
+            want, bound, rest = np.delete(want, 5), np.delete(bound, 5), np.delete(got[i], 5)
+            assert not outside(rest, want, bound), i
+            assert np.isposinf(got[i, 5]) if what == "v inf" else np.isnan(got[i, 5]), i
+
+
+@pytest.mark.parametrize("n_seqs", [70, 300])
+def test_seq_many_short(engine, dev, n_seqs):
+    """More sequences than a wave has lanes, empty ones among them."""
+    rng = np.random.default_rng(n_seqs)
+    lens = [(int(x), int(x)) for x in rng.integers(0, 6, n_seqs)]
+    lens[n_seqs // 2] = (260, 261)
+    check_seq(engine, dev, rng, "fp16", 16, 1, 1, lens, 3, 0, 1, head=131)
+
+
 def test_seq_starts_out_of_range(engine, dev):
     """Starts past the rows or out of order: rows inside the buffers at most, and the good sequences right."""
     rng = np.random.default_rng(6)
