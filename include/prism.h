@@ -484,7 +484,8 @@ int prism_rope(prism_ctx* ctx, const prism_rope_push* p, const void* in, const i
 /* A paged cache: keys and values each [n_pages][n_kv_heads][page_size]
  * [head_dim], dense, and a table int32 [n_seqs][table_pages]: token j of
  * sequence s is slot j % page_size of page table[s][j / page_size]. page_size
- * is a power of two up to 4096; head_dim 16, 32, 64 or 128. Pages and
+ * is a power of two up to 4096, table_pages * page_size at most 2^30; head_dim 16,
+ * 32, 64 or 128. Pages and
  * the table are the caller's: sequences may share pages that are only read,
  * and an entry that no call needs may hold anything. */
 typedef struct prism_cache_desc {
@@ -540,7 +541,9 @@ int prism_paged_attn(prism_ctx* ctx, const prism_paged_attn_push* p, const void*
  * + i and sees key j if j <= p + right (right < 0: no limit) and j >= p - left
  * (left < 0: no limit) or j < sinks. Heads, scale and rows without a
  * key as in prism_paged_attn. Rows of out before the first sequence and behind
- * the last one stay as they were. head_dim 16, 32, 64 or 128. */
+ * the last one stay as they were. Starts that are not in order name unspecified
+ * rows of the buffers, never others. head_dim 16, 32, 64 or 128; at most 2^30
+ * rows. */
 typedef struct prism_seq_attn_push {
     int32_t dtype, n_seqs, n_q, n_k, n_heads, n_kv_heads, head_dim;
     int32_t left, right, sinks;

@@ -95,7 +95,8 @@ struct prism_ctx {
     hipFunction_t f_enc01 = nullptr;   /* enc0 + enc1 in one launch (the encoder's first two stages) */
     hipFunction_t f_rope[2] = {};      /* [dtype] */
     hipFunction_t f_append = nullptr;
-    hipFunction_t f_paged[2][4] = {};  /* [dtype][head_dim 16, 32, 64, 128] */
+    hipFunction_t f_paged[2][4][3] = {};  /* [dtype][head_dim 16, 32, 64, 128][1, 2, more heads a key head] */
+    hipFunction_t f_paged_join[2][4] = {};
     hipFunction_t f_seq[2][4] = {};
     std::string err;
 

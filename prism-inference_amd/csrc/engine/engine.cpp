@@ -130,7 +130,9 @@ extern "C" int prism_create(prism_ctx** out, int32_t device, const char* code_ob
         all.emplace_back(&c->f_rope[t], "prism_rope_" + type);
         for (int i = 0; i < 4; ++i) {
             const std::string shape = type + "_h" + std::to_string(16 << i);
-            all.emplace_back(&c->f_paged[t][i], "prism_paged_attn_" + shape);
+            for (int g = 0; g < 3; ++g)
+                all.emplace_back(&c->f_paged[t][i][g], "prism_paged_attn_" + shape + (g == 0 ? "_g1" : g == 1 ? "_g2" : "_many"));
+            all.emplace_back(&c->f_paged_join[t][i], "prism_paged_attn_join_" + shape);
             all.emplace_back(&c->f_seq[t][i], "prism_seq_attn_" + shape);
         }
     }

@@ -4,6 +4,7 @@
 #ifndef PRISM_SEQ_RULES_H
 #define PRISM_SEQ_RULES_H
 
+#include <algorithm>
 #include <cmath>
 #include <cstdint>
 
@@ -14,6 +15,9 @@ namespace prism {
 
 /* Strides are held to 2^40 elements so that no offset passes 64 bits. */
 constexpr int64_t SEQ_MAX_STRIDE = int64_t(1) << 40;
+/* Rows of a sequence attention and tokens of a table's row: key numbers a tile past the
+ * end stay in 32 bits. */
+constexpr int64_t SEQ_MAX_ROWS = int64_t(1) << 30;
 
 inline int seq_bad(const char** why, int code, const char* text) {
     if (why) *why = text;
@@ -85,6 +89,8 @@ inline int check_cache(const prism_cache_desc& d, const char** why) {
         return seq_bad(why, PRISM_ERR_INVALID, "page_size: a power of two up to 4096");
     if (d.n_kv_heads < 1 || d.n_kv_heads > 65536 || d.n_pages < 0 || d.n_seqs < 0 || d.table_pages < 0)
         return seq_bad(why, PRISM_ERR_INVALID, "cache sizes out of range");
+    if ((int64_t)d.table_pages * d.page_size > SEQ_MAX_ROWS)
+        return seq_bad(why, PRISM_ERR_UNSUPPORTED, "a table row of more than 2^30 tokens");
     return PRISM_OK;
 }
 
@@ -108,6 +114,7 @@ inline int check_seq(const prism_seq_attn_push& p, const char** why) {
     if (int rc = check_dtype(p.dtype, why)) return rc;
     if (int rc = check_heads(p.n_heads, p.n_kv_heads, p.head_dim, why)) return rc;
     if (p.n_seqs < 0 || p.n_q < 0 || p.n_k < 0) return seq_bad(why, PRISM_ERR_INVALID, "n_seqs, n_q or n_k < 0");
+    if (p.n_q > SEQ_MAX_ROWS || p.n_k > SEQ_MAX_ROWS) return seq_bad(why, PRISM_ERR_UNSUPPORTED, "more than 2^30 rows");
     if (p.sinks < 0) return seq_bad(why, PRISM_ERR_INVALID, "sinks < 0");
     if (int rc = check_scale(p.scale, why)) return rc;
     if (int rc = check_strides(p.q_token_stride, p.q_head_stride, why)) return rc;
@@ -138,6 +145,37 @@ inline int rope_tile(int64_t n_tokens, int n_pairs) {
     int tile = 1;
     while (2 * tile <= most && n_tokens >= (int64_t)2 * tile * 4 * 256) tile *= 2;
     return tile;
+}
+
+/* How a paged attention is launched. */
+struct PagedPlan {
+    bool many;      /* the MFMA kernel */
+    int head_tiles; /* per key head */
+    int waves;      /* per item: 1 or 4 */
+    int splits;     /* workgroups per item */
+    int64_t grid;
+};
+inline PagedPlan paged_plan(const prism_paged_attn_push& p) {
+    PagedPlan r;
+    const int group = p.n_heads / p.cache.n_kv_heads;
+    r.many = group > 2;
+    r.head_tiles = (group + PAGED_TILE_HEADS - 1) / PAGED_TILE_HEADS;
+    const int64_t items = (int64_t)p.cache.n_seqs * p.cache.n_kv_heads * r.head_tiles;
+    /* keys of the longest sequence expected */
+    int64_t keys = p.max_len > 0 ? p.max_len : (int64_t)p.cache.table_pages * p.cache.page_size;
+    if (p.left >= 0 && keys > (int64_t)p.left + 1 + p.sinks) keys = (int64_t)p.left + 1 + p.sinks;
+    r.waves = items >= 4096 || keys <= 32 ? 1 : 4;
+    r.splits = 1;
+    if (r.waves == 4) {
+        int64_t want = 2048 / std::max<int64_t>(items, 1);
+        want = std::min<int64_t>(want, keys / 256);
+        r.splits = (int)std::max<int64_t>(1, std::min<int64_t>(want, PAGED_MAX_SPLITS));
+    }
+    r.grid = r.waves == 1 ? (items + 3) / 4 : items * r.splits;
+    return r;
+}
+inline int64_t paged_workspace(const prism_paged_attn_push& p, const PagedPlan& r) {
+    return r.splits == 1 ? 0 : (int64_t)p.cache.n_seqs * p.n_heads * r.splits * (p.cache.head_dim + 2) * 4;
 }
 
 /* Query tiles of a sequence attention: enough for any lengths (seq_attn.hpp's

@@ -132,14 +132,12 @@ extern "C" int64_t prism_paged_attn_workspace(const prism_paged_attn_push* p) {
     const char* why = "";
     const int rc = check_paged(*p, &why);
     if (rc) return fail(nullptr, rc, "paged attention: %s", why);
-    return 0;
+    return paged_workspace(*p, paged_plan(*p));
 }
 
 extern "C" int prism_paged_attn(prism_ctx* c, const prism_paged_attn_push* p, const void* q, const void* k_pages,
                                 const void* v_pages, const int32_t* table, const int32_t* lengths, void* out,
                                 void* workspace, int64_t workspace_bytes, void* stream) {
-    (void)workspace;
-    (void)workspace_bytes;
     if (const int rc = checked(c, p, "paged attention", check_paged)) return rc;
     const prism_cache_desc& d = p->cache;
     if (d.n_seqs == 0) return PRISM_OK;
@@ -148,6 +146,11 @@ extern "C" int prism_paged_attn(prism_ctx* c, const prism_paged_attn_push* p, co
         return fail(c, PRISM_ERR_INVALID, "paged attention: NULL cache");
     if (!aligned16(q) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(out))
         return fail(c, PRISM_ERR_INVALID, "paged attention: buffers must be 16-byte aligned");
+    const PagedPlan plan = paged_plan(*p);
+    const int64_t need = paged_workspace(*p, plan);
+    if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
+        return fail(c, PRISM_ERR_INVALID, "paged attention: workspace of %lld bytes, %lld needed, 16-byte aligned",
+                    workspace ? (long long)workspace_bytes : 0LL, (long long)need);
     PagedAttnArgs a;
     memset(&a, 0, sizeof a);
     a.q = static_cast<const uint16_t*>(q);
@@ -169,8 +172,14 @@ extern "C" int prism_paged_attn(prism_ctx* c, const prism_paged_attn_push* p, co
     a.left = p->left;
     a.sinks = p->sinks;
     a.scale_log2 = p->scale * 1.4426950408889634f;
-    return launch(c, c->f_paged[d.dtype][hd_index(d.head_dim)], "paged attention", (int64_t)d.n_seqs * p->n_heads, 64, &a,
-                  stream);
+    a.head_tiles = plan.head_tiles;
+    a.waves = plan.waves;
+    a.splits = plan.splits;
+    a.ws = static_cast<float*>(workspace);
+    const int i = hd_index(d.head_dim), kind = plan.many ? 2 : p->n_heads / d.n_kv_heads - 1;
+    const int rc = launch(c, c->f_paged[d.dtype][i][kind], "paged attention", plan.grid, 256, &a, stream);
+    if (rc || plan.splits == 1) return rc;
+    return launch(c, c->f_paged_join[d.dtype][i], "paged attention's join", (int64_t)d.n_seqs * p->n_heads, 256, &a, stream);
 }
 
 extern "C" int prism_seq_attn(prism_ctx* c, const prism_seq_attn_push* p, const void* q, const void* k, const void* v,

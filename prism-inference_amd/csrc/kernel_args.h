@@ -191,6 +191,8 @@ typedef struct AppendArgs {
     int32_t page_log2, n_pages, table_pages;
 } AppendArgs;
 
+#define PAGED_TILE_HEADS 16 /* heads of a group that a wave takes together */
+#define PAGED_MAX_SPLITS 256
 typedef struct PagedAttnArgs {
     const uint16_t* q;
     const uint16_t* k_pages;
@@ -203,6 +205,10 @@ typedef struct PagedAttnArgs {
     int32_t page_log2, n_pages, table_pages;
     int32_t left, sinks;
     float scale_log2;       /* scale * log2(e) */
+    int32_t head_tiles;     /* of PAGED_TILE_HEADS heads, per key head       */
+    int32_t waves;          /* per item: 1, or 4 (a workgroup's)              */
+    int32_t splits;         /* workgroups per item (waves = 4)                */
+    float* ws;              /* splits > 1: [n_seqs][n_heads][splits][head_dim + 2] */
 } PagedAttnArgs;
 
 #define SEQ_BM 128 /* queries per workgroup of a sequence attention */

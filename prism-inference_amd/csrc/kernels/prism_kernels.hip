@@ -16,7 +16,8 @@
  *   prism_codec_dec1_out                           dec1 + output conv + PixelShuffle + sigmoid
  *   prism_rope_{f16,bf16}                          rotary positions with several axes
  *   prism_cache_append                             new tokens into a paged cache
- *   prism_paged_attn_{f16,bf16}_h{16,32,64,128}    one new token per sequence over its paged cache
+ *   prism_paged_attn_{f16,bf16}_h{16,32,64,128}_{g1,g2,many}  one new token per sequence over its paged cache
+ *   prism_paged_attn_join_{f16,bf16}_h{16,32,64,128}  ... and the join of a split length
  *   prism_seq_attn_{f16,bf16}_h{16,32,64,128}      attention along sequences, window and sinks
  *   prism_zero_i32                                 clears routing counters
  */

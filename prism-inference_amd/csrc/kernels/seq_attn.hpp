@@ -32,13 +32,6 @@ __device__ __forceinline__ f16v mfma_32x32x16(b8 a, b8 b, f16v c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
 
-/* Transposing LDS read: 16 lanes read 4 rows of 16 values (lane i: row i / 4,
- * values 4 (i % 4) ..+3) and lane i gets column i's 4 values. */
-typedef short s4 __attribute__((ext_vector_type(4)));
-__device__ __forceinline__ s4 lds_tr4(const uint16_t* p) {
-    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)p);
-}
-
 /* One query by the whole wave, key after key, a lane per channel: the workgroup's
  * way out where zero weights would meet infinite values. */
 template <class T, int HD>

@@ -262,6 +262,23 @@ def test_paged_sharp_scores(engine, dev, group):
 
 
 @pytest.mark.parametrize("group", [1, 4])
+def test_paged_tiny_values(engine, dev, group):
+    """fp16 queries below the type's smallest normal number, a scale that makes up for it."""
+    rng = np.random.default_rng(14)
+    dtype, hd, n, page = "fp16", 64, 50, 16
+    q = to_bits(rng.standard_normal((1, group, hd)) * 2e-5, dtype)
+    kp, vp, table = paged_cache(rng, [n], 1, hd, page, dtype)
+    k, v = normal(rng, (n, 1, hd), dtype), normal(rng, (n, 1, hd), dtype)
+    fill(kp, table, 0, k)
+    fill(vp, table, 0, v)
+    got = run_paged(engine, dev, dtype, q, kp, vp, table, np.array([n], np.int32), -1, 0, 8192.0, n)
+    for h in range(group):
+        want, bound = attention_row(values(q[0, h], dtype), values(k[:, 0], dtype), values(v[:, 0], dtype), np.ones(n, bool),
+                                    8192.0, dtype)
+        assert not outside(got[0, h], want, bound), h
+
+
+@pytest.mark.parametrize("group", [1, 4])
 @pytest.mark.parametrize("hd", [16, 128])
 def test_paged_bad_tables(engine, dev, hd, group):
     """Keys of entries out of the pool are not seen; lengths out of range are brought into it."""
@@ -656,6 +673,12 @@ def test_refused_calls(hip, engine, dev):
     refused(engine.paged_attn, R.paged(), None, a, a, a, a, a, a, 1 << 20)
     refused(engine.paged_attn, R.paged(), a, a, None, a, a, a, a, 1 << 20)
     refused(engine.paged_attn, R.paged(), a, a, a, a, a, a + 4, a, 1 << 20)
+    long = R.paged(cache=R.cache(n_seqs=1, table_pages=1000), max_len=16000)
+    need = engine.paged_attn_workspace(long)
+    assert need > 0
+    refused(engine.paged_attn, long, a, a, a, a, a, a, a, need - 1)
+    refused(engine.paged_attn, long, a, a, a, a, a, a, None, need)
+    refused(engine.paged_attn, long, a, a, a, a, a, a, a + 4, need)
     refused(engine.seq_attn, R.seq(), a, None, a, a, a, a)
     refused(engine.seq_attn, R.seq(n_seqs=3), a, a, a, None, None, a)  # 10 rows are not 3 equal sequences
     refused(engine.seq_attn, R.seq(n_kv_heads=3), a, a, a, a, a, a)
@@ -675,7 +698,7 @@ def test_no_keys_at_all(engine, dev):
         out = dev.put(np.full(3 * 4 * 32, NAN["fp16"], np.uint16))
         push = R.paged(cache=R.cache(**c), max_len=0)
         need = engine.paged_attn_workspace(push)
-        ws = dev.put(np.zeros(max(need // 2, 8), np.uint16))
+        ws = dev.put(np.zeros(need // 2, np.uint16))
         engine.paged_attn(push, q, None, None, None, dev.put(np.full(3, 9, np.int32)), out, ws, need)
         assert not dev.get(out, 3 * 4 * 32).any()
     out = dev.put(np.full(10 * 4 * 64, NAN["bf16"], np.uint16))
