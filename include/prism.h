@@ -543,7 +543,7 @@ int prism_paged_attn(prism_ctx* ctx, const prism_paged_attn_push* p, const void*
  * key as in prism_paged_attn. Rows of out before the first sequence and behind
  * the last one stay as they were. Starts that are not in order name unspecified
  * rows of the buffers, never others. head_dim 16, 32, 64 or 128; at most 2^30
- * rows. */
+ * rows, k and v token strides at most 2^24. */
 typedef struct prism_seq_attn_push {
     int32_t dtype, n_seqs, n_q, n_k, n_heads, n_kv_heads, head_dim;
     int32_t left, right, sinks;

@@ -18,6 +18,8 @@ constexpr int64_t SEQ_MAX_STRIDE = int64_t(1) << 40;
 /* Rows of a sequence attention and tokens of a table's row: key numbers a tile past the
  * end stay in 32 bits. */
 constexpr int64_t SEQ_MAX_ROWS = int64_t(1) << 30;
+/* Key rows of a tile are addressed with 32 bits. */
+constexpr int64_t SEQ_MAX_KEY_STRIDE = int64_t(1) << 24;
 
 inline int seq_bad(const char** why, int code, const char* text) {
     if (why) *why = text;
@@ -120,6 +122,8 @@ inline int check_seq(const prism_seq_attn_push& p, const char** why) {
     if (int rc = check_strides(p.q_token_stride, p.q_head_stride, why)) return rc;
     if (int rc = check_strides(p.k_token_stride, p.k_head_stride, why)) return rc;
     if (int rc = check_strides(p.v_token_stride, p.v_head_stride, why)) return rc;
+    if (p.k_token_stride > SEQ_MAX_KEY_STRIDE || p.v_token_stride > SEQ_MAX_KEY_STRIDE)
+        return seq_bad(why, PRISM_ERR_UNSUPPORTED, "k and v token strides are at most 2^24");
     return check_out(p.n_q, p.n_heads, p.head_dim, p.out_token_stride, p.out_head_stride, why);
 }
 

@@ -192,7 +192,7 @@ typedef struct AppendArgs {
 } AppendArgs;
 
 #define PAGED_TILE_HEADS 16 /* heads of a group that a wave takes together */
-#define PAGED_MAX_SPLITS 256
+#define PAGED_MAX_SPLITS 64
 typedef struct PagedAttnArgs {
     const uint16_t* q;
     const uint16_t* k_pages;

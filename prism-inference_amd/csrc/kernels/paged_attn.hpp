@@ -377,24 +377,25 @@ __device__ __forceinline__ void paged_many(const PagedAttnArgs& a) {
  * 256 / HD groups of splits. */
 template <class T, int HD>
 __device__ __forceinline__ void paged_join(const PagedAttnArgs& a) {
-    __shared__ float weight[PAGED_MAX_SPLITS], part[256], red[8];
-    const int tid = threadIdx.x, wave = tid >> 6;
+    static_assert(PAGED_MAX_SPLITS == 64, "a lane per split");
+    __shared__ float weight[PAGED_MAX_SPLITS], part[256], total;
+    const int tid = threadIdx.x;
     const float* ws = a.ws + (int64_t)blockIdx.x * a.splits * (HD + 2);
-    const bool in = tid < a.splits;
+    const bool in = tid < a.splits; /* all in the first wave */
     const float m = in ? ws[tid * (HD + 2) + HD] : -INFINITY, l = in ? ws[tid * (HD + 2) + HD + 1] : 0.f;
-    float x = m;
-    for (int o = 1; o < 64; o <<= 1) x = fmaxf(x, __shfl_xor(x, o));
-    if ((tid & 63) == 0) red[wave] = x;
+    if (tid < 64) {
+        float top = m;
+        for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
+        const float f = m == -INFINITY ? 0.f : fast_exp2(m - top);
+        weight[tid] = f;
+        const float sum = wave_sum(l * f);
+        if (tid == 0) total = sum;
+    }
     __syncthreads();
-    const float top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    const float f = m == -INFINITY ? 0.f : fast_exp2(m - top);
-    weight[tid] = f;
-    x = wave_sum(l * f);
-    if ((tid & 63) == 0) red[4 + wave] = x;
-    __syncthreads();
-    const float sum = red[4] + red[5] + red[6] + red[7];
+    const float sum = total;
     const int c = tid % HD;
     float o = 0.f;
+#pragma unroll 8 /* that many loads at once: the launch is as long as their latency */
     for (int s = tid / HD; s < a.splits; s += 256 / HD) o = __builtin_fmaf(ws[s * (HD + 2) + c], weight[s], o);
     part[tid] = o;
     __syncthreads();

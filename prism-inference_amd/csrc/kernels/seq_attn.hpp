@@ -138,20 +138,30 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
 
     f16v o[DT] = {};
     float m = -INFINITY, mc = 0.f, l = 0.f; /* mc = c m, or 0 while m is -inf */
+    float limit = -INFINITY;
+    const float lag = 8.0f / a.scale_log2;
     v8 sk[CH], sv[CH];
 
     auto key0 = [&](int it) { return it < sink_tiles ? it * SEQ_BN : win0 + (it - sink_tiles) * SEQ_BN; };
     auto end_of = [&](int it) { return it < sink_tiles ? sink_end : win1; };
+    /* rows past the end lie past the buffer and read as zeros: no select that would wait for the load */
+    int koff[CH], voff[CH];
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        const int id = (threadIdx.x + 256 * c) % (SEQ_BN * CPR), r = id / CPR, e = (id % CPR) * 8;
+        koff[c] = 2 * (r * (int)a.k_token_stride + e);
+        voff[c] = 2 * (r * (int)a.v_token_stride + e);
+    }
     auto fetch = [&](int it) {
-        const int k0 = key0(it), end = end_of(it);
+        const int k0 = key0(it), rows = seq_min(end_of(it) - k0, SEQ_BN);
+        const auto kr = __builtin_amdgcn_make_buffer_rsrc((void*)(kb + k0 * a.k_token_stride), (short)0,
+                                                          2 * ((rows - 1) * (int)a.k_token_stride + HD), 0x00020000);
+        const auto vr = __builtin_amdgcn_make_buffer_rsrc((void*)(vb + k0 * a.v_token_stride), (short)0,
+                                                          2 * ((rows - 1) * (int)a.v_token_stride + HD), 0x00020000);
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
-            const int id = threadIdx.x + 256 * c, r = id / CPR, e = (id % CPR) * 8;
-            const bool ok = k0 + r < end && (SEQ_BN * CPR >= 256 || id < SEQ_BN * CPR);
-            const int64_t j = ok ? k0 + r : 0; /* n_tiles > 0: there is a key 0 */
-            const v8 x = ld8<T>(kb + j * a.k_token_stride + e), y = ld8<T>(vb + j * a.v_token_stride + e);
-            sk[c] = ok ? x : v8{};
-            sv[c] = ok ? y : v8{};
+            sk[c] = __builtin_bit_cast(v8, __builtin_amdgcn_raw_buffer_load_b128(kr, koff[c], 0, 0));
+            sv[c] = __builtin_bit_cast(v8, __builtin_amdgcn_raw_buffer_load_b128(vr, voff[c], 0, 0));
         }
     };
     auto put = [&](int it, int buf) {
@@ -181,6 +191,9 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
         fetch(0);
         put(0, 0);
     }
+    /* the queries are in from here on: a wait for them inside the loop would be one for the next tile too */
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) qf[ks] = opaque(qf[ks]);
     __syncthreads();
     for (int it = 0; it < n_tiles; ++it) {
         if (it + 1 < n_tiles) fetch(it + 1);
@@ -206,15 +219,17 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
                         sc[t][i] = j < hi && (j >= me.lo || j < a.sinks) ? sc[t][i] : -INFINITY;
                     }
             }
-            float top = m;
+            float top = sc[0][0];
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
-                for (int i = 0; i < 16; i += 2) top = fmaxf(fmaxf(top, sc[t][i]), sc[t][i + 1]);
+                for (int i = 0; i < 16; i += 2) top = vmax3(top, sc[t][i], sc[t][i + 1]);
             float x, y;
             lanes_x32(top, x, y);
-            top = fmaxf(x, y);
-            if (__any(top > m)) {
+            top = vmax(x, y);
+            /* the maximum may lag by 8 powers of two: weights up to 256 cost no precision, rescaling costs much */
+            if (__any(top > limit)) {
+                top = vmax(top, m);
                 const float tc = top == -INFINITY ? 0.f : top * a.scale_log2;
                 const float f = fast_exp2(m == -INFINITY ? -INFINITY : mc - tc);
                 l *= f;
@@ -224,6 +239,7 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
                     for (int i = 0; i < 16; ++i) o[d][i] *= f;
                 m = top;
                 mc = tc;
+                limit = top + lag;
             }
             v8 p[4];
 #pragma unroll

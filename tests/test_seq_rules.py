@@ -104,7 +104,7 @@ def test_paged_refusals(rules, bad):
 
 @pytest.mark.parametrize("bad", [
     dict(dtype=9), dict(n_seqs=-1), dict(n_q=-1), dict(n_k=-1), dict(n_heads=3), dict(n_kv_heads=0), dict(head_dim=40),
-    dict(n_q=2 ** 30 + 1), dict(n_k=MAX), dict(sinks=-2), dict(scale=0.0), dict(scale=nan), dict(out_token_stride=192), dict(out_head_stride=32),
+    dict(k_token_stride=2 ** 24 + 8), dict(v_token_stride=2 ** 24 + 8), dict(n_q=2 ** 30 + 1), dict(n_k=MAX), dict(sinks=-2), dict(scale=0.0), dict(scale=nan), dict(out_token_stride=192), dict(out_head_stride=32),
 ] + [{f: s} for f in ("q_token_stride", "k_head_stride", "v_token_stride", "out_token_stride") for s in STRIDES])
 def test_seq_refusals(rules, bad):
     assert rules.seq_check(C.byref(seq(**bad))) < 0
