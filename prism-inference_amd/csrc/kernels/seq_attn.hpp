@@ -200,14 +200,37 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
         const int k0 = key0(it), end = end_of(it), buf = it & 1;
         /* not for a tile that none of the wave's queries sees */
         if (on && k0 < wb.hi && (k0 + SEQ_BN > wa.lo || k0 < a.sinks)) {
+            /* the scores; a k-step's keys are read two steps ahead */
+            const uint16_t* krow = lk[buf] + c32 * KROW + 8 * g;
             f16v sc[2] = {};
+            v8 kf[3][2];
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks)
+            for (int ks = 0; ks < KS + 2; ++ks) {
+                if (ks < KS) {
 #pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    const v8 kf = ld8<T>(lk[buf] + (32 * t + c32) * KROW + 16 * ks + 8 * g);
-                    sc[t] = mfma_32x32x16(kf, qf[ks], sc[t]);
+                    for (int t = 0; t < 2; ++t) kf[ks % 3][t] = ld8<T>(krow + 32 * t * KROW + 16 * ks);
                 }
+                sched_fence();
+                if (ks >= 2) {
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) sc[t] = mfma_32x32x16(kf[(ks - 2) % 3][t], qf[ks - 2], sc[t]);
+                }
+            }
+            /* V^T of 16 keys: lane's rows are keys 16 t + 4 g ..+3 and 8 more on, its columns by the 16-lane group */
+            const uint16_t* vrow = lv[buf] + (4 * g + (lane & 15) / 4) * VROW + (HD >= 32 ? lane & 16 : 0) + 4 * (lane & 3);
+            union VFrag {
+                s4 h[2];
+                v8 v;
+            };
+            VFrag vf[2][DT];
+            auto read_v = [&](int t) {
+#pragma unroll
+                for (int d = 0; d < DT; ++d) {
+                    vf[t & 1][d].h[0] = lds_tr4(vrow + 16 * t * VROW + 32 * d);
+                    vf[t & 1][d].h[1] = lds_tr4(vrow + (16 * t + 8) * VROW + 32 * d);
+                }
+            };
+            read_v(0);
             const bool whole = k0 + SEQ_BN <= seq_min(wa.hi, end) && (k0 >= wb.lo || k0 + SEQ_BN <= a.sinks);
             if (!whole) {
                 const int hi = seq_min(me.hi, end);
@@ -241,30 +264,21 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
                 mc = tc;
                 limit = top + lag;
             }
-            v8 p[4];
+            /* 16 keys at a time: the next ones' V is read and their weights computed under the products */
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
+            for (int t = 0; t < 4; ++t) {
+                if (t < 3) read_v(t + 1);
+                v8 p;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float e = fast_exp2(__builtin_fmaf(sc[t][i], a.scale_log2, -mc));
+                for (int i = 0; i < 8; ++i) {
+                    const float e = fast_exp2(__builtin_fmaf(sc[t / 2][8 * (t & 1) + i], a.scale_log2, -mc));
                     l += e;
-                    p[2 * t + i / 8][i % 8] = (typename T::el)e;
+                    p[i] = (typename T::el)e;
                 }
+                sched_fence();
 #pragma unroll
-            for (int d = 0; d < DT; ++d)
-#pragma unroll
-                for (int t = 0; t < 4; ++t) {
-                    /* lane's rows: keys 16 t + 4 g ..+3 and 8 more on; its columns by the 16-lane group */
-                    const int i = lane & 15, col = HD >= 32 ? 32 * d + (lane & 16) : 0;
-                    const uint16_t* at = lv[buf] + (16 * t + 4 * g + i / 4) * VROW + col + 4 * (i & 3);
-                    union {
-                        s4 h[2];
-                        v8 v;
-                    } vf;
-                    vf.h[0] = lds_tr4(at);
-                    vf.h[1] = lds_tr4(at + 8 * VROW);
-                    o[d] = mfma_32x32x16(vf.v, p[t], o[d]);
-                }
+                for (int d = 0; d < DT; ++d) o[d] = mfma_32x32x16(vf[t & 1][d].v, p, o[d]);
+            }
         }
         if (it + 1 < n_tiles) put(it + 1, buf ^ 1);
         __syncthreads();
