@@ -186,6 +186,8 @@ inline int64_t paged_workspace(const prism_paged_attn_push& p, const PagedPlan& 
  * seq_of_tile). */
 inline int64_t seq_tiles(int64_t n_q, int64_t n_seqs) { return n_q / SEQ_BM + n_seqs; }
 
+inline bool seq_w8(int64_t grid) { return grid <= 1024; }
+
 }  // namespace prism
 
 #endif

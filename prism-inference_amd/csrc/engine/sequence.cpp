@@ -5,6 +5,7 @@
  */
 #include <hip/hip_runtime.h>
 
+#include <cstdlib>
 #include <cstring>
 
 #include "ctx.h"
@@ -216,6 +217,7 @@ extern "C" int prism_seq_attn(prism_ctx* c, const prism_seq_attn_push* p, const 
     a.right = p->right;
     a.sinks = p->sinks;
     a.scale_log2 = p->scale * 1.4426950408889634f;
-    return launch(c, c->f_seq[p->dtype][hd_index(p->head_dim)], "sequence attention", seq_tiles(p->n_q, p->n_seqs) * p->n_heads, 256,
-                  &a, stream);
+    const int64_t grid = seq_tiles(p->n_q, p->n_seqs) * p->n_heads;
+    const bool w8 = getenv("W8") ? atoi(getenv("W8")) : seq_w8(grid);
+    return launch(c, c->f_seq[p->dtype][hd_index(p->head_dim)][w8], "sequence attention", grid, w8 ? 512 : 256, &a, stream);
 }

@@ -4,7 +4,7 @@
  * p = nk - nq + i and sees keys j <= p + right with j >= p - left or j < sinks.
  *
  * A workgroup takes 128 queries of one head, 32 a wave, and goes once over the
- * keys that any of them sees, 64 at a time, with a running maximum and sum:
+ * keys that any of them sees, 64 or 128 at a time, with a running maximum and sum:
  *   S^T = K Q^T           (32x32x16 MFMA: a lane holds one query's scores)
  *   P^T = 2^(c S^T - c m) (registers; c = scale log2 e)
  *   O^T += V^T P^T        (P^T is the B operand as it lies: the MFMA's
@@ -22,8 +22,6 @@
 #include "seq_types.hpp"
 
 typedef float f16v __attribute__((ext_vector_type(16)));
-
-#define SEQ_BN 64  /* keys per tile */
 
 __device__ __forceinline__ f16v mfma_32x32x16(h8 a, h8 b, f16v c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
@@ -58,41 +56,53 @@ __device__ __forceinline__ void seq_attn_row(const SeqAttnArgs& a, const uint16_
         if (on) st1<T>(out + lane + 64 * e, l == 0.f ? 0.f : acc[e] / l);
 }
 
-/* The sequence whose query tiles include tile b: sequence s owns the tiles from
- * floor(start / SEQ_BM) + s on, which leaves each enough of them whatever
- * the lengths. 64 candidates a step. */
-__device__ __forceinline__ int seq_of_tile(const SeqAttnArgs& a, int b, int& first) {
-    int lo = 0, n = a.n_seqs, lane = lane_id();
-    first = 0;
+/* The sequence whose query tiles include tile b, and its rows: sequence s owns the
+ * tiles from floor(start / SEQ_BM) + s on, which leaves each enough of them
+ * whatever the lengths. 64 candidates a step; the last step's loads bring the
+ * rows along. */
+struct SeqTile {
+    int first;     /* the sequence's first tile */
+    RowRange q, k;
+};
+__device__ __forceinline__ SeqTile seq_of_tile(const SeqAttnArgs& a, int b) {
+    int lo = 0, n = a.n_seqs;
+    const int lane = lane_id();
     while (true) {
         const int step = (n + 63) / 64;
-        const int s = lo + lane * step;
-        bool in = false;
-        int key = 0;
-        if (lane * step < n) {
-            key = row_range(a.cu_q, s, a.n_seqs, a.n_q).start / SEQ_BM + s;
-            in = key <= b;
+        const int s = lo + min(lane, (n - 1) / step) * step; /* lanes past the end: the last one again */
+        const RowRange q = row_range(a.cu_q, s, a.n_seqs, a.n_q);
+        RowRange k{0, 0};
+        if (step == 1) k = row_range(a.cu_k, s, a.n_seqs, a.n_k);
+        const int key = q.start / SEQ_BM + s;
+        const unsigned long long mask = __ballot(key <= b);
+        const int at = mask ? min(63 - __builtin_clzll(mask), (n - 1) / step) : 0;
+        if (step == 1) {
+            const auto of = [&](int v) { return __builtin_amdgcn_readlane(v, at); };
+            return SeqTile{of(key), RowRange{of(q.start), of(q.end)}, RowRange{of(k.start), of(k.end)}};
         }
-        const unsigned long long mask = __ballot(in);
-        const int at = mask ? 63 - __builtin_clzll(mask) : 0;
         lo += at * step;
         n = min(step, n - at * step);
-        first = __builtin_amdgcn_readlane(key, at);
-        if (step == 1) return lo;
     }
 }
 
-template <class T, int HD>
+/* KW: wave groups that share a workgroup's queries, each taking 64 keys of every tile. */
+template <class T, int HD, int KW>
 __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
     typedef typename T::v8 v8;
+    constexpr int NTHR = 256 * KW, BN = 64 * KW; /* threads; keys per tile      */
     constexpr int KS = HD / 16;              /* k-steps of the scores          */
     constexpr int DT = (HD + 31) / 32;       /* 32-channel tiles of the output */
+    constexpr int NS = KS > 2 * DT ? KS : 2 * DT; /* steps of a part           */
+    constexpr int EL = 16 / NS;              /* scores per lane and step       */
     constexpr int KROW = HD + 8;             /* padded LDS rows (16-bit values): no bank conflicts for  */
     constexpr int VROW = HD + (HD >= 64 ? 32 : 0); /* 16-byte reads down rows; 8 rows of 64 bytes       */
     constexpr int CPR = HD / 8;              /* 16-byte chunks of a row        */
-    constexpr int CH = (SEQ_BN * CPR + 255) / 256; /* chunks per thread        */
-    __shared__ __attribute__((aligned(16))) uint16_t lk[2][SEQ_BN * KROW];
-    __shared__ __attribute__((aligned(16))) uint16_t lv[2][SEQ_BN * VROW];
+    constexpr int CHUNKS = BN * CPR, CH = (CHUNKS + NTHR - 1) / NTHR; /* per tile, per thread */
+    constexpr int KVBYTES = 4 * BN * (KROW + VROW), MERGE = KW > 1 ? 4 * 64 * (16 * DT + 2) * 4 : 0;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[KVBYTES > MERGE ? KVBYTES : MERGE];
+    uint16_t* const lk = reinterpret_cast<uint16_t*>(lds); /* [2][BN][KROW] */
+    uint16_t* const lv = lk + 2 * BN * KROW;               /* [2][BN][VROW] */
+    const auto uni = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
 
     /* workgroup -> (query tile, head): an XCD (workgroups b, b + 8, ...) takes a
      * run of neighbouring heads, whose keys its L2 then holds */
@@ -102,15 +112,15 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
     const int w = xcd * per + min(xcd, big) + (b >> 3);
     const int h = w / tiles, hk = h / (a.n_heads / a.n_kv_heads);
     const int tile = tiles - 1 - (w - h * tiles); /* the last, longest rows first */
-    int first;
-    const int s = __builtin_amdgcn_readfirstlane(seq_of_tile(a, tile, first));
-    const RowRange rq = row_range(a.cu_q, s, a.n_seqs, a.n_q), rk = row_range(a.cu_k, s, a.n_seqs, a.n_k);
+    const SeqTile st = seq_of_tile(a, tile);
+    const RowRange rq = st.q, rk = st.k;
+    const int first = st.first;
     const int nq = rq.end - rq.start, nk = rk.end - rk.start;
     if (tile < first || (int64_t)(tile - first) * SEQ_BM >= nq) return; /* uniform over the workgroup */
     const int q0 = (tile - first) * SEQ_BM, q1 = min(q0 + SEQ_BM, nq);
 
     const int lane = lane_id(), c32 = lane & 31, g = lane >> 5;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wave = uni(threadIdx.x >> 6) & 3, half = uni(threadIdx.x >> 8);
     const int qa = q0 + 32 * wave, qb = min(qa + 32, q1); /* the wave's queries */
     const int shift = nk - nq;                            /* position - row */
     const bool on = qa < q1;
@@ -120,16 +130,19 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
     const int qi = min(qa + c32, q1 - 1); /* this lane's query; past the end: the last one, never stored */
     const uint16_t* qp = a.q + (rq.start + qi) * a.q_token_stride + h * a.q_head_stride;
 
-    /* keys that the workgroup's, the wave's and the lane's queries see */
+    /* Keys that the workgroup's, the wave's and the lane's queries see. Tiles go over
+     * the sinks first (if a window begins behind them), then over the rest of the
+     * window, so a tile needs no more than one comparison per end. */
     const KeyRange r0 = key_range(shift + q0, nk, a.left, a.right, a.sinks);
     const KeyRange r1 = key_range(shift + q1 - 1, nk, a.left, a.right, a.sinks);
-    const KeyRange wa = key_range(shift + qa, nk, a.left, a.right, a.sinks);
-    const KeyRange wb = key_range(shift + qb - 1, nk, a.left, a.right, a.sinks);
     const KeyRange me = key_range(shift + qi, nk, a.left, a.right, a.sinks);
-    const int sink_end = seq_min(seq_min(a.sinks, r0.lo), r1.hi); /* sinks before the window */
-    const int win0 = r0.lo, win1 = r1.hi;
-    const int sink_tiles = (sink_end + SEQ_BN - 1) / SEQ_BN;
-    const int n_tiles = sink_tiles + (win1 > win0 ? (win1 - win0 + SEQ_BN - 1) / SEQ_BN : 0);
+    const int sink_end = r1.lo > 0 ? seq_min(a.sinks, r1.hi) : 0;
+    const int win0 = seq_max(r0.lo, sink_end), win1 = r1.hi;
+    const int sink_tiles = (sink_end + BN - 1) / BN;
+    const int n_tiles = sink_tiles + (win1 > win0 ? (win1 - win0 + BN - 1) / BN : 0);
+    const KeyRange ra = key_range(shift + qa, nk, a.left, a.right, a.sinks);
+    const KeyRange rb = key_range(shift + qb - 1, nk, a.left, a.right, a.sinks);
+    const int a_lo = uni(ra.lo), a_hi = uni(ra.hi), b_lo = uni(rb.lo), b_hi = uni(rb.hi);
 
     unsigned bad = 0; /* infinite or NaN V where only some of the queries look */
     v8 qf[KS];
@@ -140,43 +153,39 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
     float m = -INFINITY, mc = 0.f, l = 0.f; /* mc = c m, or 0 while m is -inf */
     float limit = -INFINITY;
     const float lag = 8.0f / a.scale_log2;
-    v8 sk[CH], sv[CH];
 
-    auto key0 = [&](int it) { return it < sink_tiles ? it * SEQ_BN : win0 + (it - sink_tiles) * SEQ_BN; };
-    auto end_of = [&](int it) { return it < sink_tiles ? sink_end : win1; };
-    /* rows past the end lie past the buffer and read as zeros: no select that would wait for the load */
+    /* k0 of tile t + 1, from tile t's; where a tile's keys end */
+    auto step = [&](int t, int k0) { return t + 1 == sink_tiles ? win0 : k0 + BN; };
+    auto end_of = [&](int t) { return t < sink_tiles ? sink_end : win1; };
+    /* Tiles through registers to LDS. Rows past the end lie past the buffer and read as zeros: no select that
+       would wait for the load. */
     int koff[CH], voff[CH];
+    v8 sk[CH], sv[CH];
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-        const int id = (threadIdx.x + 256 * c) % (SEQ_BN * CPR), r = id / CPR, e = (id % CPR) * 8;
+        const int id = (threadIdx.x + NTHR * c) % CHUNKS, r = id / CPR, e = (id % CPR) * 8;
         koff[c] = 2 * (r * (int)a.k_token_stride + e);
         voff[c] = 2 * (r * (int)a.v_token_stride + e);
     }
-    auto fetch = [&](int it) {
-        const int k0 = key0(it), rows = seq_min(end_of(it) - k0, SEQ_BN);
-        const auto kr = __builtin_amdgcn_make_buffer_rsrc((void*)(kb + k0 * a.k_token_stride), (short)0,
-                                                          2 * ((rows - 1) * (int)a.k_token_stride + HD), 0x00020000);
-        const auto vr = __builtin_amdgcn_make_buffer_rsrc((void*)(vb + k0 * a.v_token_stride), (short)0,
-                                                          2 * ((rows - 1) * (int)a.v_token_stride + HD), 0x00020000);
+    auto fetch = [&](v8 (&to)[CH], const uint16_t* base, int stride, const int (&off)[CH], int t, int k0) {
+        if (t >= n_tiles) return;
+        const int rows = seq_min(end_of(t) - k0, BN);
+        const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)(base + (int64_t)k0 * stride), (short)0,
+                                                            2 * ((rows - 1) * stride + HD), 0x00020000);
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+            to[c] = __builtin_bit_cast(v8, __builtin_amdgcn_raw_buffer_load_b128(rsrc, off[c], 0, 0));
+    };
+    auto put = [&](uint16_t* to, int row, const v8 (&from)[CH]) {
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
-            sk[c] = __builtin_bit_cast(v8, __builtin_amdgcn_raw_buffer_load_b128(kr, koff[c], 0, 0));
-            sv[c] = __builtin_bit_cast(v8, __builtin_amdgcn_raw_buffer_load_b128(vr, voff[c], 0, 0));
+            const int id = threadIdx.x + NTHR * c, r = id / CPR, e = (id % CPR) * 8;
+            if (CHUNKS % NTHR == 0 || id < CHUNKS) st8<T>(to + r * row + e, from[c]);
         }
     };
-    auto put = [&](int it, int buf) {
-#pragma unroll
-        for (int c = 0; c < CH; ++c) {
-            const int id = threadIdx.x + 256 * c, r = id / CPR, e = (id % CPR) * 8;
-            if (SEQ_BN * CPR >= 256 || id < SEQ_BN * CPR) {
-                st8<T>(lk[buf] + r * KROW + e, sk[c]);
-                st8<T>(lv[buf] + r * VROW + e, sv[c]);
-            }
-        }
-        /* seen by some queries only: are the values finite? */
-        const int k0 = key0(it);
-        if ((k0 < r1.lo && k0 + SEQ_BN > a.sinks) || k0 + SEQ_BN > r0.hi) {
-            constexpr unsigned E = sizeof(typename T::el) == 2 && __is_same(T, F16) ? 0x7C007C00u : 0x7F807F80u;
+    auto check_v = [&](int t, int k0) { /* a tile that some queries see only in part: are its V finite? */
+        if ((t >= sink_tiles && k0 < r1.lo) || k0 + BN > r0.hi) {
+            constexpr unsigned E = __is_same(T, F16) ? 0x7C007C00u : 0x7F807F80u;
             constexpr unsigned U = __is_same(T, F16) ? 0x04000400u : 0x00800080u;
 #pragma unroll
             for (int c = 0; c < CH; ++c) {
@@ -187,105 +196,147 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
         }
     };
 
-    if (n_tiles > 0) {
-        fetch(0);
-        put(0, 0);
-    }
+    /* The wave's keys go in parts of 32, two of each tile. In body(i) three parts are under way: the scores of
+       part i + 1 and the products of part i - 1 on the matrix cores, the weights of part i on the vector
+       units, a few of each at a time. */
+    union VFrag {
+        s4 h[2];
+        v8 v;
+    };
+    const uint16_t* const krow = lk + (64 * half + c32) * KROW + 8 * g;
+    const uint16_t* const vrow =
+        lv + (64 * half + 4 * g + (lane & 15) / 4) * VROW + (HD >= 32 ? lane & 16 : 0) + 4 * (lane & 3);
+    auto active = [&](int t, int k0) { /* does the wave see any of the part that starts at k0? */
+        return on && t < n_tiles && k0 < (t < sink_tiles ? seq_min(b_hi, sink_end) : b_hi) &&
+               (t < sink_tiles || k0 + 32 > a_lo);
+    };
+    auto read_v = [&](VFrag& f, const uint16_t* at, int j) { /* 16 keys j / DT, channels 32 (j % DT) ..: V^T as
+                                                              lane's rows keys 4 g ..+3 and 8 more on */
+        f.h[0] = lds_tr4(at + 16 * (j / DT) * VROW + 32 * (j % DT));
+        f.h[1] = lds_tr4(at + (16 * (j / DT) + 8) * VROW + 32 * (j % DT));
+    };
+    /* sc, p: scores and weights of the part at k0 of tile t; sn: scores of the next part (keys at ka); pl: weights
+       of the last one (values at va). A part that the wave does not see gets zero weights. */
+    auto body = [&](int t, int k0, const uint16_t* ka, const uint16_t* va, f16v& sc, f16v& sn, v8 (&p)[2], const v8 (&pl)[2]) {
+        v8 kf[3];
+        VFrag vf[3];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            if (j < KS) kf[j] = ld8<T>(ka + 16 * j);
+            if (j < 2 * DT) read_v(vf[j], va, j);
+        }
+        const int end = end_of(t), j0 = k0 + 4 * g;
+        if (k0 + 32 > seq_min(a_hi, end)) {
+            const int hi = seq_min(me.hi, end) - j0;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) sc[e] = 8 * (e / 4) + (e & 3) < hi ? sc[e] : -INFINITY;
+        }
+        if (t >= sink_tiles && k0 < b_lo) {
+            const int lo = me.lo - j0;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) sc[e] = 8 * (e / 4) + (e & 3) >= lo ? sc[e] : -INFINITY;
+        }
+        float top = vmax(sc[0], sc[1]), x, y;
+#pragma unroll
+        for (int e = 2; e < 16; e += 2) top = vmax3(top, sc[e], sc[e + 1]);
+        lanes_x32(top, x, y);
+        top = vmax(x, y);
+        /* the maximum may lag by 8 powers of two: weights up to 256 cost no precision, rescaling costs much */
+        float f = 1.f;
+        const bool scale = __any(top > limit);
+        if (scale) {
+            top = vmax(top, m);
+            const float tc = top == -INFINITY ? 0.f : top * a.scale_log2;
+            f = fast_exp2(m == -INFINITY ? -INFINITY : mc - tc);
+            l *= f;
+            m = top;
+            mc = tc;
+            limit = top + lag;
+        }
+        sn = f16v{};
+#pragma unroll
+        for (int j = 0; j < NS; ++j) {
+            if (j + 2 < KS) kf[(j + 2) % 3] = ld8<T>(ka + 16 * (j + 2));
+            if (j + 2 < 2 * DT) read_v(vf[(j + 2) % 3], va, j + 2);
+            if (j < KS) sn = mfma_32x32x16(kf[j % 3], qf[j], sn);
+#pragma unroll
+            for (int e = EL * j; e < EL * (j + 1); ++e) {
+                const float z = fast_exp2(__builtin_fmaf(sc[e], a.scale_log2, -mc));
+                l += z;
+                p[e / 8][e % 8] = (typename T::el)z;
+            }
+            if (j < 2 * DT) o[j % DT] = mfma_32x32x16(vf[j % 3].v, pl[j / DT], o[j % DT]);
+            sched_fence();
+        }
+        if (scale) {
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[d][e] *= f;
+        }
+    };
+
+    const int ks_ = (int)a.k_token_stride, vs_ = (int)a.v_token_stride;
+    int k0 = sink_tiles > 0 ? 0 : win0, k1 = step(0, k0), k2 = step(1, k1); /* of tiles t, t + 1, t + 2 */
+    fetch(sk, kb, ks_, koff, 0, k0);
+    put(lk, KROW, sk);
+    fetch(sk, kb, ks_, koff, 1, k1);
+    fetch(sv, vb, vs_, voff, 0, k0);
+    /* there is no part before the first: its weights are zero, and so is its V */
+    for (int i = threadIdx.x; i < BN * VROW / 8; i += NTHR) st8<T>(lv + BN * VROW + 8 * i, v8{});
     /* the queries are in from here on: a wait for them inside the loop would be one for the next tile too */
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) qf[ks] = opaque(qf[ks]);
     __syncthreads();
-    for (int it = 0; it < n_tiles; ++it) {
-        if (it + 1 < n_tiles) fetch(it + 1);
-        const int k0 = key0(it), end = end_of(it), buf = it & 1;
-        /* not for a tile that none of the wave's queries sees */
-        if (on && k0 < wb.hi && (k0 + SEQ_BN > wa.lo || k0 < a.sinks)) {
-            /* the scores; a k-step's keys are read two steps ahead */
-            const uint16_t* krow = lk[buf] + c32 * KROW + 8 * g;
-            f16v sc[2] = {};
-            v8 kf[3][2];
+    f16v s0 = {}, s1 = {};
+    v8 p0[2] = {}, p1[2] = {};
+    bool last = false, now0 = active(0, k0 + 64 * half);
+    if (now0) {
 #pragma unroll
-            for (int ks = 0; ks < KS + 2; ++ks) {
-                if (ks < KS) {
-#pragma unroll
-                    for (int t = 0; t < 2; ++t) kf[ks % 3][t] = ld8<T>(krow + 32 * t * KROW + 16 * ks);
-                }
-                sched_fence();
-                if (ks >= 2) {
-#pragma unroll
-                    for (int t = 0; t < 2; ++t) sc[t] = mfma_32x32x16(kf[(ks - 2) % 3][t], qf[ks - 2], sc[t]);
-                }
-            }
-            /* V^T of 16 keys: lane's rows are keys 16 t + 4 g ..+3 and 8 more on, its columns by the 16-lane group */
-            const uint16_t* vrow = lv[buf] + (4 * g + (lane & 15) / 4) * VROW + (HD >= 32 ? lane & 16 : 0) + 4 * (lane & 3);
-            union VFrag {
-                s4 h[2];
-                v8 v;
-            };
-            VFrag vf[2][DT];
-            auto read_v = [&](int t) {
-#pragma unroll
-                for (int d = 0; d < DT; ++d) {
-                    vf[t & 1][d].h[0] = lds_tr4(vrow + 16 * t * VROW + 32 * d);
-                    vf[t & 1][d].h[1] = lds_tr4(vrow + (16 * t + 8) * VROW + 32 * d);
-                }
-            };
-            read_v(0);
-            const bool whole = k0 + SEQ_BN <= seq_min(wa.hi, end) && (k0 >= wb.lo || k0 + SEQ_BN <= a.sinks);
-            if (!whole) {
-                const int hi = seq_min(me.hi, end);
-#pragma unroll
-                for (int t = 0; t < 2; ++t)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const int j = k0 + 32 * t + 8 * (i / 4) + 4 * g + (i & 3);
-                        sc[t][i] = j < hi && (j >= me.lo || j < a.sinks) ? sc[t][i] : -INFINITY;
-                    }
-            }
-            float top = sc[0][0];
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int i = 0; i < 16; i += 2) top = vmax3(top, sc[t][i], sc[t][i + 1]);
-            float x, y;
-            lanes_x32(top, x, y);
-            top = vmax(x, y);
-            /* the maximum may lag by 8 powers of two: weights up to 256 cost no precision, rescaling costs much */
-            if (__any(top > limit)) {
-                top = vmax(top, m);
-                const float tc = top == -INFINITY ? 0.f : top * a.scale_log2;
-                const float f = fast_exp2(m == -INFINITY ? -INFINITY : mc - tc);
-                l *= f;
-#pragma unroll
-                for (int d = 0; d < DT; ++d)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) o[d][i] *= f;
-                m = top;
-                mc = tc;
-                limit = top + lag;
-            }
-            /* 16 keys at a time: the next ones' V is read and their weights computed under the products */
-#pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                if (t < 3) read_v(t + 1);
-                v8 p;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float e = fast_exp2(__builtin_fmaf(sc[t / 2][8 * (t & 1) + i], a.scale_log2, -mc));
-                    l += e;
-                    p[i] = (typename T::el)e;
-                }
-                sched_fence();
-#pragma unroll
-                for (int d = 0; d < DT; ++d) o[d] = mfma_32x32x16(vf[t & 1][d].v, p, o[d]);
-            }
+        for (int j = 0; j < KS; ++j) s0 = mfma_32x32x16(ld8<T>(krow + 16 * j), qf[j], s0);
+    }
+    /* Tile t's V and tile t + 1's K are put in LDS between the bodies that last read the tiles before them
+       (before the last barrier) and those that read them (behind the next one). */
+    int kp = 0, vp = 0; /* LDS buffers of tile t */
+    for (int t = 0; t < n_tiles; ++t) {
+        const int kn = BN * KROW - kp, vn = BN * VROW - vp, at = k0 + 64 * half;
+        const bool now1 = active(t, at + 32), next0 = active(t + 1, k1 + 64 * half);
+        if (last || now0 || now1) {
+            body(t, at, krow + kp + 32 * KROW, vrow + vn + 32 * VROW, s0, s1, p0, p1);
+        } else {
+            p0[0] = p0[1] = v8{};
         }
-        if (it + 1 < n_tiles) put(it + 1, buf ^ 1);
+        put(lk + kn, KROW, sk);
+        put(lv + vp, VROW, sv);
+        check_v(t, k0);
         __syncthreads();
+        fetch(sk, kb, ks_, koff, t + 2, k2);
+        fetch(sv, vb, vs_, voff, t + 1, k1);
+        if (now0 || now1 || next0) {
+            body(t, at + 32, krow + kn, vrow + vp, s1, s0, p1, p0);
+        } else {
+            p1[0] = p1[1] = v8{};
+        }
+        last = now1;
+        now0 = next0;
+        k0 = k1;
+        k1 = k2;
+        k2 = step(t + 2, k2);
+        kp = kn;
+        vp = vn;
+    }
+    if (last) { /* the last part's products */
+        const uint16_t* va = vrow + (BN * VROW - vp) + 32 * VROW;
+#pragma unroll
+        for (int j = 0; j < 2 * DT; ++j) {
+            VFrag vf;
+            read_v(vf, va, j);
+            o[j % DT] = mfma_32x32x16(vf.v, p1[j / DT], o[j % DT]);
+        }
     }
 
     if (__syncthreads_or((bad & 0x80008000u) != 0)) {
-        for (int i = qa; i < qb; ++i)
+        for (int i = qa + half; i < qb; i += KW)
             seq_attn_row<T, HD>(a, a.q + (rq.start + i) * a.q_token_stride + h * a.q_head_stride, kb, vb,
                                 a.out + (rq.start + i) * a.out_token_stride + h * a.out_head_stride,
                                 key_range(shift + i, nk, a.left, a.right, a.sinks));
@@ -294,6 +345,26 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
     float x, y;
     lanes_x32(l, x, y);
     l = x + y;
+    if constexpr (KW > 1) { /* the other group's result through LDS (everyone is done with the tiles) */
+        float* red = reinterpret_cast<float*>(lds) + (wave * 64 + lane);
+        if (half == 1) {
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) red[(16 * d + e) * 256] = o[d][e];
+            red[16 * DT * 256] = m == -INFINITY ? m : mc;
+            red[(16 * DT + 1) * 256] = l;
+        }
+        __syncthreads();
+        if (half == 1) return;
+        const float m0 = m == -INFINITY ? m : mc, m1 = red[16 * DT * 256], top = vmax(m0, m1);
+        const float f0 = m0 == -INFINITY ? 0.f : fast_exp2(m0 - top), f1 = m1 == -INFINITY ? 0.f : fast_exp2(m1 - top);
+        l = l * f0 + red[(16 * DT + 1) * 256] * f1;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[d][e] = o[d][e] * f0 + red[(16 * d + e) * 256] * f1;
+    }
     if (!on || qa + c32 >= qb) return;
     const float inv = l == 0.f ? 0.f : 1.0f / l;
     uint16_t* out = a.out + (rq.start + qi) * a.out_token_stride + h * a.out_head_stride;
@@ -311,8 +382,9 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
         }
 }
 
-#define SEQ_ATTN(NAME, T, HD) \
-    extern "C" __global__ void __launch_bounds__(256, 2) prism_seq_attn_##NAME##_h##HD(SeqAttnArgs a) { seq_attn_body<T, HD>(a); }
+#define SEQ_ATTN(NAME, T, HD)                                                                                                       \
+    extern "C" __global__ void __launch_bounds__(256, 2) prism_seq_attn_##NAME##_h##HD(SeqAttnArgs a) { seq_attn_body<T, HD, 1>(a); } \
+    extern "C" __global__ void __launch_bounds__(512, 2) prism_seq_attn_##NAME##_h##HD##_w8(SeqAttnArgs a) { seq_attn_body<T, HD, 2>(a); }
 SEQ_ATTN(f16, F16, 16) SEQ_ATTN(f16, F16, 32) SEQ_ATTN(f16, F16, 64) SEQ_ATTN(f16, F16, 128)
 SEQ_ATTN(bf16, BF16, 16) SEQ_ATTN(bf16, BF16, 32) SEQ_ATTN(bf16, BF16, 64) SEQ_ATTN(bf16, BF16, 128)
 #undef SEQ_ATTN
