@@ -30,6 +30,27 @@ __device__ __forceinline__ f16v mfma_32x32x16(b8 a, b8 b, f16v c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
 
+/* 16 bytes a lane from a buffer straight to LDS, 1 KiB in a row from byte address `to` (the same in every
+ * lane) on; lanes past the buffer's end write zeros. In assembly because the compiler would wait for it before
+ * the next LDS read, whichever: the caller waits (vm_wait) before the barrier behind which the data is read. */
+typedef int i4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ i4 buffer_of(const void* p, int bytes) {
+    const uint64_t at = (uint64_t)p;
+    return i4{(int)at, (int)(at >> 32) & 0xFFFF, bytes, 0x00020000};
+}
+__device__ __forceinline__ void load_to_lds(i4 buffer, int offset, unsigned to) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                 ::"s"(to), "v"(offset), "s"(buffer)
+                 : "memory");
+}
+/* Computed here and not nearer to its use: keeps what goes beside the matrix products there. */
+template <class T>
+__device__ __forceinline__ T pinned(T v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
+__device__ __forceinline__ void vm_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
 /* One query by the whole wave, key after key, a lane per channel: the workgroup's
  * way out where zero weights would meet infinite values. */
 template <class T, int HD>
@@ -94,14 +115,11 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
     constexpr int DT = (HD + 31) / 32;       /* 32-channel tiles of the output */
     constexpr int NS = KS > 2 * DT ? KS : 2 * DT; /* steps of a part           */
     constexpr int EL = 16 / NS;              /* scores per lane and step       */
-    constexpr int KROW = HD + 8;             /* padded LDS rows (16-bit values): no bank conflicts for  */
-    constexpr int VROW = HD + (HD >= 64 ? 32 : 0); /* 16-byte reads down rows; 8 rows of 64 bytes       */
     constexpr int CPR = HD / 8;              /* 16-byte chunks of a row        */
     constexpr int CHUNKS = BN * CPR, CH = (CHUNKS + NTHR - 1) / NTHR; /* per tile, per thread */
-    constexpr int KVBYTES = 4 * BN * (KROW + VROW), MERGE = KW > 1 ? 4 * 64 * (16 * DT + 2) * 4 : 0;
-    __shared__ __attribute__((aligned(16))) uint8_t lds[KVBYTES > MERGE ? KVBYTES : MERGE];
-    uint16_t* const lk = reinterpret_cast<uint16_t*>(lds); /* [2][BN][KROW] */
-    uint16_t* const lv = lk + 2 * BN * KROW;               /* [2][BN][VROW] */
+    constexpr int TILE = 2 * BN * HD;        /* bytes of a tile of K or V      */
+    constexpr int KVBYTES = 4 * TILE, MERGE = KW > 1 ? 4 * 64 * (16 * DT + 2) * 4 : 0;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[KVBYTES > MERGE ? KVBYTES : MERGE]; /* K: 2 tiles, V: 2 tiles */
     const auto uni = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
 
     /* workgroup -> (query tile, head): an XCD (workgroups b, b + 8, ...) takes a
@@ -120,7 +138,7 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
     const int q0 = (tile - first) * SEQ_BM, q1 = min(q0 + SEQ_BM, nq);
 
     const int lane = lane_id(), c32 = lane & 31, g = lane >> 5;
-    const int wave = uni(threadIdx.x >> 6) & 3, half = uni(threadIdx.x >> 8);
+    const int wave8 = uni(threadIdx.x >> 6), wave = wave8 & 3, half = wave8 >> 2;
     const int qa = q0 + 32 * wave, qb = min(qa + 32, q1); /* the wave's queries */
     const int shift = nk - nq;                            /* position - row */
     const bool on = qa < q1;
@@ -157,39 +175,38 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
     /* k0 of tile t + 1, from tile t's; where a tile's keys end */
     auto step = [&](int t, int k0) { return t + 1 == sink_tiles ? win0 : k0 + BN; };
     auto end_of = [&](int t) { return t < sink_tiles ? sink_end : win1; };
-    /* Tiles through registers to LDS. Rows past the end lie past the buffer and read as zeros: no select that
-       would wait for the load. */
+    /* Tiles go from memory to LDS directly, 64 chunks of 16 bytes in a row per wave and load. A lane may choose
+       which chunk it brings, so chunk c of row r lies at place c ^ swizzle(r): for K, 16 rows' chunks of one
+       column then lie in different banks; for V, 4 rows' groups of 64 bytes. Rows past the end lie past the
+       buffer and are written as zeros. */
+    auto swizzle_k = [](int r) { return CPR < 16 ? r / (16 / CPR) & (CPR - 1) : r & 15; };
+    auto swizzle_v = [](int r) { return HD == 128 ? (r & 3) * 4 : HD == 64 ? (r >> 1 & 1) * 4 : 0; };
     int koff[CH], voff[CH];
-    v8 sk[CH], sv[CH];
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-        const int id = (threadIdx.x + NTHR * c) % CHUNKS, r = id / CPR, e = (id % CPR) * 8;
-        koff[c] = 2 * (r * (int)a.k_token_stride + e);
-        voff[c] = 2 * (r * (int)a.v_token_stride + e);
+        const int id = (threadIdx.x + NTHR * c) % CHUNKS, r = id / CPR, e = id % CPR;
+        koff[c] = 2 * (r * (int)a.k_token_stride + (e ^ swizzle_k(r)) * 8);
+        voff[c] = 2 * (r * (int)a.v_token_stride + (e ^ swizzle_v(r)) * 8);
     }
-    auto fetch = [&](v8 (&to)[CH], const uint16_t* base, int stride, const int (&off)[CH], int t, int k0) {
+    const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) uint8_t*)lds;
+    auto fetch = [&](int to, const uint16_t* base, int stride, const int (&off)[CH], int t, int k0) {
         if (t >= n_tiles) return;
         const int rows = seq_min(end_of(t) - k0, BN);
-        const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)(base + (int64_t)k0 * stride), (short)0,
-                                                            2 * ((rows - 1) * stride + HD), 0x00020000);
-#pragma unroll
-        for (int c = 0; c < CH; ++c)
-            to[c] = __builtin_bit_cast(v8, __builtin_amdgcn_raw_buffer_load_b128(rsrc, off[c], 0, 0));
-    };
-    auto put = [&](uint16_t* to, int row, const v8 (&from)[CH]) {
+        const i4 buffer = buffer_of(base + (int64_t)k0 * stride, 2 * ((rows - 1) * stride + HD));
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
-            const int id = threadIdx.x + NTHR * c, r = id / CPR, e = (id % CPR) * 8;
-            if (CHUNKS % NTHR == 0 || id < CHUNKS) st8<T>(to + r * row + e, from[c]);
+            const int id0 = 64 * wave8 + NTHR * c; /* the wave's first chunk */
+            if (CHUNKS % NTHR == 0 || id0 < CHUNKS) load_to_lds(buffer, off[c], lds0 + to + 16 * id0);
         }
     };
-    auto check_v = [&](int t, int k0) { /* a tile that some queries see only in part: are its V finite? */
+    auto check_v = [&](int at, int t, int k0) { /* a tile that some queries see only in part: finite? */
         if ((t >= sink_tiles && k0 < r1.lo) || k0 + BN > r0.hi) {
             constexpr unsigned E = __is_same(T, F16) ? 0x7C007C00u : 0x7F807F80u;
             constexpr unsigned U = __is_same(T, F16) ? 0x04000400u : 0x00800080u;
 #pragma unroll
             for (int c = 0; c < CH; ++c) {
-                const u4 d = __builtin_bit_cast(u4, sv[c]);
+                const int id = (threadIdx.x + NTHR * c) % CHUNKS;
+                const u4 d = *reinterpret_cast<const u4*>(lds + 2 * TILE + at + 16 * id);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) bad |= (d[i] & E) + U;
             }
@@ -203,26 +220,34 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
         s4 h[2];
         v8 v;
     };
-    const uint16_t* const krow = lk + (64 * half + c32) * KROW + 8 * g;
-    const uint16_t* const vrow =
-        lv + (64 * half + 4 * g + (lane & 15) / 4) * VROW + (HD >= 32 ? lane & 16 : 0) + 4 * (lane & 3);
+    /* this lane's places (bytes from lk, lv on), to be xored with 32 per k-step and 64 per 32 channels */
+    const int krow = 2 * (64 * half + c32) * HD + 16 * (g ^ swizzle_k(c32));
+    const int vrow = 2 * (64 * half + 4 * g + (lane & 15) / 4) * HD +
+                     ((HD >= 32 ? 2 * (lane & 16) : 0) ^ 16 * swizzle_v((lane & 15) / 4)) + 8 * (lane & 3);
+    auto read_k = [&](int at, int ks) { return *reinterpret_cast<const v8*>(lds + (at ^ 32 * ks)); };
     auto active = [&](int t, int k0) { /* does the wave see any of the part that starts at k0? */
         return on && t < n_tiles && k0 < (t < sink_tiles ? seq_min(b_hi, sink_end) : b_hi) &&
                (t < sink_tiles || k0 + 32 > a_lo);
     };
-    auto read_v = [&](VFrag& f, const uint16_t* at, int j) { /* 16 keys j / DT, channels 32 (j % DT) ..: V^T as
-                                                              lane's rows keys 4 g ..+3 and 8 more on */
-        f.h[0] = lds_tr4(at + 16 * (j / DT) * VROW + 32 * (j % DT));
-        f.h[1] = lds_tr4(at + (16 * (j / DT) + 8) * VROW + 32 * (j % DT));
+    auto read_v = [&](VFrag& f, int at, int j) { /* 16 keys j / DT, channels 32 (j % DT) ..: V^T as
+                                                    lane's rows keys 4 g ..+3 and 8 more on */
+        const uint8_t* v = lds + 2 * TILE + (at ^ 64 * (j % DT)) + 32 * (j / DT) * HD;
+        f.h[0] = lds_tr4(v);
+        f.h[1] = lds_tr4(v + 16 * HD);
+    };
+    auto weights = [](const unsigned (&p)[8], int i) { return __builtin_bit_cast(v8, u4{p[4 * i], p[4 * i + 1], p[4 * i + 2], p[4 * i + 3]}); };
+    auto none = [](unsigned (&p)[8]) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) p[i] = 0;
     };
     /* sc, p: scores and weights of the part at k0 of tile t; sn: scores of the next part (keys at ka); pl: weights
        of the last one (values at va). A part that the wave does not see gets zero weights. */
-    auto body = [&](int t, int k0, const uint16_t* ka, const uint16_t* va, f16v& sc, f16v& sn, v8 (&p)[2], const v8 (&pl)[2]) {
+    auto body = [&](int t, int k0, int ka, int va, f16v& sc, f16v& sn, unsigned (&p)[8], const unsigned (&pl)[8]) {
         v8 kf[3];
         VFrag vf[3];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            if (j < KS) kf[j] = ld8<T>(ka + 16 * j);
+            if (j < KS) kf[j] = read_k(ka, j);
             if (j < 2 * DT) read_v(vf[j], va, j);
         }
         const int end = end_of(t), j0 = k0 + 4 * g;
@@ -256,16 +281,19 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
         sn = f16v{};
 #pragma unroll
         for (int j = 0; j < NS; ++j) {
-            if (j + 2 < KS) kf[(j + 2) % 3] = ld8<T>(ka + 16 * (j + 2));
+            if (j + 2 < KS) kf[(j + 2) % 3] = read_k(ka, j + 2);
             if (j + 2 < 2 * DT) read_v(vf[(j + 2) % 3], va, j + 2);
             if (j < KS) sn = mfma_32x32x16(kf[j % 3], qf[j], sn);
 #pragma unroll
-            for (int e = EL * j; e < EL * (j + 1); ++e) {
-                const float z = fast_exp2(__builtin_fmaf(sc[e], a.scale_log2, -mc));
-                l += z;
-                p[e / 8][e % 8] = (typename T::el)z;
+            for (int e = EL * j; e < EL * (j + 1); e += 2) {
+                const float z0 = fast_exp2(__builtin_fmaf(sc[e], a.scale_log2, -mc));
+                const float z1 = fast_exp2(__builtin_fmaf(sc[e + 1], a.scale_log2, -mc));
+                l += z0;
+                l += z1;
+                p[e / 2] = pinned(__builtin_bit_cast(unsigned, typename T::v2{(typename T::el)z0, (typename T::el)z1}));
             }
-            if (j < 2 * DT) o[j % DT] = mfma_32x32x16(vf[j % 3].v, pl[j / DT], o[j % DT]);
+            l = pinned(l);
+            if (j < 2 * DT) o[j % DT] = mfma_32x32x16(vf[j % 3].v, weights(pl, j / DT), o[j % DT]);
             sched_fence();
         }
         if (scale) {
@@ -278,60 +306,58 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
 
     const int ks_ = (int)a.k_token_stride, vs_ = (int)a.v_token_stride;
     int k0 = sink_tiles > 0 ? 0 : win0, k1 = step(0, k0), k2 = step(1, k1); /* of tiles t, t + 1, t + 2 */
-    fetch(sk, kb, ks_, koff, 0, k0);
-    put(lk, KROW, sk);
-    fetch(sk, kb, ks_, koff, 1, k1);
-    fetch(sv, vb, vs_, voff, 0, k0);
+    fetch(0, kb, ks_, koff, 0, k0);
     /* there is no part before the first: its weights are zero, and so is its V */
-    for (int i = threadIdx.x; i < BN * VROW / 8; i += NTHR) st8<T>(lv + BN * VROW + 8 * i, v8{});
-    /* the queries are in from here on: a wait for them inside the loop would be one for the next tile too */
+    for (int i = threadIdx.x; i < TILE / 16; i += NTHR) *reinterpret_cast<v8*>(lds + 3 * TILE + 16 * i) = v8{};
+    vm_wait();
+    /* the queries are in from here on: the compiler would wait for them, and the tiles on the way, in the loop */
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) qf[ks] = opaque(qf[ks]);
     __syncthreads();
+    fetch(TILE, kb, ks_, koff, 1, k1);
+    fetch(2 * TILE, vb, vs_, voff, 0, k0);
     f16v s0 = {}, s1 = {};
-    v8 p0[2] = {}, p1[2] = {};
+    unsigned p0[8] = {}, p1[8] = {};
     bool last = false, now0 = active(0, k0 + 64 * half);
     if (now0) {
 #pragma unroll
-        for (int j = 0; j < KS; ++j) s0 = mfma_32x32x16(ld8<T>(krow + 16 * j), qf[j], s0);
+        for (int j = 0; j < KS; ++j) s0 = mfma_32x32x16(read_k(krow, j), qf[j], s0);
     }
-    /* Tile t's V and tile t + 1's K are put in LDS between the bodies that last read the tiles before them
-       (before the last barrier) and those that read them (behind the next one). */
-    int kp = 0, vp = 0; /* LDS buffers of tile t */
+    /* Tile t's V and tile t + 1's K come to LDS between the bodies that last read the tiles before them (before
+       the last barrier) and those that read them (behind the next one). */
+    int buf = 0; /* LDS buffers of tile t: buf, of the tiles next to it: other */
     for (int t = 0; t < n_tiles; ++t) {
-        const int kn = BN * KROW - kp, vn = BN * VROW - vp, at = k0 + 64 * half;
+        const int other = TILE - buf, at = k0 + 64 * half;
         const bool now1 = active(t, at + 32), next0 = active(t + 1, k1 + 64 * half);
         if (last || now0 || now1) {
-            body(t, at, krow + kp + 32 * KROW, vrow + vn + 32 * VROW, s0, s1, p0, p1);
+            body(t, at, krow + buf + 64 * HD, vrow + other + 64 * HD, s0, s1, p0, p1);
         } else {
-            p0[0] = p0[1] = v8{};
+            none(p0);
         }
-        put(lk + kn, KROW, sk);
-        put(lv + vp, VROW, sv);
-        check_v(t, k0);
+        vm_wait();
         __syncthreads();
-        fetch(sk, kb, ks_, koff, t + 2, k2);
-        fetch(sv, vb, vs_, voff, t + 1, k1);
+        fetch(buf, kb, ks_, koff, t + 2, k2);
+        fetch(2 * TILE + other, vb, vs_, voff, t + 1, k1);
+        check_v(buf, t, k0);
         if (now0 || now1 || next0) {
-            body(t, at + 32, krow + kn, vrow + vp, s1, s0, p1, p0);
+            body(t, at + 32, krow + other, vrow + buf, s1, s0, p1, p0);
         } else {
-            p1[0] = p1[1] = v8{};
+            none(p1);
         }
         last = now1;
         now0 = next0;
         k0 = k1;
         k1 = k2;
         k2 = step(t + 2, k2);
-        kp = kn;
-        vp = vn;
+        buf = other;
     }
     if (last) { /* the last part's products */
-        const uint16_t* va = vrow + (BN * VROW - vp) + 32 * VROW;
+        const int va = vrow + (TILE - buf) + 64 * HD;
 #pragma unroll
         for (int j = 0; j < 2 * DT; ++j) {
             VFrag vf;
             read_v(vf, va, j);
-            o[j % DT] = mfma_32x32x16(vf.v, p1[j / DT], o[j % DT]);
+            o[j % DT] = mfma_32x32x16(vf.v, weights(p1, j / DT), o[j % DT]);
         }
     }
 

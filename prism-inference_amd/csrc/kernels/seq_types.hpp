@@ -52,6 +52,6 @@ __device__ __forceinline__ f4 mfma_16x16x32(b8 a, b8 b, f4 c) {
 /* Transposing LDS read: 16 lanes read 4 rows of 16 values (lane i: row i / 4,
  * values 4 (i % 4) ..+3) and lane i gets column i's 4 values. */
 typedef short s4 __attribute__((ext_vector_type(4)));
-__device__ __forceinline__ s4 lds_tr4(const uint16_t* p) {
+__device__ __forceinline__ s4 lds_tr4(const void* p) {
     return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)p);
 }
