@@ -30,6 +30,14 @@ __device__ __forceinline__ f16v mfma_32x32x16(b8 a, b8 b, f16v c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
 
+template <class T>
+__device__ __forceinline__ typename T::v8 splat_one() {
+    typename T::v8 v;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = (typename T::el)1.0f;
+    return v;
+}
+
 /* 16 bytes a lane from a buffer straight to LDS, 1 KiB in a row from byte address `to` (the same in every
  * lane) on; lanes past the buffer's end write zeros. In assembly because the compiler would wait for it before
  * the next LDS read, whichever: the caller waits (vm_wait) before the barrier behind which the data is read. */
@@ -106,20 +114,22 @@ __device__ __forceinline__ SeqTile seq_of_tile(const SeqAttnArgs& a, int b) {
     }
 }
 
-/* KW: wave groups that share a workgroup's queries, each taking 64 keys of every tile. */
+/* KW: wave groups that share a workgroup's queries, each taking its keys of every tile. */
 template <class T, int HD, int KW>
 __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
     typedef typename T::v8 v8;
-    constexpr int NTHR = 256 * KW, BN = 64 * KW; /* threads; keys per tile      */
+    constexpr int NP = HD <= 32 && KW == 1 ? 4 : 2; /* parts of 32 keys that a wave has of a tile */
+    constexpr int NTHR = 256 * KW, BN = 32 * NP * KW; /* threads; keys per tile */
     constexpr int KS = HD / 16;              /* k-steps of the scores          */
     constexpr int DT = (HD + 31) / 32;       /* 32-channel tiles of the output */
+    constexpr bool ONES = HD <= 64;          /* sums of weights on the matrix cores, see below */
     constexpr int NS = KS > 2 * DT ? KS : 2 * DT; /* steps of a part           */
     constexpr int EL = 16 / NS;              /* scores per lane and step       */
     constexpr int CPR = HD / 8;              /* 16-byte chunks of a row        */
     constexpr int CHUNKS = BN * CPR, CH = (CHUNKS + NTHR - 1) / NTHR; /* per tile, per thread */
     constexpr int TILE = 2 * BN * HD;        /* bytes of a tile of K or V      */
-    constexpr int KVBYTES = 4 * TILE, MERGE = KW > 1 ? 4 * 64 * (16 * DT + 2) * 4 : 0;
-    __shared__ __attribute__((aligned(16))) uint8_t lds[KVBYTES > MERGE ? KVBYTES : MERGE]; /* K: 2 tiles, V: 2 tiles */
+    constexpr int KRING = (NP == 2 ? 2 : 3) * TILE, KVBYTES = KRING + 2 * TILE, MERGE = KW > 1 ? 4 * 64 * (16 * DT + 2) * 4 : 0;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[KVBYTES > MERGE ? KVBYTES : MERGE]; /* a ring of K tiles, two V tiles */
     const auto uni = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
 
     /* workgroup -> (query tile, head): an XCD (workgroups b, b + 8, ...) takes a
@@ -169,6 +179,11 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
 
     f16v o[DT] = {};
     float m = -INFINITY, mc = 0.f, l = 0.f; /* mc = c m, or 0 while m is -inf */
+    /* The sum of a query's weights: as many additions as weights on the vector units, or products with ones on
+       the matrix cores, which wait for the vector units up to 64 channels. (16 channels leave half of the
+       output's rows free: there V's unused rows are the ones.) The weights summed are then the rounded ones. */
+    f16v lsum = {};
+    const v8 ones = splat_one<T>();
     float limit = -INFINITY;
     const float lag = 8.0f / a.scale_log2;
 
@@ -206,14 +221,14 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
 #pragma unroll
             for (int c = 0; c < CH; ++c) {
                 const int id = (threadIdx.x + NTHR * c) % CHUNKS;
-                const u4 d = *reinterpret_cast<const u4*>(lds + 2 * TILE + at + 16 * id);
+                const u4 d = *reinterpret_cast<const u4*>(lds + KRING + at + 16 * id);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) bad |= (d[i] & E) + U;
             }
         }
     };
 
-    /* The wave's keys go in parts of 32, two of each tile. In body(i) three parts are under way: the scores of
+    /* The wave's keys go in parts of 32. In the body for part i three parts are under way: the scores of
        part i + 1 and the products of part i - 1 on the matrix cores, the weights of part i on the vector
        units, a few of each at a time. */
     union VFrag {
@@ -221,8 +236,8 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
         v8 v;
     };
     /* this lane's places (bytes from lk, lv on), to be xored with 32 per k-step and 64 per 32 channels */
-    const int krow = 2 * (64 * half + c32) * HD + 16 * (g ^ swizzle_k(c32));
-    const int vrow = 2 * (64 * half + 4 * g + (lane & 15) / 4) * HD +
+    const int krow = 2 * (32 * NP * half + c32) * HD + 16 * (g ^ swizzle_k(c32));
+    const int vrow = 2 * (32 * NP * half + 4 * g + (lane & 15) / 4) * HD +
                      ((HD >= 32 ? 2 * (lane & 16) : 0) ^ 16 * swizzle_v((lane & 15) / 4)) + 8 * (lane & 3);
     auto read_k = [&](int at, int ks) { return *reinterpret_cast<const v8*>(lds + (at ^ 32 * ks)); };
     auto active = [&](int t, int k0) { /* does the wave see any of the part that starts at k0? */
@@ -231,9 +246,13 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
     };
     auto read_v = [&](VFrag& f, int at, int j) { /* 16 keys j / DT, channels 32 (j % DT) ..: V^T as
                                                     lane's rows keys 4 g ..+3 and 8 more on */
-        const uint8_t* v = lds + 2 * TILE + (at ^ 64 * (j % DT)) + 32 * (j / DT) * HD;
+        const uint8_t* v = lds + KRING + (at ^ 64 * (j % DT)) + 32 * (j / DT) * HD;
         f.h[0] = lds_tr4(v);
         f.h[1] = lds_tr4(v + 16 * HD);
+        if constexpr (HD == 16) { /* every lane takes part in the transposing read */
+            f.v = opaque(f.v);
+            f.v = c32 >= 16 ? ones : f.v;
+        }
     };
     auto weights = [](const unsigned (&p)[8], int i) { return __builtin_bit_cast(v8, u4{p[4 * i], p[4 * i + 1], p[4 * i + 2], p[4 * i + 3]}); };
     auto none = [](unsigned (&p)[8]) {
@@ -250,16 +269,17 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
             if (j < KS) kf[j] = read_k(ka, j);
             if (j < 2 * DT) read_v(vf[j], va, j);
         }
-        const int end = end_of(t), j0 = k0 + 4 * g;
-        if (k0 + 32 > seq_min(a_hi, end)) {
-            const int hi = seq_min(me.hi, end) - j0;
+        const int end = end_of(t);
+        const bool cut_lo = t >= sink_tiles && k0 < b_lo;
+        if (k0 + 32 > seq_min(a_hi, end) || cut_lo) {
+            const int hi = seq_clamp(seq_min(me.hi, end) - k0, 0, 32), lo = cut_lo ? seq_clamp(me.lo - k0, 0, 32) : 0;
+            const unsigned seen = ((unsigned)(((uint64_t)1 << hi) - ((uint64_t)1 << seq_min(lo, hi)))) >> (4 * g);
 #pragma unroll
-            for (int e = 0; e < 16; ++e) sc[e] = 8 * (e / 4) + (e & 3) < hi ? sc[e] : -INFINITY;
-        }
-        if (t >= sink_tiles && k0 < b_lo) {
-            const int lo = me.lo - j0;
-#pragma unroll
-            for (int e = 0; e < 16; ++e) sc[e] = 8 * (e / 4) + (e & 3) >= lo ? sc[e] : -INFINITY;
+            for (int e = 0; e < 16; ++e) { /* a bit field and a bit select: no compare to wait for */
+                const int all = (int)(seen << (31 - 8 * (e / 4) - (e & 3))) >> 31;
+                const float x = sc[e];
+                sc[e] = __builtin_bit_cast(float, (__builtin_bit_cast(int, x) & all) | ((int)0xFF800000 & ~all));
+            }
         }
         float top = vmax(sc[0], sc[1]), x, y;
 #pragma unroll
@@ -273,7 +293,7 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
             top = vmax(top, m);
             const float tc = top == -INFINITY ? 0.f : top * a.scale_log2;
             f = fast_exp2(m == -INFINITY ? -INFINITY : mc - tc);
-            l *= f;
+            if (!ONES) l *= f;
             m = top;
             mc = tc;
             limit = top + lag;
@@ -288,12 +308,15 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
             for (int e = EL * j; e < EL * (j + 1); e += 2) {
                 const float z0 = fast_exp2(__builtin_fmaf(sc[e], a.scale_log2, -mc));
                 const float z1 = fast_exp2(__builtin_fmaf(sc[e + 1], a.scale_log2, -mc));
-                l += z0;
-                l += z1;
+                if (!ONES) {
+                    l += z0;
+                    l += z1;
+                }
                 p[e / 2] = pinned(__builtin_bit_cast(unsigned, typename T::v2{(typename T::el)z0, (typename T::el)z1}));
             }
-            l = pinned(l);
+            if (!ONES) l = pinned(l);
             if (j < 2 * DT) o[j % DT] = mfma_32x32x16(vf[j % 3].v, weights(pl, j / DT), o[j % DT]);
+            if (ONES && HD > 16 && j < 2) lsum = mfma_32x32x16(ones, weights(pl, j), lsum);
             sched_fence();
         }
         if (scale) {
@@ -301,6 +324,7 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
             for (int d = 0; d < DT; ++d)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) o[d][e] *= f;
+            if (ONES && HD > 16) lsum[0] *= f; /* every row holds the sum: one is kept up */
         }
     };
 
@@ -308,56 +332,69 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
     int k0 = sink_tiles > 0 ? 0 : win0, k1 = step(0, k0), k2 = step(1, k1); /* of tiles t, t + 1, t + 2 */
     fetch(0, kb, ks_, koff, 0, k0);
     /* there is no part before the first: its weights are zero, and so is its V */
-    for (int i = threadIdx.x; i < TILE / 16; i += NTHR) *reinterpret_cast<v8*>(lds + 3 * TILE + 16 * i) = v8{};
+    for (int i = threadIdx.x; i < TILE / 16; i += NTHR) *reinterpret_cast<v8*>(lds + KRING + TILE + 16 * i) = v8{};
     vm_wait();
     /* the queries are in from here on: the compiler would wait for them, and the tiles on the way, in the loop */
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) qf[ks] = opaque(qf[ks]);
     __syncthreads();
     fetch(TILE, kb, ks_, koff, 1, k1);
-    fetch(2 * TILE, vb, vs_, voff, 0, k0);
+    fetch(KRING, vb, vs_, voff, 0, k0);
     f16v s0 = {}, s1 = {};
     unsigned p0[8] = {}, p1[8] = {};
-    bool last = false, now0 = active(0, k0 + 64 * half);
+    bool last = false, now0 = active(0, k0 + 32 * NP * half);
     if (now0) {
 #pragma unroll
         for (int j = 0; j < KS; ++j) s0 = mfma_32x32x16(read_k(krow, j), qf[j], s0);
     }
-    /* Tile t's V and tile t + 1's K come to LDS between the bodies that last read the tiles before them (before
-       the last barrier) and those that read them (behind the next one). */
-    int buf = 0; /* LDS buffers of tile t: buf, of the tiles next to it: other */
+    /* Tile t's V and tile t + 1's K have come to LDS at the barrier behind the tile's first body; the next V and
+       the K after that go where the body before the barrier read last, or nobody for a tile. */
+    auto ring = [](int at) { return at + TILE < KRING ? at + TILE : 0; };
+    int kbuf = 0, vbuf = 0; /* places of tile t */
     for (int t = 0; t < n_tiles; ++t) {
-        const int other = TILE - buf, at = k0 + 64 * half;
-        const bool now1 = active(t, at + 32), next0 = active(t + 1, k1 + 64 * half);
+        const int knext = ring(kbuf), vother = TILE - vbuf, at = k0 + 32 * NP * half;
+        bool now1 = active(t, at + 32);
+        const bool next0 = active(t + 1, k1 + 32 * NP * half);
         if (last || now0 || now1) {
-            body(t, at, krow + buf + 64 * HD, vrow + other + 64 * HD, s0, s1, p0, p1);
+            body(t, at, krow + kbuf + 64 * HD, vrow + vother + (NP - 1) * 64 * HD, s0, s1, p0, p1);
         } else {
             none(p0);
         }
         vm_wait();
         __syncthreads();
-        fetch(buf, kb, ks_, koff, t + 2, k2);
-        fetch(2 * TILE + other, vb, vs_, voff, t + 1, k1);
-        check_v(buf, t, k0);
-        if (now0 || now1 || next0) {
-            body(t, at + 32, krow + other, vrow + buf, s1, s0, p1, p0);
-        } else {
-            none(p1);
+        fetch(ring(knext), kb, ks_, koff, t + 2, k2);
+        fetch(KRING + vother, vb, vs_, voff, t + 1, k1);
+        check_v(vbuf, t, k0);
+#pragma unroll
+        for (int i = 1; i < NP; ++i) {
+            const bool now2 = i + 1 < NP ? active(t, at + 32 * (i + 1)) : next0;
+            f16v &sc = i & 1 ? s1 : s0, &sn = i & 1 ? s0 : s1;
+            unsigned(&p)[8] = i & 1 ? p1 : p0;
+            if (now0 || now1 || now2) {
+                body(t, at + 32 * i, krow + (i + 1 < NP ? kbuf + 64 * HD * (i + 1) : knext), vrow + vbuf + 64 * HD * (i - 1), sc, sn,
+                     p, i & 1 ? p0 : p1);
+            } else {
+                none(p);
+            }
+            now0 = now1;
+            now1 = now2;
         }
-        last = now1;
-        now0 = next0;
+        last = now0;
+        now0 = now1;
         k0 = k1;
         k1 = k2;
         k2 = step(t + 2, k2);
-        buf = other;
+        kbuf = knext;
+        vbuf = vother;
     }
     if (last) { /* the last part's products */
-        const int va = vrow + (TILE - buf) + 64 * HD;
+        const int va = vrow + (TILE - vbuf) + (NP - 1) * 64 * HD;
 #pragma unroll
         for (int j = 0; j < 2 * DT; ++j) {
             VFrag vf;
             read_v(vf, va, j);
             o[j % DT] = mfma_32x32x16(vf.v, weights(p1, j / DT), o[j % DT]);
+            if (ONES && HD > 16 && j % DT == 0) lsum = mfma_32x32x16(ones, weights(p1, j / DT), lsum);
         }
     }
 
@@ -368,9 +405,13 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
                                 key_range(shift + i, nk, a.left, a.right, a.sinks));
         return;
     }
-    float x, y;
-    lanes_x32(l, x, y);
-    l = x + y;
+    if constexpr (ONES) {
+        l = HD == 16 ? o[0][8] : lsum[0];
+    } else {
+        float x, y;
+        lanes_x32(l, x, y);
+        l = x + y;
+    }
     if constexpr (KW > 1) { /* the other group's result through LDS (everyone is done with the tiles) */
         float* red = reinterpret_cast<float*>(lds) + (wave * 64 + lane);
         if (half == 1) {
