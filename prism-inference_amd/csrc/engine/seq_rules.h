@@ -127,18 +127,10 @@ inline int check_seq(const prism_seq_attn_push& p, const char** why) {
     return check_out(p.n_q, p.n_heads, p.head_dim, p.out_token_stride, p.out_head_stride, why);
 }
 
-/* The frequency of every turned pair in turns per unit of position, and where
- * each axis' pairs end; returns the number of pairs. */
-inline int rope_turns(const prism_rope_push& p, int32_t axis_end[4], double* turns) {
-    int n = 0, i = 0;
-    for (int a = 0; a < p.n_axes; ++a) n += p.pairs[a];
-    const double turn = (p.inverse ? -1.0 : 1.0) / 6.283185307179586476925286766559;
-    for (int a = 0; a < 4; ++a) {
-        const int pairs = a < p.n_axes ? p.pairs[a] : 0;
-        for (int j = 0; j < pairs; ++j, ++i)
-            turns[i] = turn * std::pow(p.base, p.ladder == PRISM_ROPE_ONE_LADDER ? -(double)i / n : -(double)j / pairs);
-        axis_end[a] = i;
-    }
+/* Where each axis' pairs end; returns the number of pairs. */
+inline int rope_axes(const prism_rope_push& p, int32_t axis_end[4]) {
+    int n = 0;
+    for (int a = 0; a < 4; ++a) axis_end[a] = n += a < p.n_axes ? p.pairs[a] : 0;
     return n;
 }
 

@@ -89,7 +89,10 @@ extern "C" int prism_rope(prism_ctx* c, const prism_rope_push* p, const void* in
     a.n_heads = p->n_heads;
     a.head_dim = p->head_dim;
     a.adjacent = p->layout == PRISM_ROPE_ADJACENT;
-    a.n_pairs = rope_turns(*p, a.axis_end, a.turns);
+    a.n_pairs = rope_axes(*p, a.axis_end);
+    a.one_ladder = p->ladder == PRISM_ROPE_ONE_LADDER;
+    a.turn = (p->inverse ? -1.0 : 1.0) / 6.283185307179586476925286766559;
+    a.log2_base = std::log2(p->base);
     a.copy = in != out;
     a.tile = rope_tile(p->n_tokens, a.n_pairs);
     return launch(c, c->f_rope[p->dtype], "rope", ((int64_t)p->n_tokens + a.tile - 1) / a.tile, 256, &a, stream);

@@ -175,7 +175,9 @@ typedef struct RopeArgs {
     int32_t copy;           /* write the channels that do not turn (not in place) */
     int32_t adjacent;       /* pair i = channels 2i, 2i + 1; else i, i + n_pairs */
     int32_t axis_end[4];    /* pairs [axis_end[a-1], axis_end[a]) belong to axis a */
-    double turns[ROPE_MAX_PAIRS]; /* turns per unit of position, negative for the inverse */
+    int32_t one_ladder;     /* frequencies over all pairs together, else per axis */
+    double turn;            /* 1 / (2 pi), negative for the inverse           */
+    double log2_base;
 } RopeArgs;
 
 typedef struct AppendArgs {

@@ -3,18 +3,19 @@
  *
  * Pair i of a head's channels (a, b) turns by phi = pos[axis(i)] * f_i:
  *   a' = a cos phi - b sin phi,  b' = b cos phi + a sin phi
- * The frequencies come from the host in turns (f_i / 2 pi, 64 bits; negated for
- * the inverse). phi is reduced to [-1/2, 1/2] turns in 64 bits, so a position
- * of millions keeps its angle, and sin / cos are taken in fp32.
+ * with f_i = base^-e_i in turns (64 bits, negated for the inverse). phi is
+ * reduced to [-1/2, 1/2] turns in 64 bits, so a position of millions keeps its
+ * angle, and sin / cos are taken in fp32.
  *
  * All heads of a token turn by the same angles, and an angle (64-bit product,
  * reduction, sincos: ~80 instructions) costs far more than a turn, so a
  * workgroup takes a few tokens, puts their angles' cos and sin into LDS, and
- * then streams the tokens' rows: a unit is 8 pairs of one head, 16 bytes per
- * operand. Where n is not a multiple of 8 the second operand of a HALVES unit
- * is a 16-byte access on a 2-byte boundary (global memory takes any), and
- * the last unit goes element by element. Bound by HBM traffic: x read and
- * written once.
+ * then streams the tokens' rows. A unit is 8 pairs of one head: two chunks of 16
+ * bytes (HALVES: channels i.. and i + n.., ADJACENT: 16 channels in a row; two
+ * chunks of channels that do not turn), two units a thread in flight. HALVES
+ * with n not a multiple of 8 has second chunks on 2-byte boundaries (global
+ * memory takes any) and goes the other way, one unit a time, the last pairs
+ * element by element. Bound by HBM traffic: x read and written once.
  */
 #pragma once
 #include "seq_types.hpp"
@@ -33,28 +34,70 @@ __device__ __forceinline__ void rope_turn(typename T::el& u, typename T::el& w, 
     w = (typename T::el)opaque(__builtin_fmaf(b, cs.x, a * cs.y));
 }
 
-template <class T>
-__device__ __forceinline__ void rope_body(const RopeArgs& a) {
+/* Units of two aligned chunks: HALVES with n % 8 == 0, ADJACENT. */
+template <class T, bool ADJACENT>
+__device__ __forceinline__ void rope_units(const RopeArgs& a, const float2* cs, int np, int t0, int tokens) {
     typedef typename T::v8 v8;
     typedef typename T::el el;
-    __shared__ __attribute__((aligned(16))) float2 cs[ROPE_TILE_PAIRS]; /* [token][np] cos, sin */
-    const int n = a.n_pairs, np = (n + 7) & ~7;
-    const int t0 = blockIdx.x * a.tile, tokens = min(a.tile, a.n_tokens - t0);
-    for (int i = threadIdx.x; i < tokens * np; i += 256) {
-        const int t = i / np, j = i - t * np;
-        if (j < n) {
-            const int axis = (j >= a.axis_end[0]) + (j >= a.axis_end[1]) + (j >= a.axis_end[2]);
-            const double rev = (double)a.pos[axis * a.pos_stride + t0 + t] * a.turns[j];
-            float s, c;
-            sincospif(2.0f * (float)(rev - rint(rev)), &s, &c);
-            cs[i] = float2{c, s};
+    constexpr int U = 2;
+    const int n = a.n_pairs, chunks = a.head_dim / 8;
+    const int turned = ADJACENT ? (2 * n + 15) / 16 : n / 8;
+    const int rest = chunks - 2 * turned; /* chunks behind them, of an odd number the last alone; -1: the last unit's own */
+    const int per_head = turned + (a.copy && rest > 0 ? (rest + 1) / 2 : 0);
+    const int per_token = per_head * a.n_heads, units = tokens * per_token;
+    for (int u0 = threadIdx.x; u0 < units; u0 += 256 * U) {
+        v8 p[U], q[U];
+        uint16_t* y[U];
+        int c1[U], c2[U], pair[U];
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            const int u = min(u0 + 256 * i, units - 1); /* past the end: the last one, read and not written */
+            const int t = u / per_token, r = u - t * per_token, h = r / per_head, k = r - h * per_head;
+            const bool turn = k < turned;
+            c1[i] = ADJACENT || !turn ? 2 * k : k;
+            if (!ADJACENT && !turn) c1[i] = 2 * turned + 2 * (k - turned);
+            c2[i] = min(ADJACENT || !turn ? c1[i] + 1 : k + turned, chunks - 1);
+            pair[i] = turn ? t * np + 8 * k : -1;
+            const uint16_t* x = a.in + (t0 + t) * a.in_token_stride + h * a.in_head_stride;
+            y[i] = a.out + (t0 + t) * a.out_token_stride + h * a.out_head_stride;
+            p[i] = ld8<T>(x + 8 * c1[i]);
+            q[i] = ld8<T>(x + 8 * c2[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            if (u0 + 256 * i >= units) break;
+            if (pair[i] >= 0) {
+                const int left = n - 8 * (ADJACENT ? c1[i] / 2 : c1[i]); /* pairs that turn: 8, or ADJACENT's last ones */
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    if (ADJACENT && e >= left) break;
+                    v8& vb = ADJACENT && e < 4 ? p[i] : q[i];
+                    v8& va = ADJACENT ? vb : p[i];
+                    const int ia = ADJACENT ? 2 * e % 8 : e, ib = ADJACENT ? ia + 1 : e;
+                    el b = va[ia], d = vb[ib];
+                    rope_turn<T>(b, d, cs[pair[i] + e]);
+                    va[ia] = b;
+                    vb[ib] = d;
+                }
+            }
+            if (ADJACENT && !a.copy && 16 * (c1[i] / 2) + 16 > 2 * n) { /* in place: what does not turn is not written */
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    if (8 * c1[i] + e < 2 * n) reinterpret_cast<el*>(y[i])[8 * c1[i] + e] = e < 8 ? p[i][e] : q[i][e - 8];
+            } else {
+                st8<T>(y[i] + 8 * c1[i], p[i]);
+                if (c2[i] != c1[i]) st8<T>(y[i] + 8 * c2[i], q[i]);
+            }
         }
     }
-    __syncthreads();
+}
 
-    /* a head's units: turned pairs, then chunks of channels to copy */
-    const int turned = a.adjacent ? (2 * n + 7) / 8 : np / 8;
-    const int copy0 = a.adjacent ? turned : 2 * n / 8;
+/* HALVES with n % 8 != 0 */
+template <class T>
+__device__ __forceinline__ void rope_loose_units(const RopeArgs& a, const float2* cs, int np, int t0, int tokens) {
+    typedef typename T::v8 v8;
+    typedef typename T::el el;
+    const int n = a.n_pairs, turned = np / 8, copy0 = 2 * n / 8;
     const int per_head = turned + (a.copy ? a.head_dim / 8 - copy0 : 0);
     const int per_token = per_head * a.n_heads;
     for (int u = threadIdx.x; u < tokens * per_token; u += 256) {
@@ -68,24 +111,6 @@ __device__ __forceinline__ void rope_body(const RopeArgs& a) {
                 st8<T>(y + c, ld8<T>(x + c));
             } else {
                 for (int e = 2 * n; e < c + 8; ++e) y[e] = x[e];
-            }
-        } else if (a.adjacent) {
-            v8 v = ld8<T>(x + 8 * k);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                if (4 * k + e < n) {
-                    el p = v[2 * e], q = v[2 * e + 1];
-                    rope_turn<T>(p, q, row[4 * k + e]);
-                    v[2 * e] = p;
-                    v[2 * e + 1] = q;
-                }
-            }
-            if (8 * k + 8 <= 2 * n || a.copy) { /* in place, the unturned end of a mixed chunk is not written */
-                st8<T>(y + 8 * k, v);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (8 * k + e < 2 * n) reinterpret_cast<el*>(y)[8 * k + e] = v[e];
             }
         } else if (8 * k + 8 <= n) {
             v8 p = ld8<T>(x + 8 * k), q = reinterpret_cast<const Loose8<T>*>(x + 8 * k + n)->v;
@@ -107,6 +132,34 @@ __device__ __forceinline__ void rope_body(const RopeArgs& a) {
             }
         }
     }
+}
+
+template <class T>
+__device__ __forceinline__ void rope_body(const RopeArgs& a) {
+    __shared__ __attribute__((aligned(16))) float2 cs[ROPE_TILE_PAIRS]; /* [token][np] cos, sin */
+    __shared__ double turns[ROPE_MAX_PAIRS];
+    const int n = a.n_pairs, np = (n + 7) & ~7;
+    const int t0 = blockIdx.x * a.tile, tokens = min(a.tile, a.n_tokens - t0);
+    const auto axis_of = [&](int j) { return (j >= a.axis_end[0]) + (j >= a.axis_end[1]) + (j >= a.axis_end[2]); };
+    if (threadIdx.x < n) {
+        const int j = threadIdx.x, axis = axis_of(j), first = axis ? a.axis_end[axis - 1] : 0;
+        const double e = a.one_ladder ? (double)j / n : (double)(j - first) / (a.axis_end[axis] - first);
+        turns[j] = a.turn * exp2(-e * a.log2_base);
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < tokens * np; i += 256) {
+        const int t = i / np, j = i - t * np;
+        if (j < n) {
+            const double rev = (double)a.pos[axis_of(j) * a.pos_stride + t0 + t] * turns[j];
+            float s, c;
+            sincospif(2.0f * (float)(rev - rint(rev)), &s, &c);
+            cs[i] = float2{c, s};
+        }
+    }
+    __syncthreads();
+    if (a.adjacent) rope_units<T, true>(a, cs, np, t0, tokens);
+    else if (n == np) rope_units<T, false>(a, cs, np, t0, tokens);
+    else rope_loose_units<T>(a, cs, np, t0, tokens);
 }
 
 extern "C" __global__ void __launch_bounds__(256) prism_rope_f16(RopeArgs a) { rope_body<F16>(a); }

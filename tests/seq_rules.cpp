@@ -10,7 +10,8 @@ int rope_check(const prism_rope_push* p) { const char* w; return check_rope(*p, 
 int append_check(const prism_append_push* p) { const char* w; return check_append(*p, &w); }
 int paged_check(const prism_paged_attn_push* p) { const char* w; return check_paged(*p, &w); }
 int seq_check(const prism_seq_attn_push* p) { const char* w; return check_seq(*p, &w); }
-int turns(const prism_rope_push* p, int32_t* axis_end, double* t) { return rope_turns(*p, axis_end, t); }
+int axes(const prism_rope_push* p, int32_t* axis_end) { return rope_axes(*p, axis_end); }
+int tile(long long n_tokens, int n_pairs) { return rope_tile(n_tokens, n_pairs); }
 void keys(int32_t p, int32_t n, int32_t left, int32_t right, int32_t sinks, int32_t* out) {
     const KeyRange r = key_range(p, n, left, right, sinks);
     out[0] = r.sink;

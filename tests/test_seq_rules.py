@@ -22,7 +22,7 @@ def rules(tmp_path_factory):
                     os.path.join(ROOT, "tests", "seq_rules.cpp"), "-o", so], check=True, timeout=120)
     lib = C.CDLL(so)
     lib.rows.argtypes = [C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p]
-    lib.turns.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p]
+    lib.tile.argtypes = [C.c_longlong, C.c_int]
     return lib
 
 
@@ -167,18 +167,17 @@ def test_pages_out_of_the_pool(rules):
     assert rules.page(0, 0) == 0
 
 
-@pytest.mark.parametrize("kw", [{}, dict(ladder=1), dict(inverse=1), dict(n_axes=1, pairs=(16, 3, 3, 3)),
-                                dict(pairs=(0, 5, 0, 0)), dict(n_axes=4, pairs=(1, 2, 3, 4), ladder=1)])
-def test_frequencies(rules, kw):
+@pytest.mark.parametrize("kw", [{}, dict(n_axes=1, pairs=(16, 3, 3, 3)), dict(pairs=(0, 5, 0, 0)),
+                                dict(n_axes=4, pairs=(1, 2, 3, 4))])
+def test_pairs_of_an_axis(rules, kw):
     p = rope(**kw)
-    end, t = (C.c_int32 * 4)(), (C.c_double * 128)()
-    n = rules.turns(C.byref(p), end, t)
+    end = (C.c_int32 * 4)()
     pairs = list(p.pairs)[:p.n_axes] + [0] * (4 - p.n_axes)
-    assert n == sum(pairs) and list(end) == list(np.cumsum(pairs))
-    i = 0
-    for a in range(4):
-        for j in range(pairs[a]):
-            e = i / n if p.ladder else j / pairs[a]
-            want = (-1 if p.inverse else 1) * 10000.0 ** -e / (2 * np.pi)
-            assert abs(t[i] - want) <= 4e-16 * abs(want)
-            i += 1
+    assert rules.axes(C.byref(p), end) == sum(pairs) and list(end) == list(np.cumsum(pairs))
+
+
+@pytest.mark.parametrize("tokens,pairs,tile", [(1, 1, 1), (2047, 8, 1), (2048, 8, 2), (10 ** 9, 8, 128), (10 ** 9, 128, 8),
+                                               (10 ** 9, 48, 16), (10 ** 9, 9, 64), (130560, 16, 64)])
+def test_tokens_of_a_workgroup(rules, tokens, pairs, tile):
+    """The table of angles holds them, and the GPU is filled first."""
+    assert rules.tile(tokens, pairs) == tile and tile * -(-pairs // 8) * 8 <= 1024
