@@ -172,6 +172,7 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
     const KeyRange rb = key_range(shift + qb - 1, nk, a.left, a.right, a.sinks);
     const int a_lo = uni(ra.lo), a_hi = uni(ra.hi), b_lo = uni(rb.lo), b_hi = uni(rb.hi);
 
+    const int see_hi = on ? b_hi : INT32_MIN, see_sink = seq_min(see_hi, sink_end);
     unsigned bad = 0; /* infinite or NaN V where only some of the queries look */
     v8 qf[KS];
 #pragma unroll
@@ -240,9 +241,11 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
     const int vrow = 2 * (32 * NP * half + 4 * g + (lane & 15) / 4) * HD +
                      ((HD >= 32 ? 2 * (lane & 16) : 0) ^ 16 * swizzle_v((lane & 15) / 4)) + 8 * (lane & 3);
     auto read_k = [&](int at, int ks) { return *reinterpret_cast<const v8*>(lds + (at ^ 32 * ks)); };
-    auto active = [&](int t, int k0) { /* does the wave see any of the part that starts at k0? */
-        return on && t < n_tiles && k0 < (t < sink_tiles ? seq_min(b_hi, sink_end) : b_hi) &&
-               (t < sink_tiles || k0 + 32 > a_lo);
+    /* does the wave see any of the part of tile t that starts at k0? (whole numbers: scalar code) */
+    auto active = [&](int t, int k0) -> int {
+        const int hi = t < n_tiles ? (t < sink_tiles ? see_sink : see_hi) : INT32_MIN;
+        const int lo = t < sink_tiles ? INT32_MIN : a_lo - 32;
+        return (int)(k0 < hi) & (int)(k0 > lo);
     };
     auto read_v = [&](VFrag& f, int at, int j) { /* 16 keys j / DT, channels 32 (j % DT) ..: V^T as
                                                     lane's rows keys 4 g ..+3 and 8 more on */
@@ -342,7 +345,7 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
     fetch(KRING, vb, vs_, voff, 0, k0);
     f16v s0 = {}, s1 = {};
     unsigned p0[8] = {}, p1[8] = {};
-    bool last = false, now0 = active(0, k0 + 32 * NP * half);
+    int last = 0, now0 = active(0, k0 + 32 * NP * half);
     if (now0) {
 #pragma unroll
         for (int j = 0; j < KS; ++j) s0 = mfma_32x32x16(read_k(krow, j), qf[j], s0);
@@ -353,9 +356,9 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
     int kbuf = 0, vbuf = 0; /* places of tile t */
     for (int t = 0; t < n_tiles; ++t) {
         const int knext = ring(kbuf), vother = TILE - vbuf, at = k0 + 32 * NP * half;
-        bool now1 = active(t, at + 32);
-        const bool next0 = active(t + 1, k1 + 32 * NP * half);
-        if (last || now0 || now1) {
+        int now1 = active(t, at + 32);
+        const int next0 = active(t + 1, k1 + 32 * NP * half);
+        if (last | now0 | now1) {
             body(t, at, krow + kbuf + 64 * HD, vrow + vother + (NP - 1) * 64 * HD, s0, s1, p0, p1);
         } else {
             none(p0);
@@ -367,10 +370,10 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
         check_v(vbuf, t, k0);
 #pragma unroll
         for (int i = 1; i < NP; ++i) {
-            const bool now2 = i + 1 < NP ? active(t, at + 32 * (i + 1)) : next0;
+            const int now2 = i + 1 < NP ? active(t, at + 32 * (i + 1)) : next0;
             f16v &sc = i & 1 ? s1 : s0, &sn = i & 1 ? s0 : s1;
             unsigned(&p)[8] = i & 1 ? p1 : p0;
-            if (now0 || now1 || now2) {
+            if (now0 | now1 | now2) {
                 body(t, at + 32 * i, krow + (i + 1 < NP ? kbuf + 64 * HD * (i + 1) : knext), vrow + vbuf + 64 * HD * (i - 1), sc, sn,
                      p, i & 1 ? p0 : p1);
             } else {
