@@ -178,7 +178,15 @@ inline int64_t paged_workspace(const prism_paged_attn_push& p, const PagedPlan& 
  * seq_of_tile). */
 inline int64_t seq_tiles(int64_t n_q, int64_t n_seqs) { return n_q / SEQ_BM + n_seqs; }
 
-inline bool seq_w8(int64_t grid) { return grid <= 1024; }
+/* 8 waves, of which two share each 32 queries' keys, while the workgroups are no
+ * more than four per CU: then waves are what a SIMD lacks to hide the latency of
+ * scores, maximum and weights, which follow each other. 4 and 8 waves, sequences that see
+ * all keys, 8 heads unless said: 500 queries x 64 channels (32 workgroups) 13.4 and 11.9 us,
+ * 2,000 x 32 (128) 27.5 and 24.2, 8,160 x 32, 4 heads (256) 100 and 80, 4,000 x
+ * 64, 16 heads (512) 85 and 57, 4,000 x 128, 32 heads (1,024) 169 and 164; 60 of 100 to
+ * 600 queries x 32 (1,792) 28 and 36; 2 of 5,000 x 128, 32 heads, window 2,047 (2,624) 409
+ * and 455. */
+inline bool seq_w8(int64_t grid) { return grid <= 4 * 256; }
 
 }  // namespace prism
 

@@ -5,7 +5,6 @@
  */
 #include <hip/hip_runtime.h>
 
-#include <cstdlib>
 #include <cstring>
 
 #include "ctx.h"
@@ -43,15 +42,14 @@ class OnDevice {
 };
 
 /* grid workgroups of `threads` on the context's device */
-int launch(prism_ctx* c, hipFunction_t f, const char* what, int64_t grid, unsigned threads, void* args, void* stream,
-           unsigned more_lds = 0) {
+int launch(prism_ctx* c, hipFunction_t f, const char* what, int64_t grid, unsigned threads, void* args, void* stream) {
     if (grid > INT32_MAX) return fail(c, PRISM_ERR_INVALID, "%s: %lld workgroups", what, (long long)grid);
     OnDevice on(c->device);
     if (on.error() != hipSuccess)
         return fail(c, PRISM_ERR_HIP, "hipSetDevice(%d): %s", c->device, hipGetErrorString(on.error()));
     void* params[] = {args};
     const hipError_t e =
-        hipModuleLaunchKernel(f, (unsigned)grid, 1, 1, threads, 1, 1, more_lds, (hipStream_t)stream, params, nullptr);
+        hipModuleLaunchKernel(f, (unsigned)grid, 1, 1, threads, 1, 1, 0, (hipStream_t)stream, params, nullptr);
     if (e != hipSuccess) return fail(c, PRISM_ERR_HIP, "hipModuleLaunchKernel(%s): %s", what, hipGetErrorString(e));
     return PRISM_OK;
 }
@@ -222,6 +220,6 @@ extern "C" int prism_seq_attn(prism_ctx* c, const prism_seq_attn_push* p, const 
     a.sinks = p->sinks;
     a.scale_log2 = p->scale * 1.4426950408889634f;
     const int64_t grid = seq_tiles(p->n_q, p->n_seqs) * p->n_heads;
-    const bool w8 = getenv("W8") ? atoi(getenv("W8")) : seq_w8(grid);
-    return launch(c, c->f_seq[p->dtype][hd_index(p->head_dim)][w8], "sequence attention", grid, w8 ? 512 : 256, &a, stream, getenv("ML") ? atoi(getenv("ML")) : 0);
+    const bool w8 = seq_w8(grid);
+    return launch(c, c->f_seq[p->dtype][hd_index(p->head_dim)][w8], "sequence attention", grid, w8 ? 512 : 256, &a, stream);
 }
