@@ -133,13 +133,22 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
     const auto uni = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
 
     /* workgroup -> (query tile, head): an XCD (workgroups b, b + 8, ...) takes a
-     * run of neighbouring heads, whose keys its L2 then holds */
-    const int tiles = a.n_q / SEQ_BM + a.n_seqs;
-    const int total = tiles * a.n_heads, b = blockIdx.x;
-    const int big = total & 7, per = total >> 3, xcd = b & 7;
-    const int w = xcd * per + min(xcd, big) + (b >> 3);
-    const int h = w / tiles, hk = h / (a.n_heads / a.n_kv_heads);
-    const int tile = tiles - 1 - (w - h * tiles); /* the last, longest rows first */
+     * run of neighbouring heads, whose keys its L2 then holds; the last tiles, whose
+     * queries may see the most keys, come first, so the launch ends with short ones
+     * (with whole heads per XCD, over all of them: 2 of 5,000 queries, 32 heads x
+     * 128, 409 -> 374 us) */
+    const int tiles = a.n_q / SEQ_BM + a.n_seqs, b = blockIdx.x, xcd = b & 7;
+    int h, tile;
+    if (a.n_heads % 8 == 0) {
+        const int heads = a.n_heads / 8, i = b >> 3;
+        tile = tiles - 1 - i / heads;
+        h = xcd * heads + i % heads;
+    } else {
+        const int total = tiles * a.n_heads, w = xcd * (total >> 3) + min(xcd, total & 7) + (b >> 3);
+        h = w / tiles;
+        tile = tiles - 1 - (w - h * tiles);
+    }
+    const int hk = h / (a.n_heads / a.n_kv_heads);
     const SeqTile st = seq_of_tile(a, tile);
     const RowRange rq = st.q, rk = st.k;
     const int first = st.first;
@@ -236,20 +245,25 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
         s4 h[2];
         v8 v;
     };
-    /* this lane's places (bytes from lk, lv on), to be xored with 32 per k-step and 64 per 32 channels */
+    /* this lane's places (bytes from the rings on), to be xored with 32 per k-step and 64 per 32 channels */
     const int krow = 2 * (32 * NP * half + c32) * HD + 16 * (g ^ swizzle_k(c32));
     const int vrow = 2 * (32 * NP * half + 4 * g + (lane & 15) / 4) * HD +
                      ((HD >= 32 ? 2 * (lane & 16) : 0) ^ 16 * swizzle_v((lane & 15) / 4)) + 8 * (lane & 3);
-    auto read_k = [&](int at, int ks) { return *reinterpret_cast<const v8*>(lds + (at ^ 32 * ks)); };
+    int kat[KS], vat[DT];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) kat[ks] = opaque(krow ^ 32 * ks);
+#pragma unroll
+    for (int d = 0; d < DT; ++d) vat[d] = opaque(KRING + (vrow ^ 64 * d));
+    auto read_k = [&](int off, int ks) { return *reinterpret_cast<const v8*>(lds + kat[ks] + off); };
     /* does the wave see any of the part of tile t that starts at k0? (whole numbers: scalar code) */
     auto active = [&](int t, int k0) -> int {
         const int hi = t < n_tiles ? (t < sink_tiles ? see_sink : see_hi) : INT32_MIN;
         const int lo = t < sink_tiles ? INT32_MIN : a_lo - 32;
         return (int)(k0 < hi) & (int)(k0 > lo);
     };
-    auto read_v = [&](VFrag& f, int at, int j) { /* 16 keys j / DT, channels 32 (j % DT) ..: V^T as
+    auto read_v = [&](VFrag& f, int off, int j) { /* 16 keys j / DT, channels 32 (j % DT) ..: V^T as
                                                     lane's rows keys 4 g ..+3 and 8 more on */
-        const uint8_t* v = lds + KRING + (at ^ 64 * (j % DT)) + 32 * (j / DT) * HD;
+        const uint8_t* v = lds + vat[j % DT] + (off + 32 * (j / DT) * HD);
         f.h[0] = lds_tr4(v);
         f.h[1] = lds_tr4(v + 16 * HD);
         if constexpr (HD == 16) { /* every lane takes part in the transposing read */
@@ -348,24 +362,22 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
     int last = 0, now0 = active(0, k0 + 32 * NP * half);
     if (now0) {
 #pragma unroll
-        for (int j = 0; j < KS; ++j) s0 = mfma_32x32x16(read_k(krow, j), qf[j], s0);
+        for (int j = 0; j < KS; ++j) s0 = mfma_32x32x16(read_k(0, j), qf[j], s0);
     }
     /* Tile t's V and tile t + 1's K have come to LDS at the barrier behind the tile's first body; the next V and
        the K after that go where the body before the barrier read last, or nobody for a tile. */
-    auto ring = [](int at) { return at + TILE < KRING ? at + TILE : 0; };
-    int kbuf = 0, vbuf = 0; /* places of tile t */
-    for (int t = 0; t < n_tiles; ++t) {
-        const int knext = ring(kbuf), vother = TILE - vbuf, at = k0 + 32 * NP * half;
+    auto pass = [&](int t, auto kbuf, auto knext, auto kfree, auto vbuf, auto vother) { /* places in the rings */
+        const int at = k0 + 32 * NP * half;
         int now1 = active(t, at + 32);
         const int next0 = active(t + 1, k1 + 32 * NP * half);
         if (last | now0 | now1) {
-            body(t, at, krow + kbuf + 64 * HD, vrow + vother + (NP - 1) * 64 * HD, s0, s1, p0, p1);
+            body(t, at, kbuf + 64 * HD, vother + (NP - 1) * 64 * HD, s0, s1, p0, p1);
         } else {
             none(p0);
         }
         vm_wait();
         __syncthreads();
-        fetch(ring(knext), kb, ks_, koff, t + 2, k2);
+        fetch(kfree, kb, ks_, koff, t + 2, k2);
         fetch(KRING + vother, vb, vs_, voff, t + 1, k1);
         check_v(vbuf, t, k0);
 #pragma unroll
@@ -374,8 +386,8 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
             f16v &sc = i & 1 ? s1 : s0, &sn = i & 1 ? s0 : s1;
             unsigned(&p)[8] = i & 1 ? p1 : p0;
             if (now0 | now1 | now2) {
-                body(t, at + 32 * i, krow + (i + 1 < NP ? kbuf + 64 * HD * (i + 1) : knext), vrow + vbuf + 64 * HD * (i - 1), sc, sn,
-                     p, i & 1 ? p0 : p1);
+                body(t, at + 32 * i, i + 1 < NP ? kbuf + 64 * HD * (i + 1) : knext, vbuf + 64 * HD * (i - 1), sc, sn, p,
+                     i & 1 ? p0 : p1);
             } else {
                 none(p);
             }
@@ -387,11 +399,26 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
         k0 = k1;
         k1 = k2;
         k2 = step(t + 2, k2);
-        kbuf = knext;
-        vbuf = vother;
+    };
+    int vlast = 0; /* place of the last tile's V */
+    if constexpr (KRING == 2 * TILE) { /* two tiles a turn: every LDS address a register of its own plus a constant */
+        for (int t = 0; t < n_tiles; t += 2) {
+            pass(t, 0, TILE, 0, 0, TILE);
+            vlast = 0;
+            if (t + 1 == n_tiles) break;
+            pass(t + 1, TILE, 0, TILE, TILE, 0);
+            vlast = TILE;
+        }
+    } else {
+        for (int t = 0, k = 0; t < n_tiles; ++t) {
+            const int knext = k + TILE < KRING ? k + TILE : 0, kfree = KRING - k - knext;
+            vlast = (t & 1) * TILE;
+            pass(t, k, knext, kfree, vlast, TILE - vlast);
+            k = knext;
+        }
     }
     if (last) { /* the last part's products */
-        const int va = vrow + (TILE - vbuf) + (NP - 1) * 64 * HD;
+        const int va = vlast + (NP - 1) * 64 * HD;
 #pragma unroll
         for (int j = 0; j < 2 * DT; ++j) {
             VFrag vf;
@@ -435,20 +462,29 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) o[d][e] = o[d][e] * f0 + red[(16 * d + e) * 256] * f1;
     }
-    if (!on || qa + c32 >= qb) return;
+    const bool store = on && qa + c32 < qb;
     const float inv = l == 0.f ? 0.f : 1.0f / l;
     uint16_t* out = a.out + (rq.start + qi) * a.out_token_stride + h * a.out_head_stride;
+    /* a lane has 4 channels of every 8; its partner 32 lanes on, the others: 8 and 8 after an exchange */
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-            const int ch = 32 * d + 2 * i + 4 * g;
-            if (HD >= 32 || ch < HD) {
-                typename T::v4 r;
+        for (int i = 0; i < 16; i += 8) {
+            if (32 * d + 2 * i >= HD) break;
+            u4 r;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) r[e] = (typename T::el)opaque(o[d][i + e] * inv);
-                *reinterpret_cast<typename T::v4*>(out + ch) = r;
+            for (int e = 0; e < 2; ++e) {
+                unsigned w[2];
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    const float a0 = o[d][i + 4 * x + 2 * e], a1 = o[d][i + 4 * x + 2 * e + 1];
+                    w[x] = __builtin_bit_cast(unsigned, typename T::v2{(typename T::el)opaque(a0 * inv), (typename T::el)opaque(a1 * inv)});
+                }
+                const auto sw = __builtin_amdgcn_permlane32_swap(w[0], w[1], false, false);
+                r[e] = sw[0];
+                r[2 + e] = sw[1];
             }
+            if (store) *reinterpret_cast<u4*>(out + 32 * d + 2 * i + 8 * g) = r;
         }
 }
 
