@@ -160,12 +160,21 @@ inline PagedPlan paged_plan(const prism_paged_attn_push& p) {
     /* keys of the longest sequence expected */
     int64_t keys = p.max_len > 0 ? p.max_len : (int64_t)p.cache.table_pages * p.cache.page_size;
     if (p.left >= 0 && keys > (int64_t)p.left + 1 + p.sinks) keys = (int64_t)p.left + 1 + p.sinks;
-    r.waves = items >= 4096 || keys <= 32 ? 1 : 4;
+    /* A wave alone where the waves are many and short: 64 keys, 1,600 items of 4 heads x 32 and x 128 5.6 and 12.3 us, four
+     * waves an item 8.1 and 20.1; 512 items x 128 7.2 (1 head) and 7.5 (4), and 5.1 and 8.2; 200 keys, 512 items x 128 23.5 and
+     * 13.2; 4,800 items of 64 to 1,000 keys 8.7 to 115 and 16.2 to 113. */
+    r.waves = keys <= 32 || items >= 4096 || (items >= 1024 && keys <= 128) ? 1 : 4;
+    /* Splits until the launch has about two workgroups per CU, more of them where a sequence is long (which is where
+     * lengths differ); the join costs by the splits, so their number grows with the root of the length; and the
+     * second launch has to pay. 1 head x 128 and 4 x 128, us at 1, 4, 16 and 64 splits: 8 items of 1,000 keys 19.2, 9.9, 6.9
+     * and 20.2, 11.3, 9.0; of 16,000 372, 98, 30, 18 and 271, 76, 26, 19; 128 items of 1,000 keys 29, 17, 17 and 23, 19,
+     * 26; of 16,000 541, 211, 192, 197 and 351, 197, 191, 208; 4 x 32, 8 items of 500 keys 7.4, 7.0. */
     r.splits = 1;
-    if (r.waves == 4) {
-        int64_t want = 2048 / std::max<int64_t>(items, 1);
-        want = std::min<int64_t>(want, keys / 256);
-        r.splits = (int)std::max<int64_t>(1, std::min<int64_t>(want, PAGED_MAX_SPLITS));
+    if (r.waves == 4 && keys >= 384 && keys * p.cache.head_dim >= 32 * 1024) {
+        int64_t most = 512 / std::max<int64_t>(items, 1);
+        most = std::max(most, std::min(2048 / std::max<int64_t>(items, 1), keys / 1024));
+        most = std::min(most, std::min((int64_t)(std::sqrt((double)keys) / 2), keys / 64));
+        r.splits = (int)std::max<int64_t>(1, std::min<int64_t>(most, PAGED_MAX_SPLITS));
     }
     r.grid = r.waves == 1 ? (items + 3) / 4 : items * r.splits;
     return r;
@@ -174,9 +183,15 @@ inline int64_t paged_workspace(const prism_paged_attn_push& p, const PagedPlan& 
     return r.splits == 1 ? 0 : (int64_t)p.cache.n_seqs * p.n_heads * r.splits * (p.cache.head_dim + 2) * 4;
 }
 
-/* Query tiles of a sequence attention: enough for any lengths (seq_attn.hpp's
- * seq_of_tile). */
-inline int64_t seq_tiles(int64_t n_q, int64_t n_seqs) { return n_q / SEQ_BM + n_seqs; }
+/* Heads that a workgroup of a sequence attention takes side by side: those that share
+ * a key head, unless they alone would fill it. */
+inline int seq_tile_heads(int n_heads, int n_kv_heads) {
+    const int group = n_heads / n_kv_heads;
+    return group <= SEQ_ROWS / 4 ? group : 1;
+}
+
+/* Tiles of tile_q queries: enough for any lengths (seq_attn.hpp's seq_of_tile). */
+inline int64_t seq_tiles(int64_t n_q, int64_t n_seqs, int tile_q) { return n_q / tile_q + n_seqs; }
 
 /* 8 waves, of which two share each 32 queries' keys, while the workgroups are no
  * more than four per CU: then waves are what a SIMD lacks to hide the latency of

@@ -3,7 +3,9 @@
  * sinks: query i of a sequence of nq queries and nk keys stands at position
  * p = nk - nq + i and sees keys j <= p + right with j >= p - left or j < sinks.
  *
- * A workgroup takes 128 queries of one head, 32 a wave, and goes once over the
+ * A workgroup takes 128 rows, 32 a wave: a row is a query of one head, the heads
+ * that share a key head side by side (so the workgroup's queries are fewer, and
+ * the keys that they see together too). It goes once over the
  * keys that any of them sees, 64 or 128 at a time, with a running maximum and sum:
  *   S^T = K Q^T           (32x32x16 MFMA: a lane holds one query's scores)
  *   P^T = 2^(c S^T - c m) (registers; c = scale log2 e)
@@ -86,7 +88,7 @@ __device__ __forceinline__ void seq_attn_row(const SeqAttnArgs& a, const uint16_
 }
 
 /* The sequence whose query tiles include tile b, and its rows: sequence s owns the
- * tiles from floor(start / SEQ_BM) + s on, which leaves each enough of them
+ * tiles from floor(start / tile_q) + s on, which leaves each enough of them
  * whatever the lengths. 64 candidates a step; the last step's loads bring the
  * rows along. */
 struct SeqTile {
@@ -102,7 +104,7 @@ __device__ __forceinline__ SeqTile seq_of_tile(const SeqAttnArgs& a, int b) {
         const RowRange q = row_range(a.cu_q, s, a.n_seqs, a.n_q);
         RowRange k{0, 0};
         if (step == 1) k = row_range(a.cu_k, s, a.n_seqs, a.n_k);
-        const int key = q.start / SEQ_BM + s;
+        const int key = q.start / a.tile_q + s;
         const unsigned long long mask = __ballot(key <= b);
         const int at = mask ? min(63 - __builtin_clzll(mask), (n - 1) / step) : 0;
         if (step == 1) {
@@ -122,7 +124,7 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
     constexpr int NTHR = 256 * KW, BN = 32 * NP * KW; /* threads; keys per tile */
     constexpr int KS = HD / 16;              /* k-steps of the scores          */
     constexpr int DT = (HD + 31) / 32;       /* 32-channel tiles of the output */
-    constexpr bool ONES = HD <= 64;          /* sums of weights on the matrix cores, see below */
+    constexpr bool ONES = HD == 16 || (HD <= 64 && KW == 1); /* sums of weights on the matrix cores, see below */
     constexpr int NS = KS > 2 * DT ? KS : 2 * DT; /* steps of a part           */
     constexpr int EL = 16 / NS;              /* scores per lane and step       */
     constexpr int CPR = HD / 8;              /* 16-byte chunks of a row        */
@@ -135,36 +137,38 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
     /* workgroup -> (query tile, head): an XCD (workgroups b, b + 8, ...) takes a
      * run of neighbouring heads, whose keys its L2 then holds; the last tiles, whose
      * queries may see the most keys, come first, so the launch ends with short ones
-     * (with whole heads per XCD, over all of them: 2 of 5,000 queries, 32 heads x
-     * 128, 409 -> 374 us) */
-    const int tiles = a.n_q / SEQ_BM + a.n_seqs, b = blockIdx.x, xcd = b & 7;
-    int h, tile;
-    if (a.n_heads % 8 == 0) {
-        const int heads = a.n_heads / 8, i = b >> 3;
-        tile = tiles - 1 - i / heads;
-        h = xcd * heads + i % heads;
+     * (with whole groups of heads per XCD, over all of them: 2 of 5,000 queries, 32
+     * heads x 128, 409 -> 374 us) */
+    const int tiles = a.n_q / a.tile_q + a.n_seqs, groups = a.n_heads / a.tile_heads, b = blockIdx.x, xcd = b & 7;
+    int hg, tile; /* group of heads, tile of queries */
+    if (groups % 8 == 0) {
+        const int some = groups / 8, i = b >> 3;
+        tile = tiles - 1 - i / some;
+        hg = xcd * some + i % some;
     } else {
-        const int total = tiles * a.n_heads, w = xcd * (total >> 3) + min(xcd, total & 7) + (b >> 3);
-        h = w / tiles;
-        tile = tiles - 1 - (w - h * tiles);
+        const int total = tiles * groups, w = xcd * (total >> 3) + min(xcd, total & 7) + (b >> 3);
+        hg = w / tiles;
+        tile = tiles - 1 - (w - hg * tiles);
     }
-    const int hk = h / (a.n_heads / a.n_kv_heads);
+    const int hk = hg * a.tile_heads / (a.n_heads / a.n_kv_heads);
     const SeqTile st = seq_of_tile(a, tile);
     const RowRange rq = st.q, rk = st.k;
     const int first = st.first;
     const int nq = rq.end - rq.start, nk = rk.end - rk.start;
-    if (tile < first || (int64_t)(tile - first) * SEQ_BM >= nq) return; /* uniform over the workgroup */
-    const int q0 = (tile - first) * SEQ_BM, q1 = min(q0 + SEQ_BM, nq);
+    if (tile < first || (int64_t)(tile - first) * a.tile_q >= nq) return; /* uniform over the workgroup */
+    const int q0 = (tile - first) * a.tile_q, q1 = min(q0 + a.tile_q, nq);
 
     const int lane = lane_id(), c32 = lane & 31, g = lane >> 5;
     const int wave8 = uni(threadIdx.x >> 6), wave = wave8 & 3, half = wave8 >> 2;
-    const int qa = q0 + 32 * wave, qb = min(qa + 32, q1); /* the wave's queries */
+    const int row = 32 * wave + c32; /* this lane's; the wave's queries: qa .. qb - 1 */
+    const int qa = q0 + 32 * wave / a.tile_heads, qb = min(q0 + (32 * wave + 31) / a.tile_heads + 1, q1);
     const int shift = nk - nq;                            /* position - row */
     const bool on = qa < q1;
 
     const uint16_t* kb = a.k + rk.start * a.k_token_stride + hk * a.k_head_stride;
     const uint16_t* vb = a.v + rk.start * a.v_token_stride + hk * a.v_head_stride;
-    const int qi = min(qa + c32, q1 - 1); /* this lane's query; past the end: the last one, never stored */
+    const int qrow = q0 + row / a.tile_heads, h = hg * a.tile_heads + row % a.tile_heads;
+    const int qi = min(qrow, q1 - 1); /* past the end: the last one, never stored */
     const uint16_t* qp = a.q + (rq.start + qi) * a.q_token_stride + h * a.q_head_stride;
 
     /* Keys that the workgroup's, the wave's and the lane's queries see. Tiles go over
@@ -190,8 +194,9 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
     f16v o[DT] = {};
     float m = -INFINITY, mc = 0.f, l = 0.f; /* mc = c m, or 0 while m is -inf */
     /* The sum of a query's weights: as many additions as weights on the vector units, or products with ones on
-       the matrix cores, which wait for the vector units up to 64 channels. (16 channels leave half of the
-       output's rows free: there V's unused rows are the ones.) The weights summed are then the rounded ones. */
+       the matrix cores, which wait for the vector units up to 64 channels (5 sequences of 243 to 3,788 queries, 20
+       heads x 32: 113 us and, added, 129; 8 waves have no registers for it). 16 channels leave half of the
+       output's rows free: there V's unused rows are the ones. The weights summed are then the rounded ones. */
     f16v lsum = {};
     const v8 ones = splat_one<T>();
     float limit = -INFINITY;
@@ -429,10 +434,13 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
     }
 
     if (__syncthreads_or((bad & 0x80008000u) != 0)) {
-        for (int i = qa + half; i < qb; i += KW)
-            seq_attn_row<T, HD>(a, a.q + (rq.start + i) * a.q_token_stride + h * a.q_head_stride, kb, vb,
-                                a.out + (rq.start + i) * a.out_token_stride + h * a.out_head_stride,
+        for (int r = 32 * wave + half; r < 32 * wave + 32; r += KW) {
+            const int i = q0 + r / a.tile_heads, head = hg * a.tile_heads + r % a.tile_heads;
+            if (i >= q1) break;
+            seq_attn_row<T, HD>(a, a.q + (rq.start + i) * a.q_token_stride + head * a.q_head_stride, kb, vb,
+                                a.out + (rq.start + i) * a.out_token_stride + head * a.out_head_stride,
                                 key_range(shift + i, nk, a.left, a.right, a.sinks));
+        }
         return;
     }
     if constexpr (ONES) {
@@ -462,7 +470,7 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) o[d][e] = o[d][e] * f0 + red[(16 * d + e) * 256] * f1;
     }
-    const bool store = on && qa + c32 < qb;
+    const bool store = qrow < q1;
     const float inv = l == 0.f ? 0.f : 1.0f / l;
     uint16_t* out = a.out + (rq.start + qi) * a.out_token_stride + h * a.out_head_stride;
     /* a lane has 4 channels of every 8; its partner 32 lanes on, the others: 8 and 8 after an exchange */
@@ -488,9 +496,11 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
         }
 }
 
-#define SEQ_ATTN(NAME, T, HD)                                                                                                       \
-    extern "C" __global__ void __launch_bounds__(256, 2) prism_seq_attn_##NAME##_h##HD(SeqAttnArgs a) { seq_attn_body<T, HD, 1>(a); } \
-    extern "C" __global__ void __launch_bounds__(512, 2) prism_seq_attn_##NAME##_h##HD##_w8(SeqAttnArgs a) { seq_attn_body<T, HD, 2>(a); }
-SEQ_ATTN(f16, F16, 16) SEQ_ATTN(f16, F16, 32) SEQ_ATTN(f16, F16, 64) SEQ_ATTN(f16, F16, 128)
-SEQ_ATTN(bf16, BF16, 16) SEQ_ATTN(bf16, BF16, 32) SEQ_ATTN(bf16, BF16, 64) SEQ_ATTN(bf16, BF16, 128)
+/* W4, W8: waves per SIMD that the registers have to allow. 8 waves with up to 32 channels: two workgroups per CU
+ * (8,160 queries, 8 heads x 32: 30 us; one, 36). */
+#define SEQ_ATTN(NAME, T, HD, W4, W8)                                                                                                 \
+    extern "C" __global__ void __launch_bounds__(256, W4) prism_seq_attn_##NAME##_h##HD(SeqAttnArgs a) { seq_attn_body<T, HD, 1>(a); } \
+    extern "C" __global__ void __launch_bounds__(512, W8) prism_seq_attn_##NAME##_h##HD##_w8(SeqAttnArgs a) { seq_attn_body<T, HD, 2>(a); }
+SEQ_ATTN(f16, F16, 16, 4, 4) SEQ_ATTN(f16, F16, 32, 3, 4) SEQ_ATTN(f16, F16, 64, 3, 2) SEQ_ATTN(f16, F16, 128, 2, 2)
+SEQ_ATTN(bf16, BF16, 16, 4, 4) SEQ_ATTN(bf16, BF16, 32, 3, 4) SEQ_ATTN(bf16, BF16, 64, 3, 2) SEQ_ATTN(bf16, BF16, 128, 2, 2)
 #undef SEQ_ATTN

@@ -421,6 +421,13 @@ def test_seq_long(engine, dev, dtype, hd, lens, left, sinks):
     check_seq(engine, dev, np.random.default_rng(1), dtype, hd, 1, 2, lens, left, 0, sinks)
 
 
+@pytest.mark.parametrize("hd,kv,group", [(16, 1, 32), (32, 1, 33), (64, 3, 5), (32, 2, 8), (128, 1, 16), (16, 8, 2)])
+def test_seq_shared_heads(engine, dev, hd, kv, group):
+    """Groups that fill a workgroup's rows evenly or not, with a few queries, or not at all."""
+    rng = np.random.default_rng(group)
+    check_seq(engine, dev, rng, "bf16", hd, kv, group, [(9, 20), (1, 1), (0, 3), (37, 37), (5, 2)], 12, 0, 2)
+
+
 def test_seq_sharp_scores(engine, dev):
     check_seq(engine, dev, np.random.default_rng(2), "fp16", 64, 1, 1, [(300, 300)], 100, 0, 3, big=60.0)
 
@@ -448,35 +455,40 @@ def test_seq_rising_scores(engine, dev):
 
 @pytest.mark.parametrize("dtype,hd", [("fp16", 16), ("bf16", 32), ("fp16", 64), ("bf16", 128)])
 @pytest.mark.parametrize("what", ["v nan", "v inf", "k nan"])
-def test_seq_bad_values_reach_only_who_sees_them(engine, dev, dtype, hd, what):
+@pytest.mark.parametrize("group", [1, 3])
+def test_seq_bad_values_reach_only_who_sees_them(engine, dev, dtype, hd, what, group):
     """One key's value is NaN or infinite: the queries that see it get what the formula gives, the others what they
     would get without it."""
     rng = np.random.default_rng(hd)
     n, at, left, sinks = 300, 100, 40, 2
-    q, k, v = (normal(rng, (n, 1, hd), dtype) for _ in range(3))
+    q, k, v = normal(rng, (n, group, hd), dtype), normal(rng, (n, 1, hd), dtype), normal(rng, (n, 1, hd), dtype)
     inf = 0x7C00 if dtype == "fp16" else 0x7F80
     if what == "k nan":
         k[at, 0, 3] = NAN[dtype]
     else:
         v[at, 0, 5] = inf if what == "v inf" else NAN[dtype]
-    out = dev.put(np.full((n, 1, hd), NAN[dtype], np.uint16))
-    st = {f"{x}_{y}_stride": hd for x in ("q", "k", "v", "out") for y in ("token", "head")}
-    engine.seq_attn(P.SeqAttnPush(dtype=TYPES[dtype], n_seqs=1, n_q=n, n_k=n, n_heads=1, n_kv_heads=1, head_dim=hd, left=left,
-                                  right=0, sinks=sinks, scale=0.1, **st), dev.put(q), dev.put(k), dev.put(v), None, None, out)
-    got = values(dev.get(out, (n, hd)), dtype)
-    qv, kv, vv = (values(x[:, 0], dtype) for x in (q, k, v))
-    for i in range(n):
-        seen = visible(i, n, left, 0, sinks)
-        if not seen[at]:
-            want, bound = attention_row(qv[i], kv, vv, seen, 0.1, dtype)
-            assert not outside(got[i], want, bound), i
-        elif what == "k nan":
-            assert np.isnan(got[i]).all(), i
-        else:
-            want, bound = attention_row(qv[i], kv, np.where(np.isfinite(vv), vv, 0), seen, 0.1, dtype)
-            want, bound, rest = np.delete(want, 5), np.delete(bound, 5), np.delete(got[i], 5)
-            assert not outside(rest, want, bound), i
-            assert np.isposinf(got[i, 5]) if what == "v inf" else np.isnan(got[i, 5]), i
+    out = dev.put(np.full((n, group, hd), NAN[dtype], np.uint16))
+    st = {f"{x}_{y}_stride": hd * (group if x in ("q", "out") and y == "token" else 1) for x in ("q", "k", "v", "out")
+          for y in ("token", "head")}
+    engine.seq_attn(P.SeqAttnPush(dtype=TYPES[dtype], n_seqs=1, n_q=n, n_k=n, n_heads=group, n_kv_heads=1, head_dim=hd,
+                                  left=left, right=0, sinks=sinks, scale=0.1, **st), dev.put(q), dev.put(k), dev.put(v), None,
+                    None, out)
+    got_all = values(dev.get(out, (n, group, hd)), dtype)
+    kv, vv = values(k[:, 0], dtype), values(v[:, 0], dtype)
+    for h in range(group):
+        got, qv = got_all[:, h], values(q[:, h], dtype)
+        for i in range(n):
+            seen = visible(i, n, left, 0, sinks)
+            if not seen[at]:
+                want, bound = attention_row(qv[i], kv, vv, seen, 0.1, dtype)
+                assert not outside(got[i], want, bound), i
+            elif what == "k nan":
+                assert np.isnan(got[i]).all(), i
+            else:
+                want, bound = attention_row(qv[i], kv, np.where(np.isfinite(vv), vv, 0), seen, 0.1, dtype)
+                want, bound, rest = np.delete(want, 5), np.delete(bound, 5), np.delete(got[i], 5)
+                assert not outside(rest, want, bound), i
+                assert np.isposinf(got[i, 5]) if what == "v inf" else np.isnan(got[i, 5]), i
 
 
 @pytest.mark.parametrize("n_seqs", [70, 300])
