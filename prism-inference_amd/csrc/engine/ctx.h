@@ -93,7 +93,7 @@ struct prism_ctx {
     hipFunction_t f_codec[7] = {};     /* enc0..enc3, dec3, dec2, dec1_out */
     hipFunction_t f_codec21 = nullptr; /* dec2 + dec1_out in one launch (the decoder's last two stages) */
     hipFunction_t f_enc01 = nullptr;   /* enc0 + enc1 in one launch (the encoder's first two stages) */
-    hipFunction_t f_rope[2] = {};      /* [dtype] */
+    hipFunction_t f_rope[2][2] = {};   /* [dtype][pairs in whole chunks, or not] */
     hipFunction_t f_append = nullptr;
     hipFunction_t f_paged[2][4][3] = {};  /* [dtype][head_dim 16, 32, 64, 128][1, 2, more heads a key head] */
     hipFunction_t f_paged_join[2][4] = {};

@@ -127,7 +127,8 @@ extern "C" int prism_create(prism_ctx** out, int32_t device, const char* code_ob
     all.emplace_back(&c->f_append, "prism_cache_append");
     for (int t = 0; t < 2; ++t) {
         const std::string type = t == PRISM_BF16 ? "bf16" : "f16";
-        all.emplace_back(&c->f_rope[t], "prism_rope_" + type);
+        all.emplace_back(&c->f_rope[t][0], "prism_rope_" + type);
+        all.emplace_back(&c->f_rope[t][1], "prism_rope_" + type + "_loose");
         for (int i = 0; i < 4; ++i) {
             const std::string shape = type + "_h" + std::to_string(16 << i);
             for (int g = 0; g < 3; ++g)

@@ -93,7 +93,8 @@ extern "C" int prism_rope(prism_ctx* c, const prism_rope_push* p, const void* in
     a.log2_base = std::log2(p->base);
     a.copy = in != out;
     a.tile = rope_tile(p->n_tokens, a.n_pairs);
-    return launch(c, c->f_rope[p->dtype], "rope", ((int64_t)p->n_tokens + a.tile - 1) / a.tile, 256, &a, stream);
+    const bool loose = !a.adjacent && a.n_pairs % 8 != 0;
+    return launch(c, c->f_rope[p->dtype][loose], "rope", ((int64_t)p->n_tokens + a.tile - 1) / a.tile, 256, &a, stream);
 }
 
 extern "C" int prism_cache_append(prism_ctx* c, const prism_append_push* p, const void* k, const void* v,

@@ -14,11 +14,11 @@
  *   prism_codec_enc01, prism_codec_dec21_out       the same, fused in the frame (persistent)
  *   prism_codec_enc{2,3}, prism_codec_dec3         stages and frame alike (persistent)
  *   prism_codec_dec1_out                           dec1 + output conv + PixelShuffle + sigmoid
- *   prism_rope_{f16,bf16}                          rotary positions with several axes
+ *   prism_rope_{f16,bf16}[_loose]                  rotary positions with several axes
  *   prism_cache_append                             new tokens into a paged cache
  *   prism_paged_attn_{f16,bf16}_h{16,32,64,128}_{g1,g2,many}  one new token per sequence over its paged cache
  *   prism_paged_attn_join_{f16,bf16}_h{16,32,64,128}  ... and the join of a split length
- *   prism_seq_attn_{f16,bf16}_h{16,32,64,128}      attention along sequences, window and sinks
+ *   prism_seq_attn_{f16,bf16}_h{16,32,64,128}[_w8]  attention along sequences, window and sinks
  *   prism_zero_i32                                 clears routing counters
  */
 #include "attn.hpp"

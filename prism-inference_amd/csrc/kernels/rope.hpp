@@ -13,18 +13,12 @@
  * then streams the tokens' rows. A unit is 8 pairs of one head: two chunks of 16
  * bytes (HALVES: channels i.. and i + n.., ADJACENT: 16 channels in a row; two
  * chunks of channels that do not turn), two units a thread in flight. HALVES
- * with n not a multiple of 8 has second chunks on 2-byte boundaries (global
- * memory takes any) and goes the other way, one unit a time, the last pairs
- * element by element. Bound by HBM traffic: x read and written once.
+ * with n not a multiple of 8, whose second operands lie on no 16-byte boundary,
+ * takes them from LDS, a chunk of 8 channels at a time. Bound by HBM traffic: x
+ * read and written once.
  */
 #pragma once
 #include "seq_types.hpp"
-
-/* 16 bytes on any 2-byte boundary */
-template <class T>
-struct Loose8 {
-    typename T::v8 v;
-} __attribute__((packed, aligned(2)));
 
 /* (u, w) turned by (cos, sin) cs */
 template <class T>
@@ -92,49 +86,56 @@ __device__ __forceinline__ void rope_units(const RopeArgs& a, const float2* cs, 
     }
 }
 
-/* HALVES with n % 8 != 0 */
+/* HALVES with n % 8 != 0: rows (a token's heads) through LDS, whose second operands may lie anywhere. A thread
+ * has up to two chunks of 8 channels, the next rows' on their way meanwhile. */
 template <class T>
 __device__ __forceinline__ void rope_loose_units(const RopeArgs& a, const float2* cs, int np, int t0, int tokens) {
     typedef typename T::v8 v8;
     typedef typename T::el el;
-    const int n = a.n_pairs, turned = np / 8, copy0 = 2 * n / 8;
-    const int per_head = turned + (a.copy ? a.head_dim / 8 - copy0 : 0);
-    const int per_token = per_head * a.n_heads;
-    for (int u = threadIdx.x; u < tokens * per_token; u += 256) {
-        const int t = u / per_token, r = u - t * per_token, h = r / per_head, k = r - h * per_head;
-        const uint16_t* x = a.in + (t0 + t) * a.in_token_stride + h * a.in_head_stride;
-        uint16_t* y = a.out + (t0 + t) * a.out_token_stride + h * a.out_head_stride;
-        const float2* row = cs + t * np;
-        if (k >= turned) {
-            const int c = 8 * (copy0 + k - turned);
-            if (c >= 2 * n) {
-                st8<T>(y + c, ld8<T>(x + c));
-            } else {
-                for (int e = 2 * n; e < c + 8; ++e) y[e] = x[e];
-            }
-        } else if (8 * k + 8 <= n) {
-            v8 p = ld8<T>(x + 8 * k), q = reinterpret_cast<const Loose8<T>*>(x + 8 * k + n)->v;
+    constexpr int U = 2;
+    __shared__ __attribute__((aligned(16))) uint16_t lrow[256 * U * 8];
+    const int n = a.n_pairs, chunks = a.head_dim / 8, per = 256 * U / chunks; /* rows at a time */
+    const int rows = tokens * a.n_heads;
+    v8 v[U];
+    const auto load = [&](int r0) {
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            const int id = threadIdx.x + 256 * i, r = min(r0 + id / chunks, rows - 1); /* past the end: the last row again */
+            const int t = r / a.n_heads, h = r - t * a.n_heads;
+            v[i] = ld8<T>(a.in + (t0 + t) * a.in_token_stride + h * a.in_head_stride + id % chunks * 8);
+        }
+    };
+    load(0);
+    for (int r0 = 0; r0 < rows; r0 += per) {
+#pragma unroll
+        for (int i = 0; i < U; ++i) st8<T>(lrow + 8 * (threadIdx.x + 256 * i), v[i]);
+        __syncthreads(); /* the rows are in: in place, nothing is written before they are read */
+        v8 x[U];
+#pragma unroll
+        for (int i = 0; i < U; ++i) x[i] = v[i];
+        if (r0 + per < rows) load(r0 + per);
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            const int id = threadIdx.x + 256 * i, lr = id / chunks, r = r0 + lr, c = id % chunks * 8;
+            if (lr >= per || r >= rows || (c >= 2 * n && !a.copy)) continue;
+            const int t = r / a.n_heads, h = r - t * a.n_heads;
+            const el* row = reinterpret_cast<const el*>(lrow) + lr * a.head_dim;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                el b = p[e], d = q[e];
-                rope_turn<T>(b, d, row[8 * k + e]);
-                p[e] = b;
-                q[e] = d;
+                const int at = c + e;
+                if (at >= 2 * n) break;
+                const bool second = at >= n;
+                const float2 k = cs[t * np + (second ? at - n : at)];
+                const float own = (float)x[i][e], other = (float)row[second ? at - n : at + n] * (second ? k.y : -k.y);
+                x[i][e] = (el)opaque(__builtin_fmaf(own, k.x, other));
             }
-            st8<T>(y + 8 * k, p);
-            reinterpret_cast<Loose8<T>*>(y + 8 * k + n)->v = q;
-        } else {
-            for (int i = 8 * k; i < n; ++i) {
-                el b = reinterpret_cast<const el*>(x)[i], d = reinterpret_cast<const el*>(x)[i + n];
-                rope_turn<T>(b, d, row[i]);
-                reinterpret_cast<el*>(y)[i] = b;
-                reinterpret_cast<el*>(y)[i + n] = d;
-            }
+            st8<T>(a.out + (t0 + t) * a.out_token_stride + h * a.out_head_stride + c, x[i]);
         }
+        __syncthreads(); /* everyone has read the rows */
     }
 }
 
-template <class T>
+template <class T, bool LOOSE>
 __device__ __forceinline__ void rope_body(const RopeArgs& a) {
     __shared__ __attribute__((aligned(16))) float2 cs[ROPE_TILE_PAIRS]; /* [token][np] cos, sin */
     __shared__ double turns[ROPE_MAX_PAIRS];
@@ -157,10 +158,12 @@ __device__ __forceinline__ void rope_body(const RopeArgs& a) {
         }
     }
     __syncthreads();
-    if (a.adjacent) rope_units<T, true>(a, cs, np, t0, tokens);
-    else if (n == np) rope_units<T, false>(a, cs, np, t0, tokens);
-    else rope_loose_units<T>(a, cs, np, t0, tokens);
+    if constexpr (LOOSE) rope_loose_units<T>(a, cs, np, t0, tokens);
+    else if (a.adjacent) rope_units<T, true>(a, cs, np, t0, tokens);
+    else rope_units<T, false>(a, cs, np, t0, tokens);
 }
 
-extern "C" __global__ void __launch_bounds__(256) prism_rope_f16(RopeArgs a) { rope_body<F16>(a); }
-extern "C" __global__ void __launch_bounds__(256) prism_rope_bf16(RopeArgs a) { rope_body<BF16>(a); }
+extern "C" __global__ void __launch_bounds__(256) prism_rope_f16(RopeArgs a) { rope_body<F16, false>(a); }
+extern "C" __global__ void __launch_bounds__(256) prism_rope_bf16(RopeArgs a) { rope_body<BF16, false>(a); }
+extern "C" __global__ void __launch_bounds__(256) prism_rope_f16_loose(RopeArgs a) { rope_body<F16, true>(a); }
+extern "C" __global__ void __launch_bounds__(256) prism_rope_bf16_loose(RopeArgs a) { rope_body<BF16, true>(a); }
