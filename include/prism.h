@@ -446,12 +446,13 @@ int prism_release_external_memory(prism_ctx* ctx, prism_external_buffer* buf);
  * device pointers to 16-bit values (fp16 or bf16, `dtype`), needs no model
  * loaded, keeps nothing between calls and allocates nothing, so it may be
  * captured into a graph. Sums, softmax statistics and angles are held in 32
- * bits or more; outputs are rounded once, to nearest. Pointers to values are
+ * bits or more; outputs are rounded once, to nearest, and so are softmax
+ * weights that meet their values in matrix products. Pointers to values are
  * 16-byte aligned and strides are in elements, multiples of 8, not negative
  * (0 repeats an input; an output's rows must not overlap). head_dim is the
  * innermost, contiguous dimension. The call runs on the context's device and
  * leaves the caller's current device as it was. A call without rows does
- * nothing. The reference has no counterpart: its attention sees one window of
+ * nothing; one of more than 2^32 - 1 threads is PRISM_ERR_UNSUPPORTED. The reference has no counterpart: its attention sees one window of
  * one frame (shaders/split2_qkv_attn_d256.comp.glsl:24-79). */
 #define PRISM_F16  0
 #define PRISM_BF16 1
@@ -467,7 +468,7 @@ int prism_release_external_memory(prism_ctx* ctx, prism_external_buffer* buf);
  * becomes (x cos phi - y sin phi, y cos phi + x sin phi); `inverse` turns by
  * -phi, which is also the gradient's way back. Token t of axis a is at
  * pos[a * pos_stride + t] (any int32; angles are reduced in 64 bits). head_dim
- * is a multiple of 8 up to 256; 2n <= head_dim; base > 0. in == out with equal
+ * is a multiple of 8 up to 256; 2n <= head_dim; base >= 1. in == out with equal
  * strides works in place; otherwise the two must not overlap. */
 typedef struct prism_rope_push {
     int32_t dtype, n_tokens, n_heads, head_dim;
@@ -495,7 +496,7 @@ typedef struct prism_cache_desc {
 /* Write n_new tokens' keys and values (rows of k and v) into the cache: row i is
  * token pos_of[i] of sequence seq_of[i]. A row whose sequence, position or
  * page is out of range is skipped (give padding rows sequence -1). Two rows for
- * one slot leave it unspecified which of them it holds. */
+ * one slot leave that slot's values unspecified (parts of either). */
 typedef struct prism_append_push {
     prism_cache_desc cache;
     int32_t n_new;
@@ -517,7 +518,8 @@ int prism_cache_append(prism_ctx* ctx, const prism_append_push* p, const void* k
  * it decides how the work is split; longer sequences are still right. workspace:
  * device memory of prism_paged_attn_workspace bytes (16-byte aligned; may be
  * NULL if that is 0), free to reuse after the call's work; calls that may
- * overlap need one each. scale is positive and finite. */
+ * overlap need one each. scale is positive and at most
+ * 2e38; scaled scores are fp32 and have to stay in its range. */
 typedef struct prism_paged_attn_push {
     prism_cache_desc cache;
     int32_t n_heads;
@@ -543,7 +545,7 @@ int prism_paged_attn(prism_ctx* ctx, const prism_paged_attn_push* p, const void*
  * key as in prism_paged_attn. Rows of out before the first sequence and behind
  * the last one stay as they were. Starts that are not in order name unspecified
  * rows of the buffers, never others. head_dim 16, 32, 64 or 128; at most 2^30
- * rows, k and v token strides at most 2^24. */
+ * rows, k and v token strides at most 2^22. */
 typedef struct prism_seq_attn_push {
     int32_t dtype, n_seqs, n_q, n_k, n_heads, n_kv_heads, head_dim;
     int32_t left, right, sinks;

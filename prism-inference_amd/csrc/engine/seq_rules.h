@@ -19,7 +19,7 @@ constexpr int64_t SEQ_MAX_STRIDE = int64_t(1) << 40;
  * end stay in 32 bits. */
 constexpr int64_t SEQ_MAX_ROWS = int64_t(1) << 30;
 /* Key rows of a tile are addressed with 32 bits. */
-constexpr int64_t SEQ_MAX_KEY_STRIDE = int64_t(1) << 24;
+constexpr int64_t SEQ_MAX_KEY_STRIDE = int64_t(1) << 22;
 
 inline int seq_bad(const char** why, int code, const char* text) {
     if (why) *why = text;
@@ -57,8 +57,13 @@ inline int check_heads(int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, co
     return PRISM_OK;
 }
 
+/* the kernels work with powers of two */
+inline float seq_scale_log2(float scale) { return scale * 1.4426950408889634f; }
+
 inline int check_scale(float scale, const char** why) {
-    return scale > 0.f && std::isfinite(scale) ? PRISM_OK : seq_bad(why, PRISM_ERR_INVALID, "scale is not positive");
+    return scale > 0.f && std::isfinite(seq_scale_log2(scale))
+               ? PRISM_OK
+               : seq_bad(why, PRISM_ERR_INVALID, "scale is not positive, or too large");
 }
 
 inline int check_rope(const prism_rope_push& p, const char** why) {
@@ -77,7 +82,7 @@ inline int check_rope(const prism_rope_push& p, const char** why) {
     if ((p.layout != PRISM_ROPE_HALVES && p.layout != PRISM_ROPE_ADJACENT) ||
         (p.ladder != PRISM_ROPE_AXIS_LADDER && p.ladder != PRISM_ROPE_ONE_LADDER) || (p.inverse != 0 && p.inverse != 1))
         return seq_bad(why, PRISM_ERR_INVALID, "layout, ladder or inverse");
-    if (!(p.base > 0) || !std::isfinite(p.base)) return seq_bad(why, PRISM_ERR_INVALID, "base is not positive");
+    if (!(p.base >= 1) || !std::isfinite(p.base)) return seq_bad(why, PRISM_ERR_INVALID, "base is less than 1");
     if (p.pos_stride < 0 || p.pos_stride > SEQ_MAX_STRIDE) return seq_bad(why, PRISM_ERR_INVALID, "pos_stride");
     if (int rc = check_strides(p.in_token_stride, p.in_head_stride, why)) return rc;
     return check_out(p.n_tokens, p.n_heads, p.head_dim, p.out_token_stride, p.out_head_stride, why);
@@ -123,9 +128,12 @@ inline int check_seq(const prism_seq_attn_push& p, const char** why) {
     if (int rc = check_strides(p.k_token_stride, p.k_head_stride, why)) return rc;
     if (int rc = check_strides(p.v_token_stride, p.v_head_stride, why)) return rc;
     if (p.k_token_stride > SEQ_MAX_KEY_STRIDE || p.v_token_stride > SEQ_MAX_KEY_STRIDE)
-        return seq_bad(why, PRISM_ERR_UNSUPPORTED, "k and v token strides are at most 2^24");
+        return seq_bad(why, PRISM_ERR_UNSUPPORTED, "k and v token strides are at most 2^22");
     return check_out(p.n_q, p.n_heads, p.head_dim, p.out_token_stride, p.out_head_stride, why);
 }
+
+/* A launch's threads are counted in 32 bits. */
+inline bool seq_grid_ok(int64_t grid, unsigned threads) { return grid <= (int64_t)(UINT32_MAX / threads); }
 
 /* Where each axis' pairs end; returns the number of pairs. */
 inline int rope_axes(const prism_rope_push& p, int32_t axis_end[4]) {

@@ -43,7 +43,8 @@ class OnDevice {
 
 /* grid workgroups of `threads` on the context's device */
 int launch(prism_ctx* c, hipFunction_t f, const char* what, int64_t grid, unsigned threads, void* args, void* stream) {
-    if (grid > INT32_MAX) return fail(c, PRISM_ERR_INVALID, "%s: %lld workgroups", what, (long long)grid);
+    if (!seq_grid_ok(grid, threads))
+        return fail(c, PRISM_ERR_UNSUPPORTED, "%s: %lld workgroups are more than one launch takes", what, (long long)grid);
     OnDevice on(c->device);
     if (on.error() != hipSuccess)
         return fail(c, PRISM_ERR_HIP, "hipSetDevice(%d): %s", c->device, hipGetErrorString(on.error()));
@@ -175,7 +176,7 @@ extern "C" int prism_paged_attn(prism_ctx* c, const prism_paged_attn_push* p, co
     a.table_pages = d.n_pages > 0 ? d.table_pages : 0;
     a.left = p->left;
     a.sinks = p->sinks;
-    a.scale_log2 = p->scale * 1.4426950408889634f;
+    a.scale_log2 = seq_scale_log2(p->scale);
     a.head_tiles = plan.head_tiles;
     a.waves = plan.waves;
     a.splits = plan.splits;
@@ -219,7 +220,7 @@ extern "C" int prism_seq_attn(prism_ctx* c, const prism_seq_attn_push* p, const 
     a.left = p->left;
     a.right = p->right;
     a.sinks = p->sinks;
-    a.scale_log2 = p->scale * 1.4426950408889634f;
+    a.scale_log2 = seq_scale_log2(p->scale);
     a.tile_heads = seq_tile_heads(p->n_heads, p->n_kv_heads);
     a.tile_q = SEQ_ROWS / a.tile_heads;
     const int64_t grid = seq_tiles(p->n_q, p->n_seqs, a.tile_q) * (p->n_heads / a.tile_heads);

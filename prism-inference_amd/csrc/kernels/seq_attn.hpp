@@ -4,16 +4,18 @@
  * p = nk - nq + i and sees keys j <= p + right with j >= p - left or j < sinks.
  *
  * A workgroup takes 128 rows, 32 a wave: a row is a query of one head, the heads
- * that share a key head side by side (so the workgroup's queries are fewer, and
- * the keys that they see together too). It goes once over the
- * keys that any of them sees, 64 or 128 at a time, with a running maximum and sum:
+ * that share a key head side by side (so the workgroup's queries are fewer, and the keys that they see
+ * together too). It goes once over the keys that any of them sees, in tiles of 128
+ * (64 with more than 32 channels and 4 waves), with a running maximum and sum:
  *   S^T = K Q^T           (32x32x16 MFMA: a lane holds one query's scores)
  *   P^T = 2^(c S^T - c m) (registers; c = scale log2 e)
  *   O^T += V^T P^T        (P^T is the B operand as it lies: the MFMA's
  *                          reduction index may be numbered in any order, and
  *                          V^T is read from LDS in that order by transposing
  *                          reads)
- * so a query's maximum, sum and rescaling stay in its lane (two lanes, 32
+ * The weights are rounded to the type of the values, which is what the products
+ * take (each by half a step, as much as the output's rounding). With this order
+ * a query's maximum, sum and rescaling stay in its lane (two lanes, 32
  * apart, hold halves of its keys). K and V tiles go through LDS, double
  * buffered, the next tile's loads in flight under the current tile's products.
  * Keys that no query of the workgroup sees are staged as zeros. Where only some
@@ -229,8 +231,9 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
             if (CHUNKS % NTHR == 0 || id0 < CHUNKS) load_to_lds(buffer, off[c], lds0 + to + 16 * id0);
         }
     };
-    auto check_v = [&](int at, int t, int k0) { /* a tile that some queries see only in part: finite? */
-        if ((t >= sink_tiles && k0 < r1.lo) || k0 + BN > r0.hi) {
+    auto check_v = [&](int at, int t, int k0) { /* a tile that some queries see only in part: finite? (Rows past the
+                                                    end are zeros where V's rows do not overlap.) */
+        if ((t >= sink_tiles && k0 < r1.lo) || k0 + BN > seq_min(r0.hi, end_of(t))) {
             constexpr unsigned E = __is_same(T, F16) ? 0x7C007C00u : 0x7F807F80u;
             constexpr unsigned U = __is_same(T, F16) ? 0x04000400u : 0x00800080u;
 #pragma unroll

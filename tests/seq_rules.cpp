@@ -12,6 +12,19 @@ int paged_check(const prism_paged_attn_push* p) { const char* w; return check_pa
 int seq_check(const prism_seq_attn_push* p) { const char* w; return check_seq(*p, &w); }
 int axes(const prism_rope_push* p, int32_t* axis_end) { return rope_axes(*p, axis_end); }
 int tile(long long n_tokens, int n_pairs) { return rope_tile(n_tokens, n_pairs); }
+void paged(const prism_paged_attn_push* p, long long* out) {
+    const PagedPlan r = paged_plan(*p);
+    out[0] = r.many;
+    out[1] = r.head_tiles;
+    out[2] = r.waves;
+    out[3] = r.splits;
+    out[4] = r.grid;
+    out[5] = paged_workspace(*p, r);
+}
+int tile_heads(int n_heads, int n_kv_heads) { return seq_tile_heads(n_heads, n_kv_heads); }
+long long seq_tiles(long long n_q, long long n_seqs, int tile_q) { return prism::seq_tiles(n_q, n_seqs, tile_q); }
+int grid_ok(long long grid, int threads) { return seq_grid_ok(grid, threads); }
+int seq_w8(long long grid) { return prism::seq_w8(grid); }
 void keys(int32_t p, int32_t n, int32_t left, int32_t right, int32_t sinks, int32_t* out) {
     const KeyRange r = key_range(p, n, left, right, sinks);
     out[0] = r.sink;

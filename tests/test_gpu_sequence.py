@@ -340,8 +340,10 @@ def test_paged_offsets_past_32_bits(hip, engine, dev, device_arena):
 
 # ---------------------------------------------------------------- sequences
 
-def check_seq(engine, dev, rng, dtype, hd, kv, group, lens, left, right, sinks, layout="dense", head=0, tail=3, big=1.0):
-    """lens: (queries, keys) of each sequence; head, tail: rows before the first and behind the last."""
+def check_seq(engine, dev, rng, dtype, hd, kv, group, lens, left, right, sinks, layout="dense", head=0, tail=3, big=1.0, waves=8):
+    """lens: (queries, keys) of each sequence; head, tail: rows before the first and behind the last; waves of a
+    workgroup: 4 where there are more than 1,024 workgroups (here of empty sequences)."""
+    lens = lens + [(0, 0)] * (1100 if waves == 4 else 0)
     heads, scale = kv * group, 1 / math.sqrt(hd)
     cq = (head + np.concatenate([[0], np.cumsum([a for a, _ in lens])])).astype(np.int32)
     ck = (head + np.concatenate([[0], np.cumsum([b for _, b in lens])])).astype(np.int32)
@@ -372,7 +374,7 @@ def check_seq(engine, dev, rng, dtype, hd, kv, group, lens, left, right, sinks, 
              "out_token_stride", "out_head_stride")
     push = P.SeqAttnPush(dtype=TYPES[dtype], n_seqs=len(lens), n_q=nq, n_k=nk, n_heads=heads, n_kv_heads=kv, head_dim=hd,
                          left=left, right=right, sinks=sinks, scale=scale, **dict(zip(names, st)))
-    print(f"[seq] {dtype} {heads}/{kv} x {hd} {lens} left {left} right {right} sinks {sinks} {layout}", flush=True)
+    print(f"[seq] {dtype} {heads}/{kv} x {hd} {lens[:12]} waves {waves} left {left} right {right} sinks {sinks} {layout}", flush=True)
     engine.seq_attn(push, dq, dk, dv, dev.put(cq), dev.put(ck), out)
     got = dev.get(out, (heads, nq, hd)).transpose(1, 0, 2) if layout == "heads" else dev.get(out, (nq, heads, hd))
     assert (got[:head] == NAN[dtype]).all() and (got[nq - tail:] == NAN[dtype]).all()
@@ -387,23 +389,28 @@ def check_seq(engine, dev, rng, dtype, hd, kv, group, lens, left, right, sinks, 
                 assert not msg, (s, i, h, msg)
 
 
+WAVES = pytest.mark.parametrize("waves", [8, 4])
 RAGGED = [(1, 1), (0, 0), (5, 5), (64, 64), (65, 65), (0, 7), (31, 31), (130, 130), (3, 0)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("hd", [16, 32, 64, 128])
 @pytest.mark.parametrize("kv,group", [(2, 1), (1, 3)])
-def test_seq_shapes(engine, dev, dtype, hd, kv, group):
-    check_seq(engine, dev, np.random.default_rng(hd), dtype, hd, kv, group, RAGGED, -1, 0, 0)
+@WAVES
+def test_seq_shapes(engine, dev, dtype, hd, kv, group, waves):
+    check_seq(engine, dev, np.random.default_rng(hd), dtype, hd, kv, group, RAGGED, -1, 0, 0, waves=waves)
 
 
 @pytest.mark.parametrize("left,right,sinks", [
     (-1, -1, 0), (0, 0, 0), (0, 0, 3), (7, 0, 0), (40, 0, 5), (63, 0, 100), (20, 9, 2), (0, 30, 0), (-1, 5, 0), (200, -1, 1),
     (MAX, MAX, MAX), (3, -1, 0),
 ])
-def test_seq_windows(engine, dev, left, right, sinks):
+@pytest.mark.parametrize("hd", [32, 128])
+@WAVES
+def test_seq_windows(engine, dev, left, right, sinks, hd, waves):
     rng = np.random.default_rng(abs(left) % 97 + right % 89 + sinks % 83)
-    check_seq(engine, dev, rng, "fp16", 32, 1, 2, [(150, 150), (1, 1), (33, 90), (70, 20), (200, 200)], left, right, sinks)
+    check_seq(engine, dev, rng, "fp16", hd, 1, 2, [(150, 150), (1, 1), (33, 90), (70, 20), (200, 200)], left, right, sinks,
+              waves=waves)
 
 
 @pytest.mark.parametrize("layout", ["fused", "heads"])
@@ -417,22 +424,26 @@ def test_seq_layouts(engine, dev, layout, hd):
     ("fp16", 32, [(600, 600)], 128, 20), ("bf16", 128, [(300, 900), (257, 257)], 200, 4), ("fp16", 64, [(1, 2000), (4, 700)], 511, 1),
     ("bf16", 16, [(513, 513)], -1, 0),
 ])
-def test_seq_long(engine, dev, dtype, hd, lens, left, sinks):
-    check_seq(engine, dev, np.random.default_rng(1), dtype, hd, 1, 2, lens, left, 0, sinks)
+@WAVES
+def test_seq_long(engine, dev, dtype, hd, lens, left, sinks, waves):
+    check_seq(engine, dev, np.random.default_rng(1), dtype, hd, 1, 2, lens, left, 0, sinks, waves=waves)
 
 
 @pytest.mark.parametrize("hd,kv,group", [(16, 1, 32), (32, 1, 33), (64, 3, 5), (32, 2, 8), (128, 1, 16), (16, 8, 2)])
-def test_seq_shared_heads(engine, dev, hd, kv, group):
+@WAVES
+def test_seq_shared_heads(engine, dev, hd, kv, group, waves):
     """Groups that fill a workgroup's rows evenly or not, with a few queries, or not at all."""
     rng = np.random.default_rng(group)
-    check_seq(engine, dev, rng, "bf16", hd, kv, group, [(9, 20), (1, 1), (0, 3), (37, 37), (5, 2)], 12, 0, 2)
+    check_seq(engine, dev, rng, "bf16", hd, kv, group, [(9, 20), (1, 1), (0, 3), (37, 37), (5, 2)], 12, 0, 2, waves=waves)
 
 
-def test_seq_sharp_scores(engine, dev):
-    check_seq(engine, dev, np.random.default_rng(2), "fp16", 64, 1, 1, [(300, 300)], 100, 0, 3, big=60.0)
+@WAVES
+def test_seq_sharp_scores(engine, dev, waves):
+    check_seq(engine, dev, np.random.default_rng(2), "fp16", 64, 1, 1, [(300, 300)], 100, 0, 3, big=60.0, waves=waves)
 
 
-def test_seq_rising_scores(engine, dev):
+@WAVES
+def test_seq_rising_scores(engine, dev, waves):
     """The largest score comes last, tile after tile: the running maximum moves every time."""
     rng = np.random.default_rng(4)
     dtype, hd, n = "bf16", 32, 400
@@ -442,10 +453,12 @@ def test_seq_rising_scores(engine, dev):
     q[..., 0] = np.where(np.arange(n) % 2, 4.0, -4.0)[:, None]
     q, k, v = to_bits(q, dtype), to_bits(k, dtype), normal(rng, (n, 1, hd), dtype)
     out = dev.put(np.full((n, 1, hd), NAN[dtype], np.uint16))
-    push = P.SeqAttnPush(dtype=P.BF16, n_seqs=1, n_q=n, n_k=n, n_heads=1, n_kv_heads=1, head_dim=hd, left=-1, right=0, sinks=0,
+    seqs = 1 if waves == 8 else 1100  # one sequence and empty ones, or no starts at all
+    cu = dev.put(np.array([0] + [n] * seqs, np.int32)) if seqs > 1 else None
+    push = P.SeqAttnPush(dtype=P.BF16, n_seqs=seqs, n_q=n, n_k=n, n_heads=1, n_kv_heads=1, head_dim=hd, left=-1, right=0, sinks=0,
                          scale=1.0, q_token_stride=hd, q_head_stride=hd, k_token_stride=hd, k_head_stride=hd, v_token_stride=hd,
                          v_head_stride=hd, out_token_stride=hd, out_head_stride=hd)
-    engine.seq_attn(push, dev.put(q), dev.put(k), dev.put(v), None, None, out)  # one sequence: no starts needed
+    engine.seq_attn(push, dev.put(q), dev.put(k), dev.put(v), cu, cu, out)
     got = values(dev.get(out, (n, 1, hd)), dtype)
     for i in range(n):
         want, bound = attention_row(values(q[i, 0], dtype), values(k[:, 0], dtype), values(v[:, 0], dtype),
@@ -456,7 +469,8 @@ def test_seq_rising_scores(engine, dev):
 @pytest.mark.parametrize("dtype,hd", [("fp16", 16), ("bf16", 32), ("fp16", 64), ("bf16", 128)])
 @pytest.mark.parametrize("what", ["v nan", "v inf", "k nan"])
 @pytest.mark.parametrize("group", [1, 3])
-def test_seq_bad_values_reach_only_who_sees_them(engine, dev, dtype, hd, what, group):
+@WAVES
+def test_seq_bad_values_reach_only_who_sees_them(engine, dev, dtype, hd, what, group, waves):
     """One key's value is NaN or infinite: the queries that see it get what the formula gives, the others what they
     would get without it."""
     rng = np.random.default_rng(hd)
@@ -470,9 +484,10 @@ def test_seq_bad_values_reach_only_who_sees_them(engine, dev, dtype, hd, what, g
     out = dev.put(np.full((n, group, hd), NAN[dtype], np.uint16))
     st = {f"{x}_{y}_stride": hd * (group if x in ("q", "out") and y == "token" else 1) for x in ("q", "k", "v", "out")
           for y in ("token", "head")}
-    engine.seq_attn(P.SeqAttnPush(dtype=TYPES[dtype], n_seqs=1, n_q=n, n_k=n, n_heads=group, n_kv_heads=1, head_dim=hd,
-                                  left=left, right=0, sinks=sinks, scale=0.1, **st), dev.put(q), dev.put(k), dev.put(v), None,
-                    None, out)
+    cu = dev.put(np.array([0] + [n] * (1 if waves == 8 else 1100), np.int32))  # and empty sequences
+    engine.seq_attn(P.SeqAttnPush(dtype=TYPES[dtype], n_seqs=1 if waves == 8 else 1100, n_q=n, n_k=n, n_heads=group,
+                                  n_kv_heads=1, head_dim=hd, left=left, right=0, sinks=sinks, scale=0.1, **st), dev.put(q),
+                    dev.put(k), dev.put(v), cu, cu, out)
     got_all = values(dev.get(out, (n, group, hd)), dtype)
     kv, vv = values(k[:, 0], dtype), values(v[:, 0], dtype)
     for h in range(group):
@@ -516,6 +531,72 @@ def test_seq_starts_out_of_range(engine, dev):
     for i in list(range(10)) + list(range(20, 40)):
         first = 0 if i < 10 else 10
         want, bound = attention_row(xv[i], xv[first:], xv[first:], visible(i - first, n - first, -1, 0, 0), 0.2, dtype)
+        assert not outside(got[i], want, bound), i
+
+
+@pytest.mark.parametrize("stride", [0, 8])
+@pytest.mark.parametrize("hd", [16, 128])
+@WAVES
+def test_seq_rows_that_overlap(engine, dev, stride, hd, waves):
+    """Keys and values repeated or overlapping, an infinite value among them: each channel meets it or does not."""
+    rng = np.random.default_rng(hd + stride)
+    dtype, n, sinks, left = "fp16", 300, 3, 40
+    flat = normal(rng, n * stride + hd, dtype)
+    flat[:hd:16] = to_bits(np.inf, dtype)
+    q, k = normal(rng, (n, 1, hd), dtype), normal(rng, n * stride + hd, dtype)
+    out = dev.put(np.full((n, hd), NAN[dtype], np.uint16))
+    seqs = 1 if waves == 8 else 1100
+    cu = dev.put(np.array([0] + [n] * seqs, np.int32))
+    push = P.SeqAttnPush(dtype=P.F16, n_seqs=seqs, n_q=n, n_k=n, n_heads=1, n_kv_heads=1, head_dim=hd, left=left, right=0,
+                         sinks=sinks, scale=0.1, q_token_stride=hd, q_head_stride=hd, k_token_stride=stride, k_head_stride=hd,
+                         v_token_stride=stride, v_head_stride=hd, out_token_stride=hd, out_head_stride=hd)
+    engine.seq_attn(push, dev.put(q), dev.put(k), dev.put(flat), cu, cu, out)
+    got, qv = values(dev.get(out, (n, hd)), dtype), values(q[:, 0], dtype)
+    row = lambda x: values(np.stack([x[stride * j:][:hd] for j in range(n)]), dtype)
+    kv_, vv = row(k), row(flat)
+    for i in range(n):
+        seen = visible(i, n, left, 0, sinks)
+        high = np.isinf(vv[seen]).any(0)
+        want, bound = attention_row(qv[i], kv_, np.where(np.isinf(vv), 0, vv), seen, 0.1, dtype)
+        assert np.isposinf(got[i, high]).all(), i
+        assert not outside(got[i, ~high], want[~high], bound[~high]), i
+
+
+def test_seq_largest_key_stride(hip, engine, dev, device_arena):
+    """Rows 8 MiB apart: the last of a tile's lies almost 2^30 bytes behind its first."""
+    rng = np.random.default_rng(15)
+    dtype, hd, n, far = "bf16", 32, 260, 2 ** 22
+    q, k, v = (normal(rng, (n, hd), dtype) for _ in "qkv")
+    big = device_arena(((n - 1) * far + 2 * hd) * 2, zero=False)  # a row's keys, then its values
+    for j in range(n):
+        hip.upload(big.ptr + 2 * far * j, np.concatenate([k[j], v[j]]))
+    for seqs in (1, 1100):
+        out = dev.put(np.full((n, hd), NAN[dtype], np.uint16))
+        cu = dev.put(np.array([0] + [n] * seqs, np.int32))
+        push = P.SeqAttnPush(dtype=P.BF16, n_seqs=seqs, n_q=n, n_k=n, n_heads=1, n_kv_heads=1, head_dim=hd, left=-1, right=0,
+                             sinks=0, scale=0.2, q_token_stride=hd, q_head_stride=hd, k_token_stride=far, k_head_stride=hd,
+                             v_token_stride=far, v_head_stride=hd, out_token_stride=hd, out_head_stride=hd)
+        engine.seq_attn(push, dev.put(q), big.ptr, big.ptr + 2 * hd, cu, cu, out)
+        got = values(dev.get(out, (n, hd)), dtype)
+        for i in range(n):
+            want, bound = attention_row(values(q[i], dtype), values(k, dtype), values(v, dtype), visible(i, n, -1, 0, 0), 0.2, dtype)
+            assert not outside(got[i], want, bound), i
+
+
+@pytest.mark.parametrize("hd", [16, 64])
+def test_seq_tiny_values(engine, dev, hd):
+    """fp16 queries below the type's smallest normal number, a scale that makes up for it."""
+    rng = np.random.default_rng(16)
+    dtype, n = "fp16", 100
+    q, k, v = to_bits(rng.standard_normal((n, hd)) * 2e-5, dtype), normal(rng, (n, hd), dtype), normal(rng, (n, hd), dtype)
+    out = dev.put(np.full((n, hd), NAN[dtype], np.uint16))
+    push = P.SeqAttnPush(dtype=P.F16, n_seqs=1, n_q=n, n_k=n, n_heads=1, n_kv_heads=1, head_dim=hd, left=-1, right=-1, sinks=0,
+                         scale=8192.0, q_token_stride=hd, q_head_stride=hd, k_token_stride=hd, k_head_stride=hd,
+                         v_token_stride=hd, v_head_stride=hd, out_token_stride=hd, out_head_stride=hd)
+    engine.seq_attn(push, dev.put(q), dev.put(k), dev.put(v), None, None, out)
+    got = values(dev.get(out, (n, hd)), dtype)
+    for i in range(n):
+        want, bound = attention_row(values(q[i], dtype), values(k, dtype), values(v, dtype), np.ones(n, bool), 8192.0, dtype)
         assert not outside(got[i], want, bound), i
 
 
@@ -694,6 +775,10 @@ def test_refused_calls(hip, engine, dev):
     refused(engine.seq_attn, R.seq(), a, None, a, a, a, a)
     refused(engine.seq_attn, R.seq(n_seqs=3), a, a, a, None, None, a)  # 10 rows are not 3 equal sequences
     refused(engine.seq_attn, R.seq(n_kv_heads=3), a, a, a, a, a, a)
+    # more threads than a launch has
+    refused(engine.cache_append, R.append(cache=R.cache(n_kv_heads=65536), n_new=2 ** 30), a, a, a, a, a, a, a)
+    refused(engine.paged_attn, R.paged(cache=R.cache(n_seqs=2 ** 30), out_seq_stride=128), a, a, a, a, a, a, a, 0)
+    refused(engine.seq_attn, R.seq(n_seqs=MAX), a, a, a, a, a, a)
     # calls without rows are fine, whatever the buffers are
     engine.rope(R.rope(n_tokens=0), None, None, None)
     engine.cache_append(R.append(n_new=0), *[None] * 7)

@@ -23,6 +23,8 @@ def rules(tmp_path_factory):
     lib = C.CDLL(so)
     lib.rows.argtypes = [C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p]
     lib.tile.argtypes = [C.c_longlong, C.c_int]
+    lib.seq_tiles.argtypes, lib.seq_tiles.restype = [C.c_longlong, C.c_longlong, C.c_int], C.c_longlong
+    lib.seq_w8.argtypes, lib.grid_ok.argtypes = [C.c_longlong], [C.c_longlong, C.c_int]
     return lib
 
 
@@ -63,7 +65,7 @@ STRIDES = [-8, 4, 2 ** 41]
     dict(dtype=2), dict(dtype=-1), dict(n_tokens=-1), dict(n_heads=0), dict(n_heads=65537), dict(head_dim=12),
     dict(head_dim=264), dict(head_dim=0), dict(n_axes=0), dict(n_axes=5), dict(pairs=(4, -1, 6, 0)), dict(pairs=(0, 0, 0, 9)),
     dict(pairs=(5, 6, 6, 0)), dict(pairs=(MAX, MAX, 6, 0)), dict(layout=2), dict(ladder=-1), dict(inverse=2), dict(base=0.0),
-    dict(base=-3.0), dict(base=nan), dict(base=inf), dict(pos_stride=-1), dict(out_token_stride=64),
+    dict(base=-3.0), dict(base=0.99), dict(base=nan), dict(base=inf), dict(pos_stride=-1), dict(out_token_stride=64),
     dict(out_head_stride=0), dict(out_head_stride=16), dict(out_token_stride=0),
 ] + [{f: s} for f in ("in_token_stride", "in_head_stride", "out_token_stride", "out_head_stride") for s in STRIDES])
 def test_rope_refusals(rules, bad):
@@ -94,7 +96,7 @@ def test_append_refusals(rules, bad):
 
 @pytest.mark.parametrize("bad", [dict(cache=cache(**c)) for c in CACHES] + [
     dict(n_heads=0), dict(n_heads=5), dict(n_heads=-2), dict(n_heads=65538), dict(sinks=-1), dict(max_len=-1), dict(scale=0.0),
-    dict(scale=-1.0), dict(scale=nan), dict(scale=inf), dict(out_head_stride=16), dict(out_seq_stride=96),
+    dict(scale=-1.0), dict(scale=nan), dict(scale=inf), dict(scale=3e38), dict(out_head_stride=16), dict(out_seq_stride=96),
 ] + [{f: s} for f in ("q_seq_stride", "q_head_stride", "out_seq_stride", "out_head_stride") for s in STRIDES])
 def test_paged_refusals(rules, bad):
     assert rules.paged_check(C.byref(paged(**bad))) < 0
@@ -104,7 +106,8 @@ def test_paged_refusals(rules, bad):
 
 @pytest.mark.parametrize("bad", [
     dict(dtype=9), dict(n_seqs=-1), dict(n_q=-1), dict(n_k=-1), dict(n_heads=3), dict(n_kv_heads=0), dict(head_dim=40),
-    dict(k_token_stride=2 ** 24 + 8), dict(v_token_stride=2 ** 24 + 8), dict(n_q=2 ** 30 + 1), dict(n_k=MAX), dict(sinks=-2), dict(scale=0.0), dict(scale=nan), dict(out_token_stride=192), dict(out_head_stride=32),
+    dict(k_token_stride=2 ** 22 + 8), dict(v_token_stride=2 ** 22 + 8), dict(n_q=2 ** 30 + 1), dict(n_k=MAX), dict(sinks=-2),
+    dict(scale=0.0), dict(scale=nan), dict(scale=3e38), dict(out_token_stride=192), dict(out_head_stride=32),
 ] + [{f: s} for f in ("q_token_stride", "k_head_stride", "v_token_stride", "out_token_stride") for s in STRIDES])
 def test_seq_refusals(rules, bad):
     assert rules.seq_check(C.byref(seq(**bad))) < 0
@@ -181,3 +184,56 @@ def test_pairs_of_an_axis(rules, kw):
 def test_tokens_of_a_workgroup(rules, tokens, pairs, tile):
     """The table of angles holds them, and the GPU is filled first."""
     assert rules.tile(tokens, pairs) == tile and tile * -(-pairs // 8) * 8 <= 1024
+
+
+@pytest.mark.parametrize("kw,many,tiles,waves,splits", [
+    (dict(n_heads=2), 0, 1, 4, 1), (dict(n_heads=4), 0, 1, 4, 1), (dict(n_heads=6), 1, 1, 4, 1),  # 1, 2, 3 heads a key head
+    (dict(n_heads=34), 1, 2, 4, 1),                                                   # 17
+    (dict(max_len=33), 0, 1, 4, 1), (dict(max_len=32), 0, 1, 1, 1),
+    (dict(max_len=0), 0, 1, 4, 1), (dict(max_len=10 ** 6, left=30), 0, 1, 1, 1),      # the table's 64 | the window's 31 keys
+    (dict(max_len=1023), 0, 1, 4, 1), (dict(max_len=1024), 0, 1, 4, 16),              # 32 channels: worth a second launch
+    (dict(max_len=2000, left=800, sinks=9), 0, 1, 4, 1), (dict(max_len=16000), 0, 1, 4, 63), (dict(max_len=10 ** 6), 0, 1, 4, 64),
+])
+def test_paged_plan(rules, kw, many, tiles, waves, splits):
+    out = (C.c_longlong * 6)()
+    p = paged(out_seq_stride=2048, **kw)
+    rules.paged(C.byref(p), out)
+    assert list(out)[:4] == [many, tiles, waves, splits]
+    items = 3 * 2 * tiles
+    assert out[4] == (-(-items // 4) if waves == 1 else items * splits)
+    assert out[5] == (0 if splits == 1 else 3 * p.n_heads * splits * 34 * 4) == P.lib().prism_paged_attn_workspace(C.byref(p))
+
+
+@pytest.mark.parametrize("seqs,kv,max_len,waves,splits", [
+    (24, 8, 20001, 4, 10), (1, 8, 131075, 4, 64), (8160, 8, 75, 1, 1), (128, 8, 128, 1, 1), (128, 8, 129, 4, 1), (127, 8, 128, 4, 1),
+    (16, 8, 500, 4, 4), (16, 8, 16000, 4, 15), (200, 8, 100000, 4, 1),
+])
+def test_paged_plan_of_many(rules, seqs, kv, max_len, waves, splits):
+    out = (C.c_longlong * 6)()
+    rules.paged(C.byref(paged(cache=cache(n_seqs=seqs, n_kv_heads=kv, head_dim=128), n_heads=kv, max_len=max_len)), out)
+    assert (out[2], out[3]) == (waves, splits)
+
+
+@pytest.mark.parametrize("heads,kv,side", [(8, 8, 1), (32, 8, 4), (15, 5, 3), (32, 1, 32), (33, 1, 1), (4096, 1, 1)])
+def test_seq_rows_of_a_workgroup(rules, heads, kv, side):
+    assert rules.tile_heads(heads, kv) == side and heads % side == 0
+
+
+def test_seq_tiles_suffice(rules):
+    """A sequence's tiles start at floor(start / tile) + its number: enough for its rows before the next one's."""
+    rng = np.random.default_rng(0)
+    for tile in (4, 42, 128):
+        cu = np.concatenate([[rng.integers(0, 300)], rng.integers(0, 400, 50)]).cumsum()
+        first = cu[:-1] // tile + np.arange(50)
+        need = -(-np.diff(cu) // tile)
+        assert (first[:-1] + need[:-1] <= first[1:]).all()
+        assert first[-1] + need[-1] <= rules.seq_tiles(int(cu[-1]), 50, tile)
+
+
+def test_seq_waves(rules):
+    assert [rules.seq_w8(n) for n in (1, 1024, 1025, 10 ** 6)] == [1, 1, 0, 0]
+
+
+def test_launches_fit_32_bits(rules):
+    assert [rules.grid_ok(n, 256) for n in (1, 2 ** 24 - 1, 2 ** 24, 2 ** 40)] == [1, 1, 0, 0]
+    assert [rules.grid_ok(n, 512) for n in (2 ** 23 - 1, 2 ** 23)] == [1, 0]
