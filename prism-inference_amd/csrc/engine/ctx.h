@@ -97,7 +97,7 @@ struct prism_ctx {
     hipFunction_t f_append = nullptr;
     hipFunction_t f_paged[2][4][3] = {};  /* [dtype][head_dim 16, 32, 64, 128][1, 2, more heads a key head] */
     hipFunction_t f_paged_join[2][4] = {};
-    hipFunction_t f_seq[2][4][2] = {};    /* [dtype][head_dim][4 waves, 8 waves] */
+    hipFunction_t f_seq[2][4][3] = {};    /* [dtype][head_dim][4 waves, 8 waves, 8 waves of half as many rows] */
     std::string err;
 
     bool loaded = false;

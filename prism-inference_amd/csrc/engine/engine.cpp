@@ -134,8 +134,8 @@ extern "C" int prism_create(prism_ctx** out, int32_t device, const char* code_ob
             for (int g = 0; g < 3; ++g)
                 all.emplace_back(&c->f_paged[t][i][g], "prism_paged_attn_" + shape + (g == 0 ? "_g1" : g == 1 ? "_g2" : "_many"));
             all.emplace_back(&c->f_paged_join[t][i], "prism_paged_attn_join_" + shape);
-            for (int w8 = 0; w8 < 2; ++w8)
-                all.emplace_back(&c->f_seq[t][i][w8], "prism_seq_attn_" + shape + (w8 ? "_w8" : ""));
+            for (int w = 0; w < (i < 3 ? 3 : 2); ++w)
+                all.emplace_back(&c->f_seq[t][i][w], "prism_seq_attn_" + shape + (w == 0 ? "" : w == 1 ? "_w8" : "_narrow"));
         }
     }
     for (auto& f : all) {

@@ -201,15 +201,42 @@ inline int seq_tile_heads(int n_heads, int n_kv_heads) {
 /* Tiles of tile_q queries: enough for any lengths (seq_attn.hpp's seq_of_tile). */
 inline int64_t seq_tiles(int64_t n_q, int64_t n_seqs, int tile_q) { return n_q / tile_q + n_seqs; }
 
-/* 8 waves, of which two share each 32 queries' keys, while the workgroups are no
- * more than four per CU: then waves are what a SIMD lacks to hide the latency of
- * scores, maximum and weights, which follow each other. 4 and 8 waves, sequences that see
- * all keys, 8 heads unless said: 500 queries x 64 channels (32 workgroups) 13.4 and 11.9 us,
- * 2,000 x 32 (128) 27.5 and 24.2, 8,160 x 32, 4 heads (256) 100 and 80, 4,000 x
- * 64, 16 heads (512) 85 and 57, 4,000 x 128, 32 heads (1,024) 169 and 164; 60 of 100 to
- * 600 queries x 32 (1,792) 28 and 36; 2 of 5,000 x 128, 32 heads, window 2,047 (2,624) 409
- * and 455. */
-inline bool seq_w8(int64_t grid) { return grid <= 4 * 256; }
+/* How a sequence attention is launched. The workgroup: 128 rows by 4 waves; by 8, of which
+ * two share each 32 rows' keys; or 64 rows by 8, of which four do.
+ *
+ * 8 waves while the workgroups are no more than four per CU: then waves are what a
+ * SIMD lacks to hide the latency of scores, maximum and weights, which follow each
+ * other. 4 and 8 waves, sequences that see all keys, 8 heads unless said: 500
+ * queries x 64 channels (32 workgroups) 13.4 and 11.9 us, 2,000 x 32 (128) 27.5 and 24.2,
+ * 8,160 x 32, 4 heads (256) 100 and 80, 4,000 x 64, 16 heads (512) 85 and 57, 4,000
+ * x 128, 32 heads (1,024) 169 and 164; 60 of 100 to 600 queries x 32 (1,792) 28 and
+ * 36.
+ *
+ * 64 rows while the workgroups of 128 are no more than one per CU, so that the launch lasts as long as one of them, and
+ * sequences are long enough for four waves' keys. 128 and 64 rows, 2,000 queries, 8 heads (128 workgroups) x 16 channels 21.6 and 15.1 us, x 32 23.8 and 15.7, x 64 26.8 and
+ * 19.0; 16 heads (256) 21.7 and 17.5, 24.3 and 18.9, 27.4 and 25.9; 32 heads (512) 25.4 and 27.5, 26.5 and 28.6, 33 and
+ * 49; 8 heads, window 100 8.7 and 8.6, 8.7 and 8.0, 10.0 and 9.2; 60 sequences of 32, 2 groups of 4 heads (240) 7.3 and 8.9, 7.5
+ * and 9.1, 8.0 and 14.8. 128 channels have no LDS for it. */
+enum { SEQ_FOUR = 0, SEQ_EIGHT = 1, SEQ_NARROW = 2 };
+struct SeqPlan {
+    int kind;
+    int tile_heads, tile_q; /* of a workgroup */
+    int64_t grid;
+};
+inline SeqPlan seq_plan(const prism_seq_attn_push& p) {
+    SeqPlan r;
+    r.tile_heads = seq_tile_heads(p.n_heads, p.n_kv_heads);
+    const int64_t groups = p.n_heads / r.tile_heads;
+    r.tile_q = SEQ_ROWS / r.tile_heads;
+    r.grid = seq_tiles(p.n_q, p.n_seqs, r.tile_q) * groups;
+    const bool narrow = r.grid <= 256 && p.n_k >= (int64_t)128 * p.n_seqs && p.head_dim <= 64;
+    r.kind = r.grid > 4 * 256 ? SEQ_FOUR : narrow ? SEQ_NARROW : SEQ_EIGHT;
+    if (r.kind == SEQ_NARROW) {
+        r.tile_q = SEQ_NARROW_ROWS / r.tile_heads;
+        r.grid = seq_tiles(p.n_q, p.n_seqs, r.tile_q) * groups;
+    }
+    return r;
+}
 
 }  // namespace prism
 

@@ -221,9 +221,9 @@ extern "C" int prism_seq_attn(prism_ctx* c, const prism_seq_attn_push* p, const 
     a.right = p->right;
     a.sinks = p->sinks;
     a.scale_log2 = seq_scale_log2(p->scale);
-    a.tile_heads = seq_tile_heads(p->n_heads, p->n_kv_heads);
-    a.tile_q = SEQ_ROWS / a.tile_heads;
-    const int64_t grid = seq_tiles(p->n_q, p->n_seqs, a.tile_q) * (p->n_heads / a.tile_heads);
-    const bool w8 = seq_w8(grid);
-    return launch(c, c->f_seq[p->dtype][hd_index(p->head_dim)][w8], "sequence attention", grid, w8 ? 512 : 256, &a, stream);
+    const SeqPlan plan = seq_plan(*p);
+    a.tile_heads = plan.tile_heads;
+    a.tile_q = plan.tile_q;
+    return launch(c, c->f_seq[p->dtype][hd_index(p->head_dim)][plan.kind], "sequence attention", plan.grid,
+                  plan.kind == SEQ_FOUR ? 256 : 512, &a, stream);
 }

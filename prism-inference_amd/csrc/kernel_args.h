@@ -213,7 +213,8 @@ typedef struct PagedAttnArgs {
     float* ws;              /* splits > 1: [n_seqs][n_heads][splits][head_dim + 2] */
 } PagedAttnArgs;
 
-#define SEQ_ROWS 128 /* queries x heads per workgroup of a sequence attention */
+#define SEQ_ROWS 128 /* queries x heads per workgroup of a sequence attention, */
+#define SEQ_NARROW_ROWS 64 /* and of one with few workgroups */
 typedef struct SeqAttnArgs {
     const uint16_t* q;
     const uint16_t* k;
@@ -226,7 +227,7 @@ typedef struct SeqAttnArgs {
     int32_t n_seqs, n_q, n_k, n_heads, n_kv_heads;
     int32_t left, right, sinks;
     float scale_log2;       /* scale * log2(e) */
-    int32_t tile_heads, tile_q; /* of a workgroup's rows; tile_heads * tile_q <= SEQ_ROWS */
+    int32_t tile_heads, tile_q; /* of a workgroup's rows; tile_heads * tile_q <= SEQ_ROWS, or SEQ_NARROW_ROWS */
 } SeqAttnArgs;
 
 #endif

@@ -3,10 +3,11 @@
  * sinks: query i of a sequence of nq queries and nk keys stands at position
  * p = nk - nq + i and sees keys j <= p + right with j >= p - left or j < sinks.
  *
- * A workgroup takes 128 rows, 32 a wave: a row is a query of one head, the heads
+ * A workgroup takes 128 or 64 rows, 32 a wave: a row is a query of one head, the heads
  * that share a key head side by side (so the workgroup's queries are fewer, and the keys that they see
- * together too). It goes once over the keys that any of them sees, in tiles of 128
- * (64 with more than 32 channels and 4 waves), with a running maximum and sum:
+ * together too). It goes once over the keys that any of them sees, in tiles of 64,
+ * 128 or 256, with a running maximum and sum; with few workgroups, 2 or 4 waves
+ * take the same rows, each some keys of every tile, and are joined at the end:
  *   S^T = K Q^T           (32x32x16 MFMA: a lane holds one query's scores)
  *   P^T = 2^(c S^T - c m) (registers; c = scale log2 e)
  *   O^T += V^T P^T        (P^T is the B operand as it lies: the MFMA's
@@ -118,12 +119,12 @@ __device__ __forceinline__ SeqTile seq_of_tile(const SeqAttnArgs& a, int b) {
     }
 }
 
-/* KW: wave groups that share a workgroup's queries, each taking its keys of every tile. */
-template <class T, int HD, int KW>
+/* RW: waves, 32 rows each; KW: groups of them, which share the rows, each taking its keys of every tile. */
+template <class T, int HD, int RW, int KW>
 __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
     typedef typename T::v8 v8;
     constexpr int NP = HD <= 32 && KW == 1 ? 4 : 2; /* parts of 32 keys that a wave has of a tile */
-    constexpr int NTHR = 256 * KW, BN = 32 * NP * KW; /* threads; keys per tile */
+    constexpr int NTHR = 64 * RW * KW, BN = 32 * NP * KW; /* threads; keys per tile */
     constexpr int KS = HD / 16;              /* k-steps of the scores          */
     constexpr int DT = (HD + 31) / 32;       /* 32-channel tiles of the output */
     constexpr bool ONES = HD == 16 || (HD <= 64 && KW == 1); /* sums of weights on the matrix cores, see below */
@@ -132,7 +133,7 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
     constexpr int CPR = HD / 8;              /* 16-byte chunks of a row        */
     constexpr int CHUNKS = BN * CPR, CH = (CHUNKS + NTHR - 1) / NTHR; /* per tile, per thread */
     constexpr int TILE = 2 * BN * HD;        /* bytes of a tile of K or V      */
-    constexpr int KRING = (NP == 2 ? 2 : 3) * TILE, KVBYTES = KRING + 2 * TILE, MERGE = KW > 1 ? 4 * 64 * (16 * DT + 2) * 4 : 0;
+    constexpr int KRING = (NP == 2 ? 2 : 3) * TILE, KVBYTES = KRING + 2 * TILE, MERGE = (KW - 1) * RW * 64 * (16 * DT + 2) * 4;
     __shared__ __attribute__((aligned(16))) uint8_t lds[KVBYTES > MERGE ? KVBYTES : MERGE]; /* a ring of K tiles, two V tiles */
     const auto uni = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
 
@@ -161,7 +162,7 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
     const int q0 = (tile - first) * a.tile_q, q1 = min(q0 + a.tile_q, nq);
 
     const int lane = lane_id(), c32 = lane & 31, g = lane >> 5;
-    const int wave8 = uni(threadIdx.x >> 6), wave = wave8 & 3, half = wave8 >> 2;
+    const int wave8 = uni(threadIdx.x >> 6), wave = wave8 % RW, kgroup = wave8 / RW;
     const int row = 32 * wave + c32; /* this lane's; the wave's queries: qa .. qb - 1 */
     const int qa = q0 + 32 * wave / a.tile_heads, qb = min(q0 + (32 * wave + 31) / a.tile_heads + 1, q1);
     const int shift = nk - nq;                            /* position - row */
@@ -254,8 +255,8 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
         v8 v;
     };
     /* this lane's places (bytes from the rings on), to be xored with 32 per k-step and 64 per 32 channels */
-    const int krow = 2 * (32 * NP * half + c32) * HD + 16 * (g ^ swizzle_k(c32));
-    const int vrow = 2 * (32 * NP * half + 4 * g + (lane & 15) / 4) * HD +
+    const int krow = 2 * (32 * NP * kgroup + c32) * HD + 16 * (g ^ swizzle_k(c32));
+    const int vrow = 2 * (32 * NP * kgroup + 4 * g + (lane & 15) / 4) * HD +
                      ((HD >= 32 ? 2 * (lane & 16) : 0) ^ 16 * swizzle_v((lane & 15) / 4)) + 8 * (lane & 3);
     int kat[KS], vat[DT];
 #pragma unroll
@@ -367,7 +368,7 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
     fetch(KRING, vb, vs_, voff, 0, k0);
     f16v s0 = {}, s1 = {};
     unsigned p0[8] = {}, p1[8] = {};
-    int last = 0, now0 = active(0, k0 + 32 * NP * half);
+    int last = 0, now0 = active(0, k0 + 32 * NP * kgroup);
     if (now0) {
 #pragma unroll
         for (int j = 0; j < KS; ++j) s0 = mfma_32x32x16(read_k(0, j), qf[j], s0);
@@ -375,9 +376,9 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
     /* Tile t's V and tile t + 1's K have come to LDS at the barrier behind the tile's first body; the next V and
        the K after that go where the body before the barrier read last, or nobody for a tile. */
     auto pass = [&](int t, auto kbuf, auto knext, auto kfree, auto vbuf, auto vother) { /* places in the rings */
-        const int at = k0 + 32 * NP * half;
+        const int at = k0 + 32 * NP * kgroup;
         int now1 = active(t, at + 32);
-        const int next0 = active(t + 1, k1 + 32 * NP * half);
+        const int next0 = active(t + 1, k1 + 32 * NP * kgroup);
         if (last | now0 | now1) {
             body(t, at, kbuf + 64 * HD, vother + (NP - 1) * 64 * HD, s0, s1, p0, p1);
         } else {
@@ -437,7 +438,7 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
     }
 
     if (__syncthreads_or((bad & 0x80008000u) != 0)) {
-        for (int r = 32 * wave + half; r < 32 * wave + 32; r += KW) {
+        for (int r = 32 * wave + kgroup; r < 32 * wave + 32; r += KW) {
             const int i = q0 + r / a.tile_heads, head = hg * a.tile_heads + r % a.tile_heads;
             if (i >= q1) break;
             seq_attn_row<T, HD>(a, a.q + (rq.start + i) * a.q_token_stride + head * a.q_head_stride, kb, vb,
@@ -453,25 +454,33 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
         lanes_x32(l, x, y);
         l = x + y;
     }
-    if constexpr (KW > 1) { /* the other group's result through LDS (everyone is done with the tiles) */
+    if constexpr (KW > 1) { /* the other groups' results through LDS (everyone is done with the tiles) */
+        constexpr int ST = 64 * RW, PART = (16 * DT + 2) * ST;
         float* red = reinterpret_cast<float*>(lds) + (wave * 64 + lane);
-        if (half == 1) {
+        if (kgroup > 0) {
+            float* mine = red + (kgroup - 1) * PART;
 #pragma unroll
             for (int d = 0; d < DT; ++d)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) red[(16 * d + e) * 256] = o[d][e];
-            red[16 * DT * 256] = m == -INFINITY ? m : mc;
-            red[(16 * DT + 1) * 256] = l;
+                for (int e = 0; e < 16; ++e) mine[(16 * d + e) * ST] = o[d][e];
+            mine[16 * DT * ST] = m == -INFINITY ? m : mc;
+            mine[(16 * DT + 1) * ST] = l;
         }
         __syncthreads();
-        if (half == 1) return;
-        const float m0 = m == -INFINITY ? m : mc, m1 = red[16 * DT * 256], top = vmax(m0, m1);
-        const float f0 = m0 == -INFINITY ? 0.f : fast_exp2(m0 - top), f1 = m1 == -INFINITY ? 0.f : fast_exp2(m1 - top);
-        l = l * f0 + red[(16 * DT + 1) * 256] * f1;
+        if (kgroup > 0) return;
+        float m0 = m == -INFINITY ? m : mc;
 #pragma unroll
-        for (int d = 0; d < DT; ++d)
+        for (int k = 0; k < KW - 1; ++k) {
+            const float* other = red + k * PART;
+            const float m1 = other[16 * DT * ST], top = vmax(m0, m1);
+            const float f0 = m0 == -INFINITY ? 0.f : fast_exp2(m0 - top), f1 = m1 == -INFINITY ? 0.f : fast_exp2(m1 - top);
+            l = l * f0 + other[(16 * DT + 1) * ST] * f1;
 #pragma unroll
-            for (int e = 0; e < 16; ++e) o[d][e] = o[d][e] * f0 + red[(16 * d + e) * 256] * f1;
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[d][e] = o[d][e] * f0 + other[(16 * d + e) * ST] * f1;
+            m0 = top;
+        }
     }
     const bool store = qrow < q1;
     const float inv = l == 0.f ? 0.f : 1.0f / l;
@@ -499,11 +508,16 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
         }
 }
 
-/* W4, W8: waves per SIMD that the registers have to allow. 8 waves with up to 32 channels: two workgroups per CU
+/* Which of them: seq_rules.h's seq_plan. W4, W8: waves per SIMD that the registers have to allow. 8 waves with up to 32 channels: two workgroups per CU
  * (8,160 queries, 8 heads x 32: 30 us; one, 36). */
-#define SEQ_ATTN(NAME, T, HD, W4, W8)                                                                                                 \
-    extern "C" __global__ void __launch_bounds__(256, W4) prism_seq_attn_##NAME##_h##HD(SeqAttnArgs a) { seq_attn_body<T, HD, 1>(a); } \
-    extern "C" __global__ void __launch_bounds__(512, W8) prism_seq_attn_##NAME##_h##HD##_w8(SeqAttnArgs a) { seq_attn_body<T, HD, 2>(a); }
+#define SEQ_ATTN(NAME, T, HD, W4, W8)                                                                                                    \
+    extern "C" __global__ void __launch_bounds__(256, W4) prism_seq_attn_##NAME##_h##HD(SeqAttnArgs a) { seq_attn_body<T, HD, 4, 1>(a); } \
+    extern "C" __global__ void __launch_bounds__(512, W8) prism_seq_attn_##NAME##_h##HD##_w8(SeqAttnArgs a) { seq_attn_body<T, HD, 4, 2>(a); }
+#define SEQ_ATTN_NARROW(NAME, T, HD, W8) \
+    extern "C" __global__ void __launch_bounds__(512, W8) prism_seq_attn_##NAME##_h##HD##_narrow(SeqAttnArgs a) { seq_attn_body<T, HD, 2, 4>(a); }
 SEQ_ATTN(f16, F16, 16, 4, 4) SEQ_ATTN(f16, F16, 32, 3, 4) SEQ_ATTN(f16, F16, 64, 3, 2) SEQ_ATTN(f16, F16, 128, 2, 2)
 SEQ_ATTN(bf16, BF16, 16, 4, 4) SEQ_ATTN(bf16, BF16, 32, 3, 4) SEQ_ATTN(bf16, BF16, 64, 3, 2) SEQ_ATTN(bf16, BF16, 128, 2, 2)
+SEQ_ATTN_NARROW(f16, F16, 16, 4) SEQ_ATTN_NARROW(f16, F16, 32, 4) SEQ_ATTN_NARROW(f16, F16, 64, 2)
+SEQ_ATTN_NARROW(bf16, BF16, 16, 4) SEQ_ATTN_NARROW(bf16, BF16, 32, 4) SEQ_ATTN_NARROW(bf16, BF16, 64, 2)
 #undef SEQ_ATTN
+#undef SEQ_ATTN_NARROW

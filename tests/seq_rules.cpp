@@ -24,7 +24,13 @@ void paged(const prism_paged_attn_push* p, long long* out) {
 int tile_heads(int n_heads, int n_kv_heads) { return seq_tile_heads(n_heads, n_kv_heads); }
 long long seq_tiles(long long n_q, long long n_seqs, int tile_q) { return prism::seq_tiles(n_q, n_seqs, tile_q); }
 int grid_ok(long long grid, int threads) { return seq_grid_ok(grid, threads); }
-int seq_w8(long long grid) { return prism::seq_w8(grid); }
+void seq(const prism_seq_attn_push* p, long long* out) {
+    const SeqPlan r = seq_plan(*p);
+    out[0] = r.kind;
+    out[1] = r.tile_heads;
+    out[2] = r.tile_q;
+    out[3] = r.grid;
+}
 void keys(int32_t p, int32_t n, int32_t left, int32_t right, int32_t sinks, int32_t* out) {
     const KeyRange r = key_range(p, n, left, right, sinks);
     out[0] = r.sink;

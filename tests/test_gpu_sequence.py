@@ -340,10 +340,17 @@ def test_paged_offsets_past_32_bits(hip, engine, dev, device_arena):
 
 # ---------------------------------------------------------------- sequences
 
-def check_seq(engine, dev, rng, dtype, hd, kv, group, lens, left, right, sinks, layout="dense", head=0, tail=3, big=1.0, waves=8):
-    """lens: (queries, keys) of each sequence; head, tail: rows before the first and behind the last; waves of a
-    workgroup: 4 where there are more than 1,024 workgroups (here of empty sequences)."""
-    lens = lens + [(0, 0)] * (1100 if waves == 4 else 0)
+def spare(fill, heads=1):
+    """Empty sequences that make up to 256, 1,024 or more workgroups of 128 rows."""
+    return {"few": 0, "some": -(-257 // heads), "many": 1025}[fill]
+
+
+def check_seq(engine, dev, rng, dtype, hd, kv, group, lens, left, right, sinks, layout="dense", head=0, tail=3, big=1.0, fill="some"):
+    """lens: (queries, keys) of each sequence; head, tail: rows before the first and behind the last; fill: how many
+    workgroups there are (empty sequences' as well) or, for the kernel for few of them, keys a sequence."""
+    lens = lens + [(0, 0)] * spare(fill, kv if group <= 32 else kv * group)
+    if fill == "few" and layout == "dense":
+        lens = lens + [(3, 257 * len(lens) + 259)]
     heads, scale = kv * group, 1 / math.sqrt(hd)
     cq = (head + np.concatenate([[0], np.cumsum([a for a, _ in lens])])).astype(np.int32)
     ck = (head + np.concatenate([[0], np.cumsum([b for _, b in lens])])).astype(np.int32)
@@ -374,7 +381,7 @@ def check_seq(engine, dev, rng, dtype, hd, kv, group, lens, left, right, sinks, 
              "out_token_stride", "out_head_stride")
     push = P.SeqAttnPush(dtype=TYPES[dtype], n_seqs=len(lens), n_q=nq, n_k=nk, n_heads=heads, n_kv_heads=kv, head_dim=hd,
                          left=left, right=right, sinks=sinks, scale=scale, **dict(zip(names, st)))
-    print(f"[seq] {dtype} {heads}/{kv} x {hd} {lens[:12]} waves {waves} left {left} right {right} sinks {sinks} {layout}", flush=True)
+    print(f"[seq] {dtype} {heads}/{kv} x {hd} {lens[:12]} fill {fill} left {left} right {right} sinks {sinks} {layout}", flush=True)
     engine.seq_attn(push, dq, dk, dv, dev.put(cq), dev.put(ck), out)
     got = dev.get(out, (heads, nq, hd)).transpose(1, 0, 2) if layout == "heads" else dev.get(out, (nq, heads, hd))
     assert (got[:head] == NAN[dtype]).all() and (got[nq - tail:] == NAN[dtype]).all()
@@ -389,16 +396,16 @@ def check_seq(engine, dev, rng, dtype, hd, kv, group, lens, left, right, sinks, 
                 assert not msg, (s, i, h, msg)
 
 
-WAVES = pytest.mark.parametrize("waves", [8, 4])
+FILL = pytest.mark.parametrize("fill", ["few", "some", "many"])
 RAGGED = [(1, 1), (0, 0), (5, 5), (64, 64), (65, 65), (0, 7), (31, 31), (130, 130), (3, 0)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("hd", [16, 32, 64, 128])
 @pytest.mark.parametrize("kv,group", [(2, 1), (1, 3)])
-@WAVES
-def test_seq_shapes(engine, dev, dtype, hd, kv, group, waves):
-    check_seq(engine, dev, np.random.default_rng(hd), dtype, hd, kv, group, RAGGED, -1, 0, 0, waves=waves)
+@FILL
+def test_seq_shapes(engine, dev, dtype, hd, kv, group, fill):
+    check_seq(engine, dev, np.random.default_rng(hd), dtype, hd, kv, group, RAGGED, -1, 0, 0, fill=fill)
 
 
 @pytest.mark.parametrize("left,right,sinks", [
@@ -406,11 +413,11 @@ def test_seq_shapes(engine, dev, dtype, hd, kv, group, waves):
     (MAX, MAX, MAX), (3, -1, 0),
 ])
 @pytest.mark.parametrize("hd", [32, 128])
-@WAVES
-def test_seq_windows(engine, dev, left, right, sinks, hd, waves):
+@FILL
+def test_seq_windows(engine, dev, left, right, sinks, hd, fill):
     rng = np.random.default_rng(abs(left) % 97 + right % 89 + sinks % 83)
     check_seq(engine, dev, rng, "fp16", hd, 1, 2, [(150, 150), (1, 1), (33, 90), (70, 20), (200, 200)], left, right, sinks,
-              waves=waves)
+              fill=fill)
 
 
 @pytest.mark.parametrize("layout", ["fused", "heads"])
@@ -424,26 +431,26 @@ def test_seq_layouts(engine, dev, layout, hd):
     ("fp16", 32, [(600, 600)], 128, 20), ("bf16", 128, [(300, 900), (257, 257)], 200, 4), ("fp16", 64, [(1, 2000), (4, 700)], 511, 1),
     ("bf16", 16, [(513, 513)], -1, 0),
 ])
-@WAVES
-def test_seq_long(engine, dev, dtype, hd, lens, left, sinks, waves):
-    check_seq(engine, dev, np.random.default_rng(1), dtype, hd, 1, 2, lens, left, 0, sinks, waves=waves)
+@FILL
+def test_seq_long(engine, dev, dtype, hd, lens, left, sinks, fill):
+    check_seq(engine, dev, np.random.default_rng(1), dtype, hd, 1, 2, lens, left, 0, sinks, fill=fill)
 
 
 @pytest.mark.parametrize("hd,kv,group", [(16, 1, 32), (32, 1, 33), (64, 3, 5), (32, 2, 8), (128, 1, 16), (16, 8, 2)])
-@WAVES
-def test_seq_shared_heads(engine, dev, hd, kv, group, waves):
+@FILL
+def test_seq_shared_heads(engine, dev, hd, kv, group, fill):
     """Groups that fill a workgroup's rows evenly or not, with a few queries, or not at all."""
     rng = np.random.default_rng(group)
-    check_seq(engine, dev, rng, "bf16", hd, kv, group, [(9, 20), (1, 1), (0, 3), (37, 37), (5, 2)], 12, 0, 2, waves=waves)
+    check_seq(engine, dev, rng, "bf16", hd, kv, group, [(9, 20), (1, 1), (0, 3), (37, 37), (5, 2)], 12, 0, 2, fill=fill)
 
 
-@WAVES
-def test_seq_sharp_scores(engine, dev, waves):
-    check_seq(engine, dev, np.random.default_rng(2), "fp16", 64, 1, 1, [(300, 300)], 100, 0, 3, big=60.0, waves=waves)
+@FILL
+def test_seq_sharp_scores(engine, dev, fill):
+    check_seq(engine, dev, np.random.default_rng(2), "fp16", 64, 1, 1, [(300, 300)], 100, 0, 3, big=60.0, fill=fill)
 
 
-@WAVES
-def test_seq_rising_scores(engine, dev, waves):
+@FILL
+def test_seq_rising_scores(engine, dev, fill):
     """The largest score comes last, tile after tile: the running maximum moves every time."""
     rng = np.random.default_rng(4)
     dtype, hd, n = "bf16", 32, 400
@@ -453,7 +460,7 @@ def test_seq_rising_scores(engine, dev, waves):
     q[..., 0] = np.where(np.arange(n) % 2, 4.0, -4.0)[:, None]
     q, k, v = to_bits(q, dtype), to_bits(k, dtype), normal(rng, (n, 1, hd), dtype)
     out = dev.put(np.full((n, 1, hd), NAN[dtype], np.uint16))
-    seqs = 1 if waves == 8 else 1100  # one sequence and empty ones, or no starts at all
+    seqs = 1 + spare(fill)  # one sequence and empty ones, or no starts at all
     cu = dev.put(np.array([0] + [n] * seqs, np.int32)) if seqs > 1 else None
     push = P.SeqAttnPush(dtype=P.BF16, n_seqs=seqs, n_q=n, n_k=n, n_heads=1, n_kv_heads=1, head_dim=hd, left=-1, right=0, sinks=0,
                          scale=1.0, q_token_stride=hd, q_head_stride=hd, k_token_stride=hd, k_head_stride=hd, v_token_stride=hd,
@@ -469,8 +476,8 @@ def test_seq_rising_scores(engine, dev, waves):
 @pytest.mark.parametrize("dtype,hd", [("fp16", 16), ("bf16", 32), ("fp16", 64), ("bf16", 128)])
 @pytest.mark.parametrize("what", ["v nan", "v inf", "k nan"])
 @pytest.mark.parametrize("group", [1, 3])
-@WAVES
-def test_seq_bad_values_reach_only_who_sees_them(engine, dev, dtype, hd, what, group, waves):
+@FILL
+def test_seq_bad_values_reach_only_who_sees_them(engine, dev, dtype, hd, what, group, fill):
     """One key's value is NaN or infinite: the queries that see it get what the formula gives, the others what they
     would get without it."""
     rng = np.random.default_rng(hd)
@@ -484,8 +491,9 @@ def test_seq_bad_values_reach_only_who_sees_them(engine, dev, dtype, hd, what, g
     out = dev.put(np.full((n, group, hd), NAN[dtype], np.uint16))
     st = {f"{x}_{y}_stride": hd * (group if x in ("q", "out") and y == "token" else 1) for x in ("q", "k", "v", "out")
           for y in ("token", "head")}
-    cu = dev.put(np.array([0] + [n] * (1 if waves == 8 else 1100), np.int32))  # and empty sequences
-    engine.seq_attn(P.SeqAttnPush(dtype=TYPES[dtype], n_seqs=1 if waves == 8 else 1100, n_q=n, n_k=n, n_heads=group,
+    seqs = 1 + spare(fill)
+    cu = dev.put(np.array([0] + [n] * seqs, np.int32))
+    engine.seq_attn(P.SeqAttnPush(dtype=TYPES[dtype], n_seqs=seqs, n_q=n, n_k=n, n_heads=group,
                                   n_kv_heads=1, head_dim=hd, left=left, right=0, sinks=sinks, scale=0.1, **st), dev.put(q),
                     dev.put(k), dev.put(v), cu, cu, out)
     got_all = values(dev.get(out, (n, group, hd)), dtype)
@@ -536,8 +544,8 @@ def test_seq_starts_out_of_range(engine, dev):
 
 @pytest.mark.parametrize("stride", [0, 8])
 @pytest.mark.parametrize("hd", [16, 128])
-@WAVES
-def test_seq_rows_that_overlap(engine, dev, stride, hd, waves):
+@FILL
+def test_seq_rows_that_overlap(engine, dev, stride, hd, fill):
     """Keys and values repeated or overlapping, an infinite value among them: each channel meets it or does not."""
     rng = np.random.default_rng(hd + stride)
     dtype, n, sinks, left = "fp16", 300, 3, 40
@@ -545,7 +553,7 @@ def test_seq_rows_that_overlap(engine, dev, stride, hd, waves):
     flat[:hd:16] = to_bits(np.inf, dtype)
     q, k = normal(rng, (n, 1, hd), dtype), normal(rng, n * stride + hd, dtype)
     out = dev.put(np.full((n, hd), NAN[dtype], np.uint16))
-    seqs = 1 if waves == 8 else 1100
+    seqs = 1 + spare(fill)
     cu = dev.put(np.array([0] + [n] * seqs, np.int32))
     push = P.SeqAttnPush(dtype=P.F16, n_seqs=seqs, n_q=n, n_k=n, n_heads=1, n_kv_heads=1, head_dim=hd, left=left, right=0,
                          sinks=sinks, scale=0.1, q_token_stride=hd, q_head_stride=hd, k_token_stride=stride, k_head_stride=hd,
@@ -570,7 +578,7 @@ def test_seq_largest_key_stride(hip, engine, dev, device_arena):
     big = device_arena(((n - 1) * far + 2 * hd) * 2, zero=False)  # a row's keys, then its values
     for j in range(n):
         hip.upload(big.ptr + 2 * far * j, np.concatenate([k[j], v[j]]))
-    for seqs in (1, 1100):
+    for seqs in (1, 301, 1101):
         out = dev.put(np.full((n, hd), NAN[dtype], np.uint16))
         cu = dev.put(np.array([0] + [n] * seqs, np.int32))
         push = P.SeqAttnPush(dtype=P.BF16, n_seqs=seqs, n_q=n, n_k=n, n_heads=1, n_kv_heads=1, head_dim=hd, left=-1, right=0,

@@ -24,7 +24,7 @@ def rules(tmp_path_factory):
     lib.rows.argtypes = [C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p]
     lib.tile.argtypes = [C.c_longlong, C.c_int]
     lib.seq_tiles.argtypes, lib.seq_tiles.restype = [C.c_longlong, C.c_longlong, C.c_int], C.c_longlong
-    lib.seq_w8.argtypes, lib.grid_ok.argtypes = [C.c_longlong], [C.c_longlong, C.c_int]
+    lib.grid_ok.argtypes = [C.c_longlong, C.c_int]
     return lib
 
 
@@ -230,8 +230,18 @@ def test_seq_tiles_suffice(rules):
         assert first[-1] + need[-1] <= rules.seq_tiles(int(cu[-1]), 50, tile)
 
 
-def test_seq_waves(rules):
-    assert [rules.seq_w8(n) for n in (1, 1024, 1025, 10 ** 6)] == [1, 1, 0, 0]
+@pytest.mark.parametrize("kw,kind,side,tile,grid", [
+    (dict(n_seqs=1, n_q=1, n_k=128), 2, 2, 32, 2), (dict(n_seqs=1, n_q=1, n_k=127), 1, 2, 64, 2), (dict(n_k=256, head_dim=128, k_head_stride=128, out_head_stride=128, out_token_stride=512), 1, 2, 64, 4),
+    (dict(n_seqs=126, n_q=129, n_k=10 ** 6), 2, 2, 32, 260), (dict(n_seqs=127, n_q=129, n_k=10 ** 6), 1, 2, 64, 258),  # 256 | 258 workgroups of 128 rows
+    (dict(n_seqs=500, n_q=780), 1, 2, 64, 1024), (dict(n_seqs=500, n_q=832), 0, 2, 64, 1026),
+    (dict(n_heads=32, n_kv_heads=1, n_k=256, out_token_stride=2048), 2, 32, 2, 7), (dict(n_heads=33, n_kv_heads=1, n_k=256, out_token_stride=4096), 2, 1, 64, 66),
+])
+def test_seq_plan(rules, kw, kind, side, tile, grid):
+    out = (C.c_longlong * 4)()
+    p = seq(**kw)
+    assert rules.seq_check(C.byref(p)) == 0
+    rules.seq(C.byref(p), out)
+    assert list(out) == [kind, side, tile, grid]
 
 
 def test_launches_fit_32_bits(rules):
