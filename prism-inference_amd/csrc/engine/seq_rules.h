@@ -201,22 +201,27 @@ inline int seq_tile_heads(int n_heads, int n_kv_heads) {
 /* Tiles of tile_q queries: enough for any lengths (seq_attn.hpp's seq_of_tile). */
 inline int64_t seq_tiles(int64_t n_q, int64_t n_seqs, int tile_q) { return n_q / tile_q + n_seqs; }
 
-/* How a sequence attention is launched. The workgroup: 128 rows by 4 waves; by 8, of which
- * two share each 32 rows' keys; or 64 rows by 8, of which four do.
+/* How a sequence attention is launched. The workgroup: 128 rows by 4 waves (four); by 8, of which two share each 32
+ * rows' keys (eight); or 64 rows by 8, of which four do (narrow; 128 channels have no LDS for it).
  *
- * 8 waves while the workgroups are no more than four per CU: then waves are what a
- * SIMD lacks to hide the latency of scores, maximum and weights, which follow each
- * other. 4 and 8 waves, sequences that see all keys, 8 heads unless said: 500
- * queries x 64 channels (32 workgroups) 13.4 and 11.9 us, 2,000 x 32 (128) 27.5 and 24.2,
- * 8,160 x 32, 4 heads (256) 100 and 80, 4,000 x 64, 16 heads (512) 85 and 57, 4,000
- * x 128, 32 heads (1,024) 169 and 164; 60 of 100 to 600 queries x 32 (1,792) 28 and
- * 36.
- *
- * 64 rows while the workgroups of 128 are no more than one per CU, so that the launch lasts as long as one of them, and
- * sequences are long enough for four waves' keys. 128 and 64 rows, 2,000 queries, 8 heads (128 workgroups) x 16 channels 21.6 and 15.1 us, x 32 23.8 and 15.7, x 64 26.8 and
- * 19.0; 16 heads (256) 21.7 and 17.5, 24.3 and 18.9, 27.4 and 25.9; 32 heads (512) 25.4 and 27.5, 26.5 and 28.6, 33 and
- * 49; 8 heads, window 100 8.7 and 8.6, 8.7 and 8.0, 10.0 and 9.2; 60 sequences of 32, 2 groups of 4 heads (240) 7.3 and 8.9, 7.5
- * and 9.1, 8.0 and 14.8. 128 channels have no LDS for it. */
+ * More waves to a row shorten a workgroup; four's have the least LDS and registers, so the most of them run at once.
+ * By the number of workgroups of 128 rows (those with rows, about) and the keys a query can see. us of four, eight and
+ * narrow at 16 | 64 | 128 channels (32 go as 16 do), sequences that see all keys unless a window is named:
+ *   workgroups, keys
+ *   64, 130       8.2 7.8 7.9      | 8.2 8.8 8.8    | 9.5 10.7
+ *   64, 500       10.2 9.5 8.2     | 13.0 11.7 10.5 | 16.4 15.5
+ *   160, 2,500    31.5 25.9 17.3   | 41.7 31.7 22.3 | 52.8 41.6
+ *   240, 250      9.3 10.9 10.7    | 11.8 11.9 17.6 | 15.9 16.2
+ *   256, 1,000    16.7 15.0 15.2   | 21.3 17.7 23.4 | 28.4 24.0
+ *   240, window 1,000  18.6 16.1 17.7 | 24.4 20.3 28.3 | 30.3 26.7
+ *   320, 500      12.1 12.9 14.9   | 15.9 17.9 25.6 | 21.6 26.2
+ *   320, 2,500    32.3 28.2 24.3   | 42.4 32.4 39.7 | 57.1 44.3
+ *   320, window 1,000  21.3 21.7 22.8 | 27.1 33.8 39.0 | 36.8 49.2
+ *   504, 8,000    89.0 75.1 65.4   | 124 99 116     | 178 147
+ *   512, 1,000    19.7 19.0 24.4   | 25.9 31.4 41.2 | 34.9 44.4
+ *   756, 8,000    140 131 109      | 185 183 197    | 297 264
+ *   1,000, 8,000  110 108 122      | 166 191 232    | 279 288
+ *   1,024, 1,000  29.4 34.9 42.6   | 42.8 52.9 79.2 | 62.3 75.3 */
 enum { SEQ_FOUR = 0, SEQ_EIGHT = 1, SEQ_NARROW = 2 };
 struct SeqPlan {
     int kind;
@@ -226,15 +231,17 @@ struct SeqPlan {
 inline SeqPlan seq_plan(const prism_seq_attn_push& p) {
     SeqPlan r;
     r.tile_heads = seq_tile_heads(p.n_heads, p.n_kv_heads);
-    const int64_t groups = p.n_heads / r.tile_heads;
     r.tile_q = SEQ_ROWS / r.tile_heads;
+    const int64_t groups = p.n_heads / r.tile_heads, n_seqs = std::max(p.n_seqs, 1);
+    const int64_t work = std::max(n_seqs, p.n_q / r.tile_q + n_seqs / 2) * groups;
+    int64_t keys = p.n_k / n_seqs;
+    if (p.left >= 0 && p.right >= 0) keys = std::min(keys, (int64_t)p.left + p.right + 1 + p.sinks);
+    const bool long_keys = work <= 768 && keys >= std::max<int64_t>(384, 5 * work);
+    r.kind = SEQ_FOUR;
+    if (long_keys || (work <= 256 && keys >= 384)) r.kind = SEQ_EIGHT;
+    if ((long_keys && p.head_dim <= 32) || (work <= 160 && keys >= 192 && p.head_dim <= 64)) r.kind = SEQ_NARROW;
+    if (r.kind == SEQ_NARROW) r.tile_q = SEQ_NARROW_ROWS / r.tile_heads;
     r.grid = seq_tiles(p.n_q, p.n_seqs, r.tile_q) * groups;
-    const bool narrow = r.grid <= 256 && p.n_k >= (int64_t)128 * p.n_seqs && p.head_dim <= 64;
-    r.kind = r.grid > 4 * 256 ? SEQ_FOUR : narrow ? SEQ_NARROW : SEQ_EIGHT;
-    if (r.kind == SEQ_NARROW) {
-        r.tile_q = SEQ_NARROW_ROWS / r.tile_heads;
-        r.grid = seq_tiles(p.n_q, p.n_seqs, r.tile_q) * groups;
-    }
     return r;
 }
 

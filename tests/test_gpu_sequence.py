@@ -340,21 +340,22 @@ def test_paged_offsets_past_32_bits(hip, engine, dev, device_arena):
 
 # ---------------------------------------------------------------- sequences
 
-def spare(fill, heads=1):
-    """Empty sequences that make up to 256, 1,024 or more workgroups of 128 rows."""
-    return {"few": 0, "some": -(-257 // heads), "many": 1025}[fill]
+FILL = pytest.mark.parametrize("fill", ["few", "some", "many"])
 
 
-def check_seq(engine, dev, rng, dtype, hd, kv, group, lens, left, right, sinks, layout="dense", head=0, tail=3, big=1.0, fill="some"):
-    """lens: (queries, keys) of each sequence; head, tail: rows before the first and behind the last; fill: how many
-    workgroups there are (empty sequences' as well) or, for the kernel for few of them, keys a sequence."""
-    lens = lens + [(0, 0)] * spare(fill, kv if group <= 32 else kv * group)
-    if fill == "few" and layout == "dense":
-        lens = lens + [(3, 257 * len(lens) + 259)]
+def spare(fill, groups=1):
+    """What leads to the kernels for few, some and many workgroups: (empty sequences, key rows for each sequence)."""
+    return {None: (0, 0), "few": (0, 400), "some": (-(-165 // groups), 400), "many": (1025, 0)}[fill]
+
+
+def check_seq(engine, dev, rng, dtype, hd, kv, group, lens, left, right, sinks, layout="dense", head=0, tail=3, big=1.0, fill=None):
+    """lens: (queries, keys) of each sequence; head, tail: rows before the first and behind the last; fill: see spare."""
+    empty, rows = spare(fill, kv if group <= 32 else kv * group)
+    lens = lens + [(0, 0)] * empty
     heads, scale = kv * group, 1 / math.sqrt(hd)
     cq = (head + np.concatenate([[0], np.cumsum([a for a, _ in lens])])).astype(np.int32)
     ck = (head + np.concatenate([[0], np.cumsum([b for _, b in lens])])).astype(np.int32)
-    nq, nk = int(cq[-1]) + tail, int(ck[-1]) + tail
+    nq, nk = int(cq[-1]) + tail, max(int(ck[-1]) + tail, rows * len(lens))
     q, k, v = normal(rng, (nq, heads, hd), dtype), normal(rng, (nk, kv, hd), dtype), normal(rng, (nk, kv, hd), dtype)
     if big != 1.0:
         k = to_bits(values(k, dtype) * big, dtype)
@@ -396,7 +397,6 @@ def check_seq(engine, dev, rng, dtype, hd, kv, group, lens, left, right, sinks, 
                 assert not msg, (s, i, h, msg)
 
 
-FILL = pytest.mark.parametrize("fill", ["few", "some", "many"])
 RAGGED = [(1, 1), (0, 0), (5, 5), (64, 64), (65, 65), (0, 7), (31, 31), (130, 130), (3, 0)]
 
 
@@ -410,13 +410,13 @@ def test_seq_shapes(engine, dev, dtype, hd, kv, group, fill):
 
 @pytest.mark.parametrize("left,right,sinks", [
     (-1, -1, 0), (0, 0, 0), (0, 0, 3), (7, 0, 0), (40, 0, 5), (63, 0, 100), (20, 9, 2), (0, 30, 0), (-1, 5, 0), (200, -1, 1),
-    (MAX, MAX, MAX), (3, -1, 0),
+    (MAX, MAX, MAX), (3, -1, 0), (0, 0, 384), (63, 3, 400), (150, 250, 3), (384, 0, 2), (190, 1, 0),
 ])
 @pytest.mark.parametrize("hd", [32, 128])
 @FILL
 def test_seq_windows(engine, dev, left, right, sinks, hd, fill):
     rng = np.random.default_rng(abs(left) % 97 + right % 89 + sinks % 83)
-    check_seq(engine, dev, rng, "fp16", hd, 1, 2, [(150, 150), (1, 1), (33, 90), (70, 20), (200, 200)], left, right, sinks,
+    check_seq(engine, dev, rng, "fp16", hd, 1, 2, [(150, 450), (1, 1), (33, 600), (70, 20), (200, 200)], left, right, sinks,
               fill=fill)
 
 
@@ -458,17 +458,19 @@ def test_seq_rising_scores(engine, dev, fill):
     k[..., 0] = np.linspace(-60, 60, n)[:, None]
     q = np.zeros((n, 1, hd))
     q[..., 0] = np.where(np.arange(n) % 2, 4.0, -4.0)[:, None]
-    q, k, v = to_bits(q, dtype), to_bits(k, dtype), normal(rng, (n, 1, hd), dtype)
+    empty, rows = spare(fill)  # one sequence and empty ones, or no starts at all
+    seqs, nk = 1 + empty, max(n, rows * (1 + empty))
+    q, v = to_bits(q, dtype), normal(rng, (nk, 1, hd), dtype)
+    k = np.concatenate([to_bits(k, dtype), normal(rng, (nk - n, 1, hd), dtype)])
     out = dev.put(np.full((n, 1, hd), NAN[dtype], np.uint16))
-    seqs = 1 + spare(fill)  # one sequence and empty ones, or no starts at all
     cu = dev.put(np.array([0] + [n] * seqs, np.int32)) if seqs > 1 else None
-    push = P.SeqAttnPush(dtype=P.BF16, n_seqs=seqs, n_q=n, n_k=n, n_heads=1, n_kv_heads=1, head_dim=hd, left=-1, right=0, sinks=0,
+    push = P.SeqAttnPush(dtype=P.BF16, n_seqs=seqs, n_q=n, n_k=nk, n_heads=1, n_kv_heads=1, head_dim=hd, left=-1, right=0, sinks=0,
                          scale=1.0, q_token_stride=hd, q_head_stride=hd, k_token_stride=hd, k_head_stride=hd, v_token_stride=hd,
                          v_head_stride=hd, out_token_stride=hd, out_head_stride=hd)
     engine.seq_attn(push, dev.put(q), dev.put(k), dev.put(v), cu, cu, out)
     got = values(dev.get(out, (n, 1, hd)), dtype)
     for i in range(n):
-        want, bound = attention_row(values(q[i, 0], dtype), values(k[:, 0], dtype), values(v[:, 0], dtype),
+        want, bound = attention_row(values(q[i, 0], dtype), values(k[:n, 0], dtype), values(v[:n, 0], dtype),
                                     visible(i, n, -1, 0, 0), 1.0, dtype)
         assert not outside(got[i, 0], want, bound), i
 
@@ -481,8 +483,11 @@ def test_seq_bad_values_reach_only_who_sees_them(engine, dev, dtype, hd, what, g
     """One key's value is NaN or infinite: the queries that see it get what the formula gives, the others what they
     would get without it."""
     rng = np.random.default_rng(hd)
-    n, at, left, sinks = 300, 100, 40, 2
-    q, k, v = normal(rng, (n, group, hd), dtype), normal(rng, (n, 1, hd), dtype), normal(rng, (n, 1, hd), dtype)
+    left = {"few": 200, "some": 400, "many": 40}[fill]
+    empty, rows = spare(fill)
+    n, at, sinks, seqs = 220 + 2 * left, 100, 2, 1 + empty
+    nk = max(n, rows * seqs)
+    q, k, v = normal(rng, (n, group, hd), dtype), normal(rng, (nk, 1, hd), dtype), normal(rng, (nk, 1, hd), dtype)
     inf = 0x7C00 if dtype == "fp16" else 0x7F80
     if what == "k nan":
         k[at, 0, 3] = NAN[dtype]
@@ -491,13 +496,12 @@ def test_seq_bad_values_reach_only_who_sees_them(engine, dev, dtype, hd, what, g
     out = dev.put(np.full((n, group, hd), NAN[dtype], np.uint16))
     st = {f"{x}_{y}_stride": hd * (group if x in ("q", "out") and y == "token" else 1) for x in ("q", "k", "v", "out")
           for y in ("token", "head")}
-    seqs = 1 + spare(fill)
     cu = dev.put(np.array([0] + [n] * seqs, np.int32))
-    engine.seq_attn(P.SeqAttnPush(dtype=TYPES[dtype], n_seqs=seqs, n_q=n, n_k=n, n_heads=group,
+    engine.seq_attn(P.SeqAttnPush(dtype=TYPES[dtype], n_seqs=seqs, n_q=n, n_k=nk, n_heads=group,
                                   n_kv_heads=1, head_dim=hd, left=left, right=0, sinks=sinks, scale=0.1, **st), dev.put(q),
                     dev.put(k), dev.put(v), cu, cu, out)
     got_all = values(dev.get(out, (n, group, hd)), dtype)
-    kv, vv = values(k[:, 0], dtype), values(v[:, 0], dtype)
+    kv, vv = values(k[:n, 0], dtype), values(v[:n, 0], dtype)
     for h in range(group):
         got, qv = got_all[:, h], values(q[:, h], dtype)
         for i in range(n):
@@ -548,14 +552,16 @@ def test_seq_starts_out_of_range(engine, dev):
 def test_seq_rows_that_overlap(engine, dev, stride, hd, fill):
     """Keys and values repeated or overlapping, an infinite value among them: each channel meets it or does not."""
     rng = np.random.default_rng(hd + stride)
-    dtype, n, sinks, left = "fp16", 300, 3, 40
-    flat = normal(rng, n * stride + hd, dtype)
+    left = {"few": 200, "some": 400, "many": 40}[fill]
+    empty, rows = spare(fill)
+    dtype, n, sinks, seqs = "fp16", 220 + 2 * left, 3, 1 + empty
+    nk = max(n, rows * seqs)
+    flat = normal(rng, nk * stride + hd, dtype)
     flat[:hd:16] = to_bits(np.inf, dtype)
-    q, k = normal(rng, (n, 1, hd), dtype), normal(rng, n * stride + hd, dtype)
+    q, k = normal(rng, (n, 1, hd), dtype), normal(rng, nk * stride + hd, dtype)
     out = dev.put(np.full((n, hd), NAN[dtype], np.uint16))
-    seqs = 1 + spare(fill)
     cu = dev.put(np.array([0] + [n] * seqs, np.int32))
-    push = P.SeqAttnPush(dtype=P.F16, n_seqs=seqs, n_q=n, n_k=n, n_heads=1, n_kv_heads=1, head_dim=hd, left=left, right=0,
+    push = P.SeqAttnPush(dtype=P.F16, n_seqs=seqs, n_q=n, n_k=nk, n_heads=1, n_kv_heads=1, head_dim=hd, left=left, right=0,
                          sinks=sinks, scale=0.1, q_token_stride=hd, q_head_stride=hd, k_token_stride=stride, k_head_stride=hd,
                          v_token_stride=stride, v_head_stride=hd, out_token_stride=hd, out_head_stride=hd)
     engine.seq_attn(push, dev.put(q), dev.put(k), dev.put(flat), cu, cu, out)
@@ -570,15 +576,16 @@ def test_seq_rows_that_overlap(engine, dev, stride, hd, fill):
         assert not outside(got[i, ~high], want[~high], bound[~high]), i
 
 
-def test_seq_largest_key_stride(hip, engine, dev, device_arena):
-    """Rows 8 MiB apart: the last of a tile's lies almost 2^30 bytes behind its first."""
+@pytest.mark.parametrize("hd,n,sequences", [(32, 260, (1, 1101)), (128, 400, (1, 1101))])
+def test_seq_largest_key_stride(hip, engine, dev, device_arena, hd, n, sequences):
+    """Rows 8 MiB apart: the last of a tile's lies almost 2^31 bytes behind its first."""
     rng = np.random.default_rng(15)
-    dtype, hd, n, far = "bf16", 32, 260, 2 ** 22
+    dtype, far = "bf16", 2 ** 22
     q, k, v = (normal(rng, (n, hd), dtype) for _ in "qkv")
     big = device_arena(((n - 1) * far + 2 * hd) * 2, zero=False)  # a row's keys, then its values
     for j in range(n):
         hip.upload(big.ptr + 2 * far * j, np.concatenate([k[j], v[j]]))
-    for seqs in (1, 301, 1101):
+    for seqs in sequences:
         out = dev.put(np.full((n, hd), NAN[dtype], np.uint16))
         cu = dev.put(np.array([0] + [n] * seqs, np.int32))
         push = P.SeqAttnPush(dtype=P.BF16, n_seqs=seqs, n_q=n, n_k=n, n_heads=1, n_kv_heads=1, head_dim=hd, left=-1, right=0,

@@ -230,11 +230,20 @@ def test_seq_tiles_suffice(rules):
         assert first[-1] + need[-1] <= rules.seq_tiles(int(cu[-1]), 50, tile)
 
 
-@pytest.mark.parametrize("kw,kind,side,tile,grid", [
-    (dict(n_seqs=1, n_q=1, n_k=128), 2, 2, 32, 2), (dict(n_seqs=1, n_q=1, n_k=127), 1, 2, 64, 2), (dict(n_k=256, head_dim=128, k_head_stride=128, out_head_stride=128, out_token_stride=512), 1, 2, 64, 4),
-    (dict(n_seqs=126, n_q=129, n_k=10 ** 6), 2, 2, 32, 260), (dict(n_seqs=127, n_q=129, n_k=10 ** 6), 1, 2, 64, 258),  # 256 | 258 workgroups of 128 rows
-    (dict(n_seqs=500, n_q=780), 1, 2, 64, 1024), (dict(n_seqs=500, n_q=832), 0, 2, 64, 1026),
-    (dict(n_heads=32, n_kv_heads=1, n_k=256, out_token_stride=2048), 2, 32, 2, 7), (dict(n_heads=33, n_kv_heads=1, n_k=256, out_token_stride=4096), 2, 1, 64, 66),
+FOUR, EIGHT, NARROW = 0, 1, 2
+
+
+@pytest.mark.parametrize("kw,kind,side,tile,grid", [  # 2 groups of 2 heads, 64 queries a tile of 128 rows
+    (dict(n_seqs=1, n_q=1, n_k=192), NARROW, 2, 32, 2), (dict(n_seqs=1, n_q=1, n_k=191), FOUR, 2, 64, 2),
+    (dict(n_seqs=1, n_q=80 * 64, n_k=5120), NARROW, 2, 32, 322), (dict(n_seqs=1, n_q=81 * 64, n_k=5120), EIGHT, 2, 64, 164),  # 160 | 162
+    (dict(n_seqs=1, n_q=128 * 64, n_k=384), EIGHT, 2, 64, 258), (dict(n_seqs=1, n_q=128 * 64, n_k=383), FOUR, 2, 64, 258),
+    (dict(n_seqs=1, n_q=129 * 64, n_k=1289), FOUR, 2, 64, 260), (dict(n_seqs=1, n_q=129 * 64, n_k=1290), EIGHT, 2, 64, 260),
+    (dict(n_seqs=1, n_q=129 * 64, n_k=8000, left=1200), FOUR, 2, 64, 260),
+    (dict(n_seqs=1, n_q=384 * 64, n_k=24576), EIGHT, 2, 64, 770), (dict(n_seqs=1, n_q=385 * 64, n_k=24640), FOUR, 2, 64, 772),
+    (dict(n_seqs=1, n_q=384 * 64, n_k=24576, head_dim=32), NARROW, 2, 32, 1538),
+    (dict(n_seqs=1, n_q=1, n_k=512, head_dim=128, k_head_stride=128, out_head_stride=128, out_token_stride=512), EIGHT, 2, 64, 2),
+    (dict(n_heads=32, n_kv_heads=1, n_k=400, out_token_stride=2048), NARROW, 32, 2, 7),
+    (dict(n_heads=33, n_kv_heads=1, n_k=400, out_token_stride=4096), NARROW, 1, 64, 66), (dict(n_seqs=0, n_q=0, n_k=0), FOUR, 2, 64, 0),
 ])
 def test_seq_plan(rules, kw, kind, side, tile, grid):
     out = (C.c_longlong * 4)()
