@@ -508,8 +508,8 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
         }
 }
 
-/* Which of them: seq_rules.h's seq_plan. W4, W8: waves per SIMD that the registers have to allow. 8 waves with up to 32 channels: two workgroups per CU
- * (8,160 queries, 8 heads x 32: 30 us; one, 36). */
+/* Which of them: seq_rules.h's seq_plan. W4, W8: waves per SIMD that the registers have to allow. 8 waves with up to
+ * 32 channels: two workgroups per CU (8,160 queries, 8 heads x 32, window 1,023: 30 us; one, 36). */
 #define SEQ_ATTN(NAME, T, HD, W4, W8)                                                                                                    \
     extern "C" __global__ void __launch_bounds__(256, W4) prism_seq_attn_##NAME##_h##HD(SeqAttnArgs a) { seq_attn_body<T, HD, 4, 1>(a); } \
     extern "C" __global__ void __launch_bounds__(512, W8) prism_seq_attn_##NAME##_h##HD##_w8(SeqAttnArgs a) { seq_attn_body<T, HD, 4, 2>(a); }
