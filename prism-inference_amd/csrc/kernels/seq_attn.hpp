@@ -161,6 +161,10 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
     if (tile < first || (int64_t)(tile - first) * a.tile_q >= nq) return; /* uniform over the workgroup */
     const int q0 = (tile - first) * a.tile_q, q1 = min(q0 + a.tile_q, nq);
 
+    /* A SIMD's turns go first to waves outside of the products: what they do there is one chain, maximum, exchange,
+       branch, and products are behind it. 8,160 queries, 8 heads x 32, window 1,023: 27.4 -> 25.2 us; 2,000 x 16,
+       all keys: 14.5 -> 13.2; x 64: 18.4 -> 17.7; 4,000, 32 heads x 128: 139.5 -> 136.7, x 64: 85.7 -> 87.3. */
+    __builtin_amdgcn_s_setprio(3);
     const int lane = lane_id(), c32 = lane & 31, g = lane >> 5;
     const int wave8 = uni(threadIdx.x >> 6), wave = wave8 % RW, kgroup = wave8 / RW;
     const int row = 32 * wave + c32; /* this lane's; the wave's queries: qa .. qb - 1 */
@@ -324,6 +328,7 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
             mc = tc;
             limit = top + lag;
         }
+        __builtin_amdgcn_s_setprio(0);
         sn = f16v{};
 #pragma unroll
         for (int j = 0; j < NS; ++j) {
@@ -345,6 +350,7 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
             if (ONES && HD > 16 && j < 2) lsum = mfma_32x32x16(ones, weights(pl, j), lsum);
             sched_fence();
         }
+        __builtin_amdgcn_s_setprio(3);
         if (scale) {
 #pragma unroll
             for (int d = 0; d < DT; ++d)
