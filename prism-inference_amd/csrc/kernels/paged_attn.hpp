@@ -269,7 +269,7 @@ __device__ __forceinline__ void paged_many(const PagedAttnArgs& a) {
         q[ks] = in ? x : v8{};
     }
     f4 o[DT] = {};
-    float m = -INFINITY, mc = 0.f, l = 0.f;
+    float m = -INFINITY, mu = 0.f, l = 0.f; /* mu = m, or 0 while m is -inf */
 
     const auto page_of = [&](int i) { /* lane's key of the 32 from i on */
         const int x = i + (lane & 31);
@@ -315,20 +315,21 @@ __device__ __forceinline__ void paged_many(const PagedAttnArgs& a) {
         lanes_x32(fmaxf(x, y), x, y);
         top = fmaxf(x, y);
         if (__any(top > m)) {
-            const float tc = top == -INFINITY ? 0.f : top * a.scale_log2;
-            const float f = fast_exp2(m == -INFINITY ? -INFINITY : mc - tc);
+            const float f = fast_exp2(m == -INFINITY ? -INFINITY : (m - top) * a.scale_log2);
             l *= f;
 #pragma unroll
             for (int d = 0; d < DT; ++d) o[d] *= f;
             m = top;
-            mc = tc;
+            mu = top == -INFINITY ? 0.f : top;
         }
+        /* The maximum is subtracted before the scaling: the largest weight is then 1 whatever the scores, where an FMA with
+           the rounded product c m leaves half a step of it, 2^64 at scores of 2^30. */
         v8 p;
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const float z = fast_exp2(__builtin_fmaf(s[t][e], a.scale_log2, -mc));
+                const float z = fast_exp2((s[t][e] - mu) * a.scale_log2);
                 l += z;
                 p[4 * t + e] = (typename T::el)z;
             }
@@ -377,7 +378,7 @@ __device__ __forceinline__ void paged_many(const PagedAttnArgs& a) {
     for (int d = 0; d < DT; ++d)
         *reinterpret_cast<f4*>(acc + (wave * PAGED_TILE_HEADS + l16) * HD + 16 * d + 4 * g) = o[d];
     if (g == 0) {
-        lm[wave * PAGED_TILE_HEADS + l16] = m == -INFINITY ? m : mc;
+        lm[wave * PAGED_TILE_HEADS + l16] = m * a.scale_log2;
         ll[wave * PAGED_TILE_HEADS + l16] = l;
     }
     __syncthreads();

@@ -1,0 +1,74 @@
+"""The sequence operators at the ends of their range on the GPU: scores, scales and weights of any size, against
+definitions in 64 bits."""
+import numpy as np
+import pytest
+
+import prism_amd as P
+from seqlib import HALF_STEP, NAN, SMALLEST, TYPES, Device, normal, to_bits, values
+
+pytestmark = pytest.mark.gpu
+
+@pytest.fixture
+def dev(hip, device_arena):
+    return Device(hip, device_arena)
+
+
+def run_paged(engine, dev, dtype, q, k, v, scale, max_len, page=16):
+    """One sequence: q [heads][hd] over k, v [n][kv][hd] in pages in order."""
+    heads, hd = q.shape
+    n, kv = k.shape[:2]
+    pages = -(-n // page)
+    pool = [np.full((pages * page, kv, hd), NAN[dtype], np.uint16) for _ in "kv"]
+    pool[0][:n], pool[1][:n] = k, v
+    kp, vp = (dev.put(x.reshape(pages, page, kv, hd).transpose(0, 2, 1, 3)) for x in pool)
+    out = dev.put(np.full(q.shape, NAN[dtype], np.uint16))
+    push = P.PagedAttnPush(
+        cache=P.CacheDesc(dtype=TYPES[dtype], n_kv_heads=kv, head_dim=hd, page_size=page, n_pages=pages, n_seqs=1,
+                          table_pages=pages), n_heads=heads, left=-1, sinks=0, max_len=max_len, scale=scale,
+        q_seq_stride=heads * hd, q_head_stride=hd, out_seq_stride=heads * hd, out_head_stride=hd)
+    need = engine.paged_attn_workspace(push)
+    ws = dev.put(np.full(need // 2, NAN["fp16"], np.uint16))
+    print(f"[paged] {dtype} {heads}/{kv} x {hd}, {n} keys, announced {max_len}", flush=True)
+    engine.paged_attn(push, dev.put(q), kp, vp, dev.put(np.arange(pages, dtype=np.int32)), dev.put(np.array([n], np.int32)), out,
+                      ws, need)
+    return values(dev.get(out, q.shape), dtype)
+
+
+# --------------------------------------------------------------- huge scores
+
+# q and k have one channel each that is not zero, a power of two and 2^e (128 .. 255), so every score is exact in fp32, and
+# so is its product with 1; two unlike scores differ by at least 2^22 (fp16) or 2^32 (bf16), hundreds of steps of fp32 at that
+# size, so all the weight is on the keys of the largest score, equally: the output is the mean of their values.
+HUGE = {"fp16": (2.0 ** 15, 2.0 ** 7), "bf16": (2.0 ** 20, 2.0 ** 12)}
+
+
+def huge(rng, dtype, n, heads, kv, hd, queries):
+    a, b = HUGE[dtype]
+    rank = rng.integers(128, 256, (n, kv))
+    sign = np.where(rng.random((queries, heads)) < 0.5, -1, 1)
+    q, k = np.zeros((queries, heads, hd)), rng.standard_normal((n, kv, hd))
+    q[..., 3] = a * sign
+    k[..., 3] = b * rank
+    return rank, sign, to_bits(q, dtype), to_bits(k, dtype), normal(rng, (n, kv, hd), dtype)
+
+
+def largest(rank, sign, v, seen, dtype):
+    """The mean of the values of the largest score, and its bound: weights rounded, one sum, one rounding of the output."""
+    r = np.where(seen, rank * sign, -1000)
+    top = v[r == r.max()]
+    o, size = top.mean(0), np.abs(top).mean(0)
+    return o, size * (2 * HALF_STEP[dtype] + 2.0 ** -20) + SMALLEST[dtype]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hd", [16, 128])
+@pytest.mark.parametrize("kv,group", [(2, 1), (1, 2), (2, 3), (1, 17)])
+@pytest.mark.parametrize("n,max_len", [(1, 1), (50, 16), (300, 300), (5000, 5000)])
+def test_paged_huge_scores(engine, dev, dtype, hd, kv, group, n, max_len):
+    """Scores of 2^30 (fp16) and 2^40 (bf16), where a step of fp32 is many powers of two: the largest takes all."""
+    rng = np.random.default_rng(hd + group + n)
+    rank, sign, q, k, v = huge(rng, dtype, n, kv * group, kv, hd, 1)
+    got = run_paged(engine, dev, dtype, q[0], k, v, 1.0, max_len)
+    for h in range(kv * group):
+        want, bound = largest(rank[:, h // group], sign[0, h], values(v[:, h // group], dtype), np.ones(n, bool), dtype)
+        assert (np.abs(got[h] - want) <= bound).all(), h
