@@ -21,7 +21,8 @@
  * buffered, the next tile's loads in flight under the current tile's products.
  * Keys that no query of the workgroup sees are staged as zeros. Where only some
  * queries see a tile's key, its weight is zero for the others; should such a
- * V be infinite or NaN (0 * inf), the workgroup does its rows again key by key.
+ * V be infinite or NaN (0 * inf), the workgroup does its rows again key by key,
+ * and so it does where scores pass 2^22.
  */
 #pragma once
 #include "seq_types.hpp"
@@ -65,7 +66,7 @@ __device__ __forceinline__ T pinned(T v) {
 __device__ __forceinline__ void vm_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 /* One query by the whole wave, key after key, a lane per channel: the workgroup's
- * way out where zero weights would meet infinite values. */
+ * way out where zero weights would meet infinite values, and for huge scores. */
 template <class T, int HD>
 __device__ __forceinline__ void seq_attn_row(const SeqAttnArgs& a, const uint16_t* q, const uint16_t* k, const uint16_t* v,
                                              uint16_t* out, const KeyRange kr) {
@@ -193,7 +194,10 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
     const int a_lo = uni(ra.lo), a_hi = uni(ra.hi), b_lo = uni(rb.lo), b_hi = uni(rb.hi);
 
     const int see_hi = on ? b_hi : INT32_MIN, see_sink = seq_min(see_hi, sink_end);
-    unsigned bad = 0; /* infinite or NaN V where only some of the queries look */
+    unsigned bad = 0; /* infinite or NaN V where only some of the queries look, or scores too large for mc */
+    /* c s - mc is one FMA with the rounded mc, which leaves weights a factor of up to half a step of mc: it cancels in
+       the division, but has to fit the weights' type: 2^(1/4) at 2^22, 2^64 at 2^30. */
+    constexpr float MAX_FAST = 0x1p22f;
     v8 qf[KS];
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) qf[ks] = ld8<T>(qp + 16 * ks + 8 * g);
@@ -322,6 +326,7 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
         if (scale) {
             top = vmax(top, m);
             const float tc = top == -INFINITY ? 0.f : top * a.scale_log2;
+            if (__builtin_fabsf(tc) >= MAX_FAST) bad = ~0u;
             f = fast_exp2(m == -INFINITY ? -INFINITY : mc - tc);
             if (!ONES) l *= f;
             m = top;

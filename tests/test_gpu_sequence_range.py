@@ -4,13 +4,39 @@ import numpy as np
 import pytest
 
 import prism_amd as P
-from seqlib import HALF_STEP, NAN, SMALLEST, TYPES, Device, normal, to_bits, values
+from seqlib import HALF_STEP, NAN, SMALLEST, TYPES, Device, normal, to_bits, values, visible
 
 pytestmark = pytest.mark.gpu
+KINDS = ["few", "some", "many"]  # workgroups: the three kernels of the sequence attention
+
 
 @pytest.fixture
 def dev(hip, device_arena):
     return Device(hip, device_arena)
+
+
+def spare(fill):
+    """(empty sequences, key rows for each sequence) that lead to the kernels for few, some and many workgroups."""
+    return {"few": (0, 400), "some": (165, 400), "many": (1025, 0)}[fill]
+
+
+def run_seq(engine, dev, dtype, q, k, v, left, right, sinks, scale, fill):
+    """One sequence of q [nq][heads][hd] over k, v [nk][kv][hd], and empty ones behind it."""
+    nq, heads, hd = q.shape
+    nk, kv = k.shape[:2]
+    empty, rows = spare(fill)
+    seqs = 1 + empty
+    more = max(nk, rows * seqs) - nk  # rows of no sequence
+    k, v = (np.concatenate([x, np.full((more, kv, hd), NAN[dtype], np.uint16)]) for x in (k, v))
+    cu = [dev.put(np.array([0] + [n] * seqs, np.int32)) for n in (nq, nk)]
+    out = dev.put(np.full(q.shape, NAN[dtype], np.uint16))
+    print(f"[seq] {dtype} {nq} x {nk}, {heads}/{kv} x {hd}, {fill}", flush=True)
+    engine.seq_attn(P.SeqAttnPush(
+        dtype=TYPES[dtype], n_seqs=seqs, n_q=nq, n_k=len(k), n_heads=heads, n_kv_heads=kv, head_dim=hd, left=left, right=right,
+        sinks=sinks, scale=scale, q_token_stride=heads * hd, q_head_stride=hd, k_token_stride=kv * hd, k_head_stride=hd,
+        v_token_stride=kv * hd, v_head_stride=hd, out_token_stride=heads * hd, out_head_stride=hd),
+        dev.put(q), dev.put(k), dev.put(v), cu[0], cu[1], out)
+    return values(dev.get(out, q.shape), dtype)
 
 
 def run_paged(engine, dev, dtype, q, k, v, scale, max_len, page=16):
@@ -72,3 +98,19 @@ def test_paged_huge_scores(engine, dev, dtype, hd, kv, group, n, max_len):
     for h in range(kv * group):
         want, bound = largest(rank[:, h // group], sign[0, h], values(v[:, h // group], dtype), np.ones(n, bool), dtype)
         assert (np.abs(got[h] - want) <= bound).all(), h
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hd", [16, 32, 64, 128])
+@pytest.mark.parametrize("kv,group,left", [(2, 1, -1), (1, 3, 60)])
+@pytest.mark.parametrize("fill", KINDS)
+def test_seq_huge_scores(engine, dev, dtype, hd, kv, group, left, fill):
+    rng = np.random.default_rng(hd + group)
+    n, sinks = 300, 3
+    rank, sign, q, k, v = huge(rng, dtype, n, kv * group, kv, hd, n)
+    got = run_seq(engine, dev, dtype, q, k, v, left, 0, sinks, 1.0, fill)
+    for h in range(kv * group):
+        vv = values(v[:, h // group], dtype)
+        for i in range(n):
+            want, bound = largest(rank[:, h // group], sign[i, h], vv, visible(i, n, left, 0, sinks), dtype)
+            assert (np.abs(got[i, h] - want) <= bound).all(), (i, h)
