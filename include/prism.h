@@ -446,8 +446,9 @@ int prism_release_external_memory(prism_ctx* ctx, prism_external_buffer* buf);
  * device pointers to 16-bit values (fp16 or bf16, `dtype`), needs no model
  * loaded, keeps nothing between calls and allocates nothing, so it may be
  * captured into a graph. Sums, softmax statistics and angles are held in 32
- * bits or more; outputs are rounded once, to nearest, and so are softmax
- * weights that meet their values in matrix products. Pointers to values are
+ * bits or more; outputs are rounded once, to nearest, and so are the
+ * softmax weights of prism_seq_attn, which meet their values in matrix products
+ * (those of prism_paged_attn keep twice as many bits). Pointers to values are
  * 16-byte aligned and strides are in elements, multiples of 8, not negative
  * (0 repeats an input; an output's rows must not overlap). head_dim is the
  * innermost, contiguous dimension. An output overlaps no input unless said. The

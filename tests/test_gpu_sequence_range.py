@@ -114,3 +114,82 @@ def test_seq_huge_scores(engine, dev, dtype, hd, kv, group, left, fill):
         for i in range(n):
             want, bound = largest(rank[:, h // group], sign[i, h], vv, visible(i, n, left, 0, sinks), dtype)
             assert (np.abs(got[i, h] - want) <= bound).all(), (i, h)
+
+
+# ----------------------------------------------- one key before many weak ones
+
+# Scores are exact: q is 1 in one channel, the strong key's is `ahead`, every other key's 0, scale = log(2); so the strong key
+# weighs 1 and each other 2^-ahead, off by what ahead log2(e) ln(2) is rounded by (2^-24 of it, three times) and exp2's 2^-20.
+# The strong key's value is 0, the others' are between 1 and 2: what is lost of the weak weights is not hidden by anything.
+
+def behind_one_key(dtype, ahead, n, hd, at, rng):
+    k, v = np.zeros((n, 1, hd)), 1 + rng.random((n, 1, hd))
+    k[at, 0, 5], v[at] = ahead, 0
+    v = to_bits(v, dtype)
+    x = values(v[:, 0], dtype)
+    w = 2.0 ** -float(ahead)
+    total = 1 + (n - 1) * w
+    mean = w * x.sum(0) / total
+    # every weight: 2^-20 for exp2, 3 ahead 2^-24 for its argument; n 2^-23 for the sums of weights and products
+    bound = mean * (2 * (2.0 ** -20 + 3 * ahead * 2.0 ** -24) + n * 2.0 ** -23 + HALF_STEP[dtype]) + SMALLEST[dtype]
+    return to_bits(k, dtype), v, mean, bound, x.sum(0) / total
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hd", [16, 128])
+@pytest.mark.parametrize("group", [1, 3, 17])
+@pytest.mark.parametrize("n,ahead,max_len", [(131_075, 25.5, 131_075), (20_001, 26, 16), (131_075, 30, 300)])
+@pytest.mark.parametrize("last", [False, True])
+def test_paged_many_weak_keys_behind_one(engine, dev, dtype, hd, group, n, ahead, max_len, last):
+    """The weak keys together weigh as the sum says, however many heads share a key head."""
+    k, v, mean, bound, weak = behind_one_key(dtype, ahead, n, hd, n - 1 if last else 0, np.random.default_rng(hd))
+    q = np.zeros((group, hd))
+    q[:, 5] = 1
+    got = run_paged(engine, dev, dtype, to_bits(q, dtype), k, v, np.log(2.0), max_len, page=64)
+    # weights meet the values as the sum of two 16-bit numbers: a step of one step at most, (2 u)^2, and fp16's
+    # smallest step 2^-24 of numbers of which the largest is 2^14 at least
+    two = 4 * mean * HALF_STEP[dtype] ** 2 + (2.0 ** -38 * weak if dtype == "fp16" else 0)
+    for h in range(group):
+        assert (np.abs(got[h] - mean) <= bound + two).all(), (h, np.abs(got[h] - mean).max(), mean.max())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("group", [1, 2, 3, 17])
+@pytest.mark.parametrize("pairs,max_len", [(20, 16), (300, 600), (2000, 4000)])
+def test_paged_weights_are_not_rounded_to_16_bits(engine, dev, dtype, group, pairs, max_len):
+    """Two kinds of keys, one of weight 2^-a (another a for every head), whose values cancel but for the rounding of that
+    weight to 16 bits: the output is that rounding, and a kernel that rounds the weight gives 0."""
+    rng = np.random.default_rng(group)
+    hd, n = 32, 2 * pairs
+    a = values(to_bits(np.linspace(0.03, 0.97, group), dtype), dtype)
+    k, v, q = np.zeros((n, 1, hd)), np.ones((n, 1, hd)), np.zeros((group, hd))
+    other = rng.permutation(n) < pairs
+    k[other, 0, 0] = -1
+    q[:, 0] = a
+    v[~other, 0, :group] = -values(to_bits(2.0 ** -a, dtype), dtype)  # head h's in channel h
+    got = run_paged(engine, dev, dtype, to_bits(q, dtype), to_bits(k, dtype), to_bits(v, dtype), np.log(2.0), max_len)
+    v = values(to_bits(v, dtype), dtype)[:, 0]
+    for h in range(group):
+        w = np.where(other, 2.0 ** -a[h], 1.0)
+        want, size = w @ v / w.sum(), w @ np.abs(v) / w.sum()
+        # 2^-20 for exp2 and 3 2^-24 for its argument, twice; the sums; the weight as two 16-bit numbers, a step of one
+        # step at most; one rounding of the output
+        bound = size * (2 * (2.0 ** -20 + 3 * 2.0 ** -24) + n * 2.0 ** -23 + 4 * HALF_STEP[dtype] ** 2) + \
+            HALF_STEP[dtype] * np.abs(want) + SMALLEST[dtype]
+        assert (np.abs(got[h] - want) <= bound).all(), (h, np.abs(got[h] - want).max())
+
+
+@pytest.mark.parametrize("dtype,bits", [("fp16", 0x7C00), ("bf16", 0x7F80)])
+@pytest.mark.parametrize("group", [1, 3])
+@pytest.mark.parametrize("n,max_len", [(1, 1), (1, 40), (40, 16), (700, 700), (3000, 3000)])
+def test_paged_infinite_values(engine, dev, dtype, bits, group, n, max_len):
+    """An infinite value makes its channel infinite and no other."""
+    rng = np.random.default_rng(n)
+    hd = 64
+    q, k, v = normal(rng, (group, hd), dtype), normal(rng, (n, 1, hd), dtype), normal(rng, (n, 1, hd), dtype)
+    clean = run_paged(engine, dev, dtype, q, k, v, 0.125, max_len)
+    v[n // 2, 0, 7], v[n - 1, 0, 8] = bits, bits | 0x8000
+    got = run_paged(engine, dev, dtype, q, k, v, 0.125, max_len)
+    assert np.isposinf(got[:, 7]).all() and np.isneginf(got[:, 8]).all()
+    rest = np.delete(np.arange(hd), [7, 8])
+    assert (got[:, rest] == clean[:, rest]).all()
