@@ -15,7 +15,10 @@
  *                          V^T is read from LDS in that order by transposing
  *                          reads)
  * The weights are rounded to the type of the values, which is what the products
- * take (each by half a step, as much as the output's rounding). With this order
+ * take (each by half a step, as much as the output's rounding: the two together err
+ * 1.2 to 1.4 times as much as the output's alone. A second product for what 16 bits cut
+ * off, as paged_attn.hpp has it, would be half as many products again where they bound
+ * the launch). With this order
  * a query's maximum, sum and rescaling stay in its lane (two lanes, 32
  * apart, hold halves of its keys). K and V tiles go through LDS, double
  * buffered, the next tile's loads in flight under the current tile's products.
@@ -203,7 +206,10 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
     for (int ks = 0; ks < KS; ++ks) qf[ks] = ld8<T>(qp + 16 * ks + 8 * g);
 
     f16v o[DT] = {};
-    float m = -INFINITY, mc = 0.f, l = 0.f; /* mc = c m, or 0 while m is -inf */
+    /* fp16 weights are 2^UP times as large, with which the lag (see limit) stays below 2^16: what is lost of a weight
+       is below 2^-32 of the largest, not 2^-25. Many keys behind one strong key may matter. */
+    constexpr float UP = __is_same(T, F16) ? 7.f : 0.f;
+    float m = -INFINITY, mc = 0.f, l = 0.f; /* mc = c m - UP, or 0 while m is -inf */
     /* The sum of a query's weights: as many additions as weights on the vector units, or products with ones on
        the matrix cores, which wait for the vector units up to 64 channels (5 sequences of 243 to 3,788 queries, 20
        heads x 32: 113 us and, added, 129; 8 waves have no registers for it). 16 channels leave half of the
@@ -320,12 +326,13 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
         for (int e = 2; e < 16; e += 2) top = vmax3(top, sc[e], sc[e + 1]);
         lanes_x32(top, x, y);
         top = vmax(x, y);
-        /* the maximum may lag by 8 powers of two: weights up to 256 cost no precision, rescaling costs much */
+        /* the maximum may lag by 8 powers of two: weights up to 256 (fp16: 2^15) cost no precision, rescaling
+           costs much */
         float f = 1.f;
         const bool scale = __any(top > limit);
         if (scale) {
             top = vmax(top, m);
-            const float tc = top == -INFINITY ? 0.f : top * a.scale_log2;
+            const float tc = top == -INFINITY ? 0.f : top * a.scale_log2 - UP;
             if (__builtin_fabsf(tc) >= MAX_FAST) bad = ~0u;
             f = fast_exp2(m == -INFINITY ? -INFINITY : mc - tc);
             if (!ONES) l *= f;

@@ -193,3 +193,21 @@ def test_paged_infinite_values(engine, dev, dtype, bits, group, n, max_len):
     assert np.isposinf(got[:, 7]).all() and np.isneginf(got[:, 8]).all()
     rest = np.delete(np.arange(hd), [7, 8])
     assert (got[:, rest] == clean[:, rest]).all()
+
+
+@pytest.mark.parametrize("hd", [16, 32, 64, 128])
+@pytest.mark.parametrize("n,ahead", [(131_075, 25.5), (100_000, 27)])
+@pytest.mark.parametrize("last", [False, True])
+@pytest.mark.parametrize("fill", ["few", "some", "many"])
+def test_seq_many_weak_keys_behind_one(engine, dev, hd, n, ahead, last, fill):
+    """fp16: weights below 2^-25 of the largest are not lost."""
+    dtype = "fp16"
+    k, v, mean, bound, weak = behind_one_key(dtype, ahead, n, hd, n - 1 if last else 0, np.random.default_rng(hd))
+    q = np.zeros((3, 1, hd))
+    q[..., 5] = 1
+    got = run_seq(engine, dev, dtype, to_bits(q, dtype), k, v, -1, -1, 0, np.log(2.0), fill)
+    # weights are rounded to half a step, and to fp16's smallest half step 2^-25 of numbers of which the largest is 2^7 at least;
+    # their sum may be that of the rounded ones
+    one = mean * HALF_STEP[dtype] + 2.0 ** -32 * weak
+    for i in range(3):
+        assert (np.abs(got[i, 0] - mean) <= bound + 2 * one).all(), (i, np.abs(got[i, 0] - mean).max(), mean.max())
