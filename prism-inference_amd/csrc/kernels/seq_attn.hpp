@@ -217,7 +217,7 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
     f16v lsum = {};
     const v8 ones = splat_one<T>();
     float limit = -INFINITY;
-    const float lag = 8.0f / a.scale_log2;
+    const float lag = fminf(8.0f / a.scale_log2, 0x1.fffffep127f); /* finite: -inf + lag has to stay -inf, the limit of who saw no key */
 
     /* k0 of tile t + 1, from tile t's; where a tile's keys end */
     auto step = [&](int t, int k0) { return t + 1 == sink_tiles ? win0 : k0 + BN; };

@@ -211,3 +211,38 @@ def test_seq_many_weak_keys_behind_one(engine, dev, hd, n, ahead, last, fill):
     one = mean * HALF_STEP[dtype] + 2.0 ** -32 * weak
     for i in range(3):
         assert (np.abs(got[i, 0] - mean) <= bound + 2 * one).all(), (i, np.abs(got[i, 0] - mean).max(), mean.max())
+
+
+# --------------------------------------------------------------- tiny scales
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("scale", [1e-38, 1e-40, 2e-38])
+@pytest.mark.parametrize("hd", [16, 32, 64, 128])
+@pytest.mark.parametrize("left,right,sinks", [(40, 0, 2), (9, -1, 0), (9, 400, 0)])
+@pytest.mark.parametrize("fill", KINDS)
+def test_seq_tiny_scale(engine, dev, dtype, scale, hd, left, right, sinks, fill):
+    """Any positive scale: at 1e-38 all weights are alike, and the output is the mean of the values seen. (With a window of 9,
+    rows of one wave begin to see keys in different steps.)"""
+    rng = np.random.default_rng(hd)
+    n = 330
+    q, k, v = (normal(rng, (n, 1, hd), dtype) for _ in "qkv")
+    got = run_seq(engine, dev, dtype, q, k, v, left, right, sinks, scale, fill)
+    x = values(v[:, 0], dtype)
+    for i in range(n):
+        seen = x[visible(i, n, left, right, sinks)]
+        want, size, u = seen.mean(0), np.abs(seen).mean(0), HALF_STEP[dtype]
+        # scores below 2^-110; sums; the weights' rounding; one of the output
+        bound = size * (2.0 ** -20 + n * 2.0 ** -23 + 2 * u) + u * np.abs(want) + SMALLEST[dtype]
+        assert (np.abs(got[i, 0] - want) <= bound).all(), i
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("group", [1, 3])
+@pytest.mark.parametrize("n,max_len", [(30, 30), (700, 700), (3000, 3000)])
+def test_paged_tiny_scale(engine, dev, dtype, group, n, max_len):
+    rng = np.random.default_rng(n)
+    q, k, v = normal(rng, (group, 64), dtype), normal(rng, (n, 1, 64), dtype), normal(rng, (n, 1, 64), dtype)
+    got = run_paged(engine, dev, dtype, q, k, v, 1e-40, max_len)
+    x, u = values(v[:, 0], dtype), HALF_STEP[dtype]
+    bound = np.abs(x).mean(0) * (2.0 ** -20 + n * 2.0 ** -23 + 2 * u) + u * np.abs(x.mean(0)) + SMALLEST[dtype]
+    assert (np.abs(got - x.mean(0)) <= bound).all()
