@@ -13,8 +13,9 @@
 
 namespace prism {
 
-/* Strides are held to 2^40 elements so that no offset passes 64 bits. */
+/* Strides are held to 2^40 elements, and the offset of a buffer's last row to 2^60, so that none passes 64 bits in bytes. */
 constexpr int64_t SEQ_MAX_STRIDE = int64_t(1) << 40;
+constexpr int64_t SEQ_MAX_OFFSET = int64_t(1) << 60;
 /* Rows of a sequence attention and tokens of a table's row: key numbers a tile past the
  * end stay in 32 bits. */
 constexpr int64_t SEQ_MAX_ROWS = int64_t(1) << 30;
@@ -31,16 +32,19 @@ inline int check_dtype(int32_t dtype, const char** why) {
                                                      : seq_bad(why, PRISM_ERR_INVALID, "dtype is neither PRISM_F16 nor PRISM_BF16");
 }
 
-inline int check_strides(int64_t token, int64_t head, const char** why) {
+inline int check_strides(int64_t rows, int64_t heads, int64_t token, int64_t head, const char** why) {
     if (token < 0 || head < 0 || token % 8 || head % 8 || token > SEQ_MAX_STRIDE || head > SEQ_MAX_STRIDE)
         return seq_bad(why, PRISM_ERR_INVALID, "strides are multiples of 8 from 0 to 2^40");
+    /* heads are 2^16 at most */
+    if (token > 0 && rows - 1 > (SEQ_MAX_OFFSET - (heads - 1) * head) / token)
+        return seq_bad(why, PRISM_ERR_UNSUPPORTED, "rows reach past 2^60 elements");
     return PRISM_OK;
 }
 
 /* An output's rows must not overlap: either all heads of a row lie before the
  * next row's, or all rows of a head before the next head's. */
 inline int check_out(int64_t rows, int64_t heads, int64_t head_dim, int64_t token, int64_t head, const char** why) {
-    if (int rc = check_strides(token, head, why)) return rc;
+    if (int rc = check_strides(rows, heads, token, head, why)) return rc;
     const bool rows_apart = (heads == 1 || head >= head_dim) && (rows <= 1 || token >= (heads - 1) * head + head_dim);
     const bool heads_apart = (rows <= 1 || token >= head_dim) && (heads == 1 || head >= (rows - 1) * token + head_dim);
     if (!rows_apart && !heads_apart) return seq_bad(why, PRISM_ERR_INVALID, "output rows overlap");
@@ -84,7 +88,7 @@ inline int check_rope(const prism_rope_push& p, const char** why) {
         return seq_bad(why, PRISM_ERR_INVALID, "layout, ladder or inverse");
     if (!(p.base >= 1) || !std::isfinite(p.base)) return seq_bad(why, PRISM_ERR_INVALID, "base is less than 1");
     if (p.pos_stride < 0 || p.pos_stride > SEQ_MAX_STRIDE) return seq_bad(why, PRISM_ERR_INVALID, "pos_stride");
-    if (int rc = check_strides(p.in_token_stride, p.in_head_stride, why)) return rc;
+    if (int rc = check_strides(p.n_tokens, p.n_heads, p.in_token_stride, p.in_head_stride, why)) return rc;
     return check_out(p.n_tokens, p.n_heads, p.head_dim, p.out_token_stride, p.out_head_stride, why);
 }
 
@@ -98,14 +102,18 @@ inline int check_cache(const prism_cache_desc& d, const char** why) {
         return seq_bad(why, PRISM_ERR_INVALID, "cache sizes out of range");
     if ((int64_t)d.table_pages * d.page_size > SEQ_MAX_ROWS)
         return seq_bad(why, PRISM_ERR_UNSUPPORTED, "a table row of more than 2^30 tokens");
+    if ((int64_t)d.n_pages * d.n_kv_heads * d.page_size > SEQ_MAX_OFFSET / d.head_dim ||
+        (int64_t)d.n_seqs * d.table_pages > SEQ_MAX_OFFSET)
+        return seq_bad(why, PRISM_ERR_UNSUPPORTED, "a pool or table of more than 2^60 elements");
     return PRISM_OK;
 }
 
 inline int check_append(const prism_append_push& p, const char** why) {
     if (int rc = check_cache(p.cache, why)) return rc;
     if (p.n_new < 0) return seq_bad(why, PRISM_ERR_INVALID, "n_new < 0");
-    if (int rc = check_strides(p.k_token_stride, p.k_head_stride, why)) return rc;
-    return check_strides(p.v_token_stride, p.v_head_stride, why);
+    const int64_t heads = p.cache.n_kv_heads;
+    if (int rc = check_strides(p.n_new, heads, p.k_token_stride, p.k_head_stride, why)) return rc;
+    return check_strides(p.n_new, heads, p.v_token_stride, p.v_head_stride, why);
 }
 
 inline int check_paged(const prism_paged_attn_push& p, const char** why) {
@@ -113,7 +121,7 @@ inline int check_paged(const prism_paged_attn_push& p, const char** why) {
     if (int rc = check_heads(p.n_heads, p.cache.n_kv_heads, p.cache.head_dim, why)) return rc;
     if (p.sinks < 0 || p.max_len < 0) return seq_bad(why, PRISM_ERR_INVALID, "sinks or max_len < 0");
     if (int rc = check_scale(p.scale, why)) return rc;
-    if (int rc = check_strides(p.q_seq_stride, p.q_head_stride, why)) return rc;
+    if (int rc = check_strides(p.cache.n_seqs, p.n_heads, p.q_seq_stride, p.q_head_stride, why)) return rc;
     return check_out(p.cache.n_seqs, p.n_heads, p.cache.head_dim, p.out_seq_stride, p.out_head_stride, why);
 }
 
@@ -124,9 +132,9 @@ inline int check_seq(const prism_seq_attn_push& p, const char** why) {
     if (p.n_q > SEQ_MAX_ROWS || p.n_k > SEQ_MAX_ROWS) return seq_bad(why, PRISM_ERR_UNSUPPORTED, "more than 2^30 rows");
     if (p.sinks < 0) return seq_bad(why, PRISM_ERR_INVALID, "sinks < 0");
     if (int rc = check_scale(p.scale, why)) return rc;
-    if (int rc = check_strides(p.q_token_stride, p.q_head_stride, why)) return rc;
-    if (int rc = check_strides(p.k_token_stride, p.k_head_stride, why)) return rc;
-    if (int rc = check_strides(p.v_token_stride, p.v_head_stride, why)) return rc;
+    if (int rc = check_strides(p.n_q, p.n_heads, p.q_token_stride, p.q_head_stride, why)) return rc;
+    if (int rc = check_strides(p.n_k, p.n_kv_heads, p.k_token_stride, p.k_head_stride, why)) return rc;
+    if (int rc = check_strides(p.n_k, p.n_kv_heads, p.v_token_stride, p.v_head_stride, why)) return rc;
     if (p.k_token_stride > SEQ_MAX_KEY_STRIDE || p.v_token_stride > SEQ_MAX_KEY_STRIDE)
         return seq_bad(why, PRISM_ERR_UNSUPPORTED, "k and v token strides are at most 2^22");
     return check_out(p.n_q, p.n_heads, p.head_dim, p.out_token_stride, p.out_head_stride, why);
