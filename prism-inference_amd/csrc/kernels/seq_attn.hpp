@@ -58,7 +58,7 @@ __device__ __forceinline__ i4 buffer_of(const void* p, int bytes) {
 __device__ __forceinline__ void load_to_lds(i4 buffer, int offset, unsigned to) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                  ::"s"(to), "v"(offset), "s"(buffer)
-                 : "memory");
+                 : "memory", "m0");
 }
 /* Computed here and not nearer to its use: keeps what goes beside the matrix products there. */
 template <class T>
