@@ -521,8 +521,9 @@ int prism_cache_append(prism_ctx* ctx, const prism_append_push* p, const void* k
  * device memory of prism_paged_attn_workspace bytes (16-byte aligned; may be
  * NULL if that is 0), free to reuse after the call's work; calls that may
  * overlap need one each. scale is positive and at most
- * 2e38; scores are fp32 and have to stay in its range, before the scaling and
- * after it. */
+ * 2e38; scores (before the scaling and after it) and sums of values over the
+ * keys seen are fp32 and have to stay in its range. An infinite value makes its
+ * channel infinite, or NaN where its weight rounds to zero. */
 typedef struct prism_paged_attn_push {
     prism_cache_desc cache;
     int32_t n_heads;

@@ -54,18 +54,18 @@ __device__ __forceinline__ float across(float v, F op) {
 }
 
 /* Two weights, each as the sum of two 16-bit numbers: hi has the bits cut off that the type does not hold, lo is what
- * they are, at least `least`. */
+ * they are, at least `least` where hi is not zero (r < hi then; a median of three is one instruction). */
 __device__ __forceinline__ void two_numbers(float z0, float z1, float least, h2& hi, h2& lo) {
     hi = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(z0, z1));
-    const float r0 = fmaxf(z0 - (float)hi[0], least), r1 = fmaxf(z1 - (float)hi[1], least);
-    lo = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(r0, r1));
+    const float c0 = (float)hi[0], c1 = (float)hi[1];
+    lo = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(__builtin_amdgcn_fmed3f(z0 - c0, least, c0),
+                                                           __builtin_amdgcn_fmed3f(z1 - c1, least, c1)));
 }
 __device__ __forceinline__ void two_numbers(float z0, float z1, float least, b2& hi, b2& lo) {
     const unsigned u0 = __builtin_bit_cast(unsigned, z0), u1 = __builtin_bit_cast(unsigned, z1);
     hi = __builtin_bit_cast(b2, __builtin_amdgcn_perm(u1, u0, 0x07060302));
-    const float r0 = fmaxf(z0 - __builtin_bit_cast(float, u0 & 0xFFFF0000u), least);
-    const float r1 = fmaxf(z1 - __builtin_bit_cast(float, u1 & 0xFFFF0000u), least);
-    lo = b2{(__bf16)opaque(r0), (__bf16)opaque(r1)};
+    const float c0 = __builtin_bit_cast(float, u0 & 0xFFFF0000u), c1 = __builtin_bit_cast(float, u1 & 0xFFFF0000u);
+    lo = b2{(__bf16)opaque(__builtin_amdgcn_fmed3f(z0 - c0, least, c0)), (__bf16)opaque(__builtin_amdgcn_fmed3f(z1 - c1, least, c1))};
 }
 
 template <int N>
@@ -285,12 +285,13 @@ __device__ __forceinline__ void paged_many(const PagedAttnArgs& a) {
     }
     /* A weight meets V as the sum of two 16-bit numbers (2^-15 of it off at most, where the output is rounded by 2^-8; fp16
        2^-20), fp16's from 2^15 down, so what is lost is below 2^-39 of the largest: many keys behind one strong key may matter.
-       The first is cut off and the second held above zero, so an infinite V meets no other sign. The outputs' errors are
+       The first is cut off and the second held above zero, so an infinite V meets no zero beside a weight and no other
+       sign. The outputs' errors are
        those of paged_few, which has 32-bit weights; rounded to one 16-bit number they were 1.3 times as large. us with one
-       number and with two: 24 sequences to 20,001, 32/8 x 128: 206.4, 207.4; one of 131,075: 107.6, 108.9; 64 to 1,000, 32/8 x 64:
-       21.4, 21.8; 34, 40/8 x 16, window 2,820: 21.9, 23.6. */
+       number and with two: 24 sequences to 20,001, 32/8 x 128: 207.8, 208.9; one of 131,075: 108.2, 108.8; 64 to 1,000, 32/8 x 64:
+       21.3, 21.6; 34, 40/8 x 16, window 2,820: 22.1, 24.1. */
     constexpr bool HALF = __is_same(T, F16);
-    constexpr float UP = HALF ? 15.f : 0.f, LEAST = HALF ? 0x1p-24f : 0x1p-100f;
+    constexpr float UP = HALF ? 15.f : 0.f, LEAST = HALF ? 0x1p-24f : 0x1p-133f; /* the type's smallest */
     f4 o[DT] = {};
     float m = -INFINITY, mu = 0.f, l = 0.f; /* mu = m, or 0 while m is -inf; l as the weights, 2^UP times too large */
 

@@ -246,3 +246,30 @@ def test_paged_tiny_scale(engine, dev, dtype, group, n, max_len):
     x, u = values(v[:, 0], dtype), HALF_STEP[dtype]
     bound = np.abs(x).mean(0) * (2.0 ** -20 + n * 2.0 ** -23 + 2 * u) + u * np.abs(x.mean(0)) + SMALLEST[dtype]
     assert (np.abs(got - x.mean(0)) <= bound).all()
+
+
+# ----------------------------------------------- weights of zero, large values
+
+@pytest.mark.parametrize("dtype,small,large,ahead", [("fp16", 2.0 ** -12, 60_000.0, 70), ("bf16", 1.0, 2.0 ** 100, 240)])
+@pytest.mark.parametrize("group", [1, 3])
+@pytest.mark.parametrize("n,max_len", [(40, 16), (700, 700), (70_000, 70_000)])
+def test_paged_large_values_without_weight(engine, dev, dtype, small, large, ahead, group, n, max_len):
+    """Keys `ahead` powers of two behind one: their values, however large, add nothing (n 2^-ahead large < small 2^-20). Their
+    sum stays in fp32's range, which a part of the keys without the strong one needs."""
+    hd, at = 64, n // 3
+    q, k, v = np.zeros((group, hd)), np.zeros((n, 1, hd)), np.full((n, 1, hd), large)
+    q[:, 5], k[at, 0, 5], v[at] = 1, ahead, small
+    got = run_paged(engine, dev, dtype, to_bits(q, dtype), to_bits(k, dtype), to_bits(v, dtype), np.log(2.0), max_len)
+    assert n * 2.0 ** -ahead * large < small * 2.0 ** -20
+    assert (np.abs(got - small) <= small * (2.0 ** -19 + HALF_STEP[dtype])).all(), np.abs(got - small).max()
+
+
+@pytest.mark.parametrize("dtype,small,large,ahead", [("fp16", 2.0 ** -12, 60_000.0, 70), ("bf16", 1.0, 2.0 ** 100, 240)])
+@pytest.mark.parametrize("hd", [16, 64, 128])
+@pytest.mark.parametrize("fill", KINDS)
+def test_seq_large_values_without_weight(engine, dev, dtype, small, large, ahead, hd, fill):
+    n, at = 20_000, 7
+    q, k, v = np.zeros((3, 1, hd)), np.zeros((n, 1, hd)), np.full((n, 1, hd), large)
+    q[..., 5], k[at, 0, 5], v[at] = 1, ahead, small
+    got = run_seq(engine, dev, dtype, to_bits(q, dtype), to_bits(k, dtype), to_bits(v, dtype), -1, -1, 0, np.log(2.0), fill)
+    assert (np.abs(got - small) <= small * (2.0 ** -19 + 2 * HALF_STEP[dtype])).all(), np.abs(got - small).max()
