@@ -176,7 +176,8 @@ inline PagedPlan paged_plan(const prism_paged_attn_push& p) {
     /* keys of the longest sequence expected */
     int64_t keys = p.max_len > 0 ? p.max_len : (int64_t)p.cache.table_pages * p.cache.page_size;
     if (p.left >= 0 && keys > (int64_t)p.left + 1 + p.sinks) keys = (int64_t)p.left + 1 + p.sinks;
-    /* A wave alone where the waves are many and short: 64 keys, 1,600 items of 4 heads x 32 and x 128 5.6 and 12.3 us, four
+    /* (Figures with one 16-bit number a weight; with two, 3 heads and more take up to 10 % longer.)
+     * A wave alone where the waves are many and short: 64 keys, 1,600 items of 4 heads x 32 and x 128 5.6 and 12.3 us, four
      * waves an item 8.1 and 20.1; 512 items x 128 7.2 (1 head) and 7.5 (4), and 5.1 and 8.2; 200 keys, 512 items x 128 23.5 and
      * 13.2; 4,800 items of 64 to 1,000 keys 8.7 to 115 and 16.2 to 113. */
     r.waves = keys <= 32 || items >= 4096 || (items >= 1024 && keys <= 128) ? 1 : 4;

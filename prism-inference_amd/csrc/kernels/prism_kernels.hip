@@ -19,6 +19,7 @@
  *   prism_paged_attn_{f16,bf16}_h{16,32,64,128}_{g1,g2,many}  one new token per sequence over its paged cache
  *   prism_paged_attn_join_{f16,bf16}_h{16,32,64,128}  ... and the join of a split length
  *   prism_seq_attn_{f16,bf16}_h{16,32,64,128}[_w8]  attention along sequences, window and sinks
+ *   prism_seq_attn_{f16,bf16}_h{16,32,64}_narrow   the same for few workgroups
  *   prism_zero_i32                                 clears routing counters
  */
 #include "attn.hpp"

@@ -164,8 +164,8 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
     /* workgroup -> (query tile, head): an XCD (workgroups b, b + 8, ...) takes a
      * run of neighbouring heads, whose keys its L2 then holds; the last tiles, whose
      * queries may see the most keys, come first, so the launch ends with short ones
-     * (with whole groups of heads per XCD, over all of them: 2 of 5,000 queries, 32
-     * heads x 128, 409 -> 374 us) */
+     * (with whole groups of heads per XCD, over all of them). Measured together with LDS addresses in
+     * registers and 16-byte stores: 2 of 5,000 queries, 32 heads x 128, 409 -> 374 us. */
     const int tiles = a.n_q / a.tile_q + a.n_seqs, groups = a.n_heads / a.tile_heads, b = blockIdx.x, xcd = b & 7;
     int hg, tile; /* group of heads, tile of queries */
     if (groups % 8 == 0) {
@@ -187,7 +187,8 @@ __device__ __forceinline__ void seq_attn_body(const SeqAttnArgs& a) {
 
     /* A SIMD's turns go first to waves outside of the products: what they do there is one chain, maximum, exchange,
        branch, and products are behind it. 8,160 queries, 8 heads x 32, window 1,023: 27.4 -> 25.2 us; 2,000 x 16,
-       all keys: 14.5 -> 13.2; x 64: 18.4 -> 17.7; 4,000, 32 heads x 128: 139.5 -> 136.7, x 64: 85.7 -> 87.3. */
+       all keys: 14.5 -> 13.2; x 64: 18.4 -> 17.7; 4,000, 32 heads x 128: 139.5 -> 136.7, x 64: 85.7 -> 87.3 (at 64
+       it gains with few workgroups and costs with many; one rule for all widths). */
     __builtin_amdgcn_s_setprio(3);
     const int lane = lane_id(), c32 = lane & 31, g = lane >> 5;
     const int wave8 = uni(threadIdx.x >> 6), wave = wave8 % RW, kgroup = wave8 / RW;
