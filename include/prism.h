@@ -454,8 +454,8 @@ int prism_release_external_memory(prism_ctx* ctx, prism_external_buffer* buf);
  * innermost, contiguous dimension. An output overlaps no input unless said. The
  * call runs on the context's device and leaves the caller's current device as
  * it was. A call without rows does nothing; one of more than 2^32 - 1 threads, or
- * with buffers that reach past 2^60 elements, is PRISM_ERR_UNSUPPORTED. The reference has no counterpart: its attention sees
- * one window of one frame (shaders/split2_qkv_attn_d256.comp.glsl:24-79). */
+ * with buffers that reach past 2^60 elements, is PRISM_ERR_UNSUPPORTED. The
+ * reference has no counterpart: its attention sees one window of one frame (shaders/split2_qkv_attn_d256.comp.glsl:24-79). */
 #define PRISM_F16  0
 #define PRISM_BF16 1
 

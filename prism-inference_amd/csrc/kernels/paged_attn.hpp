@@ -286,9 +286,8 @@ __device__ __forceinline__ void paged_many(const PagedAttnArgs& a) {
     /* A weight meets V as the sum of two 16-bit numbers (2^-15 of it off at most, where the output is rounded by 2^-8; fp16
        2^-20), fp16's from 2^15 down, so what is lost is below 2^-39 of the largest: many keys behind one strong key may matter.
        The first is cut off and the second held above zero, so an infinite V meets no zero beside a weight and no other
-       sign. The outputs' errors are
-       those of paged_few, which has 32-bit weights; rounded to one 16-bit number they were 1.3 times as large. us with one
-       number and with two: 24 sequences to 20,001, 32/8 x 128: 207.8, 208.9; one of 131,075: 108.2, 108.8; 64 to 1,000, 32/8 x 64:
+       sign. The outputs' errors are those of paged_few, which has 32-bit weights; rounded to one 16-bit number they were 1.3
+       times as large. us with one number and with two: 24 sequences to 20,001, 32/8 x 128: 207.8, 208.9; one of 131,075: 108.2, 108.8; 64 to 1,000, 32/8 x 64:
        21.3, 21.6; 34, 40/8 x 16, window 2,820: 22.1, 24.1. */
     constexpr bool HALF = __is_same(T, F16);
     constexpr float UP = HALF ? 15.f : 0.f, LEAST = HALF ? 0x1p-24f : 0x1p-133f; /* the type's smallest */

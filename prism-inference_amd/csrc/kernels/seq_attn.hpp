@@ -24,8 +24,8 @@
  * buffered, the next tile's loads in flight under the current tile's products.
  * Keys that no query of the workgroup sees are staged as zeros. Where only some
  * queries see a tile's key, its weight is zero for the others; should such a
- * V be infinite or NaN (0 * inf), the workgroup does its rows again key by key,
- * and so it does where scores pass 2^22.
+ * V be infinite or NaN (0 * inf), the workgroup does its rows again one by one,
+ * and so it does where scaled scores pass 2^22.
  */
 #pragma once
 #include "seq_types.hpp"
