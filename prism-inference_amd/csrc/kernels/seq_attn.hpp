@@ -15,10 +15,12 @@
  *                          V^T is read from LDS in that order by transposing
  *                          reads)
  * The weights are rounded to the type of the values, which is what the products
- * take (each by half a step, as much as the output's rounding: the two together err
- * 1.2 to 1.4 times as much as the output's alone. A second product for what 16 bits cut
- * off, as paged_attn.hpp has it, would be half as many products again where they bound
- * the launch). With this order
+ * take: each by half a step, as the output is, so that the two together err 1.2 to
+ * 1.4 times as much as the output's rounding alone (rms 1.73e-5 and 1.28e-5 at 8,160
+ * queries x 32 channels in fp16, 1.11e-4 and 7.9e-5 at 128 channels in bf16). Two 16-bit numbers a
+ * weight, as paged_attn.hpp has them where they are free, leave the output's rounding alone and
+ * took, in us: 8,160, 8 x 32, window 1,023: 41.6 instead of 29.2; 4,000, 32 x 64: 146 instead of
+ * 91; two of 4,501 and 5,800, 32/8 x 128: 404 instead of 310. With this order
  * a query's maximum, sum and rescaling stay in its lane (two lanes, 32
  * apart, hold halves of its keys). K and V tiles go through LDS, double
  * buffered, the next tile's loads in flight under the current tile's products.
