@@ -560,6 +560,114 @@ typedef struct prism_seq_attn_push {
 int prism_seq_attn(prism_ctx* ctx, const prism_seq_attn_push* p, const void* q, const void* k, const void* v,
                    const int32_t* cu_q, const int32_t* cu_k, void* out, void* stream);
 
+/* ---- a cheaper past: a cache in 4 bits, and states of fixed size ---- */
+
+/* Format of a paged cache. PRISM_CACHE_16: values of the cache's dtype, as
+ * above. PRISM_CACHE_4: a block of 32 channels of a head (16 where head_dim is
+ * 16) shares a power of two; a value is 4 bits, a sign (8) and the number of
+ * one of 0, 0.5, 1, 1.5, 2, 3, 4, 6. Pools k and v are then bytes
+ * [n_pages][n_kv_heads][page_size][head_dim / 2], channel 2i in the low half of
+ * byte i, and k_scales, v_scales bytes [n_pages][n_kv_heads][page_size]
+ * [head_dim / 32] (1 for head_dim 16): the power 2^e is the byte e + 127, and 255
+ * makes its block NaN. (Floats of two exponent bits and one fraction bit under
+ * shared exponents: the FP4 of the OCP microscaling formats.) A block is written with the
+ * smallest e for which its largest magnitude is at most 7 * 2^e, but not below
+ * -23 or above 13 (fp16; bf16: -125 and 125), so that every stored value is one
+ * of dtype's; each value becomes the nearest of those above, ties to the even
+ * number, and 6 past the last. fp16 magnitudes past 57,344 (bf16: past 2.97e38) are
+ * held as 49,152 (2.55e38). A block with an infinity or a NaN has byte 255. */
+#define PRISM_CACHE_16 0
+#define PRISM_CACHE_4  1
+typedef struct prism_cache_pages {
+    void *k, *v;               /* pools; 16-byte aligned                 */
+    void *k_scales, *v_scales; /* 16-byte aligned; not used by PRISM_CACHE_16 */
+} prism_cache_pages;
+
+/* prism_rope and prism_cache_append in one launch: n_new tokens' queries turn
+ * into q_out, their keys turn on the way into the cache, their values go there
+ * as they are. Positions and pairs as in prism_rope (pos: [n_axes][pos_stride];
+ * n_axes 0 turns nothing and takes no pos), places in the cache as in
+ * prism_cache_append: a row out of range is not kept, its queries are turned all the
+ * same. Two rows for one slot leave that slot unspecified (parts of
+ * either, with any of their scales). n_heads query heads may be 0, which takes no q
+ * and q_out. q_out == q with equal strides works in place. Angles, sines and
+ * turns are held in 64 bits, so that two values next to each other fall to the
+ * same side of a border between 4-bit values as in exact arithmetic (a turned
+ * key is rounded to fp32, and then to its format). head_dim 16, 32, 64 or 128. */
+typedef struct prism_rope_append_push {
+    prism_cache_desc cache;
+    int32_t format;
+    int32_t n_new, n_heads;
+    int32_t n_axes; /* 0..4 */
+    int32_t pairs[4];
+    int32_t layout, ladder;
+    double base;
+    int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride;
+    int64_t v_token_stride, v_head_stride, out_token_stride, out_head_stride;
+    int64_t pos_stride;
+} prism_rope_append_push;
+int prism_rope_append(prism_ctx* ctx, const prism_rope_append_push* p, const void* q, const void* k, const void* v,
+                      const int32_t* pos, void* q_out, const int32_t* seq_of, const int32_t* pos_of,
+                      const int32_t* table, const prism_cache_pages* pages, void* stream);
+
+/* Read rows of the cache back: row i of k and v becomes token pos_of[i] of
+ * sequence seq_of[i], in dtype, whatever the format; zeros where sequence,
+ * position or page is out of range. Rows of several sequences one behind the
+ * other are what prism_seq_attn takes for keys that were kept before. */
+typedef struct prism_cache_read_push {
+    prism_cache_desc cache;
+    int32_t format;
+    int32_t n_rows;
+    int64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+} prism_cache_read_push;
+int prism_cache_read(prism_ctx* ctx, const prism_cache_read_push* p, const prism_cache_pages* pages,
+                     const int32_t* seq_of, const int32_t* pos_of, const int32_t* table, void* k, void* v,
+                     void* stream);
+
+/* prism_paged_attn over a cache of PRISM_CACHE_4. */
+int64_t prism_paged_attn4_workspace(const prism_paged_attn_push* p);
+int prism_paged_attn4(prism_ctx* ctx, const prism_paged_attn_push* p, const void* q, const prism_cache_pages* pages,
+                      const int32_t* table, const int32_t* lengths, void* out, void* workspace,
+                      int64_t workspace_bytes, void* stream);
+
+/* Linear attention with a decay for each head, along n_seqs sequences that lie
+ * one behind the other in n_tokens rows (cu: n_seqs + 1 starts, as in
+ * prism_seq_attn; NULL = equal lengths). A head h of a sequence has a state, fp32
+ * [head_dim of k][head_dim of v], and for its tokens in turn
+ *   S = exp(-rates[h]) S + k^T v,   out = scale q S.
+ * rates: fp32 [n_heads] on the device, 0 or more (less, or NaN, counts as 0;
+ * infinity keeps the newest token alone). Head h reads key head h / (n_heads /
+ * n_kv_heads). States are dense [n_states][n_heads][head_dim][head_dim], 16-byte
+ * aligned; sequence s starts from number state_of[s] of state_in and leaves its
+ * last one there in state_out (state_of NULL = s itself). A number out of range, or
+ * state_in NULL, starts from zeros; a number out of range is not written, nor
+ * anything if state_out is NULL. state_in may be state_out. Two sequences of
+ * one number leave it unspecified. A sequence without tokens copies its state.
+ * Rows of out outside the sequences stay as they were. scale is finite. Sums and
+ * states are fp32 and have to stay in its range; what a matrix product takes of a
+ * state or a weight has 16 significant bits or more, what it takes for the next
+ * state 21 or more. From its token on, an infinity or NaN in q makes NaN of its row and head, in
+ * v of its channel and in k of its whole head, of state_out too; earlier tokens
+ * and other sequences do not see it. workspace as in prism_paged_attn. head_dim 16, 32,
+ * 64 or 128; at most 2^30 rows. */
+typedef struct prism_linear_attn_push {
+    int32_t dtype, n_seqs, n_tokens, n_heads, n_kv_heads, head_dim;
+    int32_t n_states;
+    float scale;
+    int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride;
+    int64_t v_token_stride, v_head_stride, out_token_stride, out_head_stride;
+} prism_linear_attn_push;
+int64_t prism_linear_attn_workspace(const prism_linear_attn_push* p);
+int prism_linear_attn(prism_ctx* ctx, const prism_linear_attn_push* p, const void* q, const void* k, const void* v,
+                      const float* rates, const int32_t* cu, const int32_t* state_of, const float* state_in, void* out,
+                      float* state_out, void* workspace, int64_t workspace_bytes, void* stream);
+/* The same for one new token per sequence (n_tokens == n_seqs, row s is sequence
+ * s), in fp32 throughout. A row whose number is out of range gets zeros. state_in and
+ * state_out are needed. */
+int prism_linear_step(prism_ctx* ctx, const prism_linear_attn_push* p, const void* q, const void* k, const void* v,
+                      const float* rates, const int32_t* state_of, const float* state_in, void* out, float* state_out,
+                      void* stream);
+
 /* aux arena size in int32 elements that a router + expert pair needs for
  * n_experts experts and batch*n_tokens tokens when laid out as
  * [assignment | counts | perm]. */

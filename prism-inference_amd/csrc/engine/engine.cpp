@@ -129,11 +129,18 @@ extern "C" int prism_create(prism_ctx** out, int32_t device, const char* code_ob
         const std::string type = t == PRISM_BF16 ? "bf16" : "f16";
         all.emplace_back(&c->f_rope[t][0], "prism_rope_" + type);
         all.emplace_back(&c->f_rope[t][1], "prism_rope_" + type + "_loose");
+        all.emplace_back(&c->f_rope_append[t][0], "prism_rope_append_" + type);
+        all.emplace_back(&c->f_rope_append[t][1], "prism_rope_append4_" + type);
+        all.emplace_back(&c->f_cache_read[t][0], "prism_cache_read");
+        all.emplace_back(&c->f_cache_read[t][1], "prism_cache_read4_" + type);
         for (int i = 0; i < 4; ++i) {
             const std::string shape = type + "_h" + std::to_string(16 << i);
             for (int g = 0; g < 3; ++g)
                 all.emplace_back(&c->f_paged[t][i][g], "prism_paged_attn_" + shape + (g == 0 ? "_g1" : g == 1 ? "_g2" : "_many"));
             all.emplace_back(&c->f_paged_join[t][i], "prism_paged_attn_join_" + shape);
+            all.emplace_back(&c->f_paged4[t][i], "prism_paged_attn4_" + shape + "_many");
+            all.emplace_back(&c->f_linear[t][i], "prism_linear_attn_" + shape);
+            all.emplace_back(&c->f_linear_step[t][i], "prism_linear_step_" + shape);
             for (int w = 0; w < (i < 3 ? 3 : 2); ++w)
                 all.emplace_back(&c->f_seq[t][i][w], "prism_seq_attn_" + shape + (w == 0 ? "" : w == 1 ? "_w8" : "_narrow"));
         }

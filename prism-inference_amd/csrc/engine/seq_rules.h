@@ -140,6 +140,67 @@ inline int check_seq(const prism_seq_attn_push& p, const char** why) {
     return check_out(p.n_q, p.n_heads, p.head_dim, p.out_token_stride, p.out_head_stride, why);
 }
 
+inline int check_format(int32_t format, const char** why) {
+    return format == PRISM_CACHE_16 || format == PRISM_CACHE_4
+               ? PRISM_OK
+               : seq_bad(why, PRISM_ERR_INVALID, "format is neither PRISM_CACHE_16 nor PRISM_CACHE_4");
+}
+
+/* the turn of a rope_append push, as a rope push of `heads` heads */
+inline prism_rope_push turn_of(const prism_rope_append_push& p, int32_t heads, int64_t in_token, int64_t in_head) {
+    prism_rope_push r = {p.cache.dtype, p.n_new, heads, p.cache.head_dim, p.n_axes, {}, p.layout, p.ladder, 0, p.base,
+                         in_token, in_head, p.out_token_stride, p.out_head_stride, p.pos_stride};
+    for (int a = 0; a < 4; ++a) r.pairs[a] = p.pairs[a];
+    return r;
+}
+
+inline int check_rope_append(const prism_rope_append_push& p, const char** why) {
+    if (int rc = check_cache(p.cache, why)) return rc;
+    if (int rc = check_format(p.format, why)) return rc;
+    if (p.n_new < 0 || p.n_heads < 0 || p.n_heads > 65536)
+        return seq_bad(why, PRISM_ERR_INVALID, "n_new or n_heads out of range");
+    prism_rope_push turn = turn_of(p, 1, 0, 0);
+    turn.out_token_stride = turn.head_dim;
+    turn.out_head_stride = turn.head_dim;
+    turn.n_tokens = 0;
+    if (p.n_axes != 0)
+        if (int rc = check_rope(turn, why)) return rc;
+    const int64_t heads = p.cache.n_kv_heads;
+    if (int rc = check_strides(p.n_new, heads, p.k_token_stride, p.k_head_stride, why)) return rc;
+    if (int rc = check_strides(p.n_new, heads, p.v_token_stride, p.v_head_stride, why)) return rc;
+    if (p.n_heads == 0) return PRISM_OK;
+    if (int rc = check_strides(p.n_new, p.n_heads, p.q_token_stride, p.q_head_stride, why)) return rc;
+    return check_out(p.n_new, p.n_heads, p.cache.head_dim, p.out_token_stride, p.out_head_stride, why);
+}
+
+inline int check_cache_read(const prism_cache_read_push& p, const char** why) {
+    if (int rc = check_cache(p.cache, why)) return rc;
+    if (int rc = check_format(p.format, why)) return rc;
+    if (p.n_rows < 0) return seq_bad(why, PRISM_ERR_INVALID, "n_rows < 0");
+    const int64_t heads = p.cache.n_kv_heads;
+    if (int rc = check_out(p.n_rows, heads, p.cache.head_dim, p.k_token_stride, p.k_head_stride, why)) return rc;
+    return check_out(p.n_rows, heads, p.cache.head_dim, p.v_token_stride, p.v_head_stride, why);
+}
+
+inline int check_linear(const prism_linear_attn_push& p, const char** why) {
+    if (int rc = check_dtype(p.dtype, why)) return rc;
+    if (int rc = check_heads(p.n_heads, p.n_kv_heads, p.head_dim, why)) return rc;
+    if (p.n_seqs < 0 || p.n_tokens < 0 || p.n_states < 0)
+        return seq_bad(why, PRISM_ERR_INVALID, "n_seqs, n_tokens or n_states < 0");
+    if (p.n_tokens > SEQ_MAX_ROWS) return seq_bad(why, PRISM_ERR_UNSUPPORTED, "more than 2^30 rows");
+    if (!std::isfinite(p.scale)) return seq_bad(why, PRISM_ERR_INVALID, "scale is not finite");
+    if ((int64_t)std::max(p.n_states, p.n_seqs) * p.n_heads > SEQ_MAX_OFFSET / (p.head_dim * p.head_dim))
+        return seq_bad(why, PRISM_ERR_UNSUPPORTED, "states of more than 2^60 elements");
+    if (int rc = check_strides(p.n_tokens, p.n_heads, p.q_token_stride, p.q_head_stride, why)) return rc;
+    if (int rc = check_strides(p.n_tokens, p.n_kv_heads, p.k_token_stride, p.k_head_stride, why)) return rc;
+    if (int rc = check_strides(p.n_tokens, p.n_kv_heads, p.v_token_stride, p.v_head_stride, why)) return rc;
+    return check_out(p.n_tokens, p.n_heads, p.head_dim, p.out_token_stride, p.out_head_stride, why);
+}
+inline int check_linear_step(const prism_linear_attn_push& p, const char** why) {
+    if (int rc = check_linear(p, why)) return rc;
+    return p.n_tokens == p.n_seqs ? PRISM_OK : seq_bad(why, PRISM_ERR_INVALID, "a step has one token a sequence");
+}
+
 /* A launch's threads are counted in 32 bits. */
 inline bool seq_grid_ok(int64_t grid, unsigned threads) { return grid <= (int64_t)(UINT32_MAX / threads); }
 

@@ -211,6 +211,8 @@ typedef struct PagedAttnArgs {
     int32_t waves;          /* per item: 1, or 4 (a workgroup's)              */
     int32_t splits;         /* workgroups per item (waves = 4)                */
     float* ws;              /* splits > 1: [n_seqs][n_heads][splits][head_dim + 2] */
+    const uint8_t* k_scales; /* 4-bit pages: the pools above are theirs too    */
+    const uint8_t* v_scales;
 } PagedAttnArgs;
 
 #define SEQ_ROWS 128 /* queries x heads per workgroup of a sequence attention, */
@@ -229,5 +231,65 @@ typedef struct SeqAttnArgs {
     float scale_log2;       /* scale * log2(e) */
     int32_t tile_heads, tile_q; /* of a workgroup's rows; tile_heads * tile_q <= SEQ_ROWS, or SEQ_NARROW_ROWS */
 } SeqAttnArgs;
+
+/* ---- a cache of 4 bits, linear attention (cache4.hpp, paged_attn4.hpp, linear_attn.hpp) */
+
+/* powers that a 4-bit block may have: all its values are numbers of the type */
+#define FP4_LOW_F16   (-23)
+#define FP4_HIGH_F16  13
+#define FP4_LOW_BF16  (-125)
+#define FP4_HIGH_BF16 125
+
+typedef struct RopeAppendArgs {
+    const uint16_t* q;
+    const uint16_t* k;
+    const uint16_t* v;
+    uint16_t* q_out;
+    uint8_t* k_pages;       /* 16-bit or 4-bit */
+    uint8_t* v_pages;
+    uint8_t* k_scales;
+    uint8_t* v_scales;
+    const int32_t* pos;     /* axis a of token t at pos[a * pos_stride + t] */
+    const int32_t* table;   /* [n_seqs][table_pages] */
+    const int32_t* seq_of;  /* [n_new] */
+    const int32_t* pos_of;  /* [n_new] */
+    int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride;
+    int64_t v_token_stride, v_head_stride, out_token_stride, out_head_stride, pos_stride;
+    int32_t n_new, n_heads, n_kv_heads, head_dim;
+    int32_t n_pairs, tile, adjacent, axis_end[4], one_ladder; /* as RopeArgs */
+    int32_t n_seqs, page_log2, n_pages, table_pages;
+    double turn, log2_base;
+} RopeAppendArgs;
+
+typedef struct CacheReadArgs {
+    const uint8_t* k_pages;
+    const uint8_t* v_pages;
+    const uint8_t* k_scales;
+    const uint8_t* v_scales;
+    const int32_t* table;
+    const int32_t* seq_of;  /* [n_rows] */
+    const int32_t* pos_of;  /* [n_rows] */
+    uint16_t* k;
+    uint16_t* v;
+    int64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+    int32_t n_rows, n_seqs, n_kv_heads, head_dim;
+    int32_t page_log2, n_pages, table_pages;
+} CacheReadArgs;
+
+typedef struct LinearAttnArgs {
+    const uint16_t* q;
+    const uint16_t* k;
+    const uint16_t* v;
+    const float* rates;     /* [n_heads] */
+    const int32_t* cu;      /* [n_seqs + 1] or NULL */
+    const int32_t* state_of; /* [n_seqs] or NULL */
+    const float* state_in;  /* [n_states][n_heads][head_dim][head_dim] or NULL */
+    uint16_t* out;
+    float* state_out;       /* or NULL */
+    int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride;
+    int64_t v_token_stride, v_head_stride, out_token_stride, out_head_stride;
+    int32_t n_seqs, n_tokens, n_heads, n_kv_heads, n_states;
+    float scale;
+} LinearAttnArgs;
 
 #endif

@@ -35,6 +35,7 @@ ROPE_HALVES = 0
 ROPE_ADJACENT = 1
 ROPE_AXIS_LADDER = 0
 ROPE_ONE_LADDER = 1
+CACHE_16, CACHE_4 = 0, 1
 
 ROUTE_RANDOM = 0
 ROUTE_UNIFORM = 1
@@ -145,6 +146,33 @@ class SeqAttnPush(C.Structure):
                  "v_token_stride", "v_head_stride", "out_token_stride", "out_head_stride")]
 
 
+class CachePages(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scales", C.c_void_p), ("v_scales", C.c_void_p)]
+
+
+class RopeAppendPush(C.Structure):
+    _fields_ = [("cache", CacheDesc), ("format", C.c_int32), ("n_new", C.c_int32), ("n_heads", C.c_int32),
+                ("n_axes", C.c_int32), ("pairs", C.c_int32 * 4), ("layout", C.c_int32), ("ladder", C.c_int32),
+                ("base", C.c_double)] + \
+               [(n, C.c_int64) for n in
+                ("q_token_stride", "q_head_stride", "k_token_stride", "k_head_stride",
+                 "v_token_stride", "v_head_stride", "out_token_stride", "out_head_stride", "pos_stride")]
+
+
+class CacheReadPush(C.Structure):
+    _fields_ = [("cache", CacheDesc), ("format", C.c_int32), ("n_rows", C.c_int32), ("k_token_stride", C.c_int64),
+                ("k_head_stride", C.c_int64), ("v_token_stride", C.c_int64), ("v_head_stride", C.c_int64)]
+
+
+class LinearAttnPush(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in
+                ("dtype", "n_seqs", "n_tokens", "n_heads", "n_kv_heads", "head_dim", "n_states")] + \
+               [("scale", C.c_float)] + \
+               [(n, C.c_int64) for n in
+                ("q_token_stride", "q_head_stride", "k_token_stride", "k_head_stride",
+                 "v_token_stride", "v_head_stride", "out_token_stride", "out_head_stride")]
+
+
 # Every entry point the header declares: name -> (restype, argtypes)
 _P = C.c_void_p
 SIGNATURES = {
@@ -196,6 +224,16 @@ SIGNATURES = {
     "prism_paged_attn_workspace": (C.c_int64, [C.POINTER(PagedAttnPush)]),
     "prism_paged_attn": (C.c_int, [_P, C.POINTER(PagedAttnPush), _P, _P, _P, _P, _P, _P, _P, C.c_int64, _P]),
     "prism_seq_attn": (C.c_int, [_P, C.POINTER(SeqAttnPush), _P, _P, _P, _P, _P, _P, _P]),
+    "prism_rope_append": (C.c_int, [_P, C.POINTER(RopeAppendPush), _P, _P, _P, _P, _P, _P, _P, _P,
+                                    C.POINTER(CachePages), _P]),
+    "prism_cache_read": (C.c_int, [_P, C.POINTER(CacheReadPush), C.POINTER(CachePages), _P, _P, _P, _P, _P, _P]),
+    "prism_paged_attn4_workspace": (C.c_int64, [C.POINTER(PagedAttnPush)]),
+    "prism_paged_attn4": (C.c_int, [_P, C.POINTER(PagedAttnPush), _P, C.POINTER(CachePages), _P, _P, _P, _P, C.c_int64,
+                                    _P]),
+    "prism_linear_attn_workspace": (C.c_int64, [C.POINTER(LinearAttnPush)]),
+    "prism_linear_attn": (C.c_int, [_P, C.POINTER(LinearAttnPush), _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, C.c_int64,
+                                    _P]),
+    "prism_linear_step": (C.c_int, [_P, C.POINTER(LinearAttnPush), _P, _P, _P, _P, _P, _P, _P, _P, _P]),
     "prism_forward_e2e": (C.c_int, [_P, _P, _P, C.c_int32, _P]),
     "prism_forward_e2e_graph": (C.c_int, [_P, _P, _P, C.c_int32, _P]),
 }
@@ -678,6 +716,46 @@ class Engine:
     def seq_attn(self, push: SeqAttnPush, q: int, k: int, v: int, cu_q: int | None, cu_k: int | None, out: int,
                  stream: int | None = None):
         _check(self.L.prism_seq_attn(self.h, C.byref(push), q, k, v, cu_q, cu_k, out, stream), self.h)
+
+    def rope_append(self, push: RopeAppendPush, q: int | None, k: int, v: int, pos: int | None, q_out: int | None,
+                    seq_of: int, pos_of: int, table: int, pages: CachePages, stream: int | None = None):
+        _check(self.L.prism_rope_append(self.h, C.byref(push), q, k, v, pos, q_out, seq_of, pos_of, table,
+                                        C.byref(pages), stream), self.h)
+
+    def cache_read(self, push: CacheReadPush, pages: CachePages, seq_of: int, pos_of: int, table: int, k: int, v: int,
+                   stream: int | None = None):
+        _check(self.L.prism_cache_read(self.h, C.byref(push), C.byref(pages), seq_of, pos_of, table, k, v, stream),
+               self.h)
+
+    def paged_attn4_workspace(self, push: PagedAttnPush) -> int:
+        """Bytes of workspace that paged_attn4 needs for this push."""
+        n = self.L.prism_paged_attn4_workspace(C.byref(push))
+        if n < 0:
+            _check(int(n))
+        return n
+
+    def paged_attn4(self, push: PagedAttnPush, q: int, pages: CachePages, table: int, lengths: int, out: int,
+                    workspace: int | None, workspace_bytes: int, stream: int | None = None):
+        _check(self.L.prism_paged_attn4(self.h, C.byref(push), q, C.byref(pages), table, lengths, out, workspace,
+                                        workspace_bytes, stream), self.h)
+
+    def linear_attn_workspace(self, push: LinearAttnPush) -> int:
+        """Bytes of workspace that linear_attn needs for this push."""
+        n = self.L.prism_linear_attn_workspace(C.byref(push))
+        if n < 0:
+            _check(int(n))
+        return n
+
+    def linear_attn(self, push: LinearAttnPush, q: int, k: int, v: int, rates: int, cu: int | None,
+                    state_of: int | None, state_in: int | None, out: int, state_out: int | None,
+                    workspace: int | None, workspace_bytes: int, stream: int | None = None):
+        _check(self.L.prism_linear_attn(self.h, C.byref(push), q, k, v, rates, cu, state_of, state_in, out, state_out,
+                                        workspace, workspace_bytes, stream), self.h)
+
+    def linear_step(self, push: LinearAttnPush, q: int, k: int, v: int, rates: int, state_of: int | None,
+                    state_in: int, out: int, state_out: int, stream: int | None = None):
+        _check(self.L.prism_linear_step(self.h, C.byref(push), q, k, v, rates, state_of, state_in, out, state_out,
+                                        stream), self.h)
 
     def chain_launch_times(self, x: int, y: int, batch: int, stream: int | None = None):
         """prism_chain_launch_times: (attention ms, expert ms, attention grid,
