@@ -102,6 +102,7 @@ struct prism_ctx {
     hipFunction_t f_cache_read[2][2] = {};  /* [dtype][16, 4 bits] */
     hipFunction_t f_paged4[2][4] = {};      /* [dtype][head_dim] */
     hipFunction_t f_linear[2][4] = {};
+    hipFunction_t f_linear_states[2][4] = {};
     hipFunction_t f_linear_step[2][4] = {};
     std::string err;
 

@@ -140,6 +140,7 @@ extern "C" int prism_create(prism_ctx** out, int32_t device, const char* code_ob
             all.emplace_back(&c->f_paged_join[t][i], "prism_paged_attn_join_" + shape);
             all.emplace_back(&c->f_paged4[t][i], "prism_paged_attn4_" + shape + "_many");
             all.emplace_back(&c->f_linear[t][i], "prism_linear_attn_" + shape);
+            all.emplace_back(&c->f_linear_states[t][i], "prism_linear_states_" + shape);
             all.emplace_back(&c->f_linear_step[t][i], "prism_linear_step_" + shape);
             for (int w = 0; w < (i < 3 ? 3 : 2); ++w)
                 all.emplace_back(&c->f_seq[t][i][w], "prism_seq_attn_" + shape + (w == 0 ? "" : w == 1 ? "_w8" : "_narrow"));

@@ -201,6 +201,30 @@ inline int check_linear_step(const prism_linear_attn_push& p, const char** why) 
     return p.n_tokens == p.n_seqs ? PRISM_OK : seq_bad(why, PRISM_ERR_INVALID, "a step has one token a sequence");
 }
 
+/* How a linear attention is launched: tokens of a segment, and segments (some of them empty). Sequences of one segment each need no
+ * first launch and no workspace. */
+struct LinearPlan {
+    int32_t segment;
+    bool split;
+    int64_t segments;
+};
+inline LinearPlan linear_plan(const prism_linear_attn_push& p) {
+    LinearPlan r = {INT32_MAX, false, std::max(p.n_seqs, 1)};
+    const int64_t n_seqs = std::max(p.n_seqs, 1), each = p.n_tokens / n_seqs;
+    const int64_t want = 768, least = 128; /* workgroups; tokens */
+    if (n_seqs * p.n_heads >= want || each < 2 * least) return r;
+    int64_t s = (int64_t)p.n_tokens * p.n_heads / want;
+    s = std::max(s, std::max(least, each / 32));
+    s = (s + LINEAR_CHUNK - 1) / LINEAR_CHUNK * LINEAR_CHUNK;
+    r.segment = (int32_t)s;
+    r.split = true;
+    r.segments = p.n_tokens / s + n_seqs;
+    return r;
+}
+inline int64_t linear_workspace(const prism_linear_attn_push& p, const LinearPlan& r) {
+    return r.split ? r.segments * p.n_heads * p.head_dim * p.head_dim * 4 : 0;
+}
+
 /* A launch's threads are counted in 32 bits. */
 inline bool seq_grid_ok(int64_t grid, unsigned threads) { return grid <= (int64_t)(UINT32_MAX / threads); }
 

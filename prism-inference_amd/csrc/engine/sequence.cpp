@@ -410,7 +410,7 @@ extern "C" int64_t prism_linear_attn_workspace(const prism_linear_attn_push* p) 
     const char* why = "";
     const int rc = check_linear(*p, &why);
     if (rc) return fail(nullptr, rc, "linear attention: %s", why);
-    return 0;
+    return linear_workspace(*p, linear_plan(*p));
 }
 
 extern "C" int prism_linear_attn(prism_ctx* c, const prism_linear_attn_push* p, const void* q, const void* k, const void* v,
@@ -424,10 +424,20 @@ extern "C" int prism_linear_attn(prism_ctx* c, const prism_linear_attn_push* p, 
         return fail(c, PRISM_ERR_INVALID, "%s: %d sequences of equal length do not fill the rows", what, p->n_seqs);
     if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || !aligned16(state_in) || !aligned16(state_out))
         return fail(c, PRISM_ERR_INVALID, "%s: buffers must be 16-byte aligned", what);
-    (void)workspace;
-    (void)workspace_bytes;
+    const LinearPlan plan = linear_plan(*p);
+    const int64_t need = linear_workspace(*p, plan);
+    if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
+        return fail(c, PRISM_ERR_INVALID, "%s: workspace of %lld bytes, %lld needed, 16-byte aligned", what,
+                    workspace ? (long long)workspace_bytes : 0LL, (long long)need);
     LinearAttnArgs a = linear_args(p, q, k, v, rates, cu, state_of, state_in, out, state_out);
-    return launch(c, c->f_linear[p->dtype][hd_index(p->head_dim)], what, (int64_t)p->n_seqs * p->n_heads, 256, &a, stream);
+    a.segment = plan.segment;
+    a.ws = static_cast<float*>(workspace);
+    const int i = hd_index(p->head_dim);
+    const unsigned threads = p->head_dim >= 64 ? 2 * p->head_dim : 64;
+    const int64_t grid = plan.segments * p->n_heads;
+    if (plan.split)
+        if (const int rc = launch(c, c->f_linear_states[p->dtype][i], what, grid, threads, &a, stream)) return rc;
+    return launch(c, c->f_linear[p->dtype][i], what, grid, threads, &a, stream);
 }
 
 extern "C" int prism_linear_step(prism_ctx* c, const prism_linear_attn_push* p, const void* q, const void* k, const void* v,

@@ -276,6 +276,7 @@ typedef struct CacheReadArgs {
     int32_t page_log2, n_pages, table_pages;
 } CacheReadArgs;
 
+#define LINEAR_CHUNK 64 /* tokens that a linear attention takes at a time */
 typedef struct LinearAttnArgs {
     const uint16_t* q;
     const uint16_t* k;
@@ -289,7 +290,9 @@ typedef struct LinearAttnArgs {
     int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride;
     int64_t v_token_stride, v_head_stride, out_token_stride, out_head_stride;
     int32_t n_seqs, n_tokens, n_heads, n_kv_heads, n_states;
+    int32_t segment;        /* tokens of a sequence that one workgroup goes through */
     float scale;
+    float* ws;              /* segments' states: [n_tokens / segment + n_seqs][n_heads][head_dim^2] */
 } LinearAttnArgs;
 
 #endif
