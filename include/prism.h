@@ -591,9 +591,10 @@ typedef struct prism_cache_pages {
  * same. Two rows for one slot leave that slot unspecified (parts of
  * either, with any of their scales). n_heads query heads may be 0, which takes no q
  * and q_out. q_out == q with equal strides works in place. Angles, sines and
- * turns are held in 64 bits, so that two values next to each other fall to the
- * same side of a border between 4-bit values as in exact arithmetic (a turned
- * key is rounded to fp32, and then to its format). head_dim 16, 32, 64 or 128. */
+ * cosines are taken in 64 bits. Queries and 16-bit keys turn in 32, 4-bit keys
+ * in 64 (rounded to fp32, and then to 4 bits), so that they fall to the same
+ * side of a border between two 4-bit values as in exact arithmetic. head_dim 16,
+ * 32, 64 or 128. */
 typedef struct prism_rope_append_push {
     prism_cache_desc cache;
     int32_t format;

@@ -244,6 +244,14 @@ inline int rope_tile(int64_t n_tokens, int n_pairs) {
     return tile;
 }
 
+/* The same for a launch that appends. */
+inline int append_tile(int64_t n_new, int head_dim) {
+    const int most = APPEND_TILE_CHANNELS / head_dim;
+    int tile = 1;
+    while (2 * tile <= most && n_new >= (int64_t)2 * tile * 4 * 256) tile *= 2;
+    return tile;
+}
+
 /* How a paged attention is launched. */
 struct PagedPlan {
     bool many;      /* the MFMA kernel */

@@ -240,6 +240,7 @@ typedef struct SeqAttnArgs {
 #define FP4_LOW_BF16  (-125)
 #define FP4_HIGH_BF16 125
 
+#define APPEND_TILE_CHANNELS 1024 /* of a workgroup's tokens together, one head's */
 typedef struct RopeAppendArgs {
     const uint16_t* q;
     const uint16_t* k;
@@ -256,7 +257,8 @@ typedef struct RopeAppendArgs {
     int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride;
     int64_t v_token_stride, v_head_stride, out_token_stride, out_head_stride, pos_stride;
     int32_t n_new, n_heads, n_kv_heads, head_dim;
-    int32_t n_pairs, tile, adjacent, axis_end[4], one_ladder; /* as RopeArgs */
+    int32_t n_pairs, adjacent, axis_end[4], one_ladder; /* as RopeArgs */
+    int32_t tile;           /* tokens per workgroup */
     int32_t n_seqs, page_log2, n_pages, table_pages;
     double turn, log2_base;
 } RopeAppendArgs;

@@ -52,30 +52,63 @@ __device__ __forceinline__ int64_t cache_slot(const Args& a, int s, int pos) {
     return (((int64_t)page * a.n_kv_heads) << a.page_log2) + (pos & ((1 << a.page_log2) - 1));
 }
 
-/* 8 channels of a row that turns, from channel c on: x as it is kept, y in fp32. cs: cos and sin of the token's pairs. */
+/* 8 values from anywhere in a row. */
 template <class T>
-__device__ __forceinline__ void turned8(const RopeAppendArgs& a, const uint16_t* row, int c, const double2* cs,
-                                        typename T::v8& x, float (&y)[8]) {
-    const int n = a.n_pairs;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const int at = c + e;
-        if (at < 2 * n) {
-            const bool second = a.adjacent ? at & 1 : at >= n;
-            const int pair = a.adjacent ? at >> 1 : second ? at - n : at;
-            const double other = ld1<T>(row + (a.adjacent ? at ^ 1 : second ? at - n : at + n));
-            const double2 k = cs[pair];
-            y[e] = (float)__builtin_fma((double)y[e], k.x, second ? other * k.y : -(other * k.y));
-            x[e] = (typename T::el)opaque(y[e]);
-        }
-    }
+__device__ __forceinline__ typename T::v8 ld8_any(const uint16_t* p) {
+    typename T::v8 v;
+    __builtin_memcpy(&v, p, 16);
+    return v;
+}
+/* v moved up by s elements (1 to 7), the lowest undefined */
+template <class V>
+__device__ __forceinline__ V shift_up(V v, int s) {
+    union {
+        V v;
+        uint64_t w[2];
+    } x{v}, y;
+    const int bits = 16 * (s & 3);
+    y.w[0] = x.w[0] << bits;
+    y.w[1] = s >= 4 ? x.w[0] << bits : x.w[1] << bits | (bits ? x.w[0] >> (64 - bits) : 0);
+    return y.v;
 }
 
+/* A chunk of 8 channels from c on of a row: itself, and the channels that its own turn with. */
+template <class T>
+struct Turned8 {
+    typename T::v8 x, other;
+};
+template <class T>
+__device__ __forceinline__ Turned8<T> turn_load(const RopeAppendArgs& a, const uint16_t* row, int c, bool turns) {
+    Turned8<T> r;
+    r.x = ld8<T>(row + c);
+    r.other = r.x;
+    const int n = a.n_pairs;
+    if (!a.adjacent && turns && c < 2 * n) {
+        /* All 8 of the first half: n channels on (16 more fit the row: n is at most head_dim / 2). The second: n back. The
+           chunk with the border inside has both, of which the second half's would begin before the row. */
+        r.other = ld8_any<T>(row + (c < n ? c + n : c - n));
+        if (c < n && c + 8 > n) {
+            const typename T::v8 back = shift_up(ld8<T>(row), n & 7);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) r.other[e] = e >= (n & 7) ? back[e] : r.other[e];
+        }
+    }
+    return r;
+}
+
+/* Tokens by a workgroup as in rope.hpp; the table holds for each channel what it is times and what its partner is times
+ * (cos, and sin with its sign), as [token][channel % 8][channel / 8], so that lanes with chunks side by side read
+ * side by side. A 4-bit key is turned in 64 bits, from a table of its own. */
 template <class T, bool FOUR>
 __device__ __forceinline__ void rope_append_body(const RopeAppendArgs& a) {
-    __shared__ __attribute__((aligned(16))) double2 cs[ROPE_TILE_PAIRS]; /* [token][np] cos, sin */
+    typedef typename T::v8 v8;
+    typedef typename T::el el;
+    constexpr int U = 2;
+    __shared__ __attribute__((aligned(16))) float2 cs[APPEND_TILE_CHANNELS];
+    __shared__ __attribute__((aligned(16))) double2 cs64[FOUR ? APPEND_TILE_CHANNELS : 1];
     __shared__ double turns[64];
-    const int n = a.n_pairs, np = (n + 7) & ~7;
+    __shared__ int64_t slots[APPEND_TILE_CHANNELS / 16];
+    const int n = a.n_pairs, hd = a.head_dim, chunks = hd / 8, lc = __builtin_ctz(chunks);
     const int t0 = blockIdx.x * a.tile, tokens = min(a.tile, a.n_new - t0);
     const auto axis_of = [&](int j) { return (j >= a.axis_end[0]) + (j >= a.axis_end[1]) + (j >= a.axis_end[2]); };
     if (threadIdx.x < n) {
@@ -83,69 +116,111 @@ __device__ __forceinline__ void rope_append_body(const RopeAppendArgs& a) {
         const double e = a.one_ladder ? (double)j / n : (double)(j - first) / (a.axis_end[axis] - first);
         turns[j] = a.turn * exp2(-e * a.log2_base);
     }
+    if (a.n_kv_heads > 0 && threadIdx.x < tokens)
+        slots[threadIdx.x] = cache_slot(a, a.seq_of[t0 + threadIdx.x], a.pos_of[t0 + threadIdx.x]);
     __syncthreads();
-    for (int i = threadIdx.x; i < tokens * np; i += 256) {
-        const int t = i / np, j = i - t * np;
-        if (j < n) {
-            const double rev = (double)a.pos[axis_of(j) * a.pos_stride + t0 + t] * turns[j];
-            double s, c;
-            sincospi(2.0 * (rev - rint(rev)), &s, &c);
-            cs[i] = double2{c, s};
+    for (int i = threadIdx.x; i < tokens * n; i += 256) {
+        const int t = i / n, j = i - t * n;
+        const double rev = (double)a.pos[axis_of(j) * a.pos_stride + t0 + t] * turns[j];
+        double s, c;
+        sincospi(2.0 * (rev - rint(rev)), &s, &c);
+        const int c1 = a.adjacent ? 2 * j : j, c2 = a.adjacent ? c1 + 1 : j + n;
+        const int i1 = t * hd + c1 % 8 * chunks + c1 / 8, i2 = t * hd + c2 % 8 * chunks + c2 / 8;
+        cs[i1] = float2{(float)c, -(float)s};
+        cs[i2] = float2{(float)c, (float)s};
+        if constexpr (FOUR) {
+            cs64[i1] = double2{c, -s};
+            cs64[i2] = double2{c, s};
         }
     }
     __syncthreads();
-    const int chunks = a.head_dim / 8, H = a.n_heads, K = a.n_kv_heads;
-    const int per_token = (H + 2 * K) * chunks, units = tokens * per_token;
-    const int block = FOUR ? min(chunks, 4) : 1; /* chunks of a 4-bit block */
-    for (int u = threadIdx.x; u < units; u += 256) { /* a block's lanes are together: chunks is a power of two */
-        const int t = u / per_token, r = u - t * per_token, row = r / chunks, c = r % chunks * 8;
-        const int64_t tok = t0 + t;
-        const bool query = row < H, value = row >= H + K;
-        const int h = query ? row : value ? row - H - K : row - H;
-        const uint16_t* x = query   ? a.q + tok * a.q_token_stride + h * a.q_head_stride
-                            : value ? a.v + tok * a.v_token_stride + h * a.v_head_stride
-                                    : a.k + tok * a.k_token_stride + h * a.k_head_stride;
-        typename T::v8 o = ld8<T>(x + c);
-        float y[8];
+    const int H = a.n_heads, K = a.n_kv_heads;
+    const int per_token = (H + 2 * K) << lc;
+    const int block = FOUR ? min(chunks, 4) : 1; /* chunks of a 4-bit block: lanes side by side, chunks is a power of two */
+    const int dt = 256 / per_token, dr = 256 % per_token;
+    int t = threadIdx.x / per_token, r = threadIdx.x % per_token;
+    while (t < tokens) {
+        Turned8<T> v[U];
+        int tt[U], row[U], c[U];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = (float)o[e];
-        if (!value) turned8<T>(a, x, c, cs + t * np, o, y);
+        for (int u = 0; u < U; ++u) {
+            tt[u] = t < tokens ? t : -1;
+            row[u] = r >> lc;
+            c[u] = (r & (chunks - 1)) * 8;
+            const int64_t tok = t0 + min(t, tokens - 1); /* past the end: read, not written */
+            const uint16_t* x = row[u] < H     ? a.q + tok * a.q_token_stride + row[u] * a.q_head_stride
+                                : row[u] < H + K ? a.k + tok * a.k_token_stride + (row[u] - H) * a.k_head_stride
+                                               : a.v + tok * a.v_token_stride + (row[u] - H - K) * a.v_head_stride;
+            v[u] = turn_load<T>(a, x, c[u], row[u] < H + K);
+            t += dt;
+            r += dr;
+            if (r >= per_token) {
+                r -= per_token;
+                ++t;
+            }
+        }
         /* in place, a row's lanes, which are in one wave, have all read before one writes */
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
-        if (query) st8<T>(a.q_out + tok * a.out_token_stride + h * a.out_head_stride + c, o);
-        float top = 0.f;
-        bool fine = true;
-        if constexpr (FOUR) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                top = fmaxf(top, fabsf(y[e]));
-                fine = fine && fabsf(y[e]) < INFINITY;
+        for (int u = 0; u < U; ++u) {
+            if (tt[u] < 0) continue;
+            const bool query = row[u] < H, value = row[u] >= H + K;
+            const int h = query ? row[u] : value ? row[u] - H - K : row[u] - H;
+            v8 o = v[u].x;
+            if (a.adjacent) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[u].other[e] = v[u].x[e ^ 1];
             }
-            top = fine ? top : INFINITY;
-            for (int w = 1; w < block; w *= 2) top = fmaxf(top, __shfl_xor(top, w));
-        }
-        const int64_t slot = query ? -1 : cache_slot(a, a.seq_of[tok], a.pos_of[tok]);
-        if (slot < 0) continue;
-        const int64_t at = slot + ((int64_t)h << a.page_log2);
-        if constexpr (!FOUR) {
-            st8<T>(reinterpret_cast<uint16_t*>(value ? a.v_pages : a.k_pages) + at * a.head_dim + c, o);
-        } else {
-            const uint32_t bits = __builtin_bit_cast(uint32_t, top);
-            /* 1.75 * 2^k = 7 * 2^(k-2) */
-            int e = (int)(bits >> 23) - 129 + ((bits & 0x7FFFFFu) > 0x600000u);
-            e = seq_clamp(e, Fp4<T>::low, Fp4<T>::high);
-            uint32_t w = 0;
-            if (top < INFINITY) {
+            float y[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] = (float)o[e];
+            if (!value) {
+                const int at = tt[u] * hd + c[u] / 8;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    if (c[u] + e >= 2 * n) break;
+                    const float other = (float)v[u].other[e];
+                    if (!FOUR || query) {
+                        const float2 k = cs[at + e * chunks];
+                        y[e] = __builtin_fmaf(y[e], k.x, other * k.y);
+                    } else {
+                        const double2 k = cs64[at + e * chunks];
+                        y[e] = (float)__builtin_fma((double)y[e], k.x, (double)other * k.y);
+                    }
+                    o[e] = (el)opaque(y[e]);
+                }
+            }
+            if (query) {
+                st8<T>(a.q_out + (t0 + tt[u]) * a.out_token_stride + h * a.out_head_stride + c[u], o);
+                continue;
+            }
+            const int64_t slot = slots[tt[u]];
+            const int64_t at = slot + ((int64_t)h << a.page_log2);
+            if constexpr (!FOUR) {
+                if (slot >= 0) st8<T>(reinterpret_cast<uint16_t*>(value ? a.v_pages : a.k_pages) + at * hd + c[u], o);
+            } else {
+                float top = 0.f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) top = vmax(top, __builtin_fabsf(y[e])); /* NaN stays */
+                top = vmax(top, dpp<0xB1>(top));
+                if (block == 4) top = vmax(top, dpp<0x4E>(top));
+                if (slot < 0) continue;
+                const uint32_t bits = __builtin_bit_cast(uint32_t, top);
+                /* 1.75 * 2^k = 7 * 2^(k-2) */
+                int e = (int)(bits >> 23) - 129 + ((bits & 0x7FFFFFu) > 0x600000u);
+                e = seq_clamp(e, Fp4<T>::low, Fp4<T>::high);
+                const bool fine = top < INFINITY;
+                uint32_t w = 0;
                 const float s = fp4_scale(e + 127);
                 w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, y[0], y[1], s, 0);
                 w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, y[2], y[3], s, 1);
                 w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, y[4], y[5], s, 2);
                 w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, y[6], y[7], s, 3);
+                *reinterpret_cast<uint32_t*>((value ? a.v_pages : a.k_pages) + at * (hd / 2) + c[u] / 2) = fine ? w : 0;
+                if ((c[u] / 8 & (block - 1)) == 0)
+                    (value ? a.v_scales : a.k_scales)[at * (chunks / block) + c[u] / 8 / block] = fine ? (uint8_t)(e + 127) : 255;
             }
-            *reinterpret_cast<uint32_t*>((value ? a.v_pages : a.k_pages) + at * (a.head_dim / 2) + c / 2) = w;
-            if (c / 8 % block == 0)
-                (value ? a.v_scales : a.k_scales)[at * (chunks / block) + c / 8 / block] = top < INFINITY ? (uint8_t)(e + 127) : 255;
         }
     }
 }

@@ -49,9 +49,11 @@ def dequantise(codes, scales):
     return (v.reshape(scales.shape + (v.shape[-1] // scales.shape[-1],)) * s[..., None]).reshape(v.shape)
 
 
-def turned(x, pos, pairs, layout, ladder, base):
+def turned(x, pos, pairs, layout, ladder, base, bits=64):
     """x [tokens][heads][hd], pos [axes][tokens] -> (turned, bound without the rounding to a type). Angle: 2^-51 of its
-    size here and there; sin, cos, products in 64 bits: 2^-50; the result in fp32: 2^-24."""
+    size here and there; sin, cos, products in 64 bits: 2^-50; the result in fp32: 2^-24. In 32 bits (queries, keys that
+    stay 16-bit) cos and sin are rounded by 2^-25 at most, the first product by 2^-24 of it: (|u| + |w|) 2^-23 more."""
+    more = 2.0 ** -23 if bits == 32 else 0.0
     n, y, bound = sum(pairs), x.copy(), np.zeros_like(x)
     i = 0
     for axis, count in enumerate(pairs):
@@ -62,7 +64,7 @@ def turned(x, pos, pairs, layout, ladder, base):
             u, w = x[..., a], x[..., b]
             y[..., a], y[..., b] = u * np.cos(phi) - w * np.sin(phi), w * np.cos(phi) + u * np.sin(phi)
             for c in (a, b):
-                bound[..., c] = (np.abs(u) + np.abs(w)) * (np.abs(phi) * 2.0 ** -50 + 2.0 ** -49) + 2.0 ** -24 * np.abs(y[..., c])
+                bound[..., c] = (np.abs(u) + np.abs(w)) * (np.abs(phi) * 2.0 ** -50 + 2.0 ** -49 + more) + 2.0 ** -24 * np.abs(y[..., c])
             i += 1
     return y, bound
 

@@ -83,9 +83,9 @@ def test_rope_append_and_read(engine, dev, four, dtype, layout, lens, heads, kv,
     print(f"[rope append] {dtype} 4 bits {four} layout {layout} {len(seq)} x {heads} + 2 x {kv} x {hd} {pairs}", flush=True)
     got, pages = append(engine, dev, cache, rows, heads, seq, at, pos, pairs, layout, ladder)
     x = values(rows, dtype)
-    y, bound = turned(x[:, :heads + kv], pos, pairs, layout, ladder, 10000.0)
+    y, bound = turned(x[:, :heads + kv], pos, pairs, layout, ladder, 10000.0, 64 if four else 32)
     if heads:
-        b = bound + HALF_STEP[dtype] * np.abs(y) + SMALLEST[dtype]
+        b = turned(x[:, :heads + kv], pos, pairs, layout, ladder, 10000.0, 32)[1] + HALF_STEP[dtype] * np.abs(y) + SMALLEST[dtype]
         assert not outside(values(got, dtype), y[:, :heads], b[:, :heads])
         assert (got[..., 2 * sum(pairs):] == rows[:, :heads, 2 * sum(pairs):]).all()  # copied bits
     pools = cache.got(dev)
