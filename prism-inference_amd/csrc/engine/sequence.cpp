@@ -433,7 +433,7 @@ extern "C" int prism_linear_attn(prism_ctx* c, const prism_linear_attn_push* p, 
     a.segment = plan.segment;
     a.ws = static_cast<float*>(workspace);
     const int i = hd_index(p->head_dim);
-    const unsigned threads = p->head_dim >= 64 ? 2 * p->head_dim : 64;
+    const unsigned threads = 4 * p->head_dim; /* a wave for 16 channels of the values */
     const int64_t grid = plan.segments * p->n_heads;
     if (plan.split)
         if (const int rc = launch(c, c->f_linear_states[p->dtype][i], what, grid, threads, &a, stream)) return rc;

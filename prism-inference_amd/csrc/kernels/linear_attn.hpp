@@ -40,17 +40,17 @@ __device__ __forceinline__ LinearTile linear_tile(const LinearAttnArgs& a, int b
     }
 }
 
-/* Two fp32 numbers as N pairs of 16-bit ones that add up to them: fp16 11 N bits (of what is above its smallest), bf16 8 N. */
+/* Two fp32 numbers as N pairs of 16-bit ones that add up to them: fp16 11 N bits (of what is above its smallest), bf16 8 N.
+ * Rounded to nearest, so that what is left has a sign and half a bit more. */
 template <class T, int N>
-__device__ __forceinline__ void parts(float x, float y, typename T::v2 (&p)[N]) {
+__device__ __forceinline__ void parts(float x, float y, uint32_t (&p)[N]) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        x = opaque(x);
-        y = opaque(y);
-        p[i] = typename T::v2{(typename T::el)x, (typename T::el)y};
+        const typename T::v2 v = {(typename T::el)x, (typename T::el)y};
+        p[i] = __builtin_bit_cast(uint32_t, v);
         if (i + 1 < N) {
-            x -= (float)p[i][0];
-            y -= (float)p[i][1];
+            x -= (float)v[0];
+            y -= (float)v[1];
         }
     }
 }
@@ -62,24 +62,45 @@ __device__ __forceinline__ float part_scale(float m) {
 __device__ __forceinline__ float part_unscale(float scale) { /* of a power of two: 1 / scale */
     return __builtin_bit_cast(float, 0x7F000000u - __builtin_bit_cast(unsigned, scale));
 }
+/* The larger of each half of two words of 16-bit values, as whole numbers. */
+typedef unsigned short us2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t most2(uint32_t a, uint32_t b) {
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(us2, a), __builtin_bit_cast(us2, b)));
+}
+/* The largest magnitude of 8 values, its bits; 2 words side by side */
+template <class V>
+__device__ __forceinline__ uint32_t most8(V v) {
+    const u4 w = __builtin_bit_cast(u4, v) & 0x7FFF7FFFu;
+    return most2(most2(w[0], w[1]), most2(w[2], w[3]));
+}
+template <class T>
+__device__ __forceinline__ bool infinite(uint32_t most) { /* bits of magnitudes, two of them */
+    constexpr uint32_t inf = __is_same(T, F16) ? 0x7C00 : 0x7F80;
+    return (most & 0xFFFF) >= inf || most >> 16 >= inf;
+}
 
-/* One segment of one head: its chunks in turn, the state in registers. STATES: only the state that the segment adds. */
+/* One segment of one head: its chunks of 64 tokens in turn,
+ *   o_i = scale (e^(-r (i+1)) q_i S + sum_{j <= i} e^(-r (i-j)) (q_i k_j) v_j),  S' = e^(-r n) S + sum_j k_j^T e^(-r (n-1-j)) v_j
+ * A wave has 16 channels of the values, so its part of the state is its own and stays in registers: 16 x 16 tiles as the
+ * product leaves them, which are at the same time what the next chunk's product q S takes. The weights (q_i k_j) are all
+ * waves' work and go through LDS. STATES: only the state that the segment adds. */
 template <class T, int HD, bool STATES>
 __device__ __forceinline__ void linear_segment(const LinearAttnArgs& a) {
     typedef typename T::v8 v8;
     typedef typename T::v4 v4;
-    typedef typename T::v2 v2;
     typedef typename T::el el;
     constexpr bool HALF = __is_same(T, F16);
     constexpr int C = LINEAR_CHUNK, QT = C / 16, M = C / 32;
-    constexpr int NW = HD >= 64 ? HD / 32 : 1, NT = 64 * NW; /* waves, threads */
-    constexpr int DV = HD >= 32 ? 2 : 1, DK = HD / 16;       /* 16-channel tiles of a wave's values, of keys */
+    constexpr int NW = HD / 16, NT = 64 * NW; /* waves, threads */
+    constexpr int DK = HD / 16;               /* 16-channel tiles of the keys */
     constexpr int KS = (HD + 31) / 32;
-    constexpr int RS = HD >= 32 ? HD + 16 : HD; /* LDS row */
-    constexpr int CPR = HD / 8, NL = C * CPR / NT; /* 16-byte chunks a row, and a thread's of a matrix */
+    constexpr int RS = HD >= 32 ? HD + 16 : HD;    /* LDS row: 4 rows' parts of a transposed read lie in different banks */
+    constexpr int CPR = HD / 8, NL = C * CPR / NT; /* 16-byte chunks a row, and a thread's of a matrix: 2 */
     constexpr int VP = HALF ? 2 : 3;               /* parts of a decayed value */
+    constexpr int TILES = QT * (QT + 1) / 2;       /* of weights */
     __shared__ __attribute__((aligned(16))) uint16_t lq[STATES ? 8 : C * RS], lk[C * RS], lv[C * RS];
-    __shared__ int lbad[2];
+    __shared__ __attribute__((aligned(16))) uint16_t lw[STATES ? 8 : QT * M * 2 * 64 * 8]; /* weights [query tile][32 keys][part] */
+    __shared__ uint32_t lmost[2][3]; /* of a chunk: an infinite value; fp16: the largest query, key */
     const int lane = lane_id(), l16 = lane & 15, g = lane >> 4, tid = threadIdx.x;
     const int wave = NW == 1 ? 0 : __builtin_amdgcn_readfirstlane(tid >> 6);
     const int b = blockIdx.x / a.n_heads, h = blockIdx.x % a.n_heads, hk = h / (a.n_heads / a.n_kv_heads);
@@ -93,35 +114,36 @@ __device__ __forceinline__ void linear_segment(const LinearAttnArgs& a) {
     const float r2 = linear_rate(a, h);
     const auto decay = [&](int n) { return fast_exp2(-r2 * (float)n); };
     const int number = linear_state(a, lt.seq);
-    const int64_t base = ((int64_t)max(number, 0) * a.n_heads + h) * HD * HD + 32 * wave + l16;
+    const int64_t base = ((int64_t)max(number, 0) * a.n_heads + h) * HD * HD + 16 * wave + l16;
     f4* const mine = reinterpret_cast<f4*>(a.ws) + ((int64_t)b * a.n_heads + h) * (HD * HD / 4) + tid; /* + NT * tile */
-    f4 S[DK][DV];
-    /* the state before the segment */
+    f4 S[DK]; /* channels 16 j + 4 g + e of the keys x channel 16 wave + l16 of the values */
 #pragma unroll
     for (int j = 0; j < DK; ++j)
 #pragma unroll
-        for (int d = 0; d < DV; ++d)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                S[j][d][e] = !STATES && a.state_in && number >= 0 ? a.state_in[base + (16 * j + 4 * g + e) * HD + 16 * d] : 0.f;
+        for (int e = 0; e < 4; ++e)
+            S[j][e] = !STATES && a.state_in && number >= 0 ? a.state_in[base + (16 * j + 4 * g + e) * HD] : 0.f;
     if constexpr (!STATES) {
         const float keep = decay(a.segment);
         for (int s = seg; s > 0; --s) {
             const f4* u = mine - (int64_t)s * a.n_heads * (HD * HD / 4);
 #pragma unroll
-            for (int j = 0; j < DK; ++j)
-#pragma unroll
-                for (int d = 0; d < DV; ++d) S[j][d] = S[j][d] * keep + u[NT * (j * DV + d)];
+            for (int j = 0; j < DK; ++j) S[j] = S[j] * keep + u[NT * j];
         }
     }
-    /* decays: of a key within a query's tile and in the tile before it, of a token up to the chunk's end */
+    /* decays: of a key in a query's tile, and in the tile before; of the state; of a token up to the chunk's end */
     float within[4], before[4], fade[M][8];
-    const float d16 = decay(16);
+    const float since = decay(l16 + 1) * a.scale;
+    if constexpr (!STATES) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const int gap = l16 - 4 * g - e;
-        within[e] = gap >= 0 ? decay(max(gap, 0)) * a.scale : 0.f;
-        before[e] = decay(16 + gap) * a.scale;
+        for (int e = 0; e < 4; ++e) {
+            const int gap = l16 - 4 * g - e;
+            within[e] = gap >= 0 ? decay(max(gap, 0)) * a.scale : 0.f;
+            before[e] = decay(16 + gap) * a.scale;
+        }
+        /* keys behind a tile's queries, in the 32 that it has a part of */
+        for (int qt = 0; qt < QT; qt += 2)
+            for (int x = tid; x < 128; x += NT)
+                *reinterpret_cast<uint64_t*>(lw + (((qt * M + qt / 2) * 2 + x / 64) * 64 + x % 64) * 8 + 4) = 0;
     }
 
     v8 rq[STATES ? 1 : NL], rk[NL], rv[NL];
@@ -141,188 +163,185 @@ __device__ __forceinline__ void linear_segment(const LinearAttnArgs& a) {
     };
     /* where channel c lies in a row of lq and lk: those that a lane takes of 32 side by side */
     const auto spot = [](int c) { return HD < 32 ? c : (c & ~31) + (c % 16 / 4) * 8 + (c % 32 / 16) * 4 + c % 4; };
+    const auto row_of = [&](const uint16_t* m, int row, int ks) {
+        if constexpr (HD >= 32) {
+            return ld8<T>(m + row * RS + 32 * ks + 8 * g);
+        } else {
+            const v4 x = *reinterpret_cast<const v4*>(m + row * RS + 4 * g);
+            return v8{x[0], x[1], x[2], x[3], (el)0.f, (el)0.f, (el)0.f, (el)0.f};
+        }
+    };
+    const auto transposed = [&](const uint16_t* m, int t, int c) { /* lane l16: channel c + l16, tokens t + 4 g.. and t + 16 + 4 g.. */
+        const uint16_t* at = m + (t + 4 * g + l16 / 4) * RS + c;
+        union {
+            s4 h[2];
+            v8 v;
+        } f;
+        f.h[0] = lds_tr4(at);
+        f.h[1] = lds_tr4(at + 16 * RS);
+        return f.v;
+    };
     if (t0 < t1) load(t0, min(C, t1 - (int)t0));
+    if (tid < 6) lmost[tid / 3][tid % 3] = 0;
     int full = -1; /* the length that fade is for */
     for (int64_t c0 = t0; c0 < t1; c0 += C) {
         const int n = min(C, t1 - (int)c0);
         const int turn = (int)((c0 - t0) / C & 1);
-        bool bad = false;
         __syncthreads(); /* the chunk before has been read */
+        if (tid < 3) lmost[turn ^ 1][tid] = 0; /* for the next chunk */
+        uint32_t mq = 0, mk = 0, mv = 0;
 #pragma unroll
         for (int i = 0; i < NL; ++i) {
             const int id = tid + NT * i, row = id / CPR, c = id % CPR * 8;
             if constexpr (!STATES) {
                 *reinterpret_cast<v4*>(lq + row * RS + spot(c)) = v4{rq[i][0], rq[i][1], rq[i][2], rq[i][3]};
                 *reinterpret_cast<v4*>(lq + row * RS + spot(c + 4)) = v4{rq[i][4], rq[i][5], rq[i][6], rq[i][7]};
-#pragma unroll
-                for (int e = 0; e < 8; ++e) bad |= !(__builtin_fabsf((float)rv[i][e]) < INFINITY);
+                if (HALF) mq = most2(mq, most8(rq[i]));
+                if (HALF) mk = most2(mk, most8(rk[i]));
+                mv = most2(mv, most8(rv[i]));
             }
             *reinterpret_cast<v4*>(lk + row * RS + spot(c)) = v4{rk[i][0], rk[i][1], rk[i][2], rk[i][3]};
             *reinterpret_cast<v4*>(lk + row * RS + spot(c + 4)) = v4{rk[i][4], rk[i][5], rk[i][6], rk[i][7]};
             st8<T>(lv + row * RS + c, rv[i]);
         }
-        if (tid == 0) lbad[turn ^ 1] = 0; /* for the next chunk */
-        if (c0 == t0 && tid == 0) lbad[0] = 0;
-        if (c0 == t0) __syncthreads();
-        if (bad) lbad[turn] = 1;
+        if constexpr (!STATES) {
+            if (infinite<T>(mv)) lmost[turn][0] = 1;
+            if constexpr (HALF) {
+                if (infinite<T>(mq) || infinite<T>(mk)) { /* the largest of the finite ones */
+                    mq = mk = 0;
+                    for (int i = 0; i < NL; ++i)
+                        for (int e = 0; e < 8; ++e) {
+                            const float x = __builtin_fabsf((float)rq[i][e]), y = __builtin_fabsf((float)rk[i][e]);
+                            if (x < INFINITY) mq = most2(mq, __builtin_bit_cast(uint16_t, (f16)x));
+                            if (y < INFINITY) mk = most2(mk, __builtin_bit_cast(uint16_t, (f16)y));
+                        }
+                }
+                atomicMax(&lmost[turn][1], max(mq & 0xFFFF, mq >> 16));
+                atomicMax(&lmost[turn][2], max(mk & 0xFFFF, mk >> 16));
+            }
+        }
         __syncthreads();
         if (c0 + C < t1) load(c0 + C, min(C, t1 - (int)c0 - C));
 
-        /* the wave's values, transposed: lane l16 is a channel, with 8 tokens of each 32 */
-        v8 v[DV][M];
+        v8 v[M]; /* lane l16 is a channel */
 #pragma unroll
-        for (int d = 0; d < DV; ++d)
-#pragma unroll
-            for (int m = 0; m < M; ++m) {
-                const uint16_t* at = lv + (32 * m + 4 * g + l16 / 4) * RS + 32 * wave + 16 * d + 4 * (l16 & 3);
-                union {
-                    s4 h[2];
-                    v8 v;
-                } f;
-                f.h[0] = lds_tr4(at);
-                f.h[1] = lds_tr4(at + 16 * RS);
-                v[d][m] = f.v;
-            }
+        for (int m = 0; m < M; ++m) v[m] = transposed(lv, 32 * m, 16 * wave + 4 * (l16 & 3));
         if constexpr (!STATES) {
-            const bool poisoned = __builtin_amdgcn_readfirstlane(lbad[turn]) != 0;
-            v8 clean[DV][M];
-#pragma unroll
-            for (int d = 0; d < DV; ++d)
-#pragma unroll
-                for (int m = 0; m < M; ++m) {
-                    clean[d][m] = v[d][m];
-                    if (poisoned)
-#pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                            clean[d][m][e] = __builtin_fabsf((float)v[d][m][e]) < INFINITY ? v[d][m][e] : (el)0.f;
-                }
-            /* the state in 16-bit parts: lane l16 is a channel of the values, with 8 of each 32 channels of the keys */
-            v8 sh[KS][DV], sl[KS][DV];
-            float back[DV][4]; /* fp16: what takes the scales out of the output's rows 4 g + e */
-#pragma unroll
-            for (int d = 0; d < DV; ++d) {
-                float up = 1.f;
-                if constexpr (HALF) {
-                    float most = 0.f;
-#pragma unroll
-                    for (int j = 0; j < DK; ++j)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) most = fmaxf(most, __builtin_fabsf(S[j][d][e]));
-                    float x, y;
-                    lanes_x16(most, x, y);
-                    lanes_x32(fmaxf(x, y), x, y);
-                    up = part_scale(fmaxf(x, y));
-                    const float down = part_unscale(up);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) back[d][e] = __shfl(down, 4 * g + e);
-                }
-#pragma unroll
-                for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-                    for (int e = 0; e < 8; e += 2) {
-                        v2 p[2] = {};
-                        const int j = 2 * ks + e / 4;
-                        if (j < DK) parts<T, 2>(S[j < DK ? j : 0][d][e % 4] * up, S[j < DK ? j : 0][d][e % 4 + 1] * up, p);
-                        sh[ks][d][e] = p[0][0];
-                        sh[ks][d][e + 1] = p[0][1];
-                        sl[ks][d][e] = p[1][0];
-                        sl[ks][d][e + 1] = p[1][1];
-                    }
+            /* fp16 weights are scaled by a power of two, after the largest that they could be: 2^15 stays above them, and
+               from there down their two parts have 40 bits */
+            float up = 1.f;
+            if constexpr (HALF) {
+                const auto largest = [&](int i) { return (float)__builtin_bit_cast(f16, (uint16_t)lmost[turn][i]); };
+                up = part_scale(largest(1) * largest(2) * (float)HD * __builtin_fabsf(a.scale));
             }
+            /* weights: lane l16 is a query, with keys 4 g + e of each 16 */
 #pragma unroll
-            for (int qt = 0; qt < QT; ++qt) {
-                v8 q[KS];
+            for (int x = wave; x < TILES; x += NW) {
+                const int qt = (x >= 1) + (x >= 3) + (x >= 6), kt = x - qt * (qt + 1) / 2;
+                f4 w = {};
 #pragma unroll
-                for (int ks = 0; ks < KS; ++ks) {
-                    if constexpr (HD >= 32) {
-                        q[ks] = ld8<T>(lq + (16 * qt + l16) * RS + 32 * ks + 8 * g);
-                    } else {
-                        const v4 x = *reinterpret_cast<const v4*>(lq + (16 * qt + l16) * RS + 4 * g);
-                        q[ks] = v8{x[0], x[1], x[2], x[3], (el)0.f, (el)0.f, (el)0.f, (el)0.f};
-                    }
+                for (int ks = 0; ks < KS; ++ks) w = mfma_16x16x32(row_of(lk, 16 * kt + l16, ks), row_of(lq, 16 * qt + l16, ks), w);
+                const float far = decay(16 * max(qt - kt - 1, 0)) * up;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float y = w[e] * ((kt == qt ? within[e] : before[e]) * far);
+                    w[e] = kt < qt || l16 >= 4 * g + e ? y : 0.f;
                 }
-                f4 o[DV] = {};
-#pragma unroll
-                for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-                    for (int d = 0; d < DV; ++d) {
-                        o[d] = mfma_16x16x32(sh[ks][d], q[ks], o[d]);
-                        o[d] = mfma_16x16x32(sl[ks][d], q[ks], o[d]);
-                    }
-                /* weights of the chunk's keys: lane l16 is a query, with keys 4 g + e of each 16 */
-                f4 w[QT] = {};
+                uint32_t p[2][2];
+                parts<T, 2>(w[0], w[1], p[0]);
+                parts<T, 2>(w[2], w[3], p[1]);
+                uint16_t* to = lw + (((qt * M + kt / 2) * 2) * 64 + lane) * 8 + kt % 2 * 4;
+                *reinterpret_cast<uint64_t*>(to) = p[0][0] | (uint64_t)p[1][0] << 32;
+                *reinterpret_cast<uint64_t*>(to + 64 * 8) = p[0][1] | (uint64_t)p[1][1] << 32;
+            }
+            /* the state in parts: lane l16 is a channel of the values, with 8 of each 32 channels of the keys */
+            v8 sh[KS], sl[KS];
+            f4 back; /* fp16: what takes the scales out of the output's rows 4 g + e */
+            float su = 1.f;
+            if constexpr (HALF) {
                 float most = 0.f;
 #pragma unroll
-                for (int kt = 0; kt <= qt; ++kt) {
+                for (int j = 0; j < DK; ++j)
 #pragma unroll
-                    for (int ks = 0; ks < KS; ++ks) {
-                        v8 k;
-                        if constexpr (HD >= 32) {
-                            k = ld8<T>(lk + (16 * kt + l16) * RS + 32 * ks + 8 * g);
-                        } else {
-                            const v4 x = *reinterpret_cast<const v4*>(lk + (16 * kt + l16) * RS + 4 * g);
-                            k = v8{x[0], x[1], x[2], x[3], (el)0.f, (el)0.f, (el)0.f, (el)0.f};
-                        }
-                        w[kt] = mfma_16x16x32(k, q[ks], w[kt]);
-                    }
-                    float far = 1.f;
-                    for (int x = kt + 1; x < qt; ++x) far *= d16;
+                    for (int e = 0; e < 4; ++e) most = fmaxf(most, __builtin_fabsf(S[j][e]));
+                float x, y;
+                lanes_x16(most, x, y);
+                lanes_x32(fmaxf(x, y), x, y);
+                su = part_scale(fmaxf(x, y));
+                const float down = part_unscale(su) * up;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        if (kt == qt) w[kt][e] = l16 >= 4 * g + e ? w[kt][e] * within[e] : 0.f;
-                        else w[kt][e] *= before[e] * far;
-                        if (HALF) most = fmaxf(most, __builtin_fabsf(w[kt][e]));
-                    }
+                for (int e = 0; e < 4; ++e) back[e] = __shfl(down, 4 * g + e);
+            }
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                u4 hi = {}, lo = {};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int j = 2 * ks + e / 2;
+                    if (j >= DK) continue;
+                    uint32_t p[2];
+                    const float x = S[j < DK ? j : 0][e % 2 * 2], y = S[j < DK ? j : 0][e % 2 * 2 + 1];
+                    parts<T, 2>(HALF ? x * su : x, HALF ? y * su : y, p);
+                    hi[e] = p[0];
+                    lo[e] = p[1];
                 }
-                const float since = decay(16 * qt + l16 + 1) * a.scale;
-                float up = 1.f;
-                if constexpr (HALF) {
-                    float x, y;
-                    lanes_x16(most, x, y);
-                    lanes_x32(fmaxf(x, y), x, y);
-                    up = part_scale(fmaxf(x, y));
+                sh[ks] = __builtin_bit_cast(v8, hi);
+                sl[ks] = __builtin_bit_cast(v8, lo);
+            }
+            f4 o[QT] = {};
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt)
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    const v8 q = row_of(lq, 16 * qt + l16, ks);
+                    o[qt] = mfma_16x16x32(sh[ks], q, o[qt]);
+                    o[qt] = mfma_16x16x32(sl[ks], q, o[qt]);
                 }
+            const float d16 = decay(16);
+            float far = since;
 #pragma unroll
-                for (int d = 0; d < DV; ++d)
+            for (int qt = 0; qt < QT; ++qt) {
+                if constexpr (HALF) o[qt] *= back;
+                o[qt] *= far;
+                far *= d16;
+            }
+            /* values that are not finite must not meet weights of zero: queries before them */
+            const bool poisoned = __builtin_amdgcn_readfirstlane(lmost[turn][0]) != 0;
+            v8 clean[M];
+            int from[4] = {C, C, C, C}; /* the first such token in channel 4 g + e */
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) o[d][e] = HALF ? o[d][e] * back[d][e] * since * up : o[d][e] * since;
+            for (int m = 0; m < M; ++m) clean[m] = v[m];
+            if (poisoned) {
+#pragma unroll
+                for (int m = 0; m < M; ++m)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) clean[m][e] = __builtin_fabsf((float)v[m][e]) < INFINITY ? v[m][e] : (el)0.f;
+                for (int t = n - 1; t >= 0; --t)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (!(__builtin_fabsf(ld1<T>(lv + t * RS + 16 * wave + 4 * g + e)) < INFINITY)) from[e] = t;
+            }
+            __syncthreads(); /* the weights are in */
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt)
 #pragma unroll
                 for (int m = 0; 2 * m <= qt; ++m) {
-                    v8 hi, lo;
-#pragma unroll
-                    for (int e = 0; e < 8; e += 2) {
-                        v2 p[2];
-                        const f4 x = w[2 * m + e / 4];
-                        parts<T, 2>(HALF ? x[e % 4] * up : x[e % 4], HALF ? x[e % 4 + 1] * up : x[e % 4 + 1], p);
-                        hi[e] = p[0][0];
-                        hi[e + 1] = p[0][1];
-                        lo[e] = p[1][0];
-                        lo[e + 1] = p[1][1];
-                    }
-#pragma unroll
-                    for (int d = 0; d < DV; ++d) {
-                        o[d] = mfma_16x16x32(clean[d][m], hi, o[d]);
-                        o[d] = mfma_16x16x32(clean[d][m], lo, o[d]);
-                    }
+                    const uint16_t* w = lw + ((qt * M + m) * 2 * 64 + lane) * 8;
+                    o[qt] = mfma_16x16x32(clean[m], ld8<T>(w), o[qt]);
+                    o[qt] = mfma_16x16x32(clean[m], ld8<T>(w + 64 * 8), o[qt]);
                 }
-                const float down = HALF ? part_unscale(up) : 1.f;
+            const float down = HALF ? part_unscale(up) : 1.f;
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt) {
                 const int i = 16 * qt + l16;
-                if (poisoned) /* queries from a value on that is not finite */
-                    for (int d = 0; d < DV; ++d)
-                        for (int e = 0; e < 4; ++e)
-                            for (int t = 0; t <= i; ++t)
-                                if (!(__builtin_fabsf(ld1<T>(lv + t * RS + 32 * wave + 16 * d + 4 * g + e)) < INFINITY))
-                                    o[d][e] = __builtin_nanf("");
-                if (i < n) {
-                    uint16_t* out = a.out + (c0 + i) * a.out_token_stride + h * a.out_head_stride + 32 * wave + 4 * g;
+                if (poisoned)
 #pragma unroll
-                    for (int d = 0; d < DV; ++d) {
-                        v4 r;
+                    for (int e = 0; e < 4; ++e) o[qt][e] = i >= from[e] ? __builtin_nanf("") : o[qt][e];
+                if (i >= n) continue;
+                v4 r;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) r[e] = (el)opaque(HALF ? o[d][e] * down : o[d][e]);
-                        *reinterpret_cast<v4*>(out + 16 * d) = r;
-                    }
-                }
+                for (int e = 0; e < 4; ++e) r[e] = (el)opaque(HALF ? o[qt][e] * down : o[qt][e]);
+                *reinterpret_cast<v4*>(a.out + (c0 + i) * a.out_token_stride + h * a.out_head_stride + 16 * wave + 4 * g) = r;
             }
         }
         /* the next state */
@@ -334,79 +353,59 @@ __device__ __forceinline__ void linear_segment(const LinearAttnArgs& a) {
                 for (int e = 0; e < 8; ++e) fade[m][e] = decay(max(n - 1 - (32 * m + e / 4 * 16 + 4 * g + e % 4), 0));
         }
         const float keep = decay(n);
-        v8 vp[DV][M][VP];
-        float down[DV];
-#pragma unroll
-        for (int d = 0; d < DV; ++d) {
-            float up = 1.f;
-            if constexpr (HALF) {
-                float most = 0.f;
-#pragma unroll
-                for (int m = 0; m < M; ++m)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) most = fmaxf(most, __builtin_fabsf((float)v[d][m][e] * fade[m][e]));
-                float x, y;
-                lanes_x16(most, x, y);
-                lanes_x32(fmaxf(x, y), x, y);
-                up = part_scale(fmaxf(x, y));
-                down[d] = part_unscale(up);
-            }
+        v8 vp[M][VP];
+        float vu = 1.f;
+        if constexpr (HALF) {
+            float most = 0.f;
 #pragma unroll
             for (int m = 0; m < M; ++m)
 #pragma unroll
-                for (int e = 0; e < 8; e += 2) {
-                    v2 p[VP];
-                    const float x = (float)v[d][m][e] * fade[m][e], y = (float)v[d][m][e + 1] * fade[m][e + 1];
-                    parts<T, VP>(HALF ? x * up : x, HALF ? y * up : y, p);
-#pragma unroll
-                    for (int i = 0; i < VP; ++i) {
-                        vp[d][m][i][e] = p[i][0];
-                        vp[d][m][i][e + 1] = p[i][1];
-                    }
-                }
+                for (int e = 0; e < 8; ++e) most = fmaxf(most, __builtin_fabsf((float)v[m][e] * fade[m][e]));
+            float x, y;
+            lanes_x16(most, x, y);
+            lanes_x32(fmaxf(x, y), x, y);
+            vu = part_scale(fmaxf(x, y));
         }
 #pragma unroll
-        for (int j = 0; j < DK; ++j) {
-            v8 k[M];
+        for (int m = 0; m < M; ++m) {
+            u4 w[VP];
 #pragma unroll
-            for (int m = 0; m < M; ++m) {
-                const uint16_t* at = lk + (32 * m + 4 * g + l16 / 4) * RS + spot(16 * j + 4 * (l16 & 3));
-                union {
-                    s4 h[2];
-                    v8 v;
-                } f;
-                f.h[0] = lds_tr4(at);
-                f.h[1] = lds_tr4(at + 16 * RS);
-                k[m] = f.v;
+            for (int e = 0; e < 4; ++e) {
+                uint32_t p[VP];
+                const float x = (float)v[m][2 * e] * fade[m][2 * e], y = (float)v[m][2 * e + 1] * fade[m][2 * e + 1];
+                parts<T, VP>(HALF ? x * vu : x, HALF ? y * vu : y, p);
+#pragma unroll
+                for (int i = 0; i < VP; ++i) w[i][e] = p[i];
             }
 #pragma unroll
-            for (int d = 0; d < DV; ++d) {
-                f4 u = HALF ? f4{} : S[j][d] * keep;
+            for (int i = 0; i < VP; ++i) vp[m][i] = __builtin_bit_cast(v8, w[i]);
+        }
+        const float vd = HALF ? part_unscale(vu) : 1.f;
 #pragma unroll
-                for (int m = 0; m < M; ++m)
+        for (int j = 0; j < DK; ++j) {
+            f4 u = HALF ? f4{} : S[j] * keep;
 #pragma unroll
-                    for (int i = 0; i < VP; ++i) u = mfma_16x16x32(k[m], vp[d][m][i], u);
-                if constexpr (HALF) {
+            for (int m = 0; m < M; ++m) {
+                const v8 k = transposed(lk, 32 * m, spot(16 * j + 4 * (l16 & 3)));
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) S[j][d][e] = __builtin_fmaf(u[e], down[d], S[j][d][e] * keep);
-                } else {
-                    S[j][d] = u;
-                }
+                for (int i = 0; i < VP; ++i) u = mfma_16x16x32(k, vp[m][i], u);
+            }
+            if constexpr (HALF) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) S[j][e] = __builtin_fmaf(u[e], vd, S[j][e] * keep);
+            } else {
+                S[j] = u;
             }
         }
     }
     if constexpr (STATES) {
 #pragma unroll
-        for (int j = 0; j < DK; ++j)
-#pragma unroll
-            for (int d = 0; d < DV; ++d) mine[NT * (j * DV + d)] = S[j][d];
+        for (int j = 0; j < DK; ++j) mine[NT * j] = S[j];
     } else if (number >= 0 && a.state_out && t1 == lt.rows.end) {
 #pragma unroll
         for (int j = 0; j < DK; ++j)
 #pragma unroll
-            for (int d = 0; d < DV; ++d)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) a.state_out[base + (16 * j + 4 * g + e) * HD + 16 * d] = S[j][d][e];
+            for (int e = 0; e < 4; ++e) a.state_out[base + (16 * j + 4 * g + e) * HD] = S[j][e];
     }
 }
 
@@ -445,8 +444,8 @@ __device__ __forceinline__ void linear_step(const LinearAttnArgs& a) {
 }
 
 #define LINEAR(NAME, T, HD)                                                                                                   \
-    extern "C" __global__ void __launch_bounds__(HD >= 64 ? 2 * HD : 64) prism_linear_attn_##NAME##_h##HD(LinearAttnArgs a) { linear_segment<T, HD, false>(a); } \
-    extern "C" __global__ void __launch_bounds__(HD >= 64 ? 2 * HD : 64) prism_linear_states_##NAME##_h##HD(LinearAttnArgs a) { linear_segment<T, HD, true>(a); } \
+    extern "C" __global__ void __launch_bounds__(4 * HD) prism_linear_attn_##NAME##_h##HD(LinearAttnArgs a) { linear_segment<T, HD, false>(a); } \
+    extern "C" __global__ void __launch_bounds__(4 * HD) prism_linear_states_##NAME##_h##HD(LinearAttnArgs a) { linear_segment<T, HD, true>(a); } \
     extern "C" __global__ void __launch_bounds__(256) prism_linear_step_##NAME##_h##HD(LinearAttnArgs a) { linear_step<T, HD>(a); }
 LINEAR(f16, F16, 16) LINEAR(f16, F16, 32) LINEAR(f16, F16, 64) LINEAR(f16, F16, 128)
 LINEAR(bf16, BF16, 16) LINEAR(bf16, BF16, 32) LINEAR(bf16, BF16, 64) LINEAR(bf16, BF16, 128)
