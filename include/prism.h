@@ -650,7 +650,7 @@ int prism_paged_attn4(prism_ctx* ctx, const prism_paged_attn_push* p, const void
  * state 21 or more. From its token on, an infinity or NaN in q makes NaN of its row and head, in
  * v of its channel and in k of its whole head, of state_out too; earlier tokens
  * and other sequences do not see it. workspace as in prism_paged_attn. head_dim 16, 32,
- * 64 or 128; at most 2^30 rows. */
+ * 64 or 128; at most 2^30 rows, token strides at most 2^22. */
 typedef struct prism_linear_attn_push {
     int32_t dtype, n_seqs, n_tokens, n_heads, n_kv_heads, head_dim;
     int32_t n_states;

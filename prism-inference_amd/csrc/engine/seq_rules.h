@@ -19,7 +19,7 @@ constexpr int64_t SEQ_MAX_OFFSET = int64_t(1) << 60;
 /* Rows of a sequence attention and tokens of a table's row: key numbers a tile past the
  * end stay in 32 bits. */
 constexpr int64_t SEQ_MAX_ROWS = int64_t(1) << 30;
-/* Key rows of a tile are addressed with 32 bits. */
+/* Key rows of a tile, and a linear attention's rows of a chunk, are addressed with 32 bits. */
 constexpr int64_t SEQ_MAX_KEY_STRIDE = int64_t(1) << 22;
 
 inline int seq_bad(const char** why, int code, const char* text) {
@@ -194,6 +194,9 @@ inline int check_linear(const prism_linear_attn_push& p, const char** why) {
     if (int rc = check_strides(p.n_tokens, p.n_heads, p.q_token_stride, p.q_head_stride, why)) return rc;
     if (int rc = check_strides(p.n_tokens, p.n_kv_heads, p.k_token_stride, p.k_head_stride, why)) return rc;
     if (int rc = check_strides(p.n_tokens, p.n_kv_heads, p.v_token_stride, p.v_head_stride, why)) return rc;
+    if (p.q_token_stride > SEQ_MAX_KEY_STRIDE || p.k_token_stride > SEQ_MAX_KEY_STRIDE || p.v_token_stride > SEQ_MAX_KEY_STRIDE ||
+        p.out_token_stride > SEQ_MAX_KEY_STRIDE)
+        return seq_bad(why, PRISM_ERR_UNSUPPORTED, "token strides are at most 2^22");
     return check_out(p.n_tokens, p.n_heads, p.head_dim, p.out_token_stride, p.out_head_stride, why);
 }
 inline int check_linear_step(const prism_linear_attn_push& p, const char** why) {

@@ -40,13 +40,14 @@ __device__ __forceinline__ LinearTile linear_tile(const LinearAttnArgs& a, int b
     }
 }
 
+typedef float f2 __attribute__((ext_vector_type(2)));
 /* Two fp32 numbers as N pairs of 16-bit ones that add up to them: fp16 11 N bits (of what is above its smallest), bf16 8 N.
  * Rounded to nearest, so that what is left has a sign and half a bit more. */
 template <class T, int N>
 __device__ __forceinline__ void parts(float x, float y, uint32_t (&p)[N]) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        const typename T::v2 v = {(typename T::el)x, (typename T::el)y};
+        const typename T::v2 v = __builtin_convertvector((f2{x, y}), typename T::v2);
         p[i] = __builtin_bit_cast(uint32_t, v);
         if (i + 1 < N) {
             x -= (float)v[0];
@@ -73,6 +74,20 @@ __device__ __forceinline__ uint32_t most8(V v) {
     const u4 w = __builtin_bit_cast(u4, v) & 0x7FFF7FFFu;
     return most2(most2(w[0], w[1]), most2(w[2], w[3]));
 }
+/* ... over the wave */
+__device__ __forceinline__ uint32_t most_of_wave(uint32_t v) {
+    const auto with = [&](auto control) {
+        v = most2(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, decltype(control)::value, 0xf, 0xf, false));
+    };
+    with(Count<0xB1>{});  /* neighbours, pairs, fours, eights: as group_sum */
+    with(Count<0x4E>{});
+    with(Count<0x140>{});
+    with(Count<0x141>{});
+    int a, b;
+    lanes_x16((int)v, a, b);
+    lanes_x32((int)most2(a, b), a, b);
+    return most2(a, b);
+}
 template <class T>
 __device__ __forceinline__ bool infinite(uint32_t most) { /* bits of magnitudes, two of them */
     constexpr uint32_t inf = __is_same(T, F16) ? 0x7C00 : 0x7F80;
@@ -82,8 +97,10 @@ __device__ __forceinline__ bool infinite(uint32_t most) { /* bits of magnitudes,
 /* One segment of one head: its chunks of 64 tokens in turn,
  *   o_i = scale (e^(-r (i+1)) q_i S + sum_{j <= i} e^(-r (i-j)) (q_i k_j) v_j),  S' = e^(-r n) S + sum_j k_j^T e^(-r (n-1-j)) v_j
  * A wave has 16 channels of the values, so its part of the state is its own and stays in registers: 16 x 16 tiles as the
- * product leaves them, which are at the same time what the next chunk's product q S takes. The weights (q_i k_j) are all
- * waves' work and go through LDS. STATES: only the state that the segment adds. */
+ * product leaves them, which are at the same time what the next chunk's product q S takes.
+ * From 64 channels on a wave has all queries (WQ = 1) and the weights (q_i k_j) are all waves' work and go through LDS.
+ * Below, where that is few waves, each has one or two of the four query tiles with weights of its own, and the
+ * state's update is done again by the waves of other tiles. STATES: only the state that the segment adds. */
 template <class T, int HD, bool STATES>
 __device__ __forceinline__ void linear_segment(const LinearAttnArgs& a) {
     typedef typename T::v8 v8;
@@ -91,18 +108,20 @@ __device__ __forceinline__ void linear_segment(const LinearAttnArgs& a) {
     typedef typename T::el el;
     constexpr bool HALF = __is_same(T, F16);
     constexpr int C = LINEAR_CHUNK, QT = C / 16, M = C / 32;
-    constexpr int NW = HD / 16, NT = 64 * NW; /* waves, threads */
-    constexpr int DK = HD / 16;               /* 16-channel tiles of the keys */
+    constexpr int WD = HD / 16, WQ = STATES || HD >= 64 ? 1 : QT / WD, QN = QT / WQ; /* waves by channels, by query tiles; a wave's */
+    constexpr bool SHARED = WQ == 1;
+    constexpr int NT = 64 * WD * WQ;
+    constexpr int DK = HD / 16; /* 16-channel tiles of the keys */
     constexpr int KS = (HD + 31) / 32;
     constexpr int RS = HD >= 32 ? HD + 16 : HD;    /* LDS row: 4 rows' parts of a transposed read lie in different banks */
-    constexpr int CPR = HD / 8, NL = C * CPR / NT; /* 16-byte chunks a row, and a thread's of a matrix: 2 */
+    constexpr int CPR = HD / 8, NL = (C * CPR + NT - 1) / NT; /* 16-byte chunks a row, and a thread's of a matrix */
     constexpr int VP = HALF ? 2 : 3;               /* parts of a decayed value */
     constexpr int TILES = QT * (QT + 1) / 2;       /* of weights */
     __shared__ __attribute__((aligned(16))) uint16_t lq[STATES ? 8 : C * RS], lk[C * RS], lv[C * RS];
-    __shared__ __attribute__((aligned(16))) uint16_t lw[STATES ? 8 : QT * M * 2 * 64 * 8]; /* weights [query tile][32 keys][part] */
-    __shared__ uint32_t lmost[2][3]; /* of a chunk: an infinite value; fp16: the largest query, key */
+    __shared__ __attribute__((aligned(16))) uint16_t lw[!STATES && SHARED ? 6 * 2 * 64 * 8 : 8]; /* weights [query tile, 32 keys][part] */
+    __shared__ __attribute__((aligned(16))) uint32_t lmost[2][2 * WD * WQ]; /* of a chunk, by waves: fp16's largest query and key; an infinite value */
     const int lane = lane_id(), l16 = lane & 15, g = lane >> 4, tid = threadIdx.x;
-    const int wave = NW == 1 ? 0 : __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wave = NT == 64 ? 0 : __builtin_amdgcn_readfirstlane(tid >> 6), wd = wave % WD, wq = wave / WD;
     const int b = blockIdx.x / a.n_heads, h = blockIdx.x % a.n_heads, hk = h / (a.n_heads / a.n_kv_heads);
     const LinearTile lt = linear_tile(a, b);
     const int seg = b - lt.first;
@@ -114,53 +133,44 @@ __device__ __forceinline__ void linear_segment(const LinearAttnArgs& a) {
     const float r2 = linear_rate(a, h);
     const auto decay = [&](int n) { return fast_exp2(-r2 * (float)n); };
     const int number = linear_state(a, lt.seq);
-    const int64_t base = ((int64_t)max(number, 0) * a.n_heads + h) * HD * HD + 16 * wave + l16;
-    f4* const mine = reinterpret_cast<f4*>(a.ws) + ((int64_t)b * a.n_heads + h) * (HD * HD / 4) + tid; /* + NT * tile */
-    f4 S[DK]; /* channels 16 j + 4 g + e of the keys x channel 16 wave + l16 of the values */
+    const int64_t base = ((int64_t)max(number, 0) * a.n_heads + h) * HD * HD + 16 * wd + l16;
+    f4* const mine = reinterpret_cast<f4*>(a.ws) + ((int64_t)b * a.n_heads + h) * (HD * HD / 4) + wd * 64 + lane; /* + 64 WD * tile */
+    f4 S[DK]; /* channels 16 j + 4 g + e of the keys x channel 16 wd + l16 of the values */
 #pragma unroll
     for (int j = 0; j < DK; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
             S[j][e] = !STATES && a.state_in && number >= 0 ? a.state_in[base + (16 * j + 4 * g + e) * HD] : 0.f;
     if constexpr (!STATES) {
+        constexpr int DEPTH = 16 / DK; /* segments asked for at once */
         const float keep = decay(a.segment);
-        for (int s = seg; s > 0; --s) {
-            const f4* u = mine - (int64_t)s * a.n_heads * (HD * HD / 4);
+        for (int s = seg; s > 0; s -= DEPTH) {
+            f4 u[DEPTH][DK];
 #pragma unroll
-            for (int j = 0; j < DK; ++j) S[j] = S[j] * keep + u[NT * j];
+            for (int i = 0; i < DEPTH; ++i)
+#pragma unroll
+                for (int j = 0; j < DK; ++j) u[i][j] = mine[64 * WD * j - (int64_t)max(s - i, 1) * a.n_heads * (HD * HD / 4)];
+#pragma unroll
+            for (int i = 0; i < DEPTH; ++i)
+                if (i < s)
+#pragma unroll
+                    for (int j = 0; j < DK; ++j) S[j] = S[j] * keep + u[i][j];
         }
     }
-    /* decays: of a key in a query's tile, and in the tile before; of the state; of a token up to the chunk's end */
-    float within[4], before[4], fade[M][8];
-    const float since = decay(l16 + 1) * a.scale;
-    if constexpr (!STATES) {
+    /* decays: of a key in a query's tile, and in the tile before; of a token up to its 16's end */
+    float within[4], before[4], fade[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int gap = l16 - 4 * g - e;
-            within[e] = gap >= 0 ? decay(max(gap, 0)) * a.scale : 0.f;
-            before[e] = decay(16 + gap) * a.scale;
-        }
-        /* keys behind a tile's queries, in the 32 that it has a part of */
-        for (int qt = 0; qt < QT; qt += 2)
-            for (int x = tid; x < 128; x += NT)
-                *reinterpret_cast<uint64_t*>(lw + (((qt * M + qt / 2) * 2 + x / 64) * 64 + x % 64) * 8 + 4) = 0;
+    for (int e = 0; e < 4; ++e) {
+        const int gap = l16 - 4 * g - e;
+        within[e] = gap >= 0 ? decay(max(gap, 0)) * a.scale : 0.f;
+        before[e] = decay(16 + gap) * a.scale;
+        fade[e] = decay(15 - 4 * g - e);
     }
+    if constexpr (!STATES && SHARED) /* keys behind a tile's queries, in the 32 that it has a part of */
+        for (int x = tid; x < 256; x += NT)
+            *reinterpret_cast<uint64_t*>(lw + ((x / 128 * 6 + x / 64 % 2) * 64 + x % 64) * 8 + 4) = 0;
+    const auto weights_at = [](int qt, int m) { return (qt + (qt == 3) + m) * 2 * 64 * 8; }; /* 0, 1, 2 3, 4 5 */
 
-    v8 rq[STATES ? 1 : NL], rk[NL], rv[NL];
-    const uint16_t* qb = a.q + h * a.q_head_stride;
-    const uint16_t* kb = a.k + hk * a.k_head_stride;
-    const uint16_t* vb = a.v + hk * a.v_head_stride;
-    const auto load = [&](int64_t c0, int n) {
-#pragma unroll
-        for (int i = 0; i < NL; ++i) {
-            const int id = tid + NT * i, row = id / CPR, c = id % CPR * 8;
-            const int64_t t = c0 + min(row, n - 1);
-            if constexpr (!STATES) rq[i] = ld8<T>(qb + t * a.q_token_stride + c);
-            rk[i] = ld8<T>(kb + t * a.k_token_stride + c);
-            rv[i] = ld8<T>(vb + t * a.v_token_stride + c);
-            if (row >= n) rk[i] = rv[i] = v8{}; /* behind the segment: no key */
-        }
-    };
     /* where channel c lies in a row of lq and lk: those that a lane takes of 32 side by side */
     const auto spot = [](int c) { return HD < 32 ? c : (c & ~31) + (c % 16 / 4) * 8 + (c % 32 / 16) * 4 + c % 4; };
     const auto row_of = [&](const uint16_t* m, int row, int ks) {
@@ -181,18 +191,33 @@ __device__ __forceinline__ void linear_segment(const LinearAttnArgs& a) {
         f.h[1] = lds_tr4(at + 16 * RS);
         return f.v;
     };
-    if (t0 < t1) load(t0, min(C, t1 - (int)t0));
-    if (tid < 6) lmost[tid / 3][tid % 3] = 0;
-    int full = -1; /* the length that fade is for */
-    for (int64_t c0 = t0; c0 < t1; c0 += C) {
-        const int n = min(C, t1 - (int)c0);
-        const int turn = (int)((c0 - t0) / C & 1);
+    /* A chunk's tokens lie at its end: a short one, the segment's last, has rows of zeros before them, so that decays up to
+       the end are always the same. Token strides are at most 2^22: 32-bit offsets from a base that is the same for all. */
+    v8 rq[STATES ? 1 : NL], rk[NL], rv[NL];
+    const auto load = [&](int c0, int skip) {
+        const auto at = [&](const uint16_t* m, int64_t stride, int64_t head, int row, int c) {
+            const uint16_t* first = m + (t0 + c0) * stride + head;
+            return ld8<T>(first + ((uint32_t)max(row - skip, 0) * (uint32_t)stride + c));
+        };
+#pragma unroll
+        for (int i = 0; i < NL; ++i) {
+            const int id = tid + NT * i, row = min(id / CPR, C - 1), c = id % CPR * 8;
+            if constexpr (!STATES) rq[i] = at(a.q, a.q_token_stride, h * a.q_head_stride, row, c);
+            rk[i] = at(a.k, a.k_token_stride, hk * a.k_head_stride, row, c);
+            rv[i] = at(a.v, a.v_token_stride, hk * a.v_head_stride, row, c);
+            if (row < skip) rk[i] = rv[i] = v8{};
+        }
+    };
+    const int len = t1 > t0 ? t1 - (int)t0 : 0;
+    if (len > 0) load(0, max(C - len, 0));
+    for (int c0 = 0; c0 < len; c0 += C) {
+        const int n = min(C, len - c0), skip = C - n, turn = c0 / C & 1;
         __syncthreads(); /* the chunk before has been read */
-        if (tid < 3) lmost[turn ^ 1][tid] = 0; /* for the next chunk */
         uint32_t mq = 0, mk = 0, mv = 0;
 #pragma unroll
         for (int i = 0; i < NL; ++i) {
             const int id = tid + NT * i, row = id / CPR, c = id % CPR * 8;
+            if (C * CPR % NT != 0 && row >= C) break;
             if constexpr (!STATES) {
                 *reinterpret_cast<v4*>(lq + row * RS + spot(c)) = v4{rq[i][0], rq[i][1], rq[i][2], rq[i][3]};
                 *reinterpret_cast<v4*>(lq + row * RS + spot(c + 4)) = v4{rq[i][4], rq[i][5], rq[i][6], rq[i][7]};
@@ -205,7 +230,8 @@ __device__ __forceinline__ void linear_segment(const LinearAttnArgs& a) {
             st8<T>(lv + row * RS + c, rv[i]);
         }
         if constexpr (!STATES) {
-            if (infinite<T>(mv)) lmost[turn][0] = 1;
+            const bool bad = __any(infinite<T>(mv));
+            uint32_t mqk = 0;
             if constexpr (HALF) {
                 if (infinite<T>(mq) || infinite<T>(mk)) { /* the largest of the finite ones */
                     mq = mk = 0;
@@ -216,28 +242,37 @@ __device__ __forceinline__ void linear_segment(const LinearAttnArgs& a) {
                             if (y < INFINITY) mk = most2(mk, __builtin_bit_cast(uint16_t, (f16)y));
                         }
                 }
-                atomicMax(&lmost[turn][1], max(mq & 0xFFFF, mq >> 16));
-                atomicMax(&lmost[turn][2], max(mk & 0xFFFF, mk >> 16));
+                mqk = most2(mq & 0xFFFF, mq >> 16) | most2(mk & 0xFFFF, mk >> 16) << 16;
+                mqk = most_of_wave(mqk);
+            }
+            if (lane == 0) {
+                lmost[turn][wave] = mqk;
+                lmost[turn][WD * WQ + wave] = bad;
             }
         }
         __syncthreads();
-        if (c0 + C < t1) load(c0 + C, min(C, t1 - (int)c0 - C));
 
         v8 v[M]; /* lane l16 is a channel */
+        const auto values = [&] {
 #pragma unroll
-        for (int m = 0; m < M; ++m) v[m] = transposed(lv, 32 * m, 16 * wave + 4 * (l16 & 3));
+            for (int m = 0; m < M; ++m) v[m] = transposed(lv, 32 * m, 16 * wd + 4 * (l16 & 3));
+        };
         if constexpr (!STATES) {
             /* fp16 weights are scaled by a power of two, after the largest that they could be: 2^15 stays above them, and
                from there down their two parts have 40 bits */
             float up = 1.f;
-            if constexpr (HALF) {
-                const auto largest = [&](int i) { return (float)__builtin_bit_cast(f16, (uint16_t)lmost[turn][i]); };
-                up = part_scale(largest(1) * largest(2) * (float)HD * __builtin_fabsf(a.scale));
-            }
-            /* weights: lane l16 is a query, with keys 4 g + e of each 16 */
+            uint32_t bad = 0;
 #pragma unroll
-            for (int x = wave; x < TILES; x += NW) {
-                const int qt = (x >= 1) + (x >= 3) + (x >= 6), kt = x - qt * (qt + 1) / 2;
+            for (int i = 0; i < WD * WQ; ++i) bad |= lmost[turn][WD * WQ + i];
+            if constexpr (HALF) {
+                uint32_t m = 0;
+#pragma unroll
+                for (int i = 0; i < WD * WQ; ++i) m = most2(m, lmost[turn][i]);
+                const h2 qk = __builtin_bit_cast(h2, m);
+                up = part_scale((float)qk[0] * (float)qk[1] * (float)HD * __builtin_fabsf(a.scale));
+            }
+            /* weights of 16 queries and 16 keys: lane l16 is a query, with keys 4 g + e; in two parts */
+            const auto weigh = [&](int qt, int kt, uint32_t (&hi)[2], uint32_t (&lo)[2]) {
                 f4 w = {};
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks) w = mfma_16x16x32(row_of(lk, 16 * kt + l16, ks), row_of(lq, 16 * qt + l16, ks), w);
@@ -250,13 +285,24 @@ __device__ __forceinline__ void linear_segment(const LinearAttnArgs& a) {
                 uint32_t p[2][2];
                 parts<T, 2>(w[0], w[1], p[0]);
                 parts<T, 2>(w[2], w[3], p[1]);
-                uint16_t* to = lw + (((qt * M + kt / 2) * 2) * 64 + lane) * 8 + kt % 2 * 4;
-                *reinterpret_cast<uint64_t*>(to) = p[0][0] | (uint64_t)p[1][0] << 32;
-                *reinterpret_cast<uint64_t*>(to + 64 * 8) = p[0][1] | (uint64_t)p[1][1] << 32;
+                hi[0] = p[0][0];
+                hi[1] = p[1][0];
+                lo[0] = p[0][1];
+                lo[1] = p[1][1];
+            };
+            const auto tile_of = [&](int i) { return WQ == 1 ? i : WQ == QT ? wq : i == 0 ? wq : QT - 1 - wq; };
+            if constexpr (SHARED) {
+                for (int x = wave; x < TILES; x += WD) {
+                    const int qt = (x >= 1) + (x >= 3) + (x >= 6), kt = x - qt * (qt + 1) / 2;
+                    uint32_t hi[2], lo[2];
+                    weigh(qt, kt, hi, lo);
+                    uint16_t* to = lw + weights_at(qt, kt / 2) + lane * 8 + kt % 2 * 4;
+                    *reinterpret_cast<uint64_t*>(to) = hi[0] | (uint64_t)hi[1] << 32;
+                    *reinterpret_cast<uint64_t*>(to + 64 * 8) = lo[0] | (uint64_t)lo[1] << 32;
+                }
             }
-            /* the state in parts: lane l16 is a channel of the values, with 8 of each 32 channels of the keys */
-            v8 sh[KS], sl[KS];
-            f4 back; /* fp16: what takes the scales out of the output's rows 4 g + e */
+            f4 o[QN] = {};
+            f4 back = {}; /* fp16: what takes the scales out of the output's rows 4 g + e */
             float su = 1.f;
             if constexpr (HALF) {
                 float most = 0.f;
@@ -272,6 +318,7 @@ __device__ __forceinline__ void linear_segment(const LinearAttnArgs& a) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) back[e] = __shfl(down, 4 * g + e);
             }
+            /* q S, the state in parts: lane l16 is a channel of the values, with 8 of each 32 channels of the keys */
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
                 u4 hi = {}, lo = {};
@@ -285,122 +332,146 @@ __device__ __forceinline__ void linear_segment(const LinearAttnArgs& a) {
                     hi[e] = p[0];
                     lo[e] = p[1];
                 }
-                sh[ks] = __builtin_bit_cast(v8, hi);
-                sl[ks] = __builtin_bit_cast(v8, lo);
+                v8 q[QN];
+#pragma unroll
+                for (int i = 0; i < QN; ++i) q[i] = row_of(lq, 16 * tile_of(i) + l16, ks);
+#pragma unroll
+                for (int i = 0; i < QN; ++i) o[i] = mfma_16x16x32(__builtin_bit_cast(v8, hi), q[i], o[i]);
+#pragma unroll
+                for (int i = 0; i < QN; ++i) o[i] = mfma_16x16x32(__builtin_bit_cast(v8, lo), q[i], o[i]);
             }
-            f4 o[QT] = {};
 #pragma unroll
-            for (int qt = 0; qt < QT; ++qt)
-#pragma unroll
-                for (int ks = 0; ks < KS; ++ks) {
-                    const v8 q = row_of(lq, 16 * qt + l16, ks);
-                    o[qt] = mfma_16x16x32(sh[ks], q, o[qt]);
-                    o[qt] = mfma_16x16x32(sl[ks], q, o[qt]);
-                }
-            const float d16 = decay(16);
-            float far = since;
-#pragma unroll
-            for (int qt = 0; qt < QT; ++qt) {
-                if constexpr (HALF) o[qt] *= back;
-                o[qt] *= far;
-                far *= d16;
+            for (int i = 0; i < QN; ++i) {
+                const float far = decay(max(16 * tile_of(i) + l16 + 1 - skip, 0)) * a.scale;
+                if constexpr (HALF) o[i] *= back;
+                o[i] *= far;
             }
             /* values that are not finite must not meet weights of zero: queries before them */
-            const bool poisoned = __builtin_amdgcn_readfirstlane(lmost[turn][0]) != 0;
-            v8 clean[M];
-            int from[4] = {C, C, C, C}; /* the first such token in channel 4 g + e */
-#pragma unroll
-            for (int m = 0; m < M; ++m) clean[m] = v[m];
-            if (poisoned) {
+            const bool poisoned = __builtin_amdgcn_readfirstlane(bad) != 0;
+            sched_fence(); /* the products' operands are dead; what follows needs its registers */
+            if constexpr (SHARED) __syncthreads(); /* the weights are in */
+            values();
+            if (poisoned)
 #pragma unroll
                 for (int m = 0; m < M; ++m)
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) clean[m][e] = __builtin_fabsf((float)v[m][e]) < INFINITY ? v[m][e] : (el)0.f;
-                for (int t = n - 1; t >= 0; --t)
+                    for (int e = 0; e < 8; ++e) v[m][e] = __builtin_fabsf((float)v[m][e]) < INFINITY ? v[m][e] : (el)0.f;
+            if constexpr (SHARED) {
+#pragma unroll
+                for (int m = 0; m < M; ++m)
+#pragma unroll
+                    for (int part = 0; part < 2; ++part)
+#pragma unroll
+                        for (int qt = 2 * m; qt < QT; ++qt)
+                            o[qt] = mfma_16x16x32(v[m], ld8<T>(lw + weights_at(qt, m) + (part * 64 + lane) * 8), o[qt]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < QN; ++i) {
+                    const int qt = tile_of(i);
+#pragma unroll
+                    for (int m = 0; m < M; ++m) {
+                        if (2 * m > qt) break;
+                        uint32_t hi[2][2], lo[2][2] = {};
+                        weigh(qt, 2 * m, hi[0], lo[0]);
+                        if (2 * m < qt) weigh(qt, 2 * m + 1, hi[1], lo[1]);
+                        else hi[1][0] = hi[1][1] = 0;
+                        o[i] = mfma_16x16x32(v[m], __builtin_bit_cast(v8, u4{hi[0][0], hi[0][1], hi[1][0], hi[1][1]}), o[i]);
+                        o[i] = mfma_16x16x32(v[m], __builtin_bit_cast(v8, u4{lo[0][0], lo[0][1], lo[1][0], lo[1][1]}), o[i]);
+                    }
+                }
+            }
+            const float down = HALF ? part_unscale(up) : 1.f;
+            if (poisoned) { /* what sees one of them */
+                int from[4] = {C, C, C, C}; /* the first in channel 4 g + e */
+                for (int t = C - 1; t >= 0; --t)
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        if (!(__builtin_fabsf(ld1<T>(lv + t * RS + 16 * wave + 4 * g + e)) < INFINITY)) from[e] = t;
+                        if (!(__builtin_fabsf(ld1<T>(lv + t * RS + 16 * wd + 4 * g + e)) < INFINITY)) from[e] = t;
+#pragma unroll
+                for (int i = 0; i < QN; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[i][e] = 16 * tile_of(i) + l16 >= from[e] ? __builtin_nanf("") : o[i][e];
             }
-            __syncthreads(); /* the weights are in */
 #pragma unroll
-            for (int qt = 0; qt < QT; ++qt)
-#pragma unroll
-                for (int m = 0; 2 * m <= qt; ++m) {
-                    const uint16_t* w = lw + ((qt * M + m) * 2 * 64 + lane) * 8;
-                    o[qt] = mfma_16x16x32(clean[m], ld8<T>(w), o[qt]);
-                    o[qt] = mfma_16x16x32(clean[m], ld8<T>(w + 64 * 8), o[qt]);
-                }
-            const float down = HALF ? part_unscale(up) : 1.f;
-#pragma unroll
-            for (int qt = 0; qt < QT; ++qt) {
-                const int i = 16 * qt + l16;
-                if (poisoned)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) o[qt][e] = i >= from[e] ? __builtin_nanf("") : o[qt][e];
-                if (i >= n) continue;
+            for (int i = 0; i < QN; ++i) {
+                const int row = 16 * tile_of(i) + l16;
+                if (row < skip) continue;
                 v4 r;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) r[e] = (el)opaque(HALF ? o[qt][e] * down : o[qt][e]);
-                *reinterpret_cast<v4*>(a.out + (c0 + i) * a.out_token_stride + h * a.out_head_stride + 16 * wave + 4 * g) = r;
+                for (int e = 0; e < 4; ++e) r[e] = (el)opaque(HALF ? o[i][e] * down : o[i][e]);
+                uint16_t* first = a.out + (t0 + c0) * a.out_token_stride + h * a.out_head_stride + 16 * wd;
+                *reinterpret_cast<v4*>(first + ((uint32_t)(row - skip) * (uint32_t)a.out_token_stride + 4 * g)) = r;
             }
         }
+        sched_fence();
+        /* the next chunk is asked for here, where it finds registers: the state's products cover some of its way, other
+           workgroups the rest */
+        if (c0 + C < len) load(c0 + C, max(2 * C - (len - c0), 0));
+        sched_fence();
         /* the next state */
-        if (n != full) {
-            full = n;
+        values();
+        float x[M][8];
+        float most = 0.f;
 #pragma unroll
-            for (int m = 0; m < M; ++m)
+        for (int m = 0; m < M; ++m)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) fade[m][e] = decay(max(n - 1 - (32 * m + e / 4 * 16 + 4 * g + e % 4), 0));
-        }
-        const float keep = decay(n);
-        v8 vp[M][VP];
+            for (int e = 0; e < 8; e += 4) {
+                const float far = decay(C - 16 - 32 * m - 4 * e);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[m][e + i] = (float)v[m][e + i] * (fade[i] * far);
+            }
         float vu = 1.f;
         if constexpr (HALF) {
-            float most = 0.f;
 #pragma unroll
             for (int m = 0; m < M; ++m)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) most = fmaxf(most, __builtin_fabsf((float)v[m][e] * fade[m][e]));
-            float x, y;
-            lanes_x16(most, x, y);
-            lanes_x32(fmaxf(x, y), x, y);
-            vu = part_scale(fmaxf(x, y));
+                for (int e = 0; e < 8; ++e) most = fmaxf(most, __builtin_fabsf(x[m][e]));
+            float y, z;
+            lanes_x16(most, y, z);
+            lanes_x32(fmaxf(y, z), y, z);
+            vu = part_scale(fmaxf(y, z));
         }
+        v8 vp[M][VP];
 #pragma unroll
         for (int m = 0; m < M; ++m) {
             u4 w[VP];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 uint32_t p[VP];
-                const float x = (float)v[m][2 * e] * fade[m][2 * e], y = (float)v[m][2 * e + 1] * fade[m][2 * e + 1];
-                parts<T, VP>(HALF ? x * vu : x, HALF ? y * vu : y, p);
+                parts<T, VP>(HALF ? x[m][2 * e] * vu : x[m][2 * e], HALF ? x[m][2 * e + 1] * vu : x[m][2 * e + 1], p);
 #pragma unroll
                 for (int i = 0; i < VP; ++i) w[i][e] = p[i];
             }
 #pragma unroll
             for (int i = 0; i < VP; ++i) vp[m][i] = __builtin_bit_cast(v8, w[i]);
         }
-        const float vd = HALF ? part_unscale(vu) : 1.f;
+        const float keep = decay(n), vd = HALF ? part_unscale(vu) : 1.f;
+        constexpr int J = DK < 4 ? DK : 4; /* tiles side by side: their products do not wait for each other */
 #pragma unroll
-        for (int j = 0; j < DK; ++j) {
-            f4 u = HALF ? f4{} : S[j] * keep;
+        for (int j0 = 0; j0 < DK; j0 += J) {
+            f4 u[J];
+#pragma unroll
+            for (int j = 0; j < J; ++j) u[j] = HALF ? f4{} : S[j0 + j] * keep;
 #pragma unroll
             for (int m = 0; m < M; ++m) {
-                const v8 k = transposed(lk, 32 * m, spot(16 * j + 4 * (l16 & 3)));
+                v8 k[J];
 #pragma unroll
-                for (int i = 0; i < VP; ++i) u = mfma_16x16x32(k, vp[m][i], u);
-            }
-            if constexpr (HALF) {
+                for (int j = 0; j < J; ++j) k[j] = transposed(lk, 32 * m, spot(16 * (j0 + j) + 4 * (l16 & 3)));
 #pragma unroll
-                for (int e = 0; e < 4; ++e) S[j][e] = __builtin_fmaf(u[e], vd, S[j][e] * keep);
-            } else {
-                S[j] = u;
+                for (int i = 0; i < VP; ++i)
+#pragma unroll
+                    for (int j = 0; j < J; ++j) u[j] = mfma_16x16x32(k[j], vp[m][i], u[j]);
             }
+#pragma unroll
+            for (int j = 0; j < J; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) S[j0 + j][e] = HALF ? __builtin_fmaf(u[j][e], vd, S[j0 + j][e] * keep) : u[j][e];
         }
     }
+    if (wq > 0) return; /* the same state */
     if constexpr (STATES) {
 #pragma unroll
-        for (int j = 0; j < DK; ++j) mine[NT * j] = S[j];
+        for (int j = 0; j < DK; ++j) mine[64 * WD * j] = S[j];
     } else if (number >= 0 && a.state_out && t1 == lt.rows.end) {
 #pragma unroll
         for (int j = 0; j < DK; ++j)
@@ -444,8 +515,8 @@ __device__ __forceinline__ void linear_step(const LinearAttnArgs& a) {
 }
 
 #define LINEAR(NAME, T, HD)                                                                                                   \
-    extern "C" __global__ void __launch_bounds__(4 * HD) prism_linear_attn_##NAME##_h##HD(LinearAttnArgs a) { linear_segment<T, HD, false>(a); } \
-    extern "C" __global__ void __launch_bounds__(4 * HD) prism_linear_states_##NAME##_h##HD(LinearAttnArgs a) { linear_segment<T, HD, true>(a); } \
+    extern "C" __global__ void __launch_bounds__(HD < 64 ? 256 : 4 * HD, HD == 64 ? 3 : HD == 128 ? 2 : 4) prism_linear_attn_##NAME##_h##HD(LinearAttnArgs a) { linear_segment<T, HD, false>(a); } \
+    extern "C" __global__ void __launch_bounds__(4 * HD, 4) prism_linear_states_##NAME##_h##HD(LinearAttnArgs a) { linear_segment<T, HD, true>(a); } \
     extern "C" __global__ void __launch_bounds__(256) prism_linear_step_##NAME##_h##HD(LinearAttnArgs a) { linear_step<T, HD>(a); }
 LINEAR(f16, F16, 16) LINEAR(f16, F16, 32) LINEAR(f16, F16, 64) LINEAR(f16, F16, 128)
 LINEAR(bf16, BF16, 16) LINEAR(bf16, BF16, 32) LINEAR(bf16, BF16, 64) LINEAR(bf16, BF16, 128)

@@ -48,11 +48,6 @@ __device__ __forceinline__ void two_numbers(float z0, float z1, float least, b2&
     lo = b2{(__bf16)opaque(__builtin_amdgcn_fmed3f(z0 - c0, least, c0)), (__bf16)opaque(__builtin_amdgcn_fmed3f(z1 - c1, least, c1))};
 }
 
-template <int N>
-struct Count {
-    static constexpr int value = N;
-};
-
 /* What a wave has to do: which sequence and heads, and which of the keys seen
  * (in the order: sinks, window). */
 struct PagedWork {

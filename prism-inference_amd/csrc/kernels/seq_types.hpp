@@ -25,6 +25,11 @@ struct BF16 {
     typedef b2 v2;
 };
 
+template <int N>
+struct Count {
+    static constexpr int value = N;
+};
+
 template <class T>
 __device__ __forceinline__ typename T::v8 ld8(const uint16_t* p) {
     return *reinterpret_cast<const typename T::v8*>(p);
