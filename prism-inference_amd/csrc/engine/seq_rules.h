@@ -205,7 +205,16 @@ inline int check_linear_step(const prism_linear_attn_push& p, const char** why) 
 }
 
 /* How a linear attention is launched: tokens of a segment, and segments (some of them empty). Sequences of one segment each need no
- * first launch and no workspace. */
+ * first launch and no workspace.
+ *
+ * A workgroup's chunks follow each other, so few sequences are split; each segment but the first then starts from the sum of those
+ * before it, which a launch of its own made: its keys and values are read twice. us without, and in segments of 64, 128, 256, 512,
+ * 1024, 1536 (heads x channels):
+ *   1 x 8,160, 8 x 32    204 | 38 22 21 27 42 59        5 x 4,500, 32 x 32   149 | 217 126 99 90 92 107
+ *   1 x 8,160, 8 x 128   598 | 230 86 60 73 118 164     5 x 4,500, 32 x 128  370 | - 689 402 330 339 293
+ *   2 x 1,000, 8 x 32    36 | 11 13 17 27               64 x 1,000, 8 x 32   41 | 103 74 65 63
+ *   3 x 500, 4 x 64      28 | 13 15 22                  64 x 1,000, 8 x 128  163 | 517 318 247 223
+ *   1 x 32,000, 4 x 128  2,317 | - - 162 105 132 173    16 x 500, 8 x 128    48 | 59 45 54 */
 struct LinearPlan {
     int32_t segment;
     bool split;
@@ -214,10 +223,10 @@ struct LinearPlan {
 inline LinearPlan linear_plan(const prism_linear_attn_push& p) {
     LinearPlan r = {INT32_MAX, false, std::max(p.n_seqs, 1)};
     const int64_t n_seqs = std::max(p.n_seqs, 1), each = p.n_tokens / n_seqs;
-    const int64_t want = 768, least = 128; /* workgroups; tokens */
-    if (n_seqs * p.n_heads >= want || each < 2 * least) return r;
-    int64_t s = (int64_t)p.n_tokens * p.n_heads / want;
-    s = std::max(s, std::max(least, each / 32));
+    const bool wide = p.head_dim >= 128; /* two workgroups fill a CU, and states are as large as chunks */
+    if (n_seqs * p.n_heads >= (wide ? 256 : 512) || each < 4 * LINEAR_CHUNK) return r;
+    /* as many workgroups as the GPU has room for, and segments as long as their number is costly */
+    int64_t s = std::max((int64_t)p.n_tokens * p.n_heads / (wide ? 480 : 768), (int64_t)std::sqrt(8.0 * (double)each));
     s = (s + LINEAR_CHUNK - 1) / LINEAR_CHUNK * LINEAR_CHUNK;
     r.segment = (int32_t)s;
     r.split = true;

@@ -433,11 +433,12 @@ extern "C" int prism_linear_attn(prism_ctx* c, const prism_linear_attn_push* p, 
     a.segment = plan.segment;
     a.ws = static_cast<float*>(workspace);
     const int i = hd_index(p->head_dim);
-    const unsigned threads = 4 * p->head_dim; /* a wave for 16 channels of the values; below 64, of the outputs' four query tiles */
+    /* a wave for 16 channels of the values (of 128, for 32); below 64, four waves by query tiles for what has queries */
+    const unsigned states = p->head_dim < 128 ? 4 * p->head_dim : 256, threads = std::max(states, 256u);
     const int64_t grid = plan.segments * p->n_heads;
     if (plan.split)
-        if (const int rc = launch(c, c->f_linear_states[p->dtype][i], what, grid, threads, &a, stream)) return rc;
-    return launch(c, c->f_linear[p->dtype][i], what, grid, std::max(threads, 256u), &a, stream);
+        if (const int rc = launch(c, c->f_linear_states[p->dtype][i], what, grid, states, &a, stream)) return rc;
+    return launch(c, c->f_linear[p->dtype][i], what, grid, threads, &a, stream);
 }
 
 extern "C" int prism_linear_step(prism_ctx* c, const prism_linear_attn_push* p, const void* q, const void* k, const void* v,

@@ -108,14 +108,14 @@ __device__ __forceinline__ void linear_segment(const LinearAttnArgs& a) {
     typedef typename T::el el;
     constexpr bool HALF = __is_same(T, F16);
     constexpr int C = LINEAR_CHUNK, QT = C / 16, M = C / 32;
-    constexpr int WD = HD / 16, WQ = STATES || HD >= 64 ? 1 : QT / WD, QN = QT / WQ; /* waves by channels, by query tiles; a wave's */
+    constexpr int DV = HD >= 128 ? 2 : 1;          /* a wave's 16-channel tiles of the values */
+    constexpr int WD = HD / 16 / DV, WQ = STATES || HD >= 64 ? 1 : QT / WD, QN = QT / WQ; /* waves by channels, by query tiles; a wave's */
     constexpr bool SHARED = WQ == 1;
     constexpr int NT = 64 * WD * WQ;
     constexpr int DK = HD / 16; /* 16-channel tiles of the keys */
     constexpr int KS = (HD + 31) / 32;
     constexpr int RS = HD >= 32 ? HD + 16 : HD;    /* LDS row: 4 rows' parts of a transposed read lie in different banks */
     constexpr int CPR = HD / 8, NL = (C * CPR + NT - 1) / NT; /* 16-byte chunks a row, and a thread's of a matrix */
-    constexpr int VP = HALF ? 2 : 3;               /* parts of a decayed value */
     constexpr int TILES = QT * (QT + 1) / 2;       /* of weights */
     __shared__ __attribute__((aligned(16))) uint16_t lq[STATES ? 8 : C * RS], lk[C * RS], lv[C * RS];
     __shared__ __attribute__((aligned(16))) uint16_t lw[!STATES && SHARED ? 6 * 2 * 64 * 8 : 8]; /* weights [query tile, 32 keys][part] */
@@ -132,39 +132,33 @@ __device__ __forceinline__ void linear_segment(const LinearAttnArgs& a) {
 
     const float r2 = linear_rate(a, h);
     const auto decay = [&](int n) { return fast_exp2(-r2 * (float)n); };
+    const float d1 = decay(1), d2 = decay(2), d3 = decay(3);
     const int number = linear_state(a, lt.seq);
-    const int64_t base = ((int64_t)max(number, 0) * a.n_heads + h) * HD * HD + 16 * wd + l16;
-    f4* const mine = reinterpret_cast<f4*>(a.ws) + ((int64_t)b * a.n_heads + h) * (HD * HD / 4) + wd * 64 + lane; /* + 64 WD * tile */
-    f4 S[DK]; /* channels 16 j + 4 g + e of the keys x channel 16 wd + l16 of the values */
+    const int64_t base = ((int64_t)max(number, 0) * a.n_heads + h) * HD * HD + 16 * DV * wd + l16;
+    f4* const mine = reinterpret_cast<f4*>(a.ws) + ((int64_t)b * a.n_heads + h) * (HD * HD / 4) + wd * 64 + lane; /* + 64 WD * (tile DV + d) */
+    f4 S[DK][DV]; /* channels 16 j + 4 g + e of the keys x channel 16 (DV wd + d) + l16 of the values */
 #pragma unroll
     for (int j = 0; j < DK; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            S[j][e] = !STATES && a.state_in && number >= 0 ? a.state_in[base + (16 * j + 4 * g + e) * HD] : 0.f;
+        for (int d = 0; d < DV; ++d)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                S[j][d][e] = !STATES && a.state_in && number >= 0 ? a.state_in[base + (16 * j + 4 * g + e) * HD + 16 * d] : 0.f;
     if constexpr (!STATES) {
-        constexpr int DEPTH = 16 / DK; /* segments asked for at once */
+        constexpr int DEPTH = DK * DV < 8 ? 16 / (DK * DV) : 2; /* segments asked for at once */
         const float keep = decay(a.segment);
         for (int s = seg; s > 0; s -= DEPTH) {
-            f4 u[DEPTH][DK];
+            f4 u[DEPTH][DK * DV];
 #pragma unroll
             for (int i = 0; i < DEPTH; ++i)
 #pragma unroll
-                for (int j = 0; j < DK; ++j) u[i][j] = mine[64 * WD * j - (int64_t)max(s - i, 1) * a.n_heads * (HD * HD / 4)];
+                for (int j = 0; j < DK * DV; ++j) u[i][j] = mine[64 * WD * j - (int64_t)max(s - i, 1) * a.n_heads * (HD * HD / 4)];
 #pragma unroll
             for (int i = 0; i < DEPTH; ++i)
                 if (i < s)
 #pragma unroll
-                    for (int j = 0; j < DK; ++j) S[j] = S[j] * keep + u[i][j];
+                    for (int j = 0; j < DK * DV; ++j) S[j / DV][j % DV] = S[j / DV][j % DV] * keep + u[i][j];
         }
-    }
-    /* decays: of a key in a query's tile, and in the tile before; of a token up to its 16's end */
-    float within[4], before[4], fade[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const int gap = l16 - 4 * g - e;
-        within[e] = gap >= 0 ? decay(max(gap, 0)) * a.scale : 0.f;
-        before[e] = decay(16 + gap) * a.scale;
-        fade[e] = decay(15 - 4 * g - e);
     }
     if constexpr (!STATES && SHARED) /* keys behind a tile's queries, in the 32 that it has a part of */
         for (int x = tid; x < 256; x += NT)
@@ -194,22 +188,37 @@ __device__ __forceinline__ void linear_segment(const LinearAttnArgs& a) {
     /* A chunk's tokens lie at its end: a short one, the segment's last, has rows of zeros before them, so that decays up to
        the end are always the same. Token strides are at most 2^22: 32-bit offsets from a base that is the same for all. */
     v8 rq[STATES ? 1 : NL], rk[NL], rv[NL];
-    const auto load = [&](int c0, int skip) {
-        const auto at = [&](const uint16_t* m, int64_t stride, int64_t head, int row, int c) {
-            const uint16_t* first = m + (t0 + c0) * stride + head;
-            return ld8<T>(first + ((uint32_t)max(row - skip, 0) * (uint32_t)stride + c));
-        };
+    const int row0 = min(tid / CPR, C - 1), col0 = tid % CPR * 8;
+    const auto load = [&](const uint16_t* m, int64_t first, uint32_t stride, uint32_t offset, v8 (&r)[NL]) { /* bytes */
 #pragma unroll
-        for (int i = 0; i < NL; ++i) {
-            const int id = tid + NT * i, row = min(id / CPR, C - 1), c = id % CPR * 8;
-            if constexpr (!STATES) rq[i] = at(a.q, a.q_token_stride, h * a.q_head_stride, row, c);
-            rk[i] = at(a.k, a.k_token_stride, hk * a.k_head_stride, row, c);
-            rv[i] = at(a.v, a.v_token_stride, hk * a.v_head_stride, row, c);
-            if (row < skip) rk[i] = rv[i] = v8{};
-        }
+        for (int i = 0; i < NL; ++i)
+            r[i] = *reinterpret_cast<const v8*>(reinterpret_cast<const char*>(m) + first + (int64_t)(NT / CPR * i) * stride + offset);
+    };
+    const uint32_t sq = 2 * (uint32_t)a.q_token_stride, sk = 2 * (uint32_t)a.k_token_stride, sv = 2 * (uint32_t)a.v_token_stride;
+    const uint32_t oq = row0 * sq + 2 * col0, ok = row0 * sk + 2 * col0, ov = row0 * sv + 2 * col0;
+    const auto load_chunk = [&](int64_t first) { /* 64 tokens from there on */
+        if constexpr (!STATES) load(a.q + h * a.q_head_stride, first * sq, sq, oq, rq);
+        load(a.k + hk * a.k_head_stride, first * sk, sk, ok, rk);
+        load(a.v + hk * a.v_head_stride, first * sv, sv, ov, rv);
+    };
+    const auto no_keys = [&](int rows) { /* the first ones are not the chunk's */
+#pragma unroll
+        for (int i = 0; i < NL; ++i)
+            if (row0 + NT / CPR * i < rows) rk[i] = rv[i] = v8{};
     };
     const int len = t1 > t0 ? t1 - (int)t0 : 0;
-    if (len > 0) load(0, max(C - len, 0));
+    if (len >= C) {
+        load_chunk(t0);
+    } else if (len > 0) { /* nothing before it is the segment's, or need exist */
+#pragma unroll
+        for (int i = 0; i < NL; ++i) {
+            const int64_t t = t0 + max(row0 + NT / CPR * i - (C - len), 0);
+            if constexpr (!STATES) rq[i] = ld8<T>(a.q + t * a.q_token_stride + h * a.q_head_stride + col0);
+            rk[i] = ld8<T>(a.k + t * a.k_token_stride + hk * a.k_head_stride + col0);
+            rv[i] = ld8<T>(a.v + t * a.v_token_stride + hk * a.v_head_stride + col0);
+        }
+        no_keys(C - len);
+    }
     for (int c0 = 0; c0 < len; c0 += C) {
         const int n = min(C, len - c0), skip = C - n, turn = c0 / C & 1;
         __syncthreads(); /* the chunk before has been read */
@@ -252,10 +261,17 @@ __device__ __forceinline__ void linear_segment(const LinearAttnArgs& a) {
         }
         __syncthreads();
 
-        v8 v[M]; /* lane l16 is a channel */
+        if (c0 + C < len) {
+            const int early = max(2 * C - (len - c0), 0);
+            load_chunk(t0 + c0 + C - early);
+            if (early > 0) no_keys(early);
+        }
+        v8 v[DV][M]; /* lane l16 is a channel */
         const auto values = [&] {
 #pragma unroll
-            for (int m = 0; m < M; ++m) v[m] = transposed(lv, 32 * m, 16 * wd + 4 * (l16 & 3));
+            for (int d = 0; d < DV; ++d)
+#pragma unroll
+                for (int m = 0; m < M; ++m) v[d][m] = transposed(lv, 32 * m, 16 * (DV * wd + d) + 4 * (l16 & 3));
         };
         if constexpr (!STATES) {
             /* fp16 weights are scaled by a power of two, after the largest that they could be: 2^15 stays above them, and
@@ -276,11 +292,16 @@ __device__ __forceinline__ void linear_segment(const LinearAttnArgs& a) {
                 f4 w = {};
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks) w = mfma_16x16x32(row_of(lk, 16 * kt + l16, ks), row_of(lq, 16 * qt + l16, ks), w);
-                const float far = decay(16 * max(qt - kt - 1, 0)) * up;
+                const int gap = 16 * (qt - kt) + l16 - 4 * g;
+                if (kt < qt) { /* gap is 4 or more */
+                    const float far = decay(gap - 3) * (a.scale * up);
+                    w[0] *= far * d3;
+                    w[1] *= far * d2;
+                    w[2] *= far * d1;
+                    w[3] *= far;
+                } else {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float y = w[e] * ((kt == qt ? within[e] : before[e]) * far);
-                    w[e] = kt < qt || l16 >= 4 * g + e ? y : 0.f;
+                    for (int e = 0; e < 4; ++e) w[e] = gap >= e ? w[e] * (decay(max(gap - e, 0)) * (a.scale * up)) : 0.f;
                 }
                 uint32_t p[2][2];
                 parts<T, 2>(w[0], w[1], p[0]);
@@ -301,69 +322,86 @@ __device__ __forceinline__ void linear_segment(const LinearAttnArgs& a) {
                     *reinterpret_cast<uint64_t*>(to + 64 * 8) = lo[0] | (uint64_t)lo[1] << 32;
                 }
             }
-            f4 o[QN] = {};
-            f4 back = {}; /* fp16: what takes the scales out of the output's rows 4 g + e */
-            float su = 1.f;
+            f4 o[QN][DV] = {};
+            f4 back[DV] = {}; /* fp16: what takes the scales out of the output's rows 4 g + e */
+            float su[DV];
             if constexpr (HALF) {
-                float most = 0.f;
 #pragma unroll
-                for (int j = 0; j < DK; ++j)
+                for (int d = 0; d < DV; ++d) {
+                    float most = 0.f, x, y;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) most = fmaxf(most, __builtin_fabsf(S[j][e]));
-                float x, y;
-                lanes_x16(most, x, y);
-                lanes_x32(fmaxf(x, y), x, y);
-                su = part_scale(fmaxf(x, y));
-                const float down = part_unscale(su) * up;
+                    for (int j = 0; j < DK; ++j)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) back[e] = __shfl(down, 4 * g + e);
+                        for (int e = 0; e < 4; ++e) most = fmaxf(most, __builtin_fabsf(S[j][d][e]));
+                    lanes_x16(most, x, y);
+                    lanes_x32(fmaxf(x, y), x, y);
+                    su[d] = part_scale(fmaxf(x, y));
+                    const float down = part_unscale(su[d]) * up;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) back[d][e] = __shfl(down, 4 * g + e);
+                }
             }
             /* q S, the state in parts: lane l16 is a channel of the values, with 8 of each 32 channels of the keys */
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
-                u4 hi = {}, lo = {};
+                v8 s[DV][2];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int j = 2 * ks + e / 2;
-                    if (j >= DK) continue;
-                    uint32_t p[2];
-                    const float x = S[j < DK ? j : 0][e % 2 * 2], y = S[j < DK ? j : 0][e % 2 * 2 + 1];
-                    parts<T, 2>(HALF ? x * su : x, HALF ? y * su : y, p);
-                    hi[e] = p[0];
-                    lo[e] = p[1];
+                for (int d = 0; d < DV; ++d) {
+                    u4 hi = {}, lo = {};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int j = 2 * ks + e / 2;
+                        if (j >= DK) continue;
+                        uint32_t p[2];
+                        const float x = S[j < DK ? j : 0][d][e % 2 * 2], y = S[j < DK ? j : 0][d][e % 2 * 2 + 1];
+                        parts<T, 2>(HALF ? x * su[d] : x, HALF ? y * su[d] : y, p);
+                        hi[e] = p[0];
+                        lo[e] = p[1];
+                    }
+                    s[d][0] = __builtin_bit_cast(v8, hi);
+                    s[d][1] = __builtin_bit_cast(v8, lo);
                 }
                 v8 q[QN];
 #pragma unroll
                 for (int i = 0; i < QN; ++i) q[i] = row_of(lq, 16 * tile_of(i) + l16, ks);
 #pragma unroll
-                for (int i = 0; i < QN; ++i) o[i] = mfma_16x16x32(__builtin_bit_cast(v8, hi), q[i], o[i]);
+                for (int part = 0; part < 2; ++part)
 #pragma unroll
-                for (int i = 0; i < QN; ++i) o[i] = mfma_16x16x32(__builtin_bit_cast(v8, lo), q[i], o[i]);
+                    for (int i = 0; i < QN; ++i)
+#pragma unroll
+                        for (int d = 0; d < DV; ++d) o[i][d] = mfma_16x16x32(s[d][part], q[i], o[i][d]);
             }
 #pragma unroll
             for (int i = 0; i < QN; ++i) {
                 const float far = decay(max(16 * tile_of(i) + l16 + 1 - skip, 0)) * a.scale;
-                if constexpr (HALF) o[i] *= back;
-                o[i] *= far;
+#pragma unroll
+                for (int d = 0; d < DV; ++d) {
+                    if constexpr (HALF) o[i][d] *= back[d];
+                    o[i][d] *= far;
+                }
             }
             /* values that are not finite must not meet weights of zero: queries before them */
             const bool poisoned = __builtin_amdgcn_readfirstlane(bad) != 0;
-            sched_fence(); /* the products' operands are dead; what follows needs its registers */
             if constexpr (SHARED) __syncthreads(); /* the weights are in */
             values();
             if (poisoned)
 #pragma unroll
-                for (int m = 0; m < M; ++m)
+                for (int d = 0; d < DV; ++d)
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) v[m][e] = __builtin_fabsf((float)v[m][e]) < INFINITY ? v[m][e] : (el)0.f;
+                    for (int m = 0; m < M; ++m)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) v[d][m][e] = __builtin_fabsf((float)v[d][m][e]) < INFINITY ? v[d][m][e] : (el)0.f;
             if constexpr (SHARED) {
 #pragma unroll
                 for (int m = 0; m < M; ++m)
 #pragma unroll
                     for (int part = 0; part < 2; ++part)
 #pragma unroll
-                        for (int qt = 2 * m; qt < QT; ++qt)
-                            o[qt] = mfma_16x16x32(v[m], ld8<T>(lw + weights_at(qt, m) + (part * 64 + lane) * 8), o[qt]);
+                        for (int qt = 2 * m; qt < QT; ++qt) {
+                            const v8 w = ld8<T>(lw + weights_at(qt, m) + (part * 64 + lane) * 8);
+#pragma unroll
+                            for (int d = 0; d < DV; ++d) o[qt][d] = mfma_16x16x32(v[d][m], w, o[qt][d]);
+                        }
             } else {
 #pragma unroll
                 for (int i = 0; i < QN; ++i) {
@@ -375,108 +413,159 @@ __device__ __forceinline__ void linear_segment(const LinearAttnArgs& a) {
                         weigh(qt, 2 * m, hi[0], lo[0]);
                         if (2 * m < qt) weigh(qt, 2 * m + 1, hi[1], lo[1]);
                         else hi[1][0] = hi[1][1] = 0;
-                        o[i] = mfma_16x16x32(v[m], __builtin_bit_cast(v8, u4{hi[0][0], hi[0][1], hi[1][0], hi[1][1]}), o[i]);
-                        o[i] = mfma_16x16x32(v[m], __builtin_bit_cast(v8, u4{lo[0][0], lo[0][1], lo[1][0], lo[1][1]}), o[i]);
+#pragma unroll
+                        for (int d = 0; d < DV; ++d) {
+                            o[i][d] = mfma_16x16x32(v[d][m], __builtin_bit_cast(v8, u4{hi[0][0], hi[0][1], hi[1][0], hi[1][1]}), o[i][d]);
+                            o[i][d] = mfma_16x16x32(v[d][m], __builtin_bit_cast(v8, u4{lo[0][0], lo[0][1], lo[1][0], lo[1][1]}), o[i][d]);
+                        }
                     }
                 }
             }
             const float down = HALF ? part_unscale(up) : 1.f;
-            if (poisoned) { /* what sees one of them */
-                int from[4] = {C, C, C, C}; /* the first in channel 4 g + e */
-                for (int t = C - 1; t >= 0; --t)
+            if (poisoned) /* what sees one of them */
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (!(__builtin_fabsf(ld1<T>(lv + t * RS + 16 * wd + 4 * g + e)) < INFINITY)) from[e] = t;
+                for (int d = 0; d < DV; ++d) {
+                    int from[4] = {C, C, C, C}; /* the first in channel 4 g + e */
+                    for (int t = C - 1; t >= 0; --t)
 #pragma unroll
-                for (int i = 0; i < QN; ++i)
+                        for (int e = 0; e < 4; ++e)
+                            if (!(__builtin_fabsf(ld1<T>(lv + t * RS + 16 * (DV * wd + d) + 4 * g + e)) < INFINITY)) from[e] = t;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) o[i][e] = 16 * tile_of(i) + l16 >= from[e] ? __builtin_nanf("") : o[i][e];
-            }
+                    for (int i = 0; i < QN; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[i][d][e] = 16 * tile_of(i) + l16 >= from[e] ? __builtin_nanf("") : o[i][d][e];
+                }
 #pragma unroll
             for (int i = 0; i < QN; ++i) {
                 const int row = 16 * tile_of(i) + l16;
                 if (row < skip) continue;
-                v4 r;
+                uint16_t* first = a.out + (t0 + c0) * a.out_token_stride + h * a.out_head_stride + 16 * DV * wd;
+                first += (uint32_t)(row - skip) * (uint32_t)a.out_token_stride + 4 * g;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) r[e] = (el)opaque(HALF ? o[i][e] * down : o[i][e]);
-                uint16_t* first = a.out + (t0 + c0) * a.out_token_stride + h * a.out_head_stride + 16 * wd;
-                *reinterpret_cast<v4*>(first + ((uint32_t)(row - skip) * (uint32_t)a.out_token_stride + 4 * g)) = r;
+                for (int d = 0; d < DV; ++d) {
+                    v4 r;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) r[e] = (el)opaque(HALF ? o[i][d][e] * down : o[i][d][e]);
+                    *reinterpret_cast<v4*>(first + 16 * d) = r;
+                }
             }
         }
-        sched_fence();
-        /* the next chunk is asked for here, where it finds registers: the state's products cover some of its way, other
-           workgroups the rest */
-        if (c0 + C < len) load(c0 + C, max(2 * C - (len - c0), 0));
-        sched_fence();
         /* the next state */
         values();
-        float x[M][8];
-        float most = 0.f;
+        const float keep = decay(n);
+        float fade[4];
 #pragma unroll
-        for (int m = 0; m < M; ++m)
+        for (int i = 0; i < 4; ++i) fade[i] = decay(15 - 4 * g - i);
+        const auto faded = [&](int d, int m, float (&x)[8]) {
 #pragma unroll
             for (int e = 0; e < 8; e += 4) {
                 const float far = decay(C - 16 - 32 * m - 4 * e);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) x[m][e + i] = (float)v[m][e + i] * (fade[i] * far);
+                for (int i = 0; i < 4; ++i) x[e + i] = (float)v[d][m][e + i] * (fade[i] * far);
             }
-        float vu = 1.f;
+        };
+        const auto key = [&](int m, int j) { return transposed(lk, 32 * m, spot(16 * j + 4 * (l16 & 3))); };
+        constexpr int J = DK < 4 / DV ? DK : 4 / DV; /* tiles side by side: their products do not wait for each other */
         if constexpr (HALF) {
+            /* scaled by a power of two to fp16's range, for each channel of the values */
+            v8 vp[DV][M][2];
+            float down[DV];
 #pragma unroll
-            for (int m = 0; m < M; ++m)
+            for (int d = 0; d < DV; ++d) {
+                float x[M][8], most = 0.f, y, z;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) most = fmaxf(most, __builtin_fabsf(x[m][e]));
-            float y, z;
-            lanes_x16(most, y, z);
-            lanes_x32(fmaxf(y, z), y, z);
-            vu = part_scale(fmaxf(y, z));
-        }
-        v8 vp[M][VP];
+                for (int m = 0; m < M; ++m) {
+                    faded(d, m, x[m]);
 #pragma unroll
-        for (int m = 0; m < M; ++m) {
-            u4 w[VP];
+                    for (int e = 0; e < 8; ++e) most = fmaxf(most, __builtin_fabsf(x[m][e]));
+                }
+                lanes_x16(most, y, z);
+                lanes_x32(fmaxf(y, z), y, z);
+                const float up = part_scale(fmaxf(y, z));
+                down[d] = part_unscale(up);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                uint32_t p[VP];
-                parts<T, VP>(HALF ? x[m][2 * e] * vu : x[m][2 * e], HALF ? x[m][2 * e + 1] * vu : x[m][2 * e + 1], p);
+                for (int m = 0; m < M; ++m) {
+                    u4 w[2];
 #pragma unroll
-                for (int i = 0; i < VP; ++i) w[i][e] = p[i];
+                    for (int e = 0; e < 4; ++e) {
+                        uint32_t p[2];
+                        parts<T, 2>(x[m][2 * e] * up, x[m][2 * e + 1] * up, p);
+                        w[0][e] = p[0];
+                        w[1][e] = p[1];
+                    }
+                    vp[d][m][0] = __builtin_bit_cast(v8, w[0]);
+                    vp[d][m][1] = __builtin_bit_cast(v8, w[1]);
+                }
             }
 #pragma unroll
-            for (int i = 0; i < VP; ++i) vp[m][i] = __builtin_bit_cast(v8, w[i]);
-        }
-        const float keep = decay(n), vd = HALF ? part_unscale(vu) : 1.f;
-        constexpr int J = DK < 4 ? DK : 4; /* tiles side by side: their products do not wait for each other */
+            for (int j0 = 0; j0 < DK; j0 += J) {
+                f4 u[J][DV] = {};
 #pragma unroll
-        for (int j0 = 0; j0 < DK; j0 += J) {
-            f4 u[J];
+                for (int m = 0; m < M; ++m) {
+                    v8 k[J];
 #pragma unroll
-            for (int j = 0; j < J; ++j) u[j] = HALF ? f4{} : S[j0 + j] * keep;
+                    for (int j = 0; j < J; ++j) k[j] = key(m, j0 + j);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int j = 0; j < J; ++j)
+#pragma unroll
+                            for (int d = 0; d < DV; ++d) u[j][d] = mfma_16x16x32(k[j], vp[d][m][i], u[j][d]);
+                }
+#pragma unroll
+                for (int j = 0; j < J; ++j)
+#pragma unroll
+                    for (int d = 0; d < DV; ++d)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) S[j0 + j][d][e] = __builtin_fmaf(u[j][d][e], down[d], S[j0 + j][d][e] * keep);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < DK; ++j)
+#pragma unroll
+                for (int d = 0; d < DV; ++d) S[j][d] *= keep;
 #pragma unroll
             for (int m = 0; m < M; ++m) {
-                v8 k[J];
+                u4 w[DV][3];
 #pragma unroll
-                for (int j = 0; j < J; ++j) k[j] = transposed(lk, 32 * m, spot(16 * (j0 + j) + 4 * (l16 & 3)));
+                for (int d = 0; d < DV; ++d) {
+                    float x[8];
+                    faded(d, m, x);
 #pragma unroll
-                for (int i = 0; i < VP; ++i)
+                    for (int e = 0; e < 4; ++e) {
+                        uint32_t p[3];
+                        parts<T, 3>(x[2 * e], x[2 * e + 1], p);
 #pragma unroll
-                    for (int j = 0; j < J; ++j) u[j] = mfma_16x16x32(k[j], vp[m][i], u[j]);
+                        for (int i = 0; i < 3; ++i) w[d][i][e] = p[i];
+                    }
+                }
+#pragma unroll
+                for (int j0 = 0; j0 < DK; j0 += J) {
+                    v8 k[J];
+#pragma unroll
+                    for (int j = 0; j < J; ++j) k[j] = key(m, j0 + j);
+#pragma unroll
+                    for (int i = 0; i < 3; ++i)
+#pragma unroll
+                        for (int j = 0; j < J; ++j)
+#pragma unroll
+                            for (int d = 0; d < DV; ++d)
+                                S[j0 + j][d] = mfma_16x16x32(k[j], __builtin_bit_cast(v8, w[d][i]), S[j0 + j][d]);
+                }
             }
-#pragma unroll
-            for (int j = 0; j < J; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) S[j0 + j][e] = HALF ? __builtin_fmaf(u[j][e], vd, S[j0 + j][e] * keep) : u[j][e];
         }
     }
     if (wq > 0) return; /* the same state */
     if constexpr (STATES) {
 #pragma unroll
-        for (int j = 0; j < DK; ++j) mine[64 * WD * j] = S[j];
+        for (int j = 0; j < DK * DV; ++j) mine[64 * WD * j] = S[j / DV][j % DV];
     } else if (number >= 0 && a.state_out && t1 == lt.rows.end) {
 #pragma unroll
         for (int j = 0; j < DK; ++j)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) a.state_out[base + (16 * j + 4 * g + e) * HD] = S[j][e];
+            for (int d = 0; d < DV; ++d)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) a.state_out[base + (16 * j + 4 * g + e) * HD + 16 * d] = S[j][d][e];
     }
 }
 
@@ -515,8 +604,8 @@ __device__ __forceinline__ void linear_step(const LinearAttnArgs& a) {
 }
 
 #define LINEAR(NAME, T, HD)                                                                                                   \
-    extern "C" __global__ void __launch_bounds__(HD < 64 ? 256 : 4 * HD, HD == 64 ? 3 : HD == 128 ? 2 : 4) prism_linear_attn_##NAME##_h##HD(LinearAttnArgs a) { linear_segment<T, HD, false>(a); } \
-    extern "C" __global__ void __launch_bounds__(4 * HD, 4) prism_linear_states_##NAME##_h##HD(LinearAttnArgs a) { linear_segment<T, HD, true>(a); } \
+    extern "C" __global__ void __launch_bounds__(256, HD < 32 ? 4 : HD < 128 ? 3 : 2) prism_linear_attn_##NAME##_h##HD(LinearAttnArgs a) { linear_segment<T, HD, false>(a); } \
+    extern "C" __global__ void __launch_bounds__(HD < 128 ? 4 * HD : 256, HD < 128 ? 3 : 2) prism_linear_states_##NAME##_h##HD(LinearAttnArgs a) { linear_segment<T, HD, true>(a); } \
     extern "C" __global__ void __launch_bounds__(256) prism_linear_step_##NAME##_h##HD(LinearAttnArgs a) { linear_step<T, HD>(a); }
 LINEAR(f16, F16, 16) LINEAR(f16, F16, 32) LINEAR(f16, F16, 64) LINEAR(f16, F16, 128)
 LINEAR(bf16, BF16, 16) LINEAR(bf16, BF16, 32) LINEAR(bf16, BF16, 64) LINEAR(bf16, BF16, 128)
