@@ -138,7 +138,8 @@ extern "C" int prism_create(prism_ctx** out, int32_t device, const char* code_ob
             for (int g = 0; g < 3; ++g)
                 all.emplace_back(&c->f_paged[t][i][g], "prism_paged_attn_" + shape + (g == 0 ? "_g1" : g == 1 ? "_g2" : "_many"));
             all.emplace_back(&c->f_paged_join[t][i], "prism_paged_attn_join_" + shape);
-            all.emplace_back(&c->f_paged4[t][i], "prism_paged_attn4_" + shape + "_many");
+            for (int g = i < 2 ? 0 : 2; g < 3; ++g)
+                all.emplace_back(&c->f_paged4[t][i][g], "prism_paged_attn4_" + shape + (g == 0 ? "_g1" : g == 1 ? "_g2" : "_many"));
             all.emplace_back(&c->f_linear[t][i], "prism_linear_attn_" + shape);
             all.emplace_back(&c->f_linear_states[t][i], "prism_linear_states_" + shape);
             all.emplace_back(&c->f_linear_step[t][i], "prism_linear_step_" + shape);

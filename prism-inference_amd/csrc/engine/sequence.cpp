@@ -188,8 +188,8 @@ int paged(prism_ctx* c, const prism_paged_attn_push* p, bool four, const void* q
     a.splits = plan.splits;
     a.ws = static_cast<float*>(workspace);
     const int i = hd_index(d.head_dim), kind = plan.many ? 2 : p->n_heads / d.n_kv_heads - 1;
-    const int rc = launch(c, four ? c->f_paged4[d.dtype][i] : c->f_paged[d.dtype][i][kind], "paged attention", plan.grid, 256,
-                          &a, stream);
+    const hipFunction_t f = four ? c->f_paged4[d.dtype][i][d.head_dim > 32 ? 2 : kind] : c->f_paged[d.dtype][i][kind];
+    const int rc = launch(c, f, "paged attention", plan.grid, 256, &a, stream);
     if (rc || plan.splits == 1) return rc;
     return launch(c, c->f_paged_join[d.dtype][i], "paged attention's join", (int64_t)d.n_seqs * p->n_heads, 256, &a, stream);
 }

@@ -40,7 +40,6 @@ __device__ __forceinline__ LinearTile linear_tile(const LinearAttnArgs& a, int b
     }
 }
 
-typedef float f2 __attribute__((ext_vector_type(2)));
 /* Two fp32 numbers as N pairs of 16-bit ones that add up to them: fp16 11 N bits (of what is above its smallest), bf16 8 N.
  * Rounded to nearest, so that what is left has a sign and half a bit more. */
 template <class T, int N>

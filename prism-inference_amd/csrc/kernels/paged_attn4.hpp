@@ -1,28 +1,185 @@
 /*
  * paged_attn4.hpp - attention of one new token per sequence over a paged cache
  * of 4 bits: paged_attn.hpp's formula, work and join; keys and values become 16-bit
- * numbers, exactly, on their way into the products.
+ * numbers, exactly, on their way into the products (a conversion instruction makes two,
+ * and takes the block's power of two along).
+ *
+ *   paged4_few   one or two heads a key head, 16 or 32 channels: a lane holds 8 or 16 channels of a key;
+ *   paged4_many  S^T = K Q^T and O^T += V^T P^T on 16x16x32 MFMAs with the heads as columns. A lane
+ *                takes a quarter of a key's row: the products only ask that queries' channels are in the
+ *                same order. V goes through a wave's own LDS, as 16-bit numbers, for transposed reads.
  */
 #pragma once
 #include "cache4.hpp"
 #include "paged_work.hpp"
 
+/* Where key i of those that the wave sees lies: its slot's number in [page][head][slot], -1 if there is none. */
+__device__ __forceinline__ int64_t paged4_slot(const PagedAttnArgs& a, const PagedWork& w, int i) {
+    if (i >= w.i1) return -1;
+    const int j = w.key(i), page = paged_page(a, w, j);
+    return page < 0 ? -1 : paged_at<1>(a, w, page, j);
+}
+
+template <class T, int HD, int G>
+__device__ __forceinline__ void paged4_few(const PagedAttnArgs& a) {
+    constexpr int CH = HD / 2 < 16 ? HD / 2 : 16; /* channels of a lane */
+    constexpr int W = CH / 8;                     /* words of codes     */
+    constexpr int LPK = HD / CH, KPS = 64 / LPK;  /* lanes a key, keys a step of the wave */
+    constexpr int U = 2;                          /* steps in flight    */
+    typedef typename T::v8 v8;
+    __shared__ float lacc[4 * G * HD], lm[4 * G], ll[4 * G];
+    const int lane = lane_id(), slot = lane / LPK, ch = lane % LPK * CH;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint8_t* kp = reinterpret_cast<const uint8_t*>(a.k_pages);
+    const uint8_t* vp = reinterpret_cast<const uint8_t*>(a.v_pages);
+    PagedWork w;
+    if (!paged_work(a, wave, w)) return; /* only where waves work alone */
+
+    v8 q[G][W];
+    float acc[G][CH] = {}, m[G], l[G];
+#pragma unroll
+    for (int h = 0; h < G; ++h) {
+#pragma unroll
+        for (int x = 0; x < W; ++x) q[h][x] = ld8<T>(a.q + w.seq * a.q_seq_stride + (w.head + h) * a.q_head_stride + ch + 8 * x);
+        m[h] = -INFINITY;
+        l[h] = 0.f;
+    }
+    const auto steps = [&](auto count, int i) {
+        constexpr int U = decltype(count)::value;
+        int64_t at[U];
+        uint32_t k[U][W], v[U][W];
+        float ks[U], vs[U];
+        bool ok[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) at[u] = paged4_slot(a, w, i + u * KPS + slot);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            ok[u] = at[u] >= 0;
+            const int64_t x = ok[u] ? at[u] : 0;
+            __builtin_memcpy(k[u], kp + x * (HD / 2) + ch / 2, 4 * W);
+            __builtin_memcpy(v[u], vp + x * (HD / 2) + ch / 2, 4 * W);
+            ks[u] = fp4_scale(a.k_scales[x]);
+            vs[u] = fp4_scale(a.v_scales[x]);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            vs[u] = ok[u] ? vs[u] : 0.f; /* 0 and any number is 0 */
+        }
+        v8 kk[U][W];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int x = 0; x < W; ++x) kk[u][x] = fp4_values<T>(k[u][x], ks[u]);
+        float s[G][U];
+#pragma unroll
+        for (int h = 0; h < G; ++h) {
+            float top = m[h];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                float d = 0.f;
+#pragma unroll
+                for (int x = 0; x < W; ++x) d = dot8(q[h][x], kk[u][x], d);
+                if constexpr (LPK == 2) d = lanes_sum<2>(d);
+                s[h][u] = ok[u] ? d * a.scale_log2 : -INFINITY;
+                top = fmaxf(top, s[h][u]);
+            }
+            const float mu = top == -INFINITY ? 0.f : top;
+            const float f = fast_exp2(m[h] - mu);
+            l[h] *= f;
+#pragma unroll
+            for (int e = 0; e < CH; ++e) acc[h][e] *= f;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                s[h][u] = fast_exp2(s[h][u] - mu);
+                l[h] += s[h][u];
+            }
+            m[h] = top;
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int x = 0; x < W; ++x) {
+                const uint32_t word = ok[u] ? v[u][x] : 0;
+                const auto two = [&](auto byte) {
+                    constexpr int B = decltype(byte)::value;
+                    const f2 y = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(word, ok[u] ? vs[u] : 1.f, B);
+#pragma unroll
+                    for (int h = 0; h < G; ++h) {
+                        acc[h][8 * x + 2 * B] = __builtin_fmaf(y[0], s[h][u], acc[h][8 * x + 2 * B]);
+                        acc[h][8 * x + 2 * B + 1] = __builtin_fmaf(y[1], s[h][u], acc[h][8 * x + 2 * B + 1]);
+                    }
+                };
+                two(Count<0>{});
+                two(Count<1>{});
+                two(Count<2>{});
+                two(Count<3>{});
+            }
+    };
+    for (int i = w.i0; i < w.i1; i += KPS * U)
+        if (w.i1 - i > KPS) steps(Count<U>{}, i);
+        else steps(Count<1>{}, i);
+    /* the wave's key slots together */
+    const auto add = [](float x, float y) { return x + y; };
+    const auto most = [](float x, float y) { return fmaxf(x, y); };
+#pragma unroll
+    for (int h = 0; h < G; ++h) {
+        const float top = across<LPK>(m[h], most);
+        const float f = m[h] == -INFINITY ? 0.f : fast_exp2(m[h] - top);
+        l[h] = across<LPK>(l[h] * f, add);
+#pragma unroll
+        for (int e = 0; e < CH; ++e) acc[h][e] = across<LPK>(acc[h][e] * f, add);
+        m[h] = top;
+    }
+    if (a.waves == 1) {
+        if (slot == 0) {
+#pragma unroll
+            for (int h = 0; h < G; ++h) {
+                const float inv = l[h] == 0.f ? 0.f : 1.0f / l[h];
+#pragma unroll
+                for (int x = 0; x < W; ++x) {
+                    v8 r;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) r[e] = (typename T::el)opaque(acc[h][8 * x + e] * inv);
+                    st8<T>(a.out + w.seq * a.out_seq_stride + (w.head + h) * a.out_head_stride + ch + 8 * x, r);
+                }
+            }
+        }
+        return;
+    }
+    if (slot == 0) {
+#pragma unroll
+        for (int h = 0; h < G; ++h) {
+#pragma unroll
+            for (int e = 0; e < CH; ++e) lacc[(wave * G + h) * HD + ch + e] = acc[h][e];
+            if (lane == 0) {
+                lm[wave * G + h] = m[h];
+                ll[wave * G + h] = l[h];
+            }
+        }
+    }
+    __syncthreads();
+    paged_join_waves<T, HD>(a, w, G, lacc, lm, ll, G);
+}
+
 template <class T, int HD>
 __device__ __forceinline__ void paged4_many(const PagedAttnArgs& a) {
     typedef typename T::v8 v8;
-    constexpr int KS = (HD + 31) / 32;             /* k-steps of the scores (16 channels: half a step, zeros) */
-    constexpr int BL = KS;                         /* blocks of a row */
-    constexpr int DT = HD / 16;                    /* 16-channel tiles of the output */
-    constexpr int VROW = HD + (HD >= 32 ? 16 : 0); /* LDS row (values) */
-    constexpr int CPR = HD / 8, RPI = 64 / CPR, NV = 32 / RPI; /* V: chunks a row, rows a load, loads for 32 keys */
-    constexpr int VBYTES = 4 * 32 * VROW * 2, ABYTES = 4 * PAGED_TILE_HEADS * HD * 4;
+    constexpr int KT = HD >= 128 ? 2 : 4, KEYS = 16 * KT; /* tiles of 16 keys a step */
+    constexpr int KS = (HD + 31) / 32;                    /* k-steps of the scores (16 channels: half a step, zeros) */
+    constexpr int QUARTER = HD >= 32 ? HD / 4 : 8;        /* channels of a lane (16: two lanes have them all) */
+    constexpr int BL = KS;                                /* blocks of a row */
+    constexpr int DT = HD / 16;                           /* 16-channel tiles of the output */
+    constexpr int VROW = HD + (HD >= 32 ? 16 : 0);        /* LDS row (values): 8 rows of 32 bytes without conflicts */
+    constexpr int VBYTES = 4 * KEYS * VROW * 2, ABYTES = 4 * PAGED_TILE_HEADS * HD * 4;
     __shared__ __attribute__((aligned(16))) uint8_t lds[VBYTES > ABYTES ? VBYTES : ABYTES];
     __shared__ float lm[4 * PAGED_TILE_HEADS], ll[4 * PAGED_TILE_HEADS];
-    const int lane = lane_id(), l16 = lane & 15, g = lane >> 4;
+    const int lane = lane_id(), l16 = lane & 15, g = lane >> 4, part = HD >= 32 ? g : g & 1;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    uint16_t* lv = reinterpret_cast<uint16_t*>(lds) + wave * 32 * VROW; /* this wave's 32 rows */
-    const uint8_t* kp = reinterpret_cast<const uint8_t*>(a.k_pages);
-    const uint8_t* vp = reinterpret_cast<const uint8_t*>(a.v_pages);
+    uint16_t* lv = reinterpret_cast<uint16_t*>(lds) + wave * KEYS * VROW; /* this wave's rows */
+    const uint8_t* kp = reinterpret_cast<const uint8_t*>(a.k_pages) + part * (QUARTER / 2);
+    const uint8_t* vp = reinterpret_cast<const uint8_t*>(a.v_pages) + part * (QUARTER / 2);
+    const uint8_t* kx = a.k_scales + part * QUARTER / 32;
+    const uint8_t* vx = a.v_scales + part * QUARTER / 32;
     PagedWork w;
     if (!paged_work(a, wave, w)) return; /* only where waves work alone */
 
@@ -30,9 +187,8 @@ __device__ __forceinline__ void paged4_many(const PagedAttnArgs& a) {
     const uint16_t* qp = a.q + w.seq * a.q_seq_stride + (w.head + min(l16, w.heads - 1)) * a.q_head_stride;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
-        const bool in = HD >= 32 || g < 2;
-        const v8 x = ld8<T>(qp + (in ? 32 * ks + 8 * g : 0));
-        q[ks] = in ? x : v8{};
+        const v8 x = ld8<T>(qp + part * QUARTER + 8 * ks);
+        q[ks] = HD >= 32 || g < 2 ? x : v8{};
     }
     /* weights as the sum of two 16-bit numbers, as in paged_attn.hpp */
     constexpr bool HALF = __is_same(T, F16);
@@ -40,45 +196,59 @@ __device__ __forceinline__ void paged4_many(const PagedAttnArgs& a) {
     f4 o[DT] = {};
     float m = -INFINITY, mu = 0.f, l = 0.f;
 
-    const auto page_of = [&](int i) { /* lane's key of the 32 from i on */
-        const int x = i + (lane & 31);
-        return x < w.i1 ? paged_page(a, w, w.key(x)) : -1;
-    };
-    int page = w.i0 < w.i1 ? page_of(w.i0) : -1;
-    for (int i = w.i0; i < w.i1; i += 32) {
-        const unsigned seen = (unsigned)__ballot(page >= 0);
-        v8 k[2][KS], v[NV];
+    int64_t slot = paged4_slot(a, w, w.i0 + (lane & (KEYS - 1))); /* a lane's key of the step */
+    for (int i = w.i0; i < w.i1; i += KEYS) {
+        const uint64_t seen = __ballot(slot >= 0);
+        /* every lane's own keys, l16 of each tile */
+        int64_t at[KT];
+        {
+            const int64_t x = slot < 0 ? 0 : slot;
+            int lo[2], hi[2];
+            lanes_x16((int)x, lo[0], lo[1]);
+            lanes_x16((int)(x >> 32), hi[0], hi[1]);
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            const int r = 16 * t + l16, p = __shfl(page, r);
-            const int64_t at = p >= 0 ? paged_at<1>(a, w, p, w.key(i + r)) : 0;
+            for (int t = 0; t < 2; ++t) {
+                if constexpr (KT == 2) {
+                    at[t] = (int64_t)hi[t] << 32 | (uint32_t)lo[t];
+                } else {
+                    int l0, l1, h0, h1;
+                    lanes_x32(lo[t], l0, l1);
+                    lanes_x32(hi[t], h0, h1);
+                    at[t] = (int64_t)h0 << 32 | (uint32_t)l0;
+                    at[t + 2] = (int64_t)h1 << 32 | (uint32_t)l1;
+                }
+            }
+        }
+        uint32_t k[KT][KS], v[KT][KS];
+        uint8_t ksc[KT], vsc[KT];
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks)
-                k[t][ks] = fp4_values<T>(*reinterpret_cast<const uint32_t*>(kp + at * (HD / 2) + (HD >= 32 ? 16 * ks + 4 * g : 4 * (g & 1))),
-                                         fp4_scale(a.k_scales[at * BL + ks]));
+        for (int t = 0; t < KT; ++t) {
+            __builtin_memcpy(k[t], __builtin_assume_aligned(kp + at[t] * (HD / 2), QUARTER / 2), QUARTER / 2);
+            ksc[t] = kx[at[t] * BL];
         }
 #pragma unroll
-        for (int n = 0; n < NV; ++n) {
-            const int r = n * RPI + lane / CPR, p = __shfl(page, r), c = lane % CPR;
-            const int64_t at = p >= 0 ? paged_at<1>(a, w, p, w.key(i + r)) : 0;
-            v[n] = fp4_values<T>(*reinterpret_cast<const uint32_t*>(vp + at * (HD / 2) + 4 * c), fp4_scale(a.v_scales[at * BL + c / 4]));
+        for (int t = 0; t < KT; ++t) {
+            __builtin_memcpy(v[t], __builtin_assume_aligned(vp + at[t] * (HD / 2), QUARTER / 2), QUARTER / 2);
+            vsc[t] = vx[at[t] * BL];
         }
-        const int next = i + 32 < w.i1 ? page_of(i + 32) : -1;
+        slot = paged4_slot(a, w, i + KEYS + (lane & (KEYS - 1)));
 
-        f4 s[2] = {};
+        f4 s[KT] = {};
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                if (HD < 32 && g >= 2) k[t][ks] = v8{}; /* channels 16.. do not exist */
-                s[t] = mfma_16x16x32(k[t][ks], q[ks], s[t]);
+            for (int t = 0; t < KT; ++t) {
+                v8 x = fp4_values<T>(k[t][ks], fp4_scale(ksc[t]));
+                if (HD < 32 && g >= 2) x = v8{}; /* channels 16.. do not exist */
+                s[t] = mfma_16x16x32(x, q[ks], s[t]);
             }
+        const bool all = seen == (KT == 2 ? 0xFFFFFFFFFFFFFFFFull : ~0ull);
         float top = m;
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < KT; ++t)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                s[t][e] = seen >> (16 * t + 4 * g + e) & 1 ? s[t][e] : -INFINITY;
+                if (!all) s[t][e] = seen >> (16 * t + 4 * g + e) & 1 ? s[t][e] : -INFINITY;
                 top = fmaxf(top, s[t][e]);
             }
         float x, y;
@@ -93,9 +263,9 @@ __device__ __forceinline__ void paged4_many(const PagedAttnArgs& a) {
             m = top;
             mu = top == -INFINITY ? 0.f : top;
         }
-        v8 p, rest;
+        v8 p[KT / 2], rest[KT / 2];
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < KT; ++t)
 #pragma unroll
             for (int e = 0; e < 4; e += 2) {
                 const float z0 = fast_exp2(__builtin_fmaf(s[t][e] - mu, a.scale_log2, UP));
@@ -104,33 +274,40 @@ __device__ __forceinline__ void paged4_many(const PagedAttnArgs& a) {
                 l += z1;
                 typename T::v2 hi, lo;
                 two_numbers(z0, z1, LEAST, hi, lo);
-                p[4 * t + e] = hi[0];
-                p[4 * t + e + 1] = hi[1];
-                rest[4 * t + e] = lo[0];
-                rest[4 * t + e + 1] = lo[1];
+                p[t / 2][4 * (t & 1) + e] = hi[0];
+                p[t / 2][4 * (t & 1) + e + 1] = hi[1];
+                rest[t / 2][4 * (t & 1) + e] = lo[0];
+                rest[t / 2][4 * (t & 1) + e + 1] = lo[1];
             }
+        /* V into the wave's rows and back transposed. The LDS works a wave's accesses off in order; the
+           fences keep the compiler from changing it. */
 #pragma unroll
-        for (int n = 0; n < NV; ++n) {
-            const int r = n * RPI + lane / CPR;
-            st8<T>(lv + r * VROW + lane % CPR * 8, seen >> r & 1 ? v[n] : v8{});
+        for (int t = 0; t < KT; ++t) {
+            const bool ok = seen >> (16 * t + l16) & 1;
+            const float scale = ok ? fp4_scale(vsc[t]) : 1.f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+                if (HD >= 32 || g < 2)
+                    st8<T>(lv + (16 * t + l16) * VROW + part * QUARTER + 8 * ks, fp4_values<T>(ok ? v[t][ks] : 0, scale));
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
-        for (int d = 0; d < DT; ++d) {
-            const uint16_t* at = lv + (4 * g + l16 / 4) * VROW + 16 * d + 4 * (l16 & 3);
-            union {
-                s4 h[2];
-                v8 v;
-            } vf;
-            vf.h[0] = lds_tr4(at);
-            vf.h[1] = lds_tr4(at + 16 * VROW);
-            o[d] = mfma_16x16x32(vf.v, p, o[d]);
-            o[d] = mfma_16x16x32(vf.v, rest, o[d]);
-        }
+        for (int n = 0; n < KT / 2; ++n)
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                const uint16_t* from = lv + (32 * n + 4 * g + l16 / 4) * VROW + 16 * d + 4 * (l16 & 3);
+                union {
+                    s4 h[2];
+                    v8 v;
+                } vf;
+                vf.h[0] = lds_tr4(from);
+                vf.h[1] = lds_tr4(from + 16 * VROW);
+                o[d] = mfma_16x16x32(vf.v, p[n], o[d]);
+                o[d] = mfma_16x16x32(vf.v, rest[n], o[d]);
+            }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
-        page = next;
     }
     l = sum_groups(l);
     if (a.waves == 1) {
@@ -165,3 +342,8 @@ __device__ __forceinline__ void paged4_many(const PagedAttnArgs& a) {
 PAGED4(f16, F16, 16) PAGED4(f16, F16, 32) PAGED4(f16, F16, 64) PAGED4(f16, F16, 128)
 PAGED4(bf16, BF16, 16) PAGED4(bf16, BF16, 32) PAGED4(bf16, BF16, 64) PAGED4(bf16, BF16, 128)
 #undef PAGED4
+#define PAGED4_FEW(NAME, T, HD) \
+    extern "C" __global__ void __launch_bounds__(256) prism_paged_attn4_##NAME##_h##HD##_g1(PagedAttnArgs a) { paged4_few<T, HD, 1>(a); } \
+    extern "C" __global__ void __launch_bounds__(256) prism_paged_attn4_##NAME##_h##HD##_g2(PagedAttnArgs a) { paged4_few<T, HD, 2>(a); }
+PAGED4_FEW(f16, F16, 16) PAGED4_FEW(f16, F16, 32) PAGED4_FEW(bf16, BF16, 16) PAGED4_FEW(bf16, BF16, 32)
+#undef PAGED4_FEW
