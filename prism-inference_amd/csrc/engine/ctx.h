@@ -101,6 +101,7 @@ struct prism_ctx {
     hipFunction_t f_rope_append[2][2] = {}; /* [dtype][16, 4 bits] */
     hipFunction_t f_cache_read[2][2] = {};  /* [dtype][16, 4 bits] */
     hipFunction_t f_paged4[2][4][3] = {};   /* [dtype][head_dim][1, 2 heads a key head and 32 channels at most; others] */
+    hipFunction_t f_paged4_join[2][4] = {};
     hipFunction_t f_linear[2][4] = {};
     hipFunction_t f_linear_states[2][4] = {};
     hipFunction_t f_linear_step[2][4] = {};

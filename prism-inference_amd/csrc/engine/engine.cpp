@@ -140,6 +140,7 @@ extern "C" int prism_create(prism_ctx** out, int32_t device, const char* code_ob
             all.emplace_back(&c->f_paged_join[t][i], "prism_paged_attn_join_" + shape);
             for (int g = i < 2 ? 0 : 2; g < 3; ++g)
                 all.emplace_back(&c->f_paged4[t][i][g], "prism_paged_attn4_" + shape + (g == 0 ? "_g1" : g == 1 ? "_g2" : "_many"));
+            all.emplace_back(&c->f_paged4_join[t][i], "prism_paged_attn4_join_" + shape);
             all.emplace_back(&c->f_linear[t][i], "prism_linear_attn_" + shape);
             all.emplace_back(&c->f_linear_states[t][i], "prism_linear_states_" + shape);
             all.emplace_back(&c->f_linear_step[t][i], "prism_linear_step_" + shape);

@@ -301,6 +301,36 @@ inline PagedPlan paged_plan(const prism_paged_attn_push& p) {
     r.grid = r.waves == 1 ? (items + 3) / 4 : items * r.splits;
     return r;
 }
+/* keys that the longest sequence expected sees */
+inline int64_t paged_keys(const prism_paged_attn_push& p) {
+    const int64_t keys = p.max_len > 0 ? p.max_len : (int64_t)p.cache.table_pages * p.cache.page_size;
+    return p.left >= 0 ? std::min(keys, (int64_t)p.left + 1 + p.sinks) : keys;
+}
+/* The same over a cache of 4 bits. The products' kernel is for more heads, and for all from 64 channels on: a lane's own channels are
+ * many there. Splits are as long as those of the longest sequence expected (paged_attn4.hpp), so that of unlike lengths about half
+ * have keys: 1,800 workgroups then are as many as the GPU holds at once, and one round of them is fastest. An odd number, so that
+ * those that many sequences lack do not fall on the same XCD. us at 1, 5, 8, 9, 15, 16, 25, 63, 95, 191 splits: 24 sequences of 1,000 to
+ * 20,001, 32/8 x 128: 249, 103, 101, 73, 81, 103, 83, 117, 138, 223; one of 131,075: 1,398, 291, 188, 167, 109, 101, 70, 46, 43, 47; one of
+ * 16,000, 8/1 x 128: 152, 40, 29, 27, 22, 19, 17, 13, 14, 16; 64 of 500 to 4,000, 8 x 128: 59, 53, 64, 55, 68, 76, 82 and more. */
+inline PagedPlan paged4_plan(const prism_paged_attn_push& p) {
+    PagedPlan r = paged_plan(p);
+    r.many = p.n_heads / p.cache.n_kv_heads > 2 || p.cache.head_dim > 32;
+    const int64_t items = std::max<int64_t>((int64_t)p.cache.n_seqs * p.cache.n_kv_heads * r.head_tiles, 1), keys = paged_keys(p);
+    /* waves by themselves: 1,600 items of 300 keys x 64 16.3 us, four a workgroup 19.7; 520 of 1,000 and more 4,000 x 128 60 and 200 */
+    r.waves = keys <= 64 || items >= 4096 || (items >= 1024 && keys <= 400) ? 1 : 4;
+    r.splits = 1;
+    if (r.waves == 4 && keys >= 384 && keys * p.cache.head_dim >= 32 * 1024) {
+        const int64_t most = std::min<int64_t>(std::min(1800 / items, keys / 320), PAGED4_MAX_SPLITS);
+        r.splits = (int)std::max<int64_t>(1, (most - 1) | 1);
+    }
+    r.grid = r.waves == 1 ? (items + 3) / 4 : items * r.splits;
+    return r;
+}
+/* Keys of a wave, of four in each split, so that they do for the longest sequence expected. */
+inline int32_t paged4_each(const prism_paged_attn_push& p, const PagedPlan& r) {
+    const int64_t each = (paged_keys(p) - 1) / (4 * r.splits) + 64;
+    return (int32_t)std::min<int64_t>(each & ~int64_t(63), int64_t(1) << 30);
+}
 inline int64_t paged_workspace(const prism_paged_attn_push& p, const PagedPlan& r) {
     return r.splits == 1 ? 0 : (int64_t)p.cache.n_seqs * p.n_heads * r.splits * (p.cache.head_dim + 2) * 4;
 }

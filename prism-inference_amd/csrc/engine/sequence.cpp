@@ -134,12 +134,12 @@ extern "C" int prism_cache_append(prism_ctx* c, const prism_append_push* p, cons
 
 namespace {
 
-int64_t paged_workspace_of(const prism_paged_attn_push* p) {
+int64_t paged_workspace_of(const prism_paged_attn_push* p, bool four) {
     if (!p) return fail(nullptr, PRISM_ERR_INVALID, "paged attention: push is NULL");
     const char* why = "";
     const int rc = check_paged(*p, &why);
     if (rc) return fail(nullptr, rc, "paged attention: %s", why);
-    return paged_workspace(*p, paged_plan(*p));
+    return paged_workspace(*p, four ? paged4_plan(*p) : paged_plan(*p));
 }
 
 /* k_scales, v_scales: of a 4-bit cache */
@@ -155,7 +155,7 @@ int paged(prism_ctx* c, const prism_paged_attn_push* p, bool four, const void* q
     if (!aligned16(q) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(k_scales) || !aligned16(v_scales) ||
         !aligned16(out))
         return fail(c, PRISM_ERR_INVALID, "paged attention: buffers must be 16-byte aligned");
-    const PagedPlan plan = paged_plan(*p);
+    const PagedPlan plan = four ? paged4_plan(*p) : paged_plan(*p);
     const int64_t need = paged_workspace(*p, plan);
     if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
         return fail(c, PRISM_ERR_INVALID, "paged attention: workspace of %lld bytes, %lld needed, 16-byte aligned",
@@ -187,16 +187,17 @@ int paged(prism_ctx* c, const prism_paged_attn_push* p, bool four, const void* q
     a.waves = plan.waves;
     a.splits = plan.splits;
     a.ws = static_cast<float*>(workspace);
+    a.each = four ? paged4_each(*p, plan) : 0;
     const int i = hd_index(d.head_dim), kind = plan.many ? 2 : p->n_heads / d.n_kv_heads - 1;
-    const hipFunction_t f = four ? c->f_paged4[d.dtype][i][d.head_dim > 32 ? 2 : kind] : c->f_paged[d.dtype][i][kind];
+    const hipFunction_t f = four ? c->f_paged4[d.dtype][i][kind] : c->f_paged[d.dtype][i][kind];
     const int rc = launch(c, f, "paged attention", plan.grid, 256, &a, stream);
     if (rc || plan.splits == 1) return rc;
-    return launch(c, c->f_paged_join[d.dtype][i], "paged attention's join", (int64_t)d.n_seqs * p->n_heads, 256, &a, stream);
+    return launch(c, four ? c->f_paged4_join[d.dtype][i] : c->f_paged_join[d.dtype][i], "paged attention's join", (int64_t)d.n_seqs * p->n_heads, 256, &a, stream);
 }
 
 }  // namespace
 
-extern "C" int64_t prism_paged_attn_workspace(const prism_paged_attn_push* p) { return paged_workspace_of(p); }
+extern "C" int64_t prism_paged_attn_workspace(const prism_paged_attn_push* p) { return paged_workspace_of(p, false); }
 
 extern "C" int prism_paged_attn(prism_ctx* c, const prism_paged_attn_push* p, const void* q, const void* k_pages,
                                 const void* v_pages, const int32_t* table, const int32_t* lengths, void* out,
@@ -204,7 +205,7 @@ extern "C" int prism_paged_attn(prism_ctx* c, const prism_paged_attn_push* p, co
     return paged(c, p, false, q, k_pages, v_pages, nullptr, nullptr, table, lengths, out, workspace, workspace_bytes, stream);
 }
 
-extern "C" int64_t prism_paged_attn4_workspace(const prism_paged_attn_push* p) { return paged_workspace_of(p); }
+extern "C" int64_t prism_paged_attn4_workspace(const prism_paged_attn_push* p) { return paged_workspace_of(p, true); }
 
 extern "C" int prism_paged_attn4(prism_ctx* c, const prism_paged_attn_push* p, const void* q, const prism_cache_pages* g,
                                  const int32_t* table, const int32_t* lengths, void* out, void* workspace,

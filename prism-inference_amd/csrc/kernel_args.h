@@ -195,6 +195,7 @@ typedef struct AppendArgs {
 
 #define PAGED_TILE_HEADS 16 /* heads of a group that a wave takes together */
 #define PAGED_MAX_SPLITS 64
+#define PAGED4_MAX_SPLITS 95
 typedef struct PagedAttnArgs {
     const uint16_t* q;
     const uint16_t* k_pages;
@@ -213,6 +214,7 @@ typedef struct PagedAttnArgs {
     float* ws;              /* splits > 1: [n_seqs][n_heads][splits][head_dim + 2] */
     const uint8_t* k_scales; /* 4-bit pages: the pools above are theirs too    */
     const uint8_t* v_scales;
+    int32_t each;           /* 4-bit pages, waves = 4: a wave's keys of the longest sequence expected */
 } PagedAttnArgs;
 
 #define SEQ_ROWS 128 /* queries x heads per workgroup of a sequence attention, */

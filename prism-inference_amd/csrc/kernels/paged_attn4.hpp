@@ -13,6 +13,39 @@
 #include "cache4.hpp"
 #include "paged_work.hpp"
 
+/* What a wave has to do, as paged_work, but with the splits of a length as long as those of the longest expected: workgroups are
+ * alike, short sequences have fewer, and those without keys leave at once. */
+__device__ __forceinline__ bool paged4_work(const PagedAttnArgs& a, int wave, PagedWork& w) {
+    const int group = a.n_heads / a.n_kv_heads;
+    const unsigned items = (unsigned)a.n_seqs * a.n_kv_heads * a.head_tiles; /* 32 bits: a launch has fewer than 2^24 workgroups */
+    unsigned item = blockIdx.x;
+    int part = 0;
+    w.split = 0;
+    if (a.waves == 1) {
+        item = item * 4 + wave;
+    } else {
+        w.split = (int)(item % (unsigned)a.splits);
+        item /= (unsigned)a.splits;
+        part = w.split * 4 + wave;
+    }
+    if (item >= items) return false;
+    const unsigned tiles = a.head_tiles, kv = a.n_kv_heads, both = item / tiles;
+    const int ht = (int)(item - both * tiles);
+    w.seq = (int)(both / kv);
+    w.hk = (int)(both - w.seq * kv);
+    w.head = w.hk * group + ht * PAGED_TILE_HEADS;
+    w.heads = min(group - ht * PAGED_TILE_HEADS, PAGED_TILE_HEADS);
+    const int n = seq_clamp(a.lengths[w.seq], 0, a.table_pages << a.page_log2);
+    w.kr = key_range(n - 1, n, a.left, 0, a.sinks);
+    const int seen = w.kr.sink + w.kr.hi - w.kr.lo, parts = a.waves * a.splits;
+    const int even = ((seen - 1) / parts + 16) & ~15; /* seen = 0: none */
+    const int each = max(even, a.each);
+    const int64_t at = (int64_t)part * each;
+    w.i0 = at < seen ? (int)at : seen;
+    w.i1 = seq_min(seen - w.i0, each) + w.i0;
+    return true;
+}
+
 /* Where key i of those that the wave sees lies: its slot's number in [page][head][slot], -1 if there is none. */
 __device__ __forceinline__ int64_t paged4_slot(const PagedAttnArgs& a, const PagedWork& w, int i) {
     if (i >= w.i1) return -1;
@@ -33,7 +66,7 @@ __device__ __forceinline__ void paged4_few(const PagedAttnArgs& a) {
     const uint8_t* kp = reinterpret_cast<const uint8_t*>(a.k_pages);
     const uint8_t* vp = reinterpret_cast<const uint8_t*>(a.v_pages);
     PagedWork w;
-    if (!paged_work(a, wave, w)) return; /* only where waves work alone */
+    if (!paged4_work(a, wave, w)) return; /* only where waves work alone */
 
     v8 q[G][W];
     float acc[G][CH] = {}, m[G], l[G];
@@ -60,10 +93,6 @@ __device__ __forceinline__ void paged4_few(const PagedAttnArgs& a) {
             __builtin_memcpy(v[u], vp + x * (HD / 2) + ch / 2, 4 * W);
             ks[u] = fp4_scale(a.k_scales[x]);
             vs[u] = fp4_scale(a.v_scales[x]);
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            vs[u] = ok[u] ? vs[u] : 0.f; /* 0 and any number is 0 */
         }
         v8 kk[U][W];
 #pragma unroll
@@ -99,7 +128,7 @@ __device__ __forceinline__ void paged4_few(const PagedAttnArgs& a) {
         for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int x = 0; x < W; ++x) {
-                const uint32_t word = ok[u] ? v[u][x] : 0;
+                const uint32_t word = ok[u] ? v[u][x] : 0; /* zeros, not what may be NaN */
                 const auto two = [&](auto byte) {
                     constexpr int B = decltype(byte)::value;
                     const f2 y = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(word, ok[u] ? vs[u] : 1.f, B);
@@ -118,43 +147,62 @@ __device__ __forceinline__ void paged4_few(const PagedAttnArgs& a) {
     for (int i = w.i0; i < w.i1; i += KPS * U)
         if (w.i1 - i > KPS) steps(Count<U>{}, i);
         else steps(Count<1>{}, i);
-    /* the wave's key slots together */
+    /* The wave's 32 key slots together, halving what a lane holds: each step pairs lanes that differ in one bit, and one
+       takes the sum of one half of the channels, the other of the other. In the end lane bits 5, 4, 3 (and 2) name a
+       channel, bit 0 the lane's half of the row. */
+    static_assert(LPK == 2, "lane bit 0: channels; 1 to 5: keys");
     const auto add = [](float x, float y) { return x + y; };
     const auto most = [](float x, float y) { return fmaxf(x, y); };
+    const bool b3 = lane & 8, b2 = lane & 4;
+    const int mine = (lane >> 5 & 1) * (CH / 2) + (lane >> 4 & 1) * (CH / 4) + (lane >> 3 & 1) * (CH / 8) + (CH == 16 ? lane >> 2 & 1 : 0);
 #pragma unroll
     for (int h = 0; h < G; ++h) {
         const float top = across<LPK>(m[h], most);
         const float f = m[h] == -INFINITY ? 0.f : fast_exp2(m[h] - top);
         l[h] = across<LPK>(l[h] * f, add);
-#pragma unroll
-        for (int e = 0; e < CH; ++e) acc[h][e] = across<LPK>(acc[h][e] * f, add);
         m[h] = top;
+        float (&x)[CH] = acc[h];
+#pragma unroll
+        for (int e = 0; e < CH; ++e) x[e] *= f;
+#pragma unroll
+        for (int e = 0; e < CH / 2; ++e) {
+            const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, x[e]), __builtin_bit_cast(unsigned, x[e + CH / 2]), false, false);
+            x[e] = __builtin_bit_cast(float, (unsigned)r[0]) + __builtin_bit_cast(float, (unsigned)r[1]);
+        }
+#pragma unroll
+        for (int e = 0; e < CH / 4; ++e) {
+            const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, x[e]), __builtin_bit_cast(unsigned, x[e + CH / 4]), false, false);
+            x[e] = __builtin_bit_cast(float, (unsigned)r[0]) + __builtin_bit_cast(float, (unsigned)r[1]);
+        }
+#pragma unroll
+        for (int e = 0; e < CH / 8; ++e) { /* row_ror 8 */
+            const float keep = b3 ? x[e + CH / 8] : x[e], give = b3 ? x[e] : x[e + CH / 8];
+            x[e] = keep + dpp<0x128>(give);
+        }
+        if constexpr (CH == 16) { /* quads mirrored in eights: lane ^ 7, and back within quads below */
+            const float keep = b2 ? x[1] : x[0], give = b2 ? x[0] : x[1];
+            const float there = dpp<0x1B>(give); /* quad_perm [3,2,1,0] */
+            x[0] = keep + dpp<0x141>(there);     /* row_half_mirror: lane ^ 7; together lane ^ 4 */
+        } else {
+            x[0] += dpp<0x141>(dpp<0x1B>(x[0]));
+        }
+        x[0] += dpp<0x4E>(x[0]); /* lane ^ 2 */
     }
+    const int c = ch + mine;
     if (a.waves == 1) {
-        if (slot == 0) {
+        if ((lane & (CH == 16 ? 2 : 6)) == 0) {
 #pragma unroll
-            for (int h = 0; h < G; ++h) {
-                const float inv = l[h] == 0.f ? 0.f : 1.0f / l[h];
-#pragma unroll
-                for (int x = 0; x < W; ++x) {
-                    v8 r;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) r[e] = (typename T::el)opaque(acc[h][8 * x + e] * inv);
-                    st8<T>(a.out + w.seq * a.out_seq_stride + (w.head + h) * a.out_head_stride + ch + 8 * x, r);
-                }
-            }
+            for (int h = 0; h < G; ++h)
+                st1<T>(a.out + w.seq * a.out_seq_stride + (w.head + h) * a.out_head_stride + c, acc[h][0] * (l[h] == 0.f ? 0.f : 1.0f / l[h]));
         }
         return;
     }
-    if (slot == 0) {
 #pragma unroll
-        for (int h = 0; h < G; ++h) {
-#pragma unroll
-            for (int e = 0; e < CH; ++e) lacc[(wave * G + h) * HD + ch + e] = acc[h][e];
-            if (lane == 0) {
-                lm[wave * G + h] = m[h];
-                ll[wave * G + h] = l[h];
-            }
+    for (int h = 0; h < G; ++h) {
+        if ((lane & (CH == 16 ? 2 : 6)) == 0) lacc[(wave * G + h) * HD + c] = acc[h][0];
+        if (lane == 0) {
+            lm[wave * G + h] = m[h];
+            ll[wave * G + h] = l[h];
         }
     }
     __syncthreads();
@@ -181,7 +229,7 @@ __device__ __forceinline__ void paged4_many(const PagedAttnArgs& a) {
     const uint8_t* kx = a.k_scales + part * QUARTER / 32;
     const uint8_t* vx = a.v_scales + part * QUARTER / 32;
     PagedWork w;
-    if (!paged_work(a, wave, w)) return; /* only where waves work alone */
+    if (!paged4_work(a, wave, w)) return; /* only where waves work alone */
 
     v8 q[KS];
     const uint16_t* qp = a.q + w.seq * a.q_seq_stride + (w.head + min(l16, w.heads - 1)) * a.q_head_stride;
@@ -242,7 +290,7 @@ __device__ __forceinline__ void paged4_many(const PagedAttnArgs& a) {
                 if (HD < 32 && g >= 2) x = v8{}; /* channels 16.. do not exist */
                 s[t] = mfma_16x16x32(x, q[ks], s[t]);
             }
-        const bool all = seen == (KT == 2 ? 0xFFFFFFFFFFFFFFFFull : ~0ull);
+        const bool all = seen == ~0ull; /* two tiles: lanes 32.. have the same keys again */
         float top = m;
 #pragma unroll
         for (int t = 0; t < KT; ++t)
@@ -283,12 +331,18 @@ __device__ __forceinline__ void paged4_many(const PagedAttnArgs& a) {
            fences keep the compiler from changing it. */
 #pragma unroll
         for (int t = 0; t < KT; ++t) {
-            const bool ok = seen >> (16 * t + l16) & 1;
-            const float scale = ok ? fp4_scale(vsc[t]) : 1.f;
+            uint32_t word[KS];
+            float scale = fp4_scale(vsc[t]);
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) word[ks] = v[t][ks];
+            if (!all && !(seen >> (16 * t + l16) & 1)) { /* zeros, not what may be NaN */
+                scale = 1.f;
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) word[ks] = 0;
+            }
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks)
-                if (HD >= 32 || g < 2)
-                    st8<T>(lv + (16 * t + l16) * VROW + part * QUARTER + 8 * ks, fp4_values<T>(ok ? v[t][ks] : 0, scale));
+                if (HD >= 32 || g < 2) st8<T>(lv + (16 * t + l16) * VROW + part * QUARTER + 8 * ks, fp4_values<T>(word[ks], scale));
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
@@ -337,8 +391,45 @@ __device__ __forceinline__ void paged4_many(const PagedAttnArgs& a) {
     paged_join_waves<T, HD>(a, w, w.heads, acc, lm, ll, PAGED_TILE_HEADS);
 }
 
+/* The splits of one (sequence, head) together: their weights by the threads of the workgroup, then HD channels by
+ * 256 / HD groups of splits. */
+template <class T, int HD>
+__device__ __forceinline__ void paged4_join(const PagedAttnArgs& a) {
+    static_assert(PAGED4_MAX_SPLITS <= 256, "a thread per split");
+    __shared__ float weight[256], part[256], tops[4], sums[4];
+    const int tid = threadIdx.x, wave = tid >> 6;
+    const float* ws = a.ws + (int64_t)blockIdx.x * a.splits * (HD + 2);
+    const bool in = tid < a.splits;
+    const float m = in ? ws[tid * (HD + 2) + HD] : -INFINITY, l = in ? ws[tid * (HD + 2) + HD + 1] : 0.f;
+    float top = m;
+    for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
+    if (lane_id() == 0) tops[wave] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+    const float f = m == -INFINITY ? 0.f : fast_exp2(m - top);
+    weight[tid] = f;
+    const float mine = wave_sum(l * f);
+    if (lane_id() == 0) sums[wave] = mine;
+    __syncthreads();
+    const float sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+    const int c = tid % HD;
+    float o = 0.f;
+#pragma unroll 8 /* that many loads at once: the launch is as long as their latency */
+    for (int s = tid / HD; s < a.splits; s += 256 / HD) o = __builtin_fmaf(ws[s * (HD + 2) + c], weight[s], o);
+    part[tid] = o;
+    __syncthreads();
+    if (tid < HD) {
+        o = 0.f;
+#pragma unroll
+        for (int k = 0; k < 256 / HD; ++k) o += part[k * HD + tid];
+        const int seq = blockIdx.x / a.n_heads, head = blockIdx.x % a.n_heads;
+        st1<T>(a.out + seq * a.out_seq_stride + head * a.out_head_stride + tid, sum == 0.f ? 0.f : o / sum);
+    }
+}
+
 #define PAGED4(NAME, T, HD) \
-    extern "C" __global__ void __launch_bounds__(256, 3) prism_paged_attn4_##NAME##_h##HD##_many(PagedAttnArgs a) { paged4_many<T, HD>(a); }
+    extern "C" __global__ void __launch_bounds__(256, 3) prism_paged_attn4_##NAME##_h##HD##_many(PagedAttnArgs a) { paged4_many<T, HD>(a); } \
+    extern "C" __global__ void __launch_bounds__(256) prism_paged_attn4_join_##NAME##_h##HD(PagedAttnArgs a) { paged4_join<T, HD>(a); }
 PAGED4(f16, F16, 16) PAGED4(f16, F16, 32) PAGED4(f16, F16, 64) PAGED4(f16, F16, 128)
 PAGED4(bf16, BF16, 16) PAGED4(bf16, BF16, 32) PAGED4(bf16, BF16, 64) PAGED4(bf16, BF16, 128)
 #undef PAGED4

@@ -59,21 +59,23 @@ struct PagedWork {
 };
 __device__ __forceinline__ bool paged_work(const PagedAttnArgs& a, int wave, PagedWork& w) {
     const int group = a.n_heads / a.n_kv_heads;
-    const int64_t items = (int64_t)a.n_seqs * a.n_kv_heads * a.head_tiles;
-    int64_t item;
+    /* a launch has fewer than 2^24 workgroups of 256, so items fit 32 bits */
+    const unsigned items = (unsigned)a.n_seqs * a.n_kv_heads * a.head_tiles;
+    unsigned item;
     int part;
     if (a.waves == 1) {
-        item = (int64_t)blockIdx.x * 4 + wave;
+        item = blockIdx.x * 4 + wave;
         w.split = part = 0;
     } else {
-        item = blockIdx.x / a.splits;
-        w.split = blockIdx.x % a.splits;
+        item = blockIdx.x / (unsigned)a.splits;
+        w.split = blockIdx.x - item * a.splits;
         part = w.split * 4 + wave;
     }
     if (item >= items) return false;
-    const int ht = (int)(item % a.head_tiles);
-    w.hk = (int)(item / a.head_tiles % a.n_kv_heads);
-    w.seq = (int)(item / a.head_tiles / a.n_kv_heads);
+    const unsigned tiles = a.head_tiles, kv = a.n_kv_heads, both = item / tiles;
+    const int ht = (int)(item - both * tiles);
+    w.seq = (int)(both / kv);
+    w.hk = (int)(both - w.seq * kv);
     w.head = w.hk * group + ht * PAGED_TILE_HEADS;
     w.heads = min(group - ht * PAGED_TILE_HEADS, PAGED_TILE_HEADS);
     const int n = seq_clamp(a.lengths[w.seq], 0, a.table_pages << a.page_log2);
