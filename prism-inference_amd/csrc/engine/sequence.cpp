@@ -187,7 +187,14 @@ int paged(prism_ctx* c, const prism_paged_attn_push* p, bool four, const void* q
     a.waves = plan.waves;
     a.splits = plan.splits;
     a.ws = static_cast<float*>(workspace);
-    a.each = four ? paged4_each(*p, plan) : 0;
+    if (four) {
+        const auto inverse = [](int32_t d) { return (uint32_t)std::min<uint64_t>((uint64_t(1) << 32) / (uint32_t)d, UINT32_MAX); };
+        a.each = paged4_each(*p, plan);
+        a.group = p->n_heads / d.n_kv_heads;
+        a.by_splits = inverse(plan.splits);
+        a.by_tiles = inverse(plan.head_tiles);
+        a.by_kv = inverse(d.n_kv_heads);
+    }
     const int i = hd_index(d.head_dim), kind = plan.many ? 2 : p->n_heads / d.n_kv_heads - 1;
     const hipFunction_t f = four ? c->f_paged4[d.dtype][i][kind] : c->f_paged[d.dtype][i][kind];
     const int rc = launch(c, f, "paged attention", plan.grid, 256, &a, stream);

@@ -214,7 +214,10 @@ typedef struct PagedAttnArgs {
     float* ws;              /* splits > 1: [n_seqs][n_heads][splits][head_dim + 2] */
     const uint8_t* k_scales; /* 4-bit pages: the pools above are theirs too    */
     const uint8_t* v_scales;
-    int32_t each;           /* 4-bit pages, waves = 4: a wave's keys of the longest sequence expected */
+    /* 4-bit pages: */
+    int32_t each;           /* waves = 4: a wave's keys of the longest sequence expected */
+    int32_t group;          /* n_heads / n_kv_heads */
+    uint32_t by_splits, by_tiles, by_kv; /* floor(2^32 / splits, head_tiles, n_kv_heads), 2^32 - 1 for 1 */
 } PagedAttnArgs;
 
 #define SEQ_ROWS 128 /* queries x heads per workgroup of a sequence attention, */

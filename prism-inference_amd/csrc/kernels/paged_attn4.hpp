@@ -16,7 +16,11 @@
 /* What a wave has to do, as paged_work, but with the splits of a length as long as those of the longest expected: workgroups are
  * alike, short sequences have fewer, and those without keys leave at once. */
 __device__ __forceinline__ bool paged4_work(const PagedAttnArgs& a, int wave, PagedWork& w) {
-    const int group = a.n_heads / a.n_kv_heads;
+    /* x / d by its inverse, one less at times */
+    const auto divide = [](unsigned x, unsigned d, unsigned inverse) {
+        const unsigned q = (unsigned)((uint64_t)x * inverse >> 32);
+        return x - q * d >= d ? q + 1 : q;
+    };
     const unsigned items = (unsigned)a.n_seqs * a.n_kv_heads * a.head_tiles; /* 32 bits: a launch has fewer than 2^24 workgroups */
     unsigned item = blockIdx.x;
     int part = 0;
@@ -24,22 +28,29 @@ __device__ __forceinline__ bool paged4_work(const PagedAttnArgs& a, int wave, Pa
     if (a.waves == 1) {
         item = item * 4 + wave;
     } else {
-        w.split = (int)(item % (unsigned)a.splits);
-        item /= (unsigned)a.splits;
+        const unsigned x = divide(item, a.splits, a.by_splits);
+        w.split = (int)(item - x * a.splits);
+        item = x;
         part = w.split * 4 + wave;
     }
     if (item >= items) return false;
-    const unsigned tiles = a.head_tiles, kv = a.n_kv_heads, both = item / tiles;
-    const int ht = (int)(item - both * tiles);
-    w.seq = (int)(both / kv);
-    w.hk = (int)(both - w.seq * kv);
-    w.head = w.hk * group + ht * PAGED_TILE_HEADS;
-    w.heads = min(group - ht * PAGED_TILE_HEADS, PAGED_TILE_HEADS);
+    const unsigned both = divide(item, a.head_tiles, a.by_tiles);
+    const int ht = (int)(item - both * a.head_tiles);
+    w.seq = (int)divide(both, a.n_kv_heads, a.by_kv);
+    w.hk = (int)(both - w.seq * a.n_kv_heads);
+    w.head = w.hk * a.group + ht * PAGED_TILE_HEADS;
+    w.heads = min(a.group - ht * PAGED_TILE_HEADS, PAGED_TILE_HEADS);
     const int n = seq_clamp(a.lengths[w.seq], 0, a.table_pages << a.page_log2);
     w.kr = key_range(n - 1, n, a.left, 0, a.sinks);
-    const int seen = w.kr.sink + w.kr.hi - w.kr.lo, parts = a.waves * a.splits;
-    const int even = ((seen - 1) / parts + 16) & ~15; /* seen = 0: none */
-    const int each = max(even, a.each);
+    const int seen = w.kr.sink + w.kr.hi - w.kr.lo;
+    if (a.waves == 1) {
+        w.i0 = 0;
+        w.i1 = seen;
+        return true;
+    }
+    const int parts = 4 * a.splits;
+    int each = a.each;
+    if ((int64_t)each * parts < seen) each = ((seen - 1) / parts + 16) & ~15; /* longer than expected */
     const int64_t at = (int64_t)part * each;
     w.i0 = at < seen ? (int)at : seen;
     w.i1 = seq_min(seen - w.i0, each) + w.i0;
