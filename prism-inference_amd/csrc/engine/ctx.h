@@ -98,8 +98,8 @@ struct prism_ctx {
     hipFunction_t f_paged[2][4][3] = {};  /* [dtype][head_dim 16, 32, 64, 128][1, 2, more heads a key head] */
     hipFunction_t f_paged_join[2][4] = {};
     hipFunction_t f_seq[2][4][3] = {};    /* [dtype][head_dim][4 waves, 8 waves, 8 waves of half as many rows] */
-    hipFunction_t f_rope_append[2][2] = {}; /* [dtype][16, 4 bits] */
-    hipFunction_t f_cache_read[2][2] = {};  /* [dtype][16, 4 bits] */
+    hipFunction_t f_rope_append[2][2][4] = {}; /* [dtype][16, 4 bits][head_dim] */
+    hipFunction_t f_cache_read[2][2][4] = {};  /* [dtype][16, 4 bits][head_dim] */
     hipFunction_t f_paged4[2][4][3] = {};   /* [dtype][head_dim][1, 2 heads a key head and 32 channels at most; others] */
     hipFunction_t f_paged4_join[2][4] = {};
     hipFunction_t f_linear[2][4] = {};

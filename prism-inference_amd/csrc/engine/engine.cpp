@@ -129,10 +129,6 @@ extern "C" int prism_create(prism_ctx** out, int32_t device, const char* code_ob
         const std::string type = t == PRISM_BF16 ? "bf16" : "f16";
         all.emplace_back(&c->f_rope[t][0], "prism_rope_" + type);
         all.emplace_back(&c->f_rope[t][1], "prism_rope_" + type + "_loose");
-        all.emplace_back(&c->f_rope_append[t][0], "prism_rope_append_" + type);
-        all.emplace_back(&c->f_rope_append[t][1], "prism_rope_append4_" + type);
-        all.emplace_back(&c->f_cache_read[t][0], "prism_cache_read");
-        all.emplace_back(&c->f_cache_read[t][1], "prism_cache_read4_" + type);
         for (int i = 0; i < 4; ++i) {
             const std::string shape = type + "_h" + std::to_string(16 << i);
             for (int g = 0; g < 3; ++g)
@@ -140,6 +136,10 @@ extern "C" int prism_create(prism_ctx** out, int32_t device, const char* code_ob
             all.emplace_back(&c->f_paged_join[t][i], "prism_paged_attn_join_" + shape);
             for (int g = i < 2 ? 0 : 2; g < 3; ++g)
                 all.emplace_back(&c->f_paged4[t][i][g], "prism_paged_attn4_" + shape + (g == 0 ? "_g1" : g == 1 ? "_g2" : "_many"));
+            all.emplace_back(&c->f_rope_append[t][0][i], "prism_rope_append_" + shape);
+            all.emplace_back(&c->f_rope_append[t][1][i], "prism_rope_append4_" + shape);
+            all.emplace_back(&c->f_cache_read[t][0][i], "prism_cache_read_h" + std::to_string(16 << i));
+            all.emplace_back(&c->f_cache_read[t][1][i], "prism_cache_read4_" + shape);
             all.emplace_back(&c->f_paged4_join[t][i], "prism_paged_attn4_join_" + shape);
             all.emplace_back(&c->f_linear[t][i], "prism_linear_attn_" + shape);
             all.emplace_back(&c->f_linear_states[t][i], "prism_linear_states_" + shape);

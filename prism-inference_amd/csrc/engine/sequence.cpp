@@ -17,6 +17,8 @@ namespace {
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 int log2_of(int32_t n) { return __builtin_ctz((unsigned)n); }
 int hd_index(int32_t hd) { return log2_of(hd) - 4; }
+/* what the kernels divide by d with */
+uint32_t inverse(int32_t d) { return d > 1 ? (uint32_t)((uint64_t(1) << 32) / (uint32_t)d) : UINT32_MAX; }
 
 /* The context's device while a call enqueues its work, the caller's after it. */
 class OnDevice {
@@ -188,7 +190,6 @@ int paged(prism_ctx* c, const prism_paged_attn_push* p, bool four, const void* q
     a.splits = plan.splits;
     a.ws = static_cast<float*>(workspace);
     if (four) {
-        const auto inverse = [](int32_t d) { return (uint32_t)std::min<uint64_t>((uint64_t(1) << 32) / (uint32_t)d, UINT32_MAX); };
         a.each = paged4_each(*p, plan);
         a.group = p->n_heads / d.n_kv_heads;
         a.by_splits = inverse(plan.splits);
@@ -322,7 +323,8 @@ extern "C" int prism_rope_append(prism_ctx* c, const prism_rope_append_push* p, 
     a.n_new = p->n_new;
     a.n_heads = p->n_heads;
     a.n_kv_heads = kept ? d.n_kv_heads : 0; /* no place: no work but the queries' */
-    a.head_dim = d.head_dim;
+    a.by_heads = inverse(a.n_heads);
+    a.by_kv = inverse(a.n_kv_heads);
     if (p->n_axes > 0) {
         a.n_pairs = rope_axes(turn_of(*p, 1, 0, 0), a.axis_end);
         a.log2_base = std::log2(p->base);
@@ -335,7 +337,7 @@ extern "C" int prism_rope_append(prism_ctx* c, const prism_rope_append_push* p, 
     a.page_log2 = log2_of(d.page_size);
     a.n_pages = d.n_pages;
     a.table_pages = d.table_pages;
-    return launch(c, c->f_rope_append[d.dtype][p->format == PRISM_CACHE_4], what,
+    return launch(c, c->f_rope_append[d.dtype][p->format == PRISM_CACHE_4][hd_index(d.head_dim)], what,
                   ((int64_t)p->n_new + a.tile - 1) / a.tile, 256, &a, stream);
 }
 
@@ -371,12 +373,12 @@ extern "C" int prism_cache_read(prism_ctx* c, const prism_cache_read_push* p, co
     a.v_head_stride = p->v_head_stride;
     a.n_rows = p->n_rows;
     a.n_kv_heads = d.n_kv_heads;
-    a.head_dim = d.head_dim;
+    a.by_kv = inverse(d.n_kv_heads);
     a.page_log2 = log2_of(d.page_size);
     a.n_pages = d.n_pages;
     a.table_pages = d.table_pages;
     const int64_t chunks = (int64_t)p->n_rows * d.n_kv_heads * (d.head_dim / 8);
-    return launch(c, c->f_cache_read[d.dtype][p->format == PRISM_CACHE_4], what, (chunks + 255) / 256, 256, &a, stream);
+    return launch(c, c->f_cache_read[d.dtype][p->format == PRISM_CACHE_4][hd_index(d.head_dim)], what, (chunks + 255) / 256, 256, &a, stream);
 }
 
 namespace {
@@ -460,5 +462,6 @@ extern "C" int prism_linear_step(prism_ctx* c, const prism_linear_attn_push* p, 
     if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || !aligned16(state_in) || !aligned16(state_out))
         return fail(c, PRISM_ERR_INVALID, "%s: buffers must be 16-byte aligned", what);
     LinearAttnArgs a = linear_args(p, q, k, v, rates, nullptr, state_of, state_in, out, state_out);
-    return launch(c, c->f_linear_step[p->dtype][hd_index(p->head_dim)], what, (int64_t)p->n_seqs * p->n_heads, 256, &a, stream);
+    const int64_t items = (int64_t)p->n_seqs * p->n_heads; /* a wave each; of 128 channels, four */
+    return launch(c, c->f_linear_step[p->dtype][hd_index(p->head_dim)], what, p->head_dim == 128 ? items : (items + 3) / 4, 256, &a, stream);
 }

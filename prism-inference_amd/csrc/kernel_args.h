@@ -217,7 +217,7 @@ typedef struct PagedAttnArgs {
     /* 4-bit pages: */
     int32_t each;           /* waves = 4: a wave's keys of the longest sequence expected */
     int32_t group;          /* n_heads / n_kv_heads */
-    uint32_t by_splits, by_tiles, by_kv; /* floor(2^32 / splits, head_tiles, n_kv_heads), 2^32 - 1 for 1 */
+    uint32_t by_splits, by_tiles, by_kv; /* inverses of splits, head_tiles and n_kv_heads */
 } PagedAttnArgs;
 
 #define SEQ_ROWS 128 /* queries x heads per workgroup of a sequence attention, */
@@ -261,9 +261,10 @@ typedef struct RopeAppendArgs {
     const int32_t* pos_of;  /* [n_new] */
     int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride;
     int64_t v_token_stride, v_head_stride, out_token_stride, out_head_stride, pos_stride;
-    int32_t n_new, n_heads, n_kv_heads, head_dim;
+    int32_t n_new, n_heads, n_kv_heads;
     int32_t n_pairs, adjacent, axis_end[4], one_ladder; /* as RopeArgs */
     int32_t tile;           /* tokens per workgroup */
+    uint32_t by_heads, by_kv; /* inverses of n_heads and n_kv_heads: floor(2^32 / n), 2^32 - 1 for 1 and 0 */
     int32_t n_seqs, page_log2, n_pages, table_pages;
     double turn, log2_base;
 } RopeAppendArgs;
@@ -279,8 +280,9 @@ typedef struct CacheReadArgs {
     uint16_t* k;
     uint16_t* v;
     int64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride;
-    int32_t n_rows, n_seqs, n_kv_heads, head_dim;
+    int32_t n_rows, n_seqs, n_kv_heads;
     int32_t page_log2, n_pages, table_pages;
+    uint32_t by_kv;
 } CacheReadArgs;
 
 #define LINEAR_CHUNK 64 /* tokens that a linear attention takes at a time */

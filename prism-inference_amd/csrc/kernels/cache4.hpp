@@ -72,44 +72,34 @@ __device__ __forceinline__ V shift_up(V v, int s) {
     return y.v;
 }
 
-/* A chunk of 8 channels from c on of a row: itself, and the channels that its own turn with. */
-template <class T>
-struct Turned8 {
-    typename T::v8 x, other;
-};
-template <class T>
-__device__ __forceinline__ Turned8<T> turn_load(const RopeAppendArgs& a, const uint16_t* row, int c, bool turns) {
-    Turned8<T> r;
-    r.x = ld8<T>(row + c);
-    r.other = r.x;
-    const int n = a.n_pairs;
-    if (!a.adjacent && turns && c < 2 * n) {
-        /* All 8 of the first half: n channels on (16 more fit the row: n is at most head_dim / 2). The second: n back. The
-           chunk with the border inside has both, of which the second half's would begin before the row. */
-        r.other = ld8_any<T>(row + (c < n ? c + n : c - n));
-        if (c < n && c + 8 > n) {
-            const typename T::v8 back = shift_up(ld8<T>(row), n & 7);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) r.other[e] = e >= (n & 7) ? back[e] : r.other[e];
-        }
-    }
-    return r;
+/* x / d by inverse = floor(2^32 / d) (2^32 - 1 for 1), which gives one less at times */
+__device__ __forceinline__ uint32_t divide(uint32_t x, uint32_t d, uint32_t inverse) {
+    const uint32_t q = __umulhi(x, inverse);
+    return x - q * d >= d ? q + 1 : q;
 }
 
-/* Tokens by a workgroup as in rope.hpp; the table holds for each channel what it is times and what its partner is times
- * (cos, and sin with its sign), as [token][channel % 8][channel / 8], so that lanes with chunks side by side read
- * side by side. A 4-bit key is turned in 64 bits, from a table of its own. */
-template <class T, bool FOUR>
+/*
+ * A workgroup takes a few tokens, as in rope.hpp. Its table holds for each channel what the channel is times and what its partner
+ * is times (cos, and sin with its sign), as [token][channel % 8][channel / 8], so that lanes with chunks of 8 side by side read
+ * side by side; a 4-bit key is turned in 64 bits, from a table of its own. Waves then take 64 chunks of queries, of keys or of values
+ * at a time, two of these in flight: what a wave does is the same for all its lanes, and a lane's channels are always the same.
+ * The partners of a chunk come as 8 values from anywhere in the row (a load that need not be aligned).
+ *
+ * Bound by HBM: 24,600 tokens of 32/8 heads x 128, 513 MB, APPENDUS us.
+ */
+template <class T, int HD, bool FOUR>
 __device__ __forceinline__ void rope_append_body(const RopeAppendArgs& a) {
     typedef typename T::v8 v8;
     typedef typename T::el el;
-    constexpr int U = 2;
-    __shared__ __attribute__((aligned(16))) float2 cs[APPEND_TILE_CHANNELS];
-    __shared__ __attribute__((aligned(16))) double2 cs64[FOUR ? APPEND_TILE_CHANNELS : 1];
+    constexpr int U = 2, CH = HD / 8, TILE = APPEND_TILE_CHANNELS / HD;
+    constexpr int BLOCK = CH < 4 ? CH : 4; /* chunks of a 4-bit block, lanes side by side */
+    __shared__ __attribute__((aligned(16))) float2 cs[TILE * HD];
+    __shared__ __attribute__((aligned(16))) double2 cs64[FOUR ? TILE * HD : 1];
     __shared__ double turns[64];
-    __shared__ int64_t slots[APPEND_TILE_CHANNELS / 16];
-    const int n = a.n_pairs, hd = a.head_dim, chunks = hd / 8, lc = __builtin_ctz(chunks);
-    const int t0 = blockIdx.x * a.tile, tokens = min(a.tile, a.n_new - t0);
+    __shared__ int64_t slots[TILE];
+    const int n = a.n_pairs, lane = lane_id();
+    const int64_t t0 = (int64_t)blockIdx.x * a.tile;
+    const int tokens = min(a.tile, (int)(a.n_new - t0));
     const auto axis_of = [&](int j) { return (j >= a.axis_end[0]) + (j >= a.axis_end[1]) + (j >= a.axis_end[2]); };
     if (threadIdx.x < n) {
         const int j = threadIdx.x, axis = axis_of(j), first = axis ? a.axis_end[axis - 1] : 0;
@@ -125,7 +115,7 @@ __device__ __forceinline__ void rope_append_body(const RopeAppendArgs& a) {
         double s, c;
         sincospi(2.0 * (rev - rint(rev)), &s, &c);
         const int c1 = a.adjacent ? 2 * j : j, c2 = a.adjacent ? c1 + 1 : j + n;
-        const int i1 = t * hd + c1 % 8 * chunks + c1 / 8, i2 = t * hd + c2 % 8 * chunks + c2 / 8;
+        const int i1 = t * HD + c1 % 8 * CH + c1 / 8, i2 = t * HD + c2 % 8 * CH + c2 / 8;
         cs[i1] = float2{(float)c, -(float)s};
         cs[i2] = float2{(float)c, (float)s};
         if constexpr (FOUR) {
@@ -134,111 +124,140 @@ __device__ __forceinline__ void rope_append_body(const RopeAppendArgs& a) {
         }
     }
     __syncthreads();
+
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int H = a.n_heads, K = a.n_kv_heads;
-    const int per_token = (H + 2 * K) << lc;
-    const int block = FOUR ? min(chunks, 4) : 1; /* chunks of a 4-bit block: lanes side by side, chunks is a power of two */
-    const int dt = 256 / per_token, dr = 256 % per_token;
-    int t = threadIdx.x / per_token, r = threadIdx.x % per_token;
-    while (t < tokens) {
-        Turned8<T> v[U];
-        int tt[U], row[U], c[U];
+    const int nq = (tokens * H * CH + 63) / 64, nk = (tokens * K * CH + 63) / 64;
+    const int k = lane % CH, c = 8 * k; /* the lane's chunk and channels */
+    const int turned = max(min(2 * n - c, 8), 0); /* of them, the first */
+    /* Partners, other than in the chunk itself: all of the first half n channels on, of the second n back. The chunk with the
+       border inside has both, of which the second half's would begin before the row. */
+    const bool far = !a.adjacent && turned > 0, border = far && c < n && c + 8 > n;
+    const int partner = far ? (c < n ? c + n : c - n) : c; /* at most HD - 8: n is at most HD / 2, and c + 8 - n < 8 here */
+
+    struct Unit {
+        int kind, t, h; /* 0 queries, 1 keys, 2 values; -1: none */
+        v8 x, other;
+    };
+    const auto load = [&](int w) {
+        Unit u;
+        u.kind = w < nq ? 0 : w < nq + nk ? 1 : w < nq + 2 * nk ? 2 : -1;
+        if (u.kind < 0) return u;
+        const uint32_t heads = u.kind == 0 ? H : K, inverse = u.kind == 0 ? a.by_heads : a.by_kv;
+        const uint32_t rows = tokens * heads, row = (w - (u.kind == 0 ? 0 : u.kind == 1 ? nq : nq + nk)) * (64 / CH) + lane / CH;
+        const uint32_t in = min(row, rows - 1);
+        u.t = divide(in, heads, inverse);
+        u.h = in - u.t * heads;
+        const uint16_t* m = u.kind == 0 ? a.q : u.kind == 1 ? a.k : a.v;
+        const int64_t ts = u.kind == 0 ? a.q_token_stride : u.kind == 1 ? a.k_token_stride : a.v_token_stride;
+        const int64_t hs = u.kind == 0 ? a.q_head_stride : u.kind == 1 ? a.k_head_stride : a.v_head_stride;
+        const uint16_t* x = m + t0 * ts + ((uint32_t)u.t * ts + (uint32_t)u.h * hs);
+        u.x = ld8<T>(x + c);
+        if (u.kind < 2) {
+            u.other = ld8_any<T>(x + partner);
+            if (border) {
+                const v8 back = shift_up(ld8<T>(x), n & 7);
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            tt[u] = t < tokens ? t : -1;
-            row[u] = r >> lc;
-            c[u] = (r & (chunks - 1)) * 8;
-            const int64_t tok = t0 + min(t, tokens - 1); /* past the end: read, not written */
-            const uint16_t* x = row[u] < H     ? a.q + tok * a.q_token_stride + row[u] * a.q_head_stride
-                                : row[u] < H + K ? a.k + tok * a.k_token_stride + (row[u] - H) * a.k_head_stride
-                                               : a.v + tok * a.v_token_stride + (row[u] - H - K) * a.v_head_stride;
-            v[u] = turn_load<T>(a, x, c[u], row[u] < H + K);
-            t += dt;
-            r += dr;
-            if (r >= per_token) {
-                r -= per_token;
-                ++t;
+                for (int e = 0; e < 8; ++e) u.other[e] = e >= (n & 7) ? back[e] : u.other[e];
             }
         }
+        if (row >= rows) u.t = -1; /* past the end: read, not written */
+        return u;
+    };
+    const auto keep = [&](const Unit& u, const float (&y)[8], v8 o) { /* into the cache; a block's lanes are all here */
+        uint8_t* pages = u.kind == 1 ? a.k_pages : a.v_pages;
+        const int64_t slot = slots[max(u.t, 0)], at = slot + ((int64_t)u.h << a.page_log2);
+        const bool on = u.t >= 0 && slot >= 0;
+        if constexpr (!FOUR) {
+            if (on) st8<T>(reinterpret_cast<uint16_t*>(pages) + at * HD + c, o);
+        } else {
+            float top = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) top = vmax(top, __builtin_fabsf(y[e])); /* NaN stays */
+            top = vmax(top, dpp<0xB1>(top));
+            if constexpr (BLOCK == 4) top = vmax(top, dpp<0x4E>(top));
+            if (!on) return;
+            const uint32_t bits = __builtin_bit_cast(uint32_t, top);
+            /* 1.75 * 2^k = 7 * 2^(k-2) */
+            int e = (int)(bits >> 23) - 129 + ((bits & 0x7FFFFFu) > 0x600000u);
+            e = seq_clamp(e, Fp4<T>::low, Fp4<T>::high);
+            const bool fine = top < INFINITY;
+            const float s = fp4_scale(e + 127);
+            uint32_t w = 0;
+            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, y[0], y[1], s, 0);
+            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, y[2], y[3], s, 1);
+            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, y[4], y[5], s, 2);
+            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, y[6], y[7], s, 3);
+            *reinterpret_cast<uint32_t*>(pages + at * (HD / 2) + c / 2) = fine ? w : 0;
+            if (k % BLOCK == 0) (u.kind == 1 ? a.k_scales : a.v_scales)[at * (CH / BLOCK) + k / BLOCK] = fine ? (uint8_t)(e + 127) : 255;
+        }
+    };
+    const auto work = [&](Unit u) {
+        if (u.kind < 0) return;
+        v8 o = u.x;
+        float y[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = (float)o[e];
+        if (u.kind < 2) {
+            if (a.adjacent) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) u.other[e] = u.x[e ^ 1];
+            }
+            const int at = max(u.t, 0) * HD + k;
+            if (!FOUR || u.kind == 0) {
+                float z[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float2 f = cs[at + e * CH];
+                    z[e] = __builtin_fmaf(y[e], f.x, (float)u.other[e] * f.y);
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (e < turned) {
+                        y[e] = z[e];
+                        o[e] = (el)opaque(y[e]);
+                    }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const double2 f = cs64[at + e * CH];
+                    const float z = (float)__builtin_fma((double)y[e], f.x, (double)(float)u.other[e] * f.y);
+                    y[e] = e < turned ? z : y[e];
+                }
+            }
+        }
+        if (u.kind == 0) {
+            if (u.t >= 0) st8<T>(a.q_out + t0 * a.out_token_stride + ((uint32_t)u.t * a.out_token_stride + (uint32_t)u.h * a.out_head_stride) + c, o);
+        } else {
+            keep(u, y, o);
+        }
+    };
+    for (int w = wave; w < nq + 2 * nk; w += 4 * U) {
+        Unit u[U];
+#pragma unroll
+        for (int i = 0; i < U; ++i) u[i] = load(w + 4 * i);
         /* in place, a row's lanes, which are in one wave, have all read before one writes */
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (tt[u] < 0) continue;
-            const bool query = row[u] < H, value = row[u] >= H + K;
-            const int h = query ? row[u] : value ? row[u] - H - K : row[u] - H;
-            v8 o = v[u].x;
-            if (a.adjacent) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[u].other[e] = v[u].x[e ^ 1];
-            }
-            float y[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) y[e] = (float)o[e];
-            if (!value) {
-                const int at = tt[u] * hd + c[u] / 8;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    if (c[u] + e >= 2 * n) break;
-                    const float other = (float)v[u].other[e];
-                    if (!FOUR || query) {
-                        const float2 k = cs[at + e * chunks];
-                        y[e] = __builtin_fmaf(y[e], k.x, other * k.y);
-                    } else {
-                        const double2 k = cs64[at + e * chunks];
-                        y[e] = (float)__builtin_fma((double)y[e], k.x, (double)other * k.y);
-                    }
-                    o[e] = (el)opaque(y[e]);
-                }
-            }
-            if (query) {
-                st8<T>(a.q_out + (t0 + tt[u]) * a.out_token_stride + h * a.out_head_stride + c[u], o);
-                continue;
-            }
-            const int64_t slot = slots[tt[u]];
-            const int64_t at = slot + ((int64_t)h << a.page_log2);
-            if constexpr (!FOUR) {
-                if (slot >= 0) st8<T>(reinterpret_cast<uint16_t*>(value ? a.v_pages : a.k_pages) + at * hd + c[u], o);
-            } else {
-                float top = 0.f;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) top = vmax(top, __builtin_fabsf(y[e])); /* NaN stays */
-                top = vmax(top, dpp<0xB1>(top));
-                if (block == 4) top = vmax(top, dpp<0x4E>(top));
-                if (slot < 0) continue;
-                const uint32_t bits = __builtin_bit_cast(uint32_t, top);
-                /* 1.75 * 2^k = 7 * 2^(k-2) */
-                int e = (int)(bits >> 23) - 129 + ((bits & 0x7FFFFFu) > 0x600000u);
-                e = seq_clamp(e, Fp4<T>::low, Fp4<T>::high);
-                const bool fine = top < INFINITY;
-                uint32_t w = 0;
-                const float s = fp4_scale(e + 127);
-                w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, y[0], y[1], s, 0);
-                w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, y[2], y[3], s, 1);
-                w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, y[4], y[5], s, 2);
-                w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, y[6], y[7], s, 3);
-                *reinterpret_cast<uint32_t*>((value ? a.v_pages : a.k_pages) + at * (hd / 2) + c[u] / 2) = fine ? w : 0;
-                if ((c[u] / 8 & (block - 1)) == 0)
-                    (value ? a.v_scales : a.k_scales)[at * (chunks / block) + c[u] / 8 / block] = fine ? (uint8_t)(e + 127) : 255;
-            }
-        }
+        for (int i = 0; i < U; ++i) work(u[i]);
     }
 }
 
-template <class T, bool FOUR>
+template <class T, int HD, bool FOUR>
 __device__ __forceinline__ void cache_read_body(const CacheReadArgs& a) {
-    const int chunks = a.head_dim / 8, block = min(chunks, 4);
-    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int64_t per_token = (int64_t)a.n_kv_heads * chunks;
-    if (id >= a.n_rows * per_token) return;
-    const int64_t t = id / per_token;
-    const int r = (int)(id - t * per_token), h = r / chunks, c = r % chunks;
+    constexpr int CH = HD / 8, BLOCK = CH < 4 ? CH : 4;
+    const uint32_t id = blockIdx.x * 256 + threadIdx.x, row = id / CH; /* 32 bits: a launch has fewer than 2^32 threads */
+    const int c = id % CH;
+    const int64_t t = divide(row, a.n_kv_heads, a.by_kv);
+    const int h = (int)(row - (uint32_t)t * a.n_kv_heads);
+    if (t >= a.n_rows) return;
     const int64_t slot = a.n_seqs > 0 ? cache_slot(a, a.seq_of[t], a.pos_of[t]) : -1; /* no sequences: no arrays either */
     typename T::v8 k{}, v{};
     if (slot >= 0) {
-        const int64_t at = slot + ((int64_t)h << a.page_log2), i = at * chunks + c;
+        const int64_t at = slot + ((int64_t)h << a.page_log2), i = at * CH + c;
         if constexpr (FOUR) {
-            const int64_t j = at * (chunks / block) + c / block;
+            const int64_t j = at * (CH / BLOCK) + c / BLOCK;
             k = fp4_values<T>(reinterpret_cast<const uint32_t*>(a.k_pages)[i], fp4_scale(a.k_scales[j]));
             v = fp4_values<T>(reinterpret_cast<const uint32_t*>(a.v_pages)[i], fp4_scale(a.v_scales[j]));
         } else {
@@ -250,10 +269,14 @@ __device__ __forceinline__ void cache_read_body(const CacheReadArgs& a) {
     st8<T>(a.v + t * a.v_token_stride + h * a.v_head_stride + 8 * c, v);
 }
 
-#define CACHE4(NAME, T)                                                                                                      \
-    extern "C" __global__ void __launch_bounds__(256) prism_rope_append_##NAME(RopeAppendArgs a) { rope_append_body<T, false>(a); } \
-    extern "C" __global__ void __launch_bounds__(256) prism_rope_append4_##NAME(RopeAppendArgs a) { rope_append_body<T, true>(a); } \
-    extern "C" __global__ void __launch_bounds__(256) prism_cache_read4_##NAME(CacheReadArgs a) { cache_read_body<T, true>(a); }
-CACHE4(f16, F16) CACHE4(bf16, BF16)
+#define CACHE4(NAME, T, HD)                                                                                                        \
+    extern "C" __global__ void __launch_bounds__(256) prism_rope_append_##NAME##_h##HD(RopeAppendArgs a) { rope_append_body<T, HD, false>(a); } \
+    extern "C" __global__ void __launch_bounds__(256) prism_rope_append4_##NAME##_h##HD(RopeAppendArgs a) { rope_append_body<T, HD, true>(a); } \
+    extern "C" __global__ void __launch_bounds__(256) prism_cache_read4_##NAME##_h##HD(CacheReadArgs a) { cache_read_body<T, HD, true>(a); }
+CACHE4(f16, F16, 16) CACHE4(f16, F16, 32) CACHE4(f16, F16, 64) CACHE4(f16, F16, 128)
+CACHE4(bf16, BF16, 16) CACHE4(bf16, BF16, 32) CACHE4(bf16, BF16, 64) CACHE4(bf16, BF16, 128)
 #undef CACHE4
-extern "C" __global__ void __launch_bounds__(256) prism_cache_read(CacheReadArgs a) { cache_read_body<F16, false>(a); }
+#define CACHE16(HD) \
+    extern "C" __global__ void __launch_bounds__(256) prism_cache_read_h##HD(CacheReadArgs a) { cache_read_body<F16, HD, false>(a); }
+CACHE16(16) CACHE16(32) CACHE16(64) CACHE16(128)
+#undef CACHE16

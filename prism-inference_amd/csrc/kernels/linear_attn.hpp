@@ -568,37 +568,70 @@ __device__ __forceinline__ void linear_segment(const LinearAttnArgs& a) {
     }
 }
 
-/* One token of a sequence and head by a workgroup. */
+/* One token of a sequence and head, in fp32: a wave (128 channels: four), whose lanes have four columns of R rows of the state
+ * each, 16 bytes a load; sums over the rows meet across lanes. Bound by HBM: the state read and written once, 8,160 x 8 x 32 x 32
+ * STEPUS us (535 MB). */
 template <class T, int HD>
 __device__ __forceinline__ void linear_step(const LinearAttnArgs& a) {
-    constexpr int P = 256 / HD, R = HD / P;
-    __shared__ float part[256];
-    const int s = blockIdx.x / a.n_heads, h = blockIdx.x % a.n_heads, hk = h / (a.n_heads / a.n_kv_heads);
-    const int c = threadIdx.x % HD, p = threadIdx.x / HD;
+    typedef typename T::v4 v4;
+    constexpr int WPI = HD == 128 ? 4 : 1, COLS = HD / 4, R = HD / (64 / COLS) / WPI; /* waves a head; lanes a row; rows of a lane */
+    __shared__ f4 part[WPI > 1 ? 4 * 32 : 1];
+    const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t item = WPI > 1 ? blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
+    if (item >= (int64_t)a.n_seqs * a.n_heads) return;
+    const int s = (int)(item / a.n_heads), h = (int)(item % a.n_heads), hk = h / (a.n_heads / a.n_kv_heads);
+    const int c = lane % COLS * 4, r0 = ((WPI > 1 ? wave : 0) * (64 / COLS) + lane / COLS) * R;
     const int number = linear_state(a, s);
     uint16_t* out = a.out + s * a.out_token_stride + h * a.out_head_stride + c;
+    const bool first = lane < COLS && (WPI == 1 || wave == 0);
     if (number < 0) {
-        if (p == 0) st1<T>(out, 0.f);
+        if (first) *reinterpret_cast<v4*>(out) = v4{};
         return;
     }
-    const int64_t base = ((int64_t)number * a.n_heads + h) * HD * HD;
+    const int64_t at = ((int64_t)number * a.n_heads + h) * HD * HD + r0 * HD + c;
+    f4 S[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) S[i] = *reinterpret_cast<const f4*>(a.state_in + at + i * HD);
     const float keep = fast_exp2(-linear_rate(a, h));
-    const uint16_t* q = a.q + s * a.q_token_stride + h * a.q_head_stride;
-    const uint16_t* k = a.k + s * a.k_token_stride + hk * a.k_head_stride;
-    const float v = ld1<T>(a.v + s * a.v_token_stride + hk * a.v_head_stride + c);
-    float o = 0.f;
+    const uint16_t* q = a.q + s * a.q_token_stride + h * a.q_head_stride + r0;
+    const uint16_t* k = a.k + s * a.k_token_stride + hk * a.k_head_stride + r0;
+    const v4 vv = *reinterpret_cast<const v4*>(a.v + s * a.v_token_stride + hk * a.v_head_stride + c);
+    const f4 v = __builtin_convertvector(vv, f4);
+    typename T::el kr[R], qr[R];
+    __builtin_memcpy(kr, k, 2 * R);
+    __builtin_memcpy(qr, q, 2 * R);
+    f4 o = {};
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-        const int64_t at = base + (p + P * i) * HD + c;
-        const float S = __builtin_fmaf(ld1<T>(k + p + P * i), v, a.state_in[at] * keep);
-        a.state_out[at] = S;
-        o = __builtin_fmaf(ld1<T>(q + p + P * i), S, o);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            S[i][e] = __builtin_fmaf((float)kr[i], v[e], S[i][e] * keep);
+            o[e] = __builtin_fmaf((float)qr[i], S[i][e], o[e]);
+        }
+        *reinterpret_cast<f4*>(a.state_out + at + i * HD) = S[i];
     }
-    part[threadIdx.x] = o;
-    __syncthreads();
-    if (p == 0) {
-        for (int i = 1; i < P; ++i) o += part[i * HD + c];
-        st1<T>(out, o * a.scale);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        float x, y;
+        if constexpr (COLS <= 4) o[e] += dpp<0x141>(dpp<0x1B>(o[e])); /* lane ^ 4: quads mirrored in eights, and back within */
+        if constexpr (COLS <= 8) o[e] += dpp<0x128>(o[e]);            /* lane ^ 8 */
+        if constexpr (COLS <= 16) {
+            lanes_x16(o[e], x, y);
+            o[e] = x + y;
+        }
+        lanes_x32(o[e], x, y);
+        o[e] = x + y;
+    }
+    if constexpr (WPI > 1) {
+        if (lane < COLS) part[wave * 32 + lane] = o;
+        __syncthreads();
+        if (first) o = (part[lane] + part[32 + lane]) + (part[64 + lane] + part[96 + lane]);
+    }
+    if (first) {
+        v4 r;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r[e] = (typename T::el)opaque(o[e] * a.scale);
+        *reinterpret_cast<v4*>(out) = r;
     }
 }
 

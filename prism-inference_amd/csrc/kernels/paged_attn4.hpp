@@ -16,11 +16,6 @@
 /* What a wave has to do, as paged_work, but with the splits of a length as long as those of the longest expected: workgroups are
  * alike, short sequences have fewer, and those without keys leave at once. */
 __device__ __forceinline__ bool paged4_work(const PagedAttnArgs& a, int wave, PagedWork& w) {
-    /* x / d by its inverse, one less at times */
-    const auto divide = [](unsigned x, unsigned d, unsigned inverse) {
-        const unsigned q = (unsigned)((uint64_t)x * inverse >> 32);
-        return x - q * d >= d ? q + 1 : q;
-    };
     const unsigned items = (unsigned)a.n_seqs * a.n_kv_heads * a.head_tiles; /* 32 bits: a launch has fewer than 2^24 workgroups */
     unsigned item = blockIdx.x;
     int part = 0;
