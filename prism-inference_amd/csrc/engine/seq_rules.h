@@ -256,11 +256,15 @@ inline int rope_tile(int64_t n_tokens, int n_pairs) {
     return tile;
 }
 
-/* The same for a launch that appends. */
-inline int append_tile(int64_t n_new, int head_dim) {
+/* Tokens per workgroup of a launch that appends, as its tables allow: 12 wave's steps of 64 chunks at least where workgroups stay as many as
+ * CUs, and up to 48 where they are many. us at 1, 2, 4, 8, 16, 32 tokens: 24,600 tokens, 48 heads x 128: 150, 126, 123, 132; 8,160,
+ * 24 x 32: 23, 14, 12, 11, 12, 16; 50,000: 121, 66, 46, 37, 35, 38; 4,000, 24 x 64: 12, 9, 8, 9, 11; 40,000, 48 x 16: 94, 52, 36, 29, 26, 25. */
+inline int append_tile(int64_t n_new, int64_t heads, int head_dim) {
     const int most = APPEND_TILE_CHANNELS / head_dim;
+    const auto chunks = [&](int tile) { return tile * heads * (head_dim / 8); };
     int tile = 1;
-    while (2 * tile <= most && n_new >= (int64_t)2 * tile * 4 * 256) tile *= 2;
+    while (2 * tile <= most && chunks(tile) < 12 * 64 && n_new / (2 * tile) >= 256) tile *= 2;
+    while (2 * tile <= most && chunks(2 * tile) <= 48 * 64 && n_new / (2 * tile) >= 2500) tile *= 2;
     return tile;
 }
 

@@ -332,7 +332,7 @@ extern "C" int prism_rope_append(prism_ctx* c, const prism_rope_append_push* p, 
     a.adjacent = p->layout == PRISM_ROPE_ADJACENT;
     a.one_ladder = p->ladder == PRISM_ROPE_ONE_LADDER;
     a.turn = 1.0 / 6.283185307179586476925286766559;
-    a.tile = append_tile(p->n_new, d.head_dim);
+    a.tile = append_tile(p->n_new, a.n_heads + 2 * a.n_kv_heads, d.head_dim);
     a.n_seqs = d.n_seqs;
     a.page_log2 = log2_of(d.page_size);
     a.n_pages = d.n_pages;

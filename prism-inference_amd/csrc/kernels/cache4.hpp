@@ -85,12 +85,11 @@ __device__ __forceinline__ uint32_t divide(uint32_t x, uint32_t d, uint32_t inve
  * at a time, two of these in flight: what a wave does is the same for all its lanes, and a lane's channels are always the same.
  * The partners of a chunk come as 8 values from anywhere in the row (a load that need not be aligned).
  *
- * Bound by HBM: 24,600 tokens of 32/8 heads x 128, 513 MB, APPENDUS us.
+ * Bound by HBM: 24,600 tokens of 32/8 heads x 128, 4 bits, 531 MB, 123 us (a copy of as much: 104); the vector units are half busy.
  */
 template <class T, int HD, bool FOUR>
 __device__ __forceinline__ void rope_append_body(const RopeAppendArgs& a) {
     typedef typename T::v8 v8;
-    typedef typename T::el el;
     constexpr int U = 2, CH = HD / 8, TILE = APPEND_TILE_CHANNELS / HD;
     constexpr int BLOCK = CH < 4 ? CH : 4; /* chunks of a 4-bit block, lanes side by side */
     __shared__ __attribute__((aligned(16))) float2 cs[TILE * HD];
@@ -153,7 +152,7 @@ __device__ __forceinline__ void rope_append_body(const RopeAppendArgs& a) {
         const int64_t hs = u.kind == 0 ? a.q_head_stride : u.kind == 1 ? a.k_head_stride : a.v_head_stride;
         const uint16_t* x = m + t0 * ts + ((uint32_t)u.t * ts + (uint32_t)u.h * hs);
         u.x = ld8<T>(x + c);
-        if (u.kind < 2) {
+        if (u.kind < 2 && !a.adjacent) {
             u.other = ld8_any<T>(x + partner);
             if (border) {
                 const v8 back = shift_up(ld8<T>(x), n & 7);
@@ -192,44 +191,44 @@ __device__ __forceinline__ void rope_append_body(const RopeAppendArgs& a) {
             if (k % BLOCK == 0) (u.kind == 1 ? a.k_scales : a.v_scales)[at * (CH / BLOCK) + k / BLOCK] = fine ? (uint8_t)(e + 127) : 255;
         }
     };
-    const auto work = [&](Unit u) {
+    const bool none = turned == 0, some = !none && turned < 8;
+    const auto work = [&](const Unit& u) {
         if (u.kind < 0) return;
-        v8 o = u.x;
-        float y[8];
+        float y[8], z[8], p[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = (float)o[e];
-        if (u.kind < 2) {
-            if (a.adjacent) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) u.other[e] = u.x[e ^ 1];
-            }
-            const int at = max(u.t, 0) * HD + k;
-            if (!FOUR || u.kind == 0) {
-                float z[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float2 f = cs[at + e * CH];
-                    z[e] = __builtin_fmaf(y[e], f.x, (float)u.other[e] * f.y);
-                }
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (e < turned) {
-                        y[e] = z[e];
-                        o[e] = (el)opaque(y[e]);
-                    }
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const double2 f = cs64[at + e * CH];
-                    const float z = (float)__builtin_fma((double)y[e], f.x, (double)(float)u.other[e] * f.y);
-                    y[e] = e < turned ? z : y[e];
-                }
-            }
+        for (int e = 0; e < 8; ++e) y[e] = (float)u.x[e];
+        if (u.kind == 2) {
+            keep(u, y, u.x);
+            return;
         }
-        if (u.kind == 0) {
-            if (u.t >= 0) st8<T>(a.q_out + t0 * a.out_token_stride + ((uint32_t)u.t * a.out_token_stride + (uint32_t)u.h * a.out_head_stride) + c, o);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) p[e] = a.adjacent ? y[e ^ 1] : (float)u.other[e];
+        const int at = max(u.t, 0) * HD + k;
+        if (!FOUR || u.kind == 0) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float2 f = cs[at + e * CH];
+                z[e] = __builtin_fmaf(y[e], f.x, p[e] * f.y);
+            }
+            u4 w, x = __builtin_bit_cast(u4, u.x);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f2{opaque(z[2 * e]), opaque(z[2 * e + 1])}), typename T::v2));
+            v8 o = __builtin_bit_cast(v8, none ? x : w); /* what does not turn keeps its bits, those of a NaN too */
+            if (some)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) o[e] = e < turned ? o[e] : u.x[e];
+            if (u.kind == 1) keep(u, y, o);
+            else if (u.t >= 0)
+                st8<T>(a.q_out + t0 * a.out_token_stride + ((uint32_t)u.t * a.out_token_stride + (uint32_t)u.h * a.out_head_stride) + c, o);
         } else {
-            keep(u, y, o);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const double2 f = cs64[at + e * CH];
+                z[e] = (float)__builtin_fma((double)y[e], f.x, (double)p[e] * f.y);
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] = none || (some && e >= turned) ? y[e] : z[e];
+            keep(u, y, u.x);
         }
     };
     for (int w = wave; w < nq + 2 * nk; w += 4 * U) {
