@@ -112,6 +112,8 @@ __device__ __forceinline__ void linear_segment(const LinearAttnArgs& a) {
     constexpr bool SHARED = WQ == 1;
     constexpr int NT = 64 * WD * WQ;
     constexpr int DK = HD / 16; /* 16-channel tiles of the keys */
+    /* of row or column r of a wave's tile d: a lane's 4 outputs of two tiles lie side by side, 16 bytes a store */
+    const auto channel = [](int d, int r) { return 4 * DV * (r / 4) + 4 * d + r % 4; };
     constexpr int KS = (HD + 31) / 32;
     constexpr int RS = HD >= 32 ? HD + 16 : HD;    /* LDS row: 4 rows' parts of a transposed read lie in different banks */
     constexpr int CPR = HD / 8, NL = (C * CPR + NT - 1) / NT; /* 16-byte chunks a row, and a thread's of a matrix */
@@ -126,23 +128,33 @@ __device__ __forceinline__ void linear_segment(const LinearAttnArgs& a) {
     const int seg = b - lt.first;
     if (seg < 0) return; /* only where starts are not in order */
     const int64_t t0 = lt.rows.start + (int64_t)seg * a.segment;
-    if (STATES ? t0 + a.segment >= lt.rows.end : seg > 0 && t0 >= lt.rows.end) return;
+    const bool last = t0 + a.segment >= lt.rows.end;
+    if (STATES ? last && (seg == 0 || t0 >= lt.rows.end) : seg > 0 && t0 >= lt.rows.end) return;
     const int t1 = (int)min(t0 + a.segment, (int64_t)lt.rows.end);
 
     const float r2 = linear_rate(a, h);
     const auto decay = [&](int n) { return fast_exp2(-r2 * (float)n); };
     const float d1 = decay(1), d2 = decay(2), d3 = decay(3);
     const int number = linear_state(a, lt.seq);
-    const int64_t base = ((int64_t)max(number, 0) * a.n_heads + h) * HD * HD + 16 * DV * wd + l16;
+    const int64_t base = ((int64_t)max(number, 0) * a.n_heads + h) * HD * HD + 16 * DV * wd;
     f4* const mine = reinterpret_cast<f4*>(a.ws) + ((int64_t)b * a.n_heads + h) * (HD * HD / 4) + wd * 64 + lane; /* + 64 WD * (tile DV + d) */
-    f4 S[DK][DV]; /* channels 16 j + 4 g + e of the keys x channel 16 (DV wd + d) + l16 of the values */
+    f4 S[DK][DV]; /* rows 16 j + 4 g + e, channels 16 DV wd + channel(d, l16) of the values */
+    /* state_out may be state_in, and a sequence's last segment may end before the first one begins: where there are
+       several, the launch before this one has read state_in. Its first segment goes on from there, and the last, which
+       adds to nothing, leaves a copy for the first. */
+    const bool begins = number >= 0 && a.state_in && (STATES ? seg == 0 || last : seg == 0 && last);
 #pragma unroll
     for (int j = 0; j < DK; ++j)
 #pragma unroll
         for (int d = 0; d < DV; ++d)
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                S[j][d][e] = !STATES && a.state_in && number >= 0 ? a.state_in[base + (16 * j + 4 * g + e) * HD + 16 * d] : 0.f;
+            for (int e = 0; e < 4; ++e) S[j][d][e] = begins ? a.state_in[base + (16 * j + 4 * g + e) * HD + channel(d, l16)] : 0.f;
+    if constexpr (!STATES)
+        if (seg == 0 && !last) {
+            const f4* const copy = mine + (int64_t)((lt.rows.end - lt.rows.start - 1) / a.segment) * a.n_heads * (HD * HD / 4);
+#pragma unroll
+            for (int j = 0; j < DK * DV; ++j) S[j / DV][j % DV] = copy[64 * WD * j];
+        }
     if constexpr (!STATES) {
         constexpr int DEPTH = DK * DV < 8 ? 16 / (DK * DV) : 2; /* segments asked for at once */
         const float keep = decay(a.segment);
@@ -205,7 +217,7 @@ __device__ __forceinline__ void linear_segment(const LinearAttnArgs& a) {
         for (int i = 0; i < NL; ++i)
             if (row0 + NT / CPR * i < rows) rk[i] = rv[i] = v8{};
     };
-    const int len = t1 > t0 ? t1 - (int)t0 : 0;
+    const int len = t1 > t0 && !(STATES && last) ? t1 - (int)t0 : 0;
     if (len >= C) {
         load_chunk(t0);
     } else if (len > 0) { /* nothing before it is the segment's, or need exist */
@@ -270,7 +282,7 @@ __device__ __forceinline__ void linear_segment(const LinearAttnArgs& a) {
 #pragma unroll
             for (int d = 0; d < DV; ++d)
 #pragma unroll
-                for (int m = 0; m < M; ++m) v[d][m] = transposed(lv, 32 * m, 16 * (DV * wd + d) + 4 * (l16 & 3));
+                for (int m = 0; m < M; ++m) v[d][m] = transposed(lv, 32 * m, 16 * DV * wd + channel(d, 4 * (l16 & 3)));
         };
         if constexpr (!STATES) {
             /* fp16 weights are scaled by a power of two, after the largest that they could be: 2^15 stays above them, and
@@ -428,7 +440,7 @@ __device__ __forceinline__ void linear_segment(const LinearAttnArgs& a) {
                     for (int t = C - 1; t >= 0; --t)
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
-                            if (!(__builtin_fabsf(ld1<T>(lv + t * RS + 16 * (DV * wd + d) + 4 * g + e)) < INFINITY)) from[e] = t;
+                            if (!(__builtin_fabsf(ld1<T>(lv + t * RS + 16 * DV * wd + channel(d, 4 * g + e))) < INFINITY)) from[e] = t;
 #pragma unroll
                     for (int i = 0; i < QN; ++i)
 #pragma unroll
@@ -439,14 +451,11 @@ __device__ __forceinline__ void linear_segment(const LinearAttnArgs& a) {
                 const int row = 16 * tile_of(i) + l16;
                 if (row < skip) continue;
                 uint16_t* first = a.out + (t0 + c0) * a.out_token_stride + h * a.out_head_stride + 16 * DV * wd;
-                first += (uint32_t)(row - skip) * (uint32_t)a.out_token_stride + 4 * g;
+                first += (uint32_t)(row - skip) * (uint32_t)a.out_token_stride + channel(0, 4 * g);
+                el r[4 * DV];
 #pragma unroll
-                for (int d = 0; d < DV; ++d) {
-                    v4 r;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) r[e] = (el)opaque(HALF ? o[i][d][e] * down : o[i][d][e]);
-                    *reinterpret_cast<v4*>(first + 16 * d) = r;
-                }
+                for (int x = 0; x < 4 * DV; ++x) r[x] = (el)opaque(HALF ? o[i][x / 4][x % 4] * down : o[i][x / 4][x % 4]);
+                __builtin_memcpy(__builtin_assume_aligned(first, 8 * DV), r, sizeof(r));
             }
         }
         /* the next state */
@@ -564,13 +573,13 @@ __device__ __forceinline__ void linear_segment(const LinearAttnArgs& a) {
 #pragma unroll
             for (int d = 0; d < DV; ++d)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) a.state_out[base + (16 * j + 4 * g + e) * HD + 16 * d] = S[j][d][e];
+                for (int e = 0; e < 4; ++e) a.state_out[base + (16 * j + 4 * g + e) * HD + channel(d, l16)] = S[j][d][e];
     }
 }
 
 /* One token of a sequence and head, in fp32: a wave (128 channels: four), whose lanes have four columns of R rows of the state
  * each, 16 bytes a load; sums over the rows meet across lanes. Bound by HBM: the state read and written once, 8,160 x 8 x 32 x 32
- * STEPUS us (535 MB). */
+ * 95 us (551 MB, 5.8 TB/s; a copy of as much 108). A lane a column, 4 bytes a load, took 129. */
 template <class T, int HD>
 __device__ __forceinline__ void linear_step(const LinearAttnArgs& a) {
     typedef typename T::v4 v4;

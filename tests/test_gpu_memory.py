@@ -696,3 +696,182 @@ def test_calls_without_rows(engine, dev):
                        None, 0)
     got = dev.get(new, s0.shape, np.float32)
     assert (got[:5] == s0[:5]).all() and np.isnan(got[5:]).all()
+
+
+# ------------------------------------------- calls that the documentation allows
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hd,lens", [(16, [1500, 777, 0, 3]), (32, [2300, 64]), (64, [777, 1500]), (128, [1900, 300]), (128, [63, 65])])
+def test_linear_state_in_place(engine, dev, dtype, hd, lens):
+    """state_out = state_in: the same bits, whether a sequence is split or not."""
+    rng, heads, n = np.random.default_rng(hd), 3, len(lens)
+    rows = normal(rng, (sum(lens), 3 * heads, hd), dtype)
+    s0 = rng.standard_normal((n, heads, hd, hd)).astype(np.float32)
+    push = linear_push(dtype, n, sum(lens), heads, heads, hd, n, 0.1, 3 * heads * hd)
+    need = engine.linear_attn_workspace(push)
+    assert (need > 0) == (max(lens) > 256)
+    x, rates = dev.put(rows), dev.put(np.array([0.0, 0.001, 0.3], np.float32))
+    cu = dev.put(np.concatenate([[0], np.cumsum(lens)]).astype(np.int32))
+
+    def run(old, new):
+        out, ws = dev.put(np.full((sum(lens), heads, hd), NAN[dtype], np.uint16)), dev.put(np.full(max(need, 16) // 4, np.nan, np.float32))
+        engine.linear_attn(push, x, x + 2 * heads * hd, x + 4 * heads * hd, rates, cu, None, old, out, new, ws, need)
+        return dev.get(out, (sum(lens), heads, hd)), dev.get(new, s0.shape, np.float32)
+
+    apart, same = dev.put(s0), dev.put(s0)
+    want, state = run(apart, dev.put(np.full(s0.shape, np.nan, np.float32)))
+    got, left = run(same, same)
+    assert (got == want).all() and (left == state).all() and not np.isnan(state).any()
+    assert (dev.get(apart, s0.shape, np.float32) == s0).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hd", [16, 32, 64, 128])
+def test_linear_strides(engine, dev, dtype, hd):
+    """Heads that read the same queries and the same values (head strides of 0), rows with room in them, outputs head by
+    head: the same bits as from dense rows; along a sequence and a token at a time."""
+    rng, heads, n, room = np.random.default_rng(hd), 4, 70, 24
+    q, k, v = (normal(rng, (n, h, hd), dtype) for h in (1, heads, 1))
+    dense = [dev.put(np.ascontiguousarray(np.broadcast_to(a, (n, heads, hd)))) for a in (q, k, v)]
+    odd = np.full((n, heads * (hd + 8) + room), NAN[dtype], np.uint16)
+    odd[:, :heads * (hd + 8)].reshape(n, heads, hd + 8)[..., :hd] = k
+    s0 = dev.put(rng.standard_normal((n, heads, hd, hd)).astype(np.float32))
+    rates = dev.put(np.array([0.0, 0.01, 0.3, 3.0], np.float32))
+
+    def push(seqs, **kw):
+        p = linear_push(dtype, seqs, n, heads, heads, hd, n, 0.25, heads * hd)
+        for name, value in kw.items():
+            setattr(p, name, value)
+        return p
+
+    strides = dict(q_token_stride=hd, q_head_stride=0, k_token_stride=odd.shape[1], k_head_stride=hd + 8, v_token_stride=hd,
+                   v_head_stride=0, out_token_stride=hd + 8, out_head_stride=n * (hd + 8))
+    for seqs in (1, n):
+        for step in (False, True)[:1 if seqs == 1 else 2]:
+            outs, states = [], []
+            for x, p in ((dense, push(seqs)), ([dev.put(q), dev.put(odd), dev.put(v)], push(seqs, **strides))):
+                new = dev.put(np.full((n, heads, hd, hd), np.nan, np.float32))
+                out = dev.put(np.full((heads, n, hd + 8), NAN[dtype], np.uint16))
+                if step:
+                    engine.linear_step(p, *x, rates, None, s0, out, new)
+                else:
+                    assert engine.linear_attn_workspace(p) == 0
+                    engine.linear_attn(p, *x, rates, None, None, s0, out, new, None, 0)
+                outs.append(dev.get(out, (heads, n, hd + 8)))
+                states.append(dev.get(new, (seqs, heads, hd, hd), np.float32))
+            plain = outs[0].reshape(-1)[:n * heads * hd].reshape(n, heads, hd).transpose(1, 0, 2)
+            assert (outs[1][..., :hd] == plain).all() and (outs[1][..., hd:] == NAN[dtype]).all()
+            assert (states[0] == states[1]).all() and not np.isnan(states[0]).any()
+
+
+def test_linear_thousands_of_sequences(engine, dev):
+    """More than the 64 x 64 that two looks at the starts find."""
+    rng = np.random.default_rng(14)
+    check_linear(engine, dev, rng, "bf16", 16, 1, 1, [int(x) for x in rng.integers(0, 4, 4500)])
+
+
+def test_linear_starts_that_are_not_in_order(engine, dev):
+    """What they give is not specified; rows and states that are not the call's stay as they were."""
+    rng, heads, hd, n = np.random.default_rng(15), 2, 32, 3
+    for cu in ([700, 100, 900, 50], [0, 2000, -5, 1000], [1000, 0, 0, 0]):
+        x, out = dev.put(normal(rng, (1000, 3 * heads, hd), "fp16")), dev.put(np.full((1002, heads, hd), NAN["fp16"], np.uint16))
+        push = linear_push("fp16", n, 1000, heads, heads, hd, n, 0.1, 3 * heads * hd)
+        need = engine.linear_attn_workspace(push)
+        ws, new = dev.put(np.zeros(need // 4 + 64, np.float32)), dev.put(np.full((n + 1, heads, hd, hd), 7.0, np.float32))
+        assert need > 0
+        engine.linear_attn(push, x, x + 2 * heads * hd, x + 4 * heads * hd, dev.put(np.zeros(heads, np.float32)), dev.put(np.array(cu, np.int32)),
+                           None, None, out, new, ws, need)
+        assert (dev.get(out, (1002, heads, hd))[1000:] == NAN["fp16"]).all()
+        assert (dev.get(new, (n + 1, heads, hd, hd), np.float32)[n] == 7.0).all()
+        assert (dev.get(ws, need // 4 + 64, np.float32)[need // 4:] == 0).all()
+
+
+@pytest.mark.parametrize("four", [False, True])
+def test_a_pool_past_32_bits(engine, dev, device_arena, four):
+    """Pages whose offsets, in elements and in bytes, pass 2^32: written, read back and attended to as in a small pool."""
+    rng, dtype, hd, kv, heads, page, n = np.random.default_rng(16), "bf16", 128, 8, 16, 128, 300
+    pages = 2 ** 32 // (kv * page * hd) * (2 if four else 1) + 300  # elements, and in 4 bits also bytes
+    big = [device_arena(pages * kv * page * b, zero=False).ptr for b in ([hd // 2] * 2 + [hd // 32] * 2 if four else [2 * hd] * 2)]
+    big = P.CachePages(**dict(zip(("k", "v", "k_scales", "v_scales"), big)))
+    small = P.CachePages(**{name: device_arena(300 * kv * page * (hd // 32 if name[1:] else hd // 2 if four else 2 * hd)).ptr
+                            for name in (("k", "v", "k_scales", "v_scales") if four else ("k", "v"))})
+    rows = normal(rng, (n, heads + 2 * kv, hd), dtype)
+    x, row = dev.put(rows), (heads + 2 * kv) * hd
+    seq, at = dev.put(np.repeat([0, 1], n // 2).astype(np.int32)), dev.put(np.tile(np.arange(n // 2), 2).astype(np.int32))
+    pos, lengths = dev.put(np.arange(n, dtype=np.int32)), dev.put(np.array([n // 2, 140], np.int32))
+    print(f"[big pool] {pages} pages, four {four}", flush=True)
+    got = []
+    for count, pool in ((300, small), (pages, big)):
+        table = dev.put((count - 1 - np.array([[0, 7], [200, 3]])).astype(np.int32))
+        cache = P.CacheDesc(dtype=TYPES[dtype], n_kv_heads=kv, head_dim=hd, page_size=page, n_pages=count, n_seqs=2, table_pages=2)
+        push = P.RopeAppendPush(cache=cache, format=P.CACHE_4 if four else P.CACHE_16, n_new=n, n_heads=heads, n_axes=1,
+                                pairs=(64, 0, 0, 0), layout=0, ladder=0, base=10000.0, q_token_stride=row, q_head_stride=hd,
+                                k_token_stride=row, k_head_stride=hd, v_token_stride=row, v_head_stride=hd,
+                                out_token_stride=heads * hd, out_head_stride=hd, pos_stride=n)
+        q, k, v, o = (dev.put(np.full((n, heads, hd), NAN[dtype], np.uint16)) for _ in range(4))
+        engine.rope_append(push, x, x + 2 * heads * hd, x + 2 * (heads + kv) * hd, pos, q, seq, at, table, pool)
+        read = P.CacheReadPush(cache=cache, format=push.format, n_rows=n, k_token_stride=heads * hd, k_head_stride=hd,
+                               v_token_stride=heads * hd, v_head_stride=hd)
+        engine.cache_read(read, pool, seq, at, table, k, v)
+        parts = [dev.get(a, (n, heads, hd)) for a in (q, k, v)]
+        if four:
+            for group in (2, 1):
+                one = P.PagedAttnPush(cache=cache, n_heads=kv * group, left=-1, sinks=0, max_len=n // 2, scale=0.1,
+                                      q_seq_stride=heads * hd, q_head_stride=hd, out_seq_stride=heads * hd, out_head_stride=hd)
+                assert engine.paged_attn4_workspace(one) == 0
+                engine.paged_attn4(one, q, pool, table, lengths, o, None, 0)
+                parts.append(dev.get(o, (2, heads, hd))[:, :kv * group])
+        got.append(parts)
+    for a, b in zip(*got):
+        assert (a == b).all()
+    assert (got[0][1][:, :kv] != NAN[dtype]).any() and (got[0][1][:, kv:] == NAN[dtype]).all()
+
+
+def test_two_streams_at_once(hip, engine, dev):
+    """Calls on two streams, each with a workspace and outputs of its own: the bits of either alone."""
+    rng, dtype, hd, heads, n = np.random.default_rng(17), "bf16", 64, 4, 1200
+    rows = normal(rng, (n, 3 * heads, hd), dtype)
+    x, rates, cu = dev.put(rows), dev.put(np.array([0.0, 0.01, 0.1, 1.0], np.float32)), dev.put(np.array([0, 900, n], np.int32))
+    push = linear_push(dtype, 2, n, heads, heads, hd, 2, 0.125, 3 * heads * hd)
+    need = engine.linear_attn_workspace(push)
+    cache = Cache(rng, [2500, 60], 2, hd, 64, dtype, True)
+    for s, ln in enumerate((2500, 60)):
+        cache.fill(s, np.arange(ln), rng.standard_normal((ln, 2, hd)), rng.standard_normal((ln, 2, hd)))
+    pages, table, lengths, q = cache.put(dev), dev.put(cache.table), dev.put(np.array([2500, 60], np.int32)), dev.put(normal(rng, (2, 8, hd), dtype))
+    one = P.PagedAttnPush(cache=cache.desc(), n_heads=8, left=-1, sinks=0, max_len=2500, scale=0.125, q_seq_stride=8 * hd,
+                          q_head_stride=hd, out_seq_stride=8 * hd, out_head_stride=hd)
+    need4 = engine.paged_attn4_workspace(one)
+    assert need > 0 and need4 > 0
+    streams = [hip.stream(), hip.stream()]
+    mine = [dict(out=dev.put(np.zeros((n, heads, hd), np.uint16)), state=dev.put(np.zeros((2, heads, hd, hd), np.float32)), a=dev.put(np.zeros((2, 8, hd), np.uint16)),
+                 ws=dev.put(np.full(need // 4, np.nan, np.float32)), ws4=dev.put(np.full(need4 // 4, np.nan, np.float32))) for _ in range(3)]
+    hip.sync()
+
+    def calls(d, s):
+        engine.linear_attn(push, x, x + 2 * heads * hd, x + 4 * heads * hd, rates, cu, None, None, d["out"], d["state"], d["ws"], need, s)
+        engine.paged_attn4(one, q, pages, table, lengths, d["a"], d["ws4"], need4, s)
+
+    calls(mine[2], None)
+    hip.sync()
+    for _ in range(5):
+        for d, s in zip(mine, streams):
+            calls(d, s)
+    hip.sync()
+    for name, shape, t in (("out", (n, heads, hd), np.uint16), ("state", (2, heads, hd, hd), np.float32), ("a", (2, 8, hd), np.uint16)):
+        want = dev.get(mine[2][name], shape, t)
+        assert want.any() and all((dev.get(d[name], shape, t) == want).all() for d in mine[:2])
+
+
+def test_a_page_of_two_streams(engine, dev):
+    """A prompt's pages in two streams' tables: each attends as if they were its own."""
+    rng, dtype, hd, kv, page = np.random.default_rng(18), "fp16", 32, 2, 16
+    cache = Cache(rng, [48, 48], kv, hd, page, dtype, True)
+    for j in range(48):
+        k, v = rng.standard_normal((2, kv, hd))
+        cache.write(0, j, k, v)
+        cache.write(1, j, k, v)
+    q = np.repeat(normal(rng, (1, 4, hd), dtype), 2, 0)
+    apart = run_paged4(engine, dev, cache, q, [48, 48], -1, 0, 0.2, 48)
+    cache.table[1, :2] = cache.table[0, :2]
+    together = run_paged4(engine, dev, cache, q, [48, 48], -1, 0, 0.2, 48)
+    assert (apart == together).all() and (apart[0] == apart[1]).all() and np.isfinite(apart).all()

@@ -113,6 +113,59 @@ def test_entries_without_a_context():
     assert lib.prism_linear_attn_workspace(C.byref(linear())) >= 0
 
 
+def numbers(call, push, n):
+    out = (C.c_int64 * n)()
+    call(C.byref(push), out)
+    return list(out)
+
+
+@pytest.mark.parametrize("hd", [16, 32, 64, 128])
+def test_tokens_that_are_turned_together(rules, hd):
+    """Fit their tables in LDS, at any size, and are never none."""
+    most = rules.append_tile_channels() // hd
+    for n in (1, 255, 256, 8160, 10 ** 6, MAX):
+        for heads in (1, 3, 24, 65536 + 2 * 65536):
+            tile = rules.append_tile_of(C.c_int64(n), C.c_int64(heads), hd)
+            assert 1 <= tile <= most and tile & (tile - 1) == 0
+
+
+@pytest.mark.parametrize("hd", [16, 32, 64, 128])
+@pytest.mark.parametrize("kv,group", [(1, 1), (8, 1), (2, 3), (1, 65536), (8, 4)])
+def test_splits_of_a_long_cache(rules, hd, kv, group):
+    """All keys expected have a wave, whole tiles each; splits are what the joining launch has room for and an odd number."""
+    for n in (1, 5, 64, 8160):
+        for page, pages in ((1, 1), (16, 4), (16, 1000), (64, 3000), (4096, 2 ** 18)):
+            for max_len, left, sinks in ((0, -1, 0), (300, -1, 0), (5000, 0, 0), (0, MAX, MAX), (0, 700, 5), (MAX, -1, 0)):
+                p = P.PagedAttnPush(cache=cache(n_kv_heads=kv, head_dim=hd, page_size=page, n_pages=9, n_seqs=n, table_pages=pages),
+                                    n_heads=kv * group, left=left, sinks=sinks, max_len=max_len, scale=1.0)
+                many, tiles, waves, splits, grid, each, keys, space = numbers(rules.paged4_of, p, 8)
+                assert tiles * 16 >= group and waves in (1, 4) and 1 <= splits <= 95 and splits % 2 == 1
+                assert many or (group <= 2 and hd <= 32)
+                assert each % 64 == 0 and each > 0 and (4 * splits * each >= keys or each == 2 ** 30)
+                assert grid == (-(-n * kv * tiles // 4) if waves == 1 else n * kv * tiles * splits) and (waves == 4 or splits == 1)
+                assert space == (0 if splits == 1 else n * kv * group * splits * (hd + 2) * 4)
+
+
+@pytest.mark.parametrize("hd", [16, 32, 64, 128])
+@pytest.mark.parametrize("heads", [1, 5, 32])
+def test_segments_of_long_sequences(rules, hd, heads):
+    """Whole chunks, and a number for each of them whatever the lengths: sequence s has those from start / segment + s on."""
+    rng = np.random.default_rng(hd)
+    for n, tokens in ((1, 1), (1, 255), (1, 256), (1, 8160), (3, 1000), (9, 3), (64, 64000), (1, 2 ** 30), (511, 2 ** 20), (2, 0)):
+        p = linear(n_seqs=n, n_tokens=tokens, n_heads=heads, n_kv_heads=heads, head_dim=hd)
+        segment, split, segments, space = numbers(rules.linear_of, p, 4)
+        assert space == (segments * heads * hd * hd * 4 if split else 0)
+        if not split:
+            assert segments == n and segment == MAX
+            continue
+        assert segment % 64 == 0 and segment > 0
+        for _ in range(20):
+            cuts = np.sort(rng.integers(0, tokens + 1, n + 1))
+            first = cuts[:-1] // segment + np.arange(n)
+            last = first + np.maximum(np.diff(cuts) - 1, 0) // segment
+            assert last[-1] < segments and (last[:-1] < first[1:]).all()
+
+
 @pytest.mark.parametrize("dtype", ["fp16", "bf16"])
 def test_the_definition_of_a_block(dtype):
     """Against a search over all sixteen numbers; what fits comes back as it was."""
