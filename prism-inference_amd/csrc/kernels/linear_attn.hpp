@@ -132,6 +132,40 @@ __device__ __forceinline__ void linear_segment(const LinearAttnArgs& a) {
     if (STATES ? last && (seg == 0 || t0 >= lt.rows.end) : seg > 0 && t0 >= lt.rows.end) return;
     const int t1 = (int)min(t0 + a.segment, (int64_t)lt.rows.end);
 
+    /* The first chunk is asked for before anything else is waited for. A chunk's tokens lie at its end: a short one, the segment's last, has rows of zeros before them, so that decays up to
+       the end are always the same. Token strides are at most 2^22: 32-bit offsets from a base that is the same for all. */
+    v8 rq[STATES ? 1 : NL], rk[NL], rv[NL];
+    const int row0 = min(tid / CPR, C - 1), col0 = tid % CPR * 8;
+    const auto load = [&](const uint16_t* m, int64_t first, uint32_t stride, uint32_t offset, v8 (&r)[NL]) { /* bytes */
+#pragma unroll
+        for (int i = 0; i < NL; ++i)
+            r[i] = *reinterpret_cast<const v8*>(reinterpret_cast<const char*>(m) + first + (int64_t)(NT / CPR * i) * stride + offset);
+    };
+    const uint32_t sq = 2 * (uint32_t)a.q_token_stride, sk = 2 * (uint32_t)a.k_token_stride, sv = 2 * (uint32_t)a.v_token_stride;
+    const uint32_t oq = row0 * sq + 2 * col0, ok = row0 * sk + 2 * col0, ov = row0 * sv + 2 * col0;
+    const auto load_chunk = [&](int64_t first) { /* 64 tokens from there on */
+        if constexpr (!STATES) load(a.q + h * a.q_head_stride, first * sq, sq, oq, rq);
+        load(a.k + hk * a.k_head_stride, first * sk, sk, ok, rk);
+        load(a.v + hk * a.v_head_stride, first * sv, sv, ov, rv);
+    };
+    const auto no_keys = [&](int rows) { /* the first ones are not the chunk's */
+#pragma unroll
+        for (int i = 0; i < NL; ++i)
+            if (row0 + NT / CPR * i < rows) rk[i] = rv[i] = v8{};
+    };
+    const int len = t1 > t0 && !(STATES && last) ? t1 - (int)t0 : 0;
+    if (len >= C) {
+        load_chunk(t0);
+    } else if (len > 0) { /* nothing before it is the segment's, or need exist */
+#pragma unroll
+        for (int i = 0; i < NL; ++i) {
+            const int64_t t = t0 + max(row0 + NT / CPR * i - (C - len), 0);
+            if constexpr (!STATES) rq[i] = ld8<T>(a.q + t * a.q_token_stride + h * a.q_head_stride + col0);
+            rk[i] = ld8<T>(a.k + t * a.k_token_stride + hk * a.k_head_stride + col0);
+            rv[i] = ld8<T>(a.v + t * a.v_token_stride + hk * a.v_head_stride + col0);
+        }
+    }
+
     const float r2 = linear_rate(a, h);
     const auto decay = [&](int n) { return fast_exp2(-r2 * (float)n); };
     const float d1 = decay(1), d2 = decay(2), d3 = decay(3);
@@ -156,7 +190,7 @@ __device__ __forceinline__ void linear_segment(const LinearAttnArgs& a) {
             for (int j = 0; j < DK * DV; ++j) S[j / DV][j % DV] = copy[64 * WD * j];
         }
     if constexpr (!STATES) {
-        constexpr int DEPTH = DK * DV < 8 ? 16 / (DK * DV) : 2; /* segments asked for at once */
+        constexpr int DEPTH = DK <= 2 ? 16 : DK <= 4 ? 4 : 2; /* segments asked for at once */
         const float keep = decay(a.segment);
         for (int s = seg; s > 0; s -= DEPTH) {
             f4 u[DEPTH][DK * DV];
@@ -196,40 +230,7 @@ __device__ __forceinline__ void linear_segment(const LinearAttnArgs& a) {
         f.h[1] = lds_tr4(at + 16 * RS);
         return f.v;
     };
-    /* A chunk's tokens lie at its end: a short one, the segment's last, has rows of zeros before them, so that decays up to
-       the end are always the same. Token strides are at most 2^22: 32-bit offsets from a base that is the same for all. */
-    v8 rq[STATES ? 1 : NL], rk[NL], rv[NL];
-    const int row0 = min(tid / CPR, C - 1), col0 = tid % CPR * 8;
-    const auto load = [&](const uint16_t* m, int64_t first, uint32_t stride, uint32_t offset, v8 (&r)[NL]) { /* bytes */
-#pragma unroll
-        for (int i = 0; i < NL; ++i)
-            r[i] = *reinterpret_cast<const v8*>(reinterpret_cast<const char*>(m) + first + (int64_t)(NT / CPR * i) * stride + offset);
-    };
-    const uint32_t sq = 2 * (uint32_t)a.q_token_stride, sk = 2 * (uint32_t)a.k_token_stride, sv = 2 * (uint32_t)a.v_token_stride;
-    const uint32_t oq = row0 * sq + 2 * col0, ok = row0 * sk + 2 * col0, ov = row0 * sv + 2 * col0;
-    const auto load_chunk = [&](int64_t first) { /* 64 tokens from there on */
-        if constexpr (!STATES) load(a.q + h * a.q_head_stride, first * sq, sq, oq, rq);
-        load(a.k + hk * a.k_head_stride, first * sk, sk, ok, rk);
-        load(a.v + hk * a.v_head_stride, first * sv, sv, ov, rv);
-    };
-    const auto no_keys = [&](int rows) { /* the first ones are not the chunk's */
-#pragma unroll
-        for (int i = 0; i < NL; ++i)
-            if (row0 + NT / CPR * i < rows) rk[i] = rv[i] = v8{};
-    };
-    const int len = t1 > t0 && !(STATES && last) ? t1 - (int)t0 : 0;
-    if (len >= C) {
-        load_chunk(t0);
-    } else if (len > 0) { /* nothing before it is the segment's, or need exist */
-#pragma unroll
-        for (int i = 0; i < NL; ++i) {
-            const int64_t t = t0 + max(row0 + NT / CPR * i - (C - len), 0);
-            if constexpr (!STATES) rq[i] = ld8<T>(a.q + t * a.q_token_stride + h * a.q_head_stride + col0);
-            rk[i] = ld8<T>(a.k + t * a.k_token_stride + hk * a.k_head_stride + col0);
-            rv[i] = ld8<T>(a.v + t * a.v_token_stride + hk * a.v_head_stride + col0);
-        }
-        no_keys(C - len);
-    }
+    if (len < C) no_keys(C - len);
     for (int c0 = 0; c0 < len; c0 += C) {
         const int n = min(C, len - c0), skip = C - n, turn = c0 / C & 1;
         __syncthreads(); /* the chunk before has been read */
