@@ -93,7 +93,12 @@ __device__ __forceinline__ bool infinite(uint32_t most) { /* bits of magnitudes,
     return (most & 0xFFFF) >= inf || most >> 16 >= inf;
 }
 
-/* One segment of one head: its chunks of 64 tokens in turn,
+/* What bounds it. Few short sequences: a chain of launch, starts, tokens and products; 9 up to 130, 8 x 16, 8 us. 8,160 tokens,
+ * 8 x 32: 16 us behind 5 for the segments' states, of which each chunk is 1 and the rest latency. 5 sequences of 22,400 tokens, 32 x 128:
+ * 212 us behind 87 (805 MB: 3.8 TB/s); matrix cores 30 %, vector units 39 % busy. Without any product the kernel still takes 0.8 of
+ * that: loads, staging in LDS, barriers and stores, with two workgroups a CU (256 registers, 67 KB of LDS).
+ *
+ * One segment of one head: its chunks of 64 tokens in turn,
  *   o_i = scale (e^(-r (i+1)) q_i S + sum_{j <= i} e^(-r (i-j)) (q_i k_j) v_j),  S' = e^(-r n) S + sum_j k_j^T e^(-r (n-1-j)) v_j
  * A wave has 16 channels of the values, so its part of the state is its own and stays in registers: 16 x 16 tiles as the
  * product leaves them, which are at the same time what the next chunk's product q S takes.
