@@ -94,7 +94,7 @@ __device__ __forceinline__ bool infinite(uint32_t most) { /* bits of magnitudes,
 }
 
 /* What bounds it. Few short sequences: a chain of launch, starts, tokens and products; 9 up to 130, 8 x 16, 8 us. 8,160 tokens,
- * 8 x 32: 16 us behind 5 for the segments' states, of which each chunk is 1 and the rest latency. 5 sequences of 22,400 tokens, 32 x 128:
+ * 8 x 32: 16 us behind 5 for the segments' states, of which each chunk is 1 and the rest latency. 23,000 tokens of 5 sequences, 32 x 128:
  * 212 us behind 87 (805 MB: 3.8 TB/s); matrix cores 30 %, vector units 39 % busy. Without any product the kernel still takes 0.8 of
  * that: loads, staging in LDS, barriers and stores, with two workgroups a CU (256 registers, 67 KB of LDS).
  *
