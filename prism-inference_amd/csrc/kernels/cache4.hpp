@@ -99,31 +99,6 @@ __device__ __forceinline__ void rope_append_body(const RopeAppendArgs& a) {
     const int n = a.n_pairs, lane = lane_id();
     const int64_t t0 = (int64_t)blockIdx.x * a.tile;
     const int tokens = min(a.tile, (int)(a.n_new - t0));
-    const auto axis_of = [&](int j) { return (j >= a.axis_end[0]) + (j >= a.axis_end[1]) + (j >= a.axis_end[2]); };
-    if (threadIdx.x < n) {
-        const int j = threadIdx.x, axis = axis_of(j), first = axis ? a.axis_end[axis - 1] : 0;
-        const double e = a.one_ladder ? (double)j / n : (double)(j - first) / (a.axis_end[axis] - first);
-        turns[j] = a.turn * exp2(-e * a.log2_base);
-    }
-    if (a.n_kv_heads > 0 && threadIdx.x < tokens)
-        slots[threadIdx.x] = cache_slot(a, a.seq_of[t0 + threadIdx.x], a.pos_of[t0 + threadIdx.x]);
-    __syncthreads();
-    for (int i = threadIdx.x; i < tokens * n; i += 256) {
-        const int t = i / n, j = i - t * n;
-        const double rev = (double)a.pos[axis_of(j) * a.pos_stride + t0 + t] * turns[j];
-        double s, c;
-        sincospi(2.0 * (rev - rint(rev)), &s, &c);
-        const int c1 = a.adjacent ? 2 * j : j, c2 = a.adjacent ? c1 + 1 : j + n;
-        const int i1 = t * HD + c1 % 8 * CH + c1 / 8, i2 = t * HD + c2 % 8 * CH + c2 / 8;
-        cs[i1] = float2{(float)c, -(float)s};
-        cs[i2] = float2{(float)c, (float)s};
-        if constexpr (FOUR) {
-            cs64[i1] = double2{c, -s};
-            cs64[i2] = double2{c, s};
-        }
-    }
-    __syncthreads();
-
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int H = a.n_heads, K = a.n_kv_heads;
     const int nq = (tokens * H * CH + 63) / 64, nk = (tokens * K * CH + 63) / 64;
@@ -163,6 +138,36 @@ __device__ __forceinline__ void rope_append_body(const RopeAppendArgs& a) {
         if (row >= rows) u.t = -1; /* past the end: read, not written */
         return u;
     };
+    /* The first rows are asked for before the angles. In place, a row's lanes, which are in one wave, have all read before
+       one writes. */
+    Unit u[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) u[i] = load(wave + 4 * i);
+    const auto axis_of = [&](int j) { return (j >= a.axis_end[0]) + (j >= a.axis_end[1]) + (j >= a.axis_end[2]); };
+    if (threadIdx.x < n) {
+        const int j = threadIdx.x, axis = axis_of(j), first = axis ? a.axis_end[axis - 1] : 0;
+        const double e = a.one_ladder ? (double)j / n : (double)(j - first) / (a.axis_end[axis] - first);
+        turns[j] = a.turn * exp2(-e * a.log2_base);
+    }
+    if (a.n_kv_heads > 0 && threadIdx.x < tokens)
+        slots[threadIdx.x] = cache_slot(a, a.seq_of[t0 + threadIdx.x], a.pos_of[t0 + threadIdx.x]);
+    __syncthreads();
+    for (int i = threadIdx.x; i < tokens * n; i += 256) {
+        const int t = i / n, j = i - t * n;
+        const double rev = (double)a.pos[axis_of(j) * a.pos_stride + t0 + t] * turns[j];
+        double s, c;
+        sincospi(2.0 * (rev - rint(rev)), &s, &c);
+        const int c1 = a.adjacent ? 2 * j : j, c2 = a.adjacent ? c1 + 1 : j + n;
+        const int i1 = t * HD + c1 % 8 * CH + c1 / 8, i2 = t * HD + c2 % 8 * CH + c2 / 8;
+        cs[i1] = float2{(float)c, -(float)s};
+        cs[i2] = float2{(float)c, (float)s};
+        if constexpr (FOUR) {
+            cs64[i1] = double2{c, -s};
+            cs64[i2] = double2{c, s};
+        }
+    }
+    __syncthreads();
+
     const auto keep = [&](const Unit& u, const float (&y)[8], v8 o) { /* into the cache; a block's lanes are all here */
         uint8_t* pages = u.kind == 1 ? a.k_pages : a.v_pages;
         const int64_t slot = slots[max(u.t, 0)], at = slot + ((int64_t)u.h << a.page_log2);
@@ -231,15 +236,14 @@ __device__ __forceinline__ void rope_append_body(const RopeAppendArgs& a) {
             keep(u, y, u.x);
         }
     };
-    for (int w = wave; w < nq + 2 * nk; w += 4 * U) {
-        Unit u[U];
-#pragma unroll
-        for (int i = 0; i < U; ++i) u[i] = load(w + 4 * i);
-        /* in place, a row's lanes, which are in one wave, have all read before one writes */
+    for (int w = wave; w < nq + 2 * nk;) {
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
         for (int i = 0; i < U; ++i) work(u[i]);
+        w += 4 * U;
+#pragma unroll
+        for (int i = 0; i < U; ++i) u[i] = load(w + 4 * i);
     }
 }
 
