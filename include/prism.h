@@ -560,7 +560,8 @@ typedef struct prism_seq_attn_push {
 int prism_seq_attn(prism_ctx* ctx, const prism_seq_attn_push* p, const void* q, const void* k, const void* v,
                    const int32_t* cu_q, const int32_t* cu_k, void* out, void* stream);
 
-/* ---- a cheaper past: a cache in 4 bits, and states of fixed size ---- */
+/* ---- a cheaper past: a cache in 4 bits, and states of fixed size ----
+ * Strides, alignment, streams, workspaces and what outputs may overlap as in the sequence operators above. */
 
 /* Format of a paged cache. PRISM_CACHE_16: values of the cache's dtype, as
  * above. PRISM_CACHE_4: a block of 32 channels of a head (16 where head_dim is
