@@ -58,11 +58,20 @@ __device__ __forceinline__ bool paged4_work(const PagedAttnArgs& a, int wave, Pa
     return true;
 }
 
-/* Where key i of those that the wave sees lies: its slot's number in [page][head][slot], -1 if there is none. */
-__device__ __forceinline__ int64_t paged4_slot(const PagedAttnArgs& a, const PagedWork& w, int i) {
-    if (i >= w.i1) return -1;
-    const int j = w.key(i), page = paged_page(a, w, j);
-    return page < 0 ? -1 : paged_at<1>(a, w, page, j);
+/* Key i of those that the wave sees, of which there are some: its table entry, past the end the last one's. A load for every lane, and
+ * nothing that waits for it: the entries of several keys are asked for together. */
+__device__ __forceinline__ int paged4_entry(const PagedAttnArgs& a, const PagedWork& w, int i) {
+    return a.table[(int64_t)w.seq * a.table_pages + (w.key(min(i, w.i1 - 1)) >> a.page_log2)];
+}
+/* ... and where it lies, its slot's number in [page][head][slot]; a slot of the first page if it is not seen. */
+struct Paged4Key {
+    int64_t at;
+    bool seen;
+};
+__device__ __forceinline__ Paged4Key paged4_key(const PagedAttnArgs& a, const PagedWork& w, int i, int entry) {
+    const bool seen = i < w.i1 && page_ok(entry, a.n_pages);
+    const int slot = w.key(min(i, w.i1 - 1)) & ((1 << a.page_log2) - 1);
+    return Paged4Key{(int64_t)((((uint64_t)(uint32_t)(seen ? entry : 0) * (uint32_t)a.n_kv_heads + (uint32_t)w.hk) << a.page_log2) + (uint32_t)slot), seen};
 }
 
 template <class T, int HD, int G>
@@ -91,26 +100,26 @@ __device__ __forceinline__ void paged4_few(const PagedAttnArgs& a) {
     }
     const auto steps = [&](auto count, int i) {
         constexpr int U = decltype(count)::value;
-        int64_t at[U];
+        int entry[U];
         uint32_t k[U][W], v[U][W];
-        float ks[U], vs[U];
+        uint8_t ks[U], vs[U];
         bool ok[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) at[u] = paged4_slot(a, w, i + u * KPS + slot);
+        for (int u = 0; u < U; ++u) entry[u] = paged4_entry(a, w, i + u * KPS + slot);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            ok[u] = at[u] >= 0;
-            const int64_t x = ok[u] ? at[u] : 0;
-            __builtin_memcpy(k[u], kp + x * (HD / 2) + ch / 2, 4 * W);
-            __builtin_memcpy(v[u], vp + x * (HD / 2) + ch / 2, 4 * W);
-            ks[u] = fp4_scale(a.k_scales[x]);
-            vs[u] = fp4_scale(a.v_scales[x]);
+            const Paged4Key key = paged4_key(a, w, i + u * KPS + slot, entry[u]);
+            ok[u] = key.seen;
+            __builtin_memcpy(k[u], kp + key.at * (HD / 2) + ch / 2, 4 * W);
+            __builtin_memcpy(v[u], vp + key.at * (HD / 2) + ch / 2, 4 * W);
+            ks[u] = a.k_scales[key.at];
+            vs[u] = a.v_scales[key.at];
         }
         v8 kk[U][W];
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int x = 0; x < W; ++x) kk[u][x] = fp4_values<T>(k[u][x], ks[u]);
+            for (int x = 0; x < W; ++x) kk[u][x] = fp4_values<T>(k[u][x], fp4_scale(ks[u]));
         float s[G][U];
 #pragma unroll
         for (int h = 0; h < G; ++h) {
@@ -143,7 +152,7 @@ __device__ __forceinline__ void paged4_few(const PagedAttnArgs& a) {
                 const uint32_t word = ok[u] ? v[u][x] : 0; /* zeros, not what may be NaN */
                 const auto two = [&](auto byte) {
                     constexpr int B = decltype(byte)::value;
-                    const f2 y = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(word, ok[u] ? vs[u] : 1.f, B);
+                    const f2 y = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(word, ok[u] ? fp4_scale(vs[u]) : 1.f, B);
 #pragma unroll
                     for (int h = 0; h < G; ++h) {
                         acc[h][8 * x + 2 * B] = __builtin_fmaf(y[0], s[h][u], acc[h][8 * x + 2 * B]);
@@ -156,9 +165,9 @@ __device__ __forceinline__ void paged4_few(const PagedAttnArgs& a) {
                 two(Count<3>{});
             }
     };
-    for (int i = w.i0; i < w.i1; i += KPS * U)
-        if (w.i1 - i > KPS) steps(Count<U>{}, i);
-        else steps(Count<1>{}, i);
+    int i = w.i0;
+    for (; w.i1 - i > KPS; i += KPS * U) steps(Count<U>{}, i);
+    if (i < w.i1) steps(Count<1>{}, i);
     /* The wave's 32 key slots together, halving what a lane holds: each step pairs lanes that differ in one bit, and one
        takes the sum of one half of the channels, the other of the other. In the end lane bits 5, 4, 3 (and 2) name a
        channel, bit 0 the lane's half of the row. */
@@ -256,13 +265,15 @@ __device__ __forceinline__ void paged4_many(const PagedAttnArgs& a) {
     f4 o[DT] = {};
     float m = -INFINITY, mu = 0.f, l = 0.f;
 
-    int64_t slot = paged4_slot(a, w, w.i0 + (lane & (KEYS - 1))); /* a lane's key of the step */
+    const int key = lane & (KEYS - 1); /* a lane's of the step */
+    int entry = w.i0 < w.i1 ? paged4_entry(a, w, w.i0 + key) : -1;
     for (int i = w.i0; i < w.i1; i += KEYS) {
-        const uint64_t seen = __ballot(slot >= 0);
+        const Paged4Key own = paged4_key(a, w, i + key, entry);
+        const uint64_t seen = __ballot(own.seen);
         /* every lane's own keys, l16 of each tile */
         int64_t at[KT];
         {
-            const int64_t x = slot < 0 ? 0 : slot;
+            const int64_t x = own.at;
             int lo[2], hi[2];
             lanes_x16((int)x, lo[0], lo[1]);
             lanes_x16((int)(x >> 32), hi[0], hi[1]);
@@ -291,7 +302,7 @@ __device__ __forceinline__ void paged4_many(const PagedAttnArgs& a) {
             __builtin_memcpy(v[t], __builtin_assume_aligned(vp + at[t] * (HD / 2), QUARTER / 2), QUARTER / 2);
             vsc[t] = vx[at[t] * BL];
         }
-        slot = paged4_slot(a, w, i + KEYS + (lane & (KEYS - 1)));
+        entry = paged4_entry(a, w, i + KEYS + key);
 
         f4 s[KT] = {};
 #pragma unroll
