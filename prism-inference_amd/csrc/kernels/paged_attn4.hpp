@@ -61,7 +61,9 @@ __device__ __forceinline__ bool paged4_work(const PagedAttnArgs& a, int wave, Pa
 /* Key i of those that the wave sees, of which there are some: its table entry, past the end the last one's. A load for every lane, and
  * nothing that waits for it: the entries of several keys are asked for together. */
 __device__ __forceinline__ int paged4_entry(const PagedAttnArgs& a, const PagedWork& w, int i) {
-    return a.table[(int64_t)w.seq * a.table_pages + (w.key(min(i, w.i1 - 1)) >> a.page_log2)];
+    const int32_t* row = a.table + (int64_t)w.seq * a.table_pages; /* of 2^30 entries at most: 32-bit offsets */
+    const uint32_t page = (uint32_t)w.key(min(i, w.i1 - 1)) >> a.page_log2;
+    return *reinterpret_cast<const int32_t*>(reinterpret_cast<const char*>(row) + 4 * page);
 }
 /* ... and where it lies, its slot's number in [page][head][slot]; a slot of the first page if it is not seen. */
 struct Paged4Key {
@@ -98,6 +100,8 @@ __device__ __forceinline__ void paged4_few(const PagedAttnArgs& a) {
         m[h] = -INFINITY;
         l[h] = 0.f;
     }
+    const auto add = [](float x, float y) { return x + y; };
+    const auto most = [](float x, float y) { return vmax(x, y); };
     const auto steps = [&](auto count, int i) {
         constexpr int U = decltype(count)::value;
         int entry[U];
@@ -123,7 +127,7 @@ __device__ __forceinline__ void paged4_few(const PagedAttnArgs& a) {
         float s[G][U];
 #pragma unroll
         for (int h = 0; h < G; ++h) {
-            float top = m[h];
+            float top = -INFINITY;
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 float d = 0.f;
@@ -131,25 +135,30 @@ __device__ __forceinline__ void paged4_few(const PagedAttnArgs& a) {
                 for (int x = 0; x < W; ++x) d = dot8(q[h][x], kk[u][x], d);
                 if constexpr (LPK == 2) d = lanes_sum<2>(d);
                 s[h][u] = ok[u] ? d * a.scale_log2 : -INFINITY;
-                top = fmaxf(top, s[h][u]);
+                top = vmax(top, s[h][u]);
             }
-            const float mu = top == -INFINITY ? 0.f : top;
-            const float f = fast_exp2(m[h] - mu);
-            l[h] *= f;
+            top = across<LPK>(top, most);
+            if (__builtin_amdgcn_readfirstlane(top > m[h])) { /* the same for all lanes; not where a score is NaN: weights are then */
+                if (i > w.i0) {
+                    const float f = fast_exp2(m[h] - top);
+                    l[h] *= f;
 #pragma unroll
-            for (int e = 0; e < CH; ++e) acc[h][e] *= f;
+                    for (int e = 0; e < CH; ++e) acc[h][e] *= f;
+                }
+                m[h] = top;
+            }
+            const float mu = m[h] == -INFINITY ? 0.f : m[h];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 s[h][u] = fast_exp2(s[h][u] - mu);
                 l[h] += s[h][u];
             }
-            m[h] = top;
         }
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int x = 0; x < W; ++x) {
-                const uint32_t word = ok[u] ? v[u][x] : 0; /* zeros, not what may be NaN */
+                const uint32_t word = v[u][x];
                 const auto two = [&](auto byte) {
                     constexpr int B = decltype(byte)::value;
                     const f2 y = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(word, ok[u] ? fp4_scale(vs[u]) : 1.f, B);
@@ -172,19 +181,12 @@ __device__ __forceinline__ void paged4_few(const PagedAttnArgs& a) {
        takes the sum of one half of the channels, the other of the other. In the end lane bits 5, 4, 3 (and 2) name a
        channel, bit 0 the lane's half of the row. */
     static_assert(LPK == 2, "lane bit 0: channels; 1 to 5: keys");
-    const auto add = [](float x, float y) { return x + y; };
-    const auto most = [](float x, float y) { return fmaxf(x, y); };
     const bool b3 = lane & 8, b2 = lane & 4;
     const int mine = (lane >> 5 & 1) * (CH / 2) + (lane >> 4 & 1) * (CH / 4) + (lane >> 3 & 1) * (CH / 8) + (CH == 16 ? lane >> 2 & 1 : 0);
 #pragma unroll
     for (int h = 0; h < G; ++h) {
-        const float top = across<LPK>(m[h], most);
-        const float f = m[h] == -INFINITY ? 0.f : fast_exp2(m[h] - top);
-        l[h] = across<LPK>(l[h] * f, add);
-        m[h] = top;
+        l[h] = across<LPK>(l[h], add);
         float (&x)[CH] = acc[h];
-#pragma unroll
-        for (int e = 0; e < CH; ++e) x[e] *= f;
 #pragma unroll
         for (int e = 0; e < CH / 2; ++e) {
             const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, x[e]), __builtin_bit_cast(unsigned, x[e + CH / 2]), false, false);
