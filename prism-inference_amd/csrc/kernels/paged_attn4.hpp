@@ -10,9 +10,9 @@
  *                same order. V goes through a wave's own LDS, as 16-bit numbers, for transposed reads.
  *
  * A key and a value are 17/16 of a byte a channel, a quarter of 16-bit ones, so that the vector units come close to memory:
- *   paged4_few   8,160 streams of 52 keys, 8 x 32: 40 us for 117 MB, vector units 83 to 95 % busy with 330 instructions a wave (of 20 keys 31 us: most
- *                is a wave's beginning and end). A maximum for the whole wave instead of one a lane took as long.
- *   paged4_many  24 streams of 1,000 to 20,001, 32 over 8 x 128: 68 us for 276 MB (4.1 TB/s), its loads alone 53; one of 131,075: 36 for 143 MB.
+ *   paged4_few   8,160 streams of 52 keys, 8 x 32: 31 us for 117 MB, vector units 96 % busy. One maximum for the wave: 40 us with one a lane,
+ *                whose sums are scaled once more at the end.
+ *   paged4_many  24 streams of 1,000 to 20,001, 32 over 8 x 128: 64 us for 276 MB (4.3 TB/s), its loads alone 53; one of 131,075: 34 for 143 MB.
  *                Keys through LDS in whole lines, and the next step's asked for ahead of the softmax, were slower or equal.
  */
 #pragma once
