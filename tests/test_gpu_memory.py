@@ -875,3 +875,21 @@ def test_a_page_of_two_streams(engine, dev):
     cache.table[1, :2] = cache.table[0, :2]
     together = run_paged4(engine, dev, cache, q, [48, 48], -1, 0, 0.2, 48)
     assert (apart == together).all() and (apart[0] == apart[1]).all() and np.isfinite(apart).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hd,group", [(16, 1), (16, 2), (32, 1), (32, 2), (64, 1), (128, 4)])
+@pytest.mark.parametrize("at", [0, 20, 69, 70])
+def test_paged4_a_key_of_nan_reaches_its_head_alone(engine, dev, dtype, hd, group, at):
+    """A key of NaN makes NaN of the heads that share it, in the stream that sees it (70 keys); one behind the last is not seen."""
+    rng = np.random.default_rng(19)
+    kv, page, lengths = 2, 16, [71, 70, 71]
+    cache = Cache(rng, lengths, kv, hd, page, dtype, True)
+    for s, n in enumerate(lengths):
+        cache.fill(s, np.arange(n), rng.standard_normal((n, kv, hd)), rng.standard_normal((n, kv, hd)))
+    p, slot = cache.place(1, at)
+    cache.ks[p, 0, slot, 0] = 255
+    got = run_paged4(engine, dev, cache, normal(rng, (3, kv * group, hd), dtype), lengths, -1, 0, 0.2, 71)
+    bad = np.zeros(got.shape, bool)
+    bad[1, :group] = at < 70
+    assert (np.isnan(got) == bad).all()
