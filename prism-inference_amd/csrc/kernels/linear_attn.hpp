@@ -54,6 +54,21 @@ __device__ __forceinline__ void parts(float x, float y, uint32_t (&p)[N]) {
         }
     }
 }
+/* 8 values as numbers of bf16 that add up to them, exactly: fp16's 11 bits are two. Products of fp16 with what is not fp16 (weights, which
+ * differ by more than fp16's powers of two beside each other) are taken in bf16, whose powers are fp32's. */
+__device__ __forceinline__ void numbers(b8 v, b8 (&n)[1]) { n[0] = v; }
+__device__ __forceinline__ void numbers(h8 v, b8 (&n)[2]) {
+    u4 w[2];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        uint32_t p[2];
+        parts<BF16, 2>((float)v[2 * e], (float)v[2 * e + 1], p);
+        w[0][e] = p[0];
+        w[1][e] = p[1];
+    }
+    n[0] = __builtin_bit_cast(b8, w[0]);
+    n[1] = __builtin_bit_cast(b8, w[1]);
+}
 /* 2^k that brings the largest magnitude m (of fp16 parts' numbers) to 2^13 .. 2^14; 1 for 0; k from -120 to 60 */
 __device__ __forceinline__ float part_scale(float m) {
     const int e = (int)(__builtin_bit_cast(unsigned, m) >> 23); /* m >= 0 */
@@ -72,20 +87,6 @@ template <class V>
 __device__ __forceinline__ uint32_t most8(V v) {
     const u4 w = __builtin_bit_cast(u4, v) & 0x7FFF7FFFu;
     return most2(most2(w[0], w[1]), most2(w[2], w[3]));
-}
-/* ... over the wave */
-__device__ __forceinline__ uint32_t most_of_wave(uint32_t v) {
-    const auto with = [&](auto control) {
-        v = most2(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, decltype(control)::value, 0xf, 0xf, false));
-    };
-    with(Count<0xB1>{});  /* neighbours, pairs, fours, eights: as group_sum */
-    with(Count<0x4E>{});
-    with(Count<0x140>{});
-    with(Count<0x141>{});
-    int a, b;
-    lanes_x16((int)v, a, b);
-    lanes_x32((int)most2(a, b), a, b);
-    return most2(a, b);
 }
 template <class T>
 __device__ __forceinline__ bool infinite(uint32_t most) { /* bits of magnitudes, two of them */
@@ -111,6 +112,7 @@ __device__ __forceinline__ void linear_segment(const LinearAttnArgs& a) {
     typedef typename T::v4 v4;
     typedef typename T::el el;
     constexpr bool HALF = __is_same(T, F16);
+    constexpr int IN = HALF ? 2 : 1; /* numbers of bf16 that an input is */
     constexpr int C = LINEAR_CHUNK, QT = C / 16, M = C / 32;
     constexpr int DV = HD >= 128 ? 2 : 1;          /* a wave's 16-channel tiles of the values */
     constexpr int WD = HD / 16 / DV, WQ = STATES || HD >= 64 ? 1 : QT / WD, QN = QT / WQ; /* waves by channels, by query tiles; a wave's */
@@ -125,7 +127,7 @@ __device__ __forceinline__ void linear_segment(const LinearAttnArgs& a) {
     constexpr int TILES = QT * (QT + 1) / 2;       /* of weights */
     __shared__ __attribute__((aligned(16))) uint16_t lq[STATES ? 8 : C * RS], lk[C * RS], lv[C * RS];
     __shared__ __attribute__((aligned(16))) uint16_t lw[!STATES && SHARED ? 6 * 2 * 64 * 8 : 8]; /* weights [query tile, 32 keys][part] */
-    __shared__ __attribute__((aligned(16))) uint32_t lmost[2][2 * WD * WQ]; /* of a chunk, by waves: fp16's largest query and key; an infinite value */
+    __shared__ uint32_t lbad[2][WD * WQ]; /* of a chunk, by waves: a value that is not finite */
     const int lane = lane_id(), l16 = lane & 15, g = lane >> 4, tid = threadIdx.x;
     const int wave = NT == 64 ? 0 : __builtin_amdgcn_readfirstlane(tid >> 6), wd = wave % WD, wq = wave / WD;
     const int b = blockIdx.x / a.n_heads, h = blockIdx.x % a.n_heads, hk = h / (a.n_heads / a.n_kv_heads);
@@ -239,7 +241,7 @@ __device__ __forceinline__ void linear_segment(const LinearAttnArgs& a) {
     for (int c0 = 0; c0 < len; c0 += C) {
         const int n = min(C, len - c0), skip = C - n, turn = c0 / C & 1;
         __syncthreads(); /* the chunk before has been read */
-        uint32_t mq = 0, mk = 0, mv = 0;
+        uint32_t mv = 0;
 #pragma unroll
         for (int i = 0; i < NL; ++i) {
             const int id = tid + NT * i, row = id / CPR, c = id % CPR * 8;
@@ -247,8 +249,6 @@ __device__ __forceinline__ void linear_segment(const LinearAttnArgs& a) {
             if constexpr (!STATES) {
                 *reinterpret_cast<v4*>(lq + row * RS + spot(c)) = v4{rq[i][0], rq[i][1], rq[i][2], rq[i][3]};
                 *reinterpret_cast<v4*>(lq + row * RS + spot(c + 4)) = v4{rq[i][4], rq[i][5], rq[i][6], rq[i][7]};
-                if (HALF) mq = most2(mq, most8(rq[i]));
-                if (HALF) mk = most2(mk, most8(rk[i]));
                 mv = most2(mv, most8(rv[i]));
             }
             *reinterpret_cast<v4*>(lk + row * RS + spot(c)) = v4{rk[i][0], rk[i][1], rk[i][2], rk[i][3]};
@@ -257,24 +257,7 @@ __device__ __forceinline__ void linear_segment(const LinearAttnArgs& a) {
         }
         if constexpr (!STATES) {
             const bool bad = __any(infinite<T>(mv));
-            uint32_t mqk = 0;
-            if constexpr (HALF) {
-                if (infinite<T>(mq) || infinite<T>(mk)) { /* the largest of the finite ones */
-                    mq = mk = 0;
-                    for (int i = 0; i < NL; ++i)
-                        for (int e = 0; e < 8; ++e) {
-                            const float x = __builtin_fabsf((float)rq[i][e]), y = __builtin_fabsf((float)rk[i][e]);
-                            if (x < INFINITY) mq = most2(mq, __builtin_bit_cast(uint16_t, (f16)x));
-                            if (y < INFINITY) mk = most2(mk, __builtin_bit_cast(uint16_t, (f16)y));
-                        }
-                }
-                mqk = most2(mq & 0xFFFF, mq >> 16) | most2(mk & 0xFFFF, mk >> 16) << 16;
-                mqk = most_of_wave(mqk);
-            }
-            if (lane == 0) {
-                lmost[turn][wave] = mqk;
-                lmost[turn][WD * WQ + wave] = bad;
-            }
+            if (lane == 0) lbad[turn][wave] = bad;
         }
         __syncthreads();
 
@@ -291,38 +274,28 @@ __device__ __forceinline__ void linear_segment(const LinearAttnArgs& a) {
                 for (int m = 0; m < M; ++m) v[d][m] = transposed(lv, 32 * m, 16 * DV * wd + channel(d, 4 * (l16 & 3)));
         };
         if constexpr (!STATES) {
-            /* fp16 weights are scaled by a power of two, after the largest that they could be: 2^15 stays above them, and
-               from there down their two parts have 40 bits */
-            float up = 1.f;
             uint32_t bad = 0;
 #pragma unroll
-            for (int i = 0; i < WD * WQ; ++i) bad |= lmost[turn][WD * WQ + i];
-            if constexpr (HALF) {
-                uint32_t m = 0;
-#pragma unroll
-                for (int i = 0; i < WD * WQ; ++i) m = most2(m, lmost[turn][i]);
-                const h2 qk = __builtin_bit_cast(h2, m);
-                up = part_scale((float)qk[0] * (float)qk[1] * (float)HD * __builtin_fabsf(a.scale));
-            }
-            /* weights of 16 queries and 16 keys: lane l16 is a query, with keys 4 g + e; in two parts */
+            for (int i = 0; i < WD * WQ; ++i) bad |= lbad[turn][i];
+            /* weights of 16 queries and 16 keys: lane l16 is a query, with keys 4 g + e; as two numbers of bf16 */
             const auto weigh = [&](int qt, int kt, uint32_t (&hi)[2], uint32_t (&lo)[2]) {
                 f4 w = {};
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks) w = mfma_16x16x32(row_of(lk, 16 * kt + l16, ks), row_of(lq, 16 * qt + l16, ks), w);
                 const int gap = 16 * (qt - kt) + l16 - 4 * g;
                 if (kt < qt) { /* gap is 4 or more */
-                    const float far = decay(gap - 3) * (a.scale * up);
+                    const float far = decay(gap - 3) * a.scale;
                     w[0] *= far * d3;
                     w[1] *= far * d2;
                     w[2] *= far * d1;
                     w[3] *= far;
                 } else {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) w[e] = gap >= e ? w[e] * (decay(max(gap - e, 0)) * (a.scale * up)) : 0.f;
+                    for (int e = 0; e < 4; ++e) w[e] = gap >= e ? w[e] * (decay(max(gap - e, 0)) * a.scale) : 0.f;
                 }
                 uint32_t p[2][2];
-                parts<T, 2>(w[0], w[1], p[0]);
-                parts<T, 2>(w[2], w[3], p[1]);
+                parts<BF16, 2>(w[0], w[1], p[0]);
+                parts<BF16, 2>(w[2], w[3], p[1]);
                 hi[0] = p[0][0];
                 hi[1] = p[1][0];
                 lo[0] = p[0][1];
@@ -353,7 +326,7 @@ __device__ __forceinline__ void linear_segment(const LinearAttnArgs& a) {
                     lanes_x16(most, x, y);
                     lanes_x32(fmaxf(x, y), x, y);
                     su[d] = part_scale(fmaxf(x, y));
-                    const float down = part_unscale(su[d]) * up;
+                    const float down = part_unscale(su[d]);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) back[d][e] = __shfl(down, 4 * g + e);
                 }
@@ -408,6 +381,12 @@ __device__ __forceinline__ void linear_segment(const LinearAttnArgs& a) {
                     for (int m = 0; m < M; ++m)
 #pragma unroll
                         for (int e = 0; e < 8; ++e) v[d][m][e] = __builtin_fabsf((float)v[d][m][e]) < INFINITY ? v[d][m][e] : (el)0.f;
+            b8 vb[DV][M][IN];
+#pragma unroll
+            for (int d = 0; d < DV; ++d)
+#pragma unroll
+                for (int m = 0; m < M; ++m) numbers(v[d][m], vb[d][m]);
+            /* the product of both second numbers is at most 2^-18 of a term, as is what two numbers leave of a weight: not taken */
             if constexpr (SHARED) {
 #pragma unroll
                 for (int m = 0; m < M; ++m)
@@ -415,9 +394,11 @@ __device__ __forceinline__ void linear_segment(const LinearAttnArgs& a) {
                     for (int part = 0; part < 2; ++part)
 #pragma unroll
                         for (int qt = 2 * m; qt < QT; ++qt) {
-                            const v8 w = ld8<T>(lw + weights_at(qt, m) + (part * 64 + lane) * 8);
+                            const b8 w = ld8<BF16>(lw + weights_at(qt, m) + (part * 64 + lane) * 8);
 #pragma unroll
-                            for (int d = 0; d < DV; ++d) o[qt][d] = mfma_16x16x32(v[d][m], w, o[qt][d]);
+                            for (int i = 0; i < IN - part * (IN - 1); ++i)
+#pragma unroll
+                                for (int d = 0; d < DV; ++d) o[qt][d] = mfma_16x16x32(vb[d][m][i], w, o[qt][d]);
                         }
             } else {
 #pragma unroll
@@ -430,15 +411,17 @@ __device__ __forceinline__ void linear_segment(const LinearAttnArgs& a) {
                         weigh(qt, 2 * m, hi[0], lo[0]);
                         if (2 * m < qt) weigh(qt, 2 * m + 1, hi[1], lo[1]);
                         else hi[1][0] = hi[1][1] = 0;
+                        const b8 first = __builtin_bit_cast(b8, u4{hi[0][0], hi[0][1], hi[1][0], hi[1][1]});
+                        const b8 second = __builtin_bit_cast(b8, u4{lo[0][0], lo[0][1], lo[1][0], lo[1][1]});
 #pragma unroll
                         for (int d = 0; d < DV; ++d) {
-                            o[i][d] = mfma_16x16x32(v[d][m], __builtin_bit_cast(v8, u4{hi[0][0], hi[0][1], hi[1][0], hi[1][1]}), o[i][d]);
-                            o[i][d] = mfma_16x16x32(v[d][m], __builtin_bit_cast(v8, u4{lo[0][0], lo[0][1], lo[1][0], lo[1][1]}), o[i][d]);
+#pragma unroll
+                            for (int x = 0; x < IN; ++x) o[i][d] = mfma_16x16x32(vb[d][m][x], first, o[i][d]);
+                            o[i][d] = mfma_16x16x32(vb[d][m][0], second, o[i][d]);
                         }
                     }
                 }
             }
-            const float down = HALF ? part_unscale(up) : 1.f;
             if (poisoned) /* what sees one of them */
 #pragma unroll
                 for (int d = 0; d < DV; ++d) {
@@ -460,7 +443,7 @@ __device__ __forceinline__ void linear_segment(const LinearAttnArgs& a) {
                 first += (uint32_t)(row - skip) * (uint32_t)a.out_token_stride + channel(0, 4 * g);
                 el r[4 * DV];
 #pragma unroll
-                for (int x = 0; x < 4 * DV; ++x) r[x] = (el)opaque(HALF ? o[i][x / 4][x % 4] * down : o[i][x / 4][x % 4]);
+                for (int x = 0; x < 4 * DV; ++x) r[x] = (el)opaque(o[i][x / 4][x % 4]);
                 __builtin_memcpy(__builtin_assume_aligned(first, 8 * DV), r, sizeof(r));
             }
         }

@@ -1,0 +1,53 @@
+"""Linear attention where rows of one call differ much in size, against memlib.py's definition and bounds."""
+import numpy as np
+import pytest
+
+from memlib import linear
+from seqlib import NAN, TYPES, Device, to_bits, values
+from test_gpu_memory import outside, run_linear
+
+pytestmark = pytest.mark.gpu
+GUARD = 3
+
+
+@pytest.fixture
+def dev(hip, device_arena):
+    return Device(hip, device_arena)
+
+
+def check_rows(engine, dev, dtype, q, k, v, lens, rates, state_in=None):
+    """q, k, v [tokens][heads][hd] in 64 bits, sequences one behind the other; every output and state within its bound."""
+    tokens, heads, hd = q.shape
+    rows = np.full((tokens + 2 * GUARD, 3 * heads, hd), NAN[dtype], np.uint16)
+    rows[GUARD:-GUARD] = to_bits(np.concatenate((q, k, v), 1), dtype)
+    x = values(rows[GUARD:-GUARD], dtype)
+    assert np.isfinite(x).all()
+    rates = np.array(rates, np.float32)
+    print(f"[linear] {dtype} {heads} x {hd} lengths {lens}", flush=True)
+    got, new = run_linear(engine, dev, dtype, rows, heads, heads, lens, rates, None, state_in, len(lens), None, GUARD)
+    at = 0
+    for s, n in enumerate(lens):
+        for h in range(heads):
+            first = np.zeros((hd, hd)) if state_in is None else state_in[s, h].astype(np.float64)
+            part = x[at:at + n]
+            o, b, S, B = linear(part[:, h], part[:, heads + h], part[:, 2 * heads + h], float(rates[h]), first, hd ** -0.5, dtype)
+            assert not outside(values(got[GUARD + at:GUARD + at + n, h], dtype), o, b), (s, h)
+            assert not outside(new[s, h].astype(np.float64), S, B), (s, h)
+        at += n
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hd", [16, 32, 64, 128])
+@pytest.mark.parametrize("usual,large", [(1.0, 8000.0), (1.0, 40000.0), (0.1, 65000.0)])
+@pytest.mark.parametrize("lens,query,key", [
+    ([64], 63, 63), ([40], 39, 39), ([104], 103, 103), ([90, 70], 60, 89),  # the chunk's last; a query of the chunk before a short one
+    ([64], 0, 0), ([100], 70, 20)])
+def test_linear_one_large_token(engine, dev, dtype, hd, usual, large, lens, query, key):
+    """One channel of one query and another of one key are large: tokens that do not see it keep their bits, as do those whose
+    weights are small beside it. Values are small, so that outputs stay in fp16's range (65,000 sqrt(64) 4 / 64)."""
+    rng = np.random.default_rng(hd)
+    tokens, heads = sum(lens), 4
+    q, k, v = (rng.standard_normal((tokens, heads, hd)) * usual for _ in "qkv")
+    q[query, :, 3] = large
+    k[key, :, 7] = -large
+    check_rows(engine, dev, dtype, q, k, v / 64, lens, [0.0, 0.003, 0.05, 0.7])
