@@ -313,28 +313,10 @@ __device__ __forceinline__ void linear_segment(const LinearAttnArgs& a) {
                 }
             }
             f4 o[QN][DV] = {};
-            f4 back[DV] = {}; /* fp16: what takes the scales out of the output's rows 4 g + e */
-            float su[DV];
-            if constexpr (HALF) {
-#pragma unroll
-                for (int d = 0; d < DV; ++d) {
-                    float most = 0.f, x, y;
-#pragma unroll
-                    for (int j = 0; j < DK; ++j)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) most = fmaxf(most, __builtin_fabsf(S[j][d][e]));
-                    lanes_x16(most, x, y);
-                    lanes_x32(fmaxf(x, y), x, y);
-                    su[d] = part_scale(fmaxf(x, y));
-                    const float down = part_unscale(su[d]);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) back[d][e] = __shfl(down, 4 * g + e);
-                }
-            }
-            /* q S, the state in parts: lane l16 is a channel of the values, with 8 of each 32 channels of the keys */
+            /* q S, the state as two numbers of bf16: lane l16 is a channel of the values, with 8 of each 32 channels of the keys */
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
-                v8 s[DV][2];
+                b8 s[DV][2];
 #pragma unroll
                 for (int d = 0; d < DV; ++d) {
                     u4 hi = {}, lo = {};
@@ -344,31 +326,30 @@ __device__ __forceinline__ void linear_segment(const LinearAttnArgs& a) {
                         if (j >= DK) continue;
                         uint32_t p[2];
                         const float x = S[j < DK ? j : 0][d][e % 2 * 2], y = S[j < DK ? j : 0][d][e % 2 * 2 + 1];
-                        parts<T, 2>(HALF ? x * su[d] : x, HALF ? y * su[d] : y, p);
+                        parts<BF16, 2>(x, y, p);
                         hi[e] = p[0];
                         lo[e] = p[1];
                     }
-                    s[d][0] = __builtin_bit_cast(v8, hi);
-                    s[d][1] = __builtin_bit_cast(v8, lo);
+                    s[d][0] = __builtin_bit_cast(b8, hi);
+                    s[d][1] = __builtin_bit_cast(b8, lo);
                 }
-                v8 q[QN];
+                b8 q[QN][IN];
 #pragma unroll
-                for (int i = 0; i < QN; ++i) q[i] = row_of(lq, 16 * tile_of(i) + l16, ks);
+                for (int i = 0; i < QN; ++i) numbers(row_of(lq, 16 * tile_of(i) + l16, ks), q[i]);
 #pragma unroll
                 for (int part = 0; part < 2; ++part)
 #pragma unroll
-                    for (int i = 0; i < QN; ++i)
+                    for (int x = 0; x < IN - part * (IN - 1); ++x)
 #pragma unroll
-                        for (int d = 0; d < DV; ++d) o[i][d] = mfma_16x16x32(s[d][part], q[i], o[i][d]);
+                        for (int i = 0; i < QN; ++i)
+#pragma unroll
+                            for (int d = 0; d < DV; ++d) o[i][d] = mfma_16x16x32(s[d][part], q[i][x], o[i][d]);
             }
 #pragma unroll
             for (int i = 0; i < QN; ++i) {
                 const float far = decay(max(16 * tile_of(i) + l16 + 1 - skip, 0)) * a.scale;
 #pragma unroll
-                for (int d = 0; d < DV; ++d) {
-                    if constexpr (HALF) o[i][d] *= back[d];
-                    o[i][d] *= far;
-                }
+                for (int d = 0; d < DV; ++d) o[i][d] *= far;
             }
             /* values that are not finite must not meet weights of zero: queries before them */
             const bool poisoned = __builtin_amdgcn_readfirstlane(bad) != 0;

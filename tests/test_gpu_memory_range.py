@@ -51,3 +51,16 @@ def test_linear_one_large_token(engine, dev, dtype, hd, usual, large, lens, quer
     q[query, :, 3] = large
     k[key, :, 7] = -large
     check_rows(engine, dev, dtype, q, k, v / 64, lens, [0.0, 0.003, 0.05, 0.7])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hd", [16, 32, 64, 128])
+def test_linear_states_of_unlike_sizes(engine, dev, dtype, hd):
+    """A row of the carried state is 2^30 and no query looks at its channel: the others' bits stay."""
+    rng = np.random.default_rng(hd)
+    lens, heads = [70, 5, 600], 2
+    q, k, v = (rng.standard_normal((sum(lens), heads, hd)) for _ in "qkv")
+    s0 = (rng.standard_normal((len(lens), heads, hd, hd))).astype(np.float32)
+    s0[:, :, hd // 2] = 2.0 ** 30
+    q[:, :, hd // 2] = 0
+    check_rows(engine, dev, dtype, q, k / 64, v / 64, lens, [0.0, 0.01], s0)
