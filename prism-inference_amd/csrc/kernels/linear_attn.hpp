@@ -40,13 +40,13 @@ __device__ __forceinline__ LinearTile linear_tile(const LinearAttnArgs& a, int b
     }
 }
 
-/* Two fp32 numbers as N pairs of 16-bit ones that add up to them: fp16 11 N bits (of what is above its smallest), bf16 8 N.
- * Rounded to nearest, so that what is left has a sign and half a bit more. */
-template <class T, int N>
+/* Two fp32 numbers as N pairs of bf16 numbers that add up to them, to 2^-9N (rounded to nearest, so that what is left has a sign and half a bit
+ * more). bf16's exponents are fp32's: the bits do not depend on what else is in a product. */
+template <int N>
 __device__ __forceinline__ void parts(float x, float y, uint32_t (&p)[N]) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        const typename T::v2 v = __builtin_convertvector((f2{x, y}), typename T::v2);
+        const b2 v = __builtin_convertvector((f2{x, y}), b2);
         p[i] = __builtin_bit_cast(uint32_t, v);
         if (i + 1 < N) {
             x -= (float)v[0];
@@ -54,28 +54,21 @@ __device__ __forceinline__ void parts(float x, float y, uint32_t (&p)[N]) {
         }
     }
 }
-/* 8 values as numbers of bf16 that add up to them, exactly: fp16's 11 bits are two. Products of fp16 with what is not fp16 (weights, which
- * differ by more than fp16's powers of two beside each other) are taken in bf16, whose powers are fp32's. */
+/* 8 values as numbers of bf16 that add up to them, exactly: fp16's 11 bits are two. Products of two inputs take fp16 as it is; weights,
+ * states and decayed values, which differ by more than fp16's powers of two beside each other, meet them in bf16. The product of both second
+ * numbers, 2^-18 of a term at most, is not taken where the other factor has two numbers, which hold it to 2^-18. */
 __device__ __forceinline__ void numbers(b8 v, b8 (&n)[1]) { n[0] = v; }
 __device__ __forceinline__ void numbers(h8 v, b8 (&n)[2]) {
     u4 w[2];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         uint32_t p[2];
-        parts<BF16, 2>((float)v[2 * e], (float)v[2 * e + 1], p);
+        parts<2>((float)v[2 * e], (float)v[2 * e + 1], p);
         w[0][e] = p[0];
         w[1][e] = p[1];
     }
     n[0] = __builtin_bit_cast(b8, w[0]);
     n[1] = __builtin_bit_cast(b8, w[1]);
-}
-/* 2^k that brings the largest magnitude m (of fp16 parts' numbers) to 2^13 .. 2^14; 1 for 0; k from -120 to 60 */
-__device__ __forceinline__ float part_scale(float m) {
-    const int e = (int)(__builtin_bit_cast(unsigned, m) >> 23); /* m >= 0 */
-    return m == 0.f ? 1.f : __builtin_bit_cast(float, (unsigned)seq_clamp(267 - e, 7, 187) << 23);
-}
-__device__ __forceinline__ float part_unscale(float scale) { /* of a power of two: 1 / scale */
-    return __builtin_bit_cast(float, 0x7F000000u - __builtin_bit_cast(unsigned, scale));
 }
 /* The larger of each half of two words of 16-bit values, as whole numbers. */
 typedef unsigned short us2 __attribute__((ext_vector_type(2)));
@@ -111,8 +104,7 @@ __device__ __forceinline__ void linear_segment(const LinearAttnArgs& a) {
     typedef typename T::v8 v8;
     typedef typename T::v4 v4;
     typedef typename T::el el;
-    constexpr bool HALF = __is_same(T, F16);
-    constexpr int IN = HALF ? 2 : 1; /* numbers of bf16 that an input is */
+    constexpr int IN = __is_same(T, F16) ? 2 : 1; /* numbers of bf16 that an input is */
     constexpr int C = LINEAR_CHUNK, QT = C / 16, M = C / 32;
     constexpr int DV = HD >= 128 ? 2 : 1;          /* a wave's 16-channel tiles of the values */
     constexpr int WD = HD / 16 / DV, WQ = STATES || HD >= 64 ? 1 : QT / WD, QN = QT / WQ; /* waves by channels, by query tiles; a wave's */
@@ -294,8 +286,8 @@ __device__ __forceinline__ void linear_segment(const LinearAttnArgs& a) {
                     for (int e = 0; e < 4; ++e) w[e] = gap >= e ? w[e] * (decay(max(gap - e, 0)) * a.scale) : 0.f;
                 }
                 uint32_t p[2][2];
-                parts<BF16, 2>(w[0], w[1], p[0]);
-                parts<BF16, 2>(w[2], w[3], p[1]);
+                parts<2>(w[0], w[1], p[0]);
+                parts<2>(w[2], w[3], p[1]);
                 hi[0] = p[0][0];
                 hi[1] = p[1][0];
                 lo[0] = p[0][1];
@@ -326,7 +318,7 @@ __device__ __forceinline__ void linear_segment(const LinearAttnArgs& a) {
                         if (j >= DK) continue;
                         uint32_t p[2];
                         const float x = S[j < DK ? j : 0][d][e % 2 * 2], y = S[j < DK ? j : 0][d][e % 2 * 2 + 1];
-                        parts<BF16, 2>(x, y, p);
+                        parts<2>(x, y, p);
                         hi[e] = p[0];
                         lo[e] = p[1];
                     }
@@ -367,7 +359,6 @@ __device__ __forceinline__ void linear_segment(const LinearAttnArgs& a) {
             for (int d = 0; d < DV; ++d)
 #pragma unroll
                 for (int m = 0; m < M; ++m) numbers(v[d][m], vb[d][m]);
-            /* the product of both second numbers is at most 2^-18 of a term, as is what two numbers leave of a weight: not taken */
             if constexpr (SHARED) {
 #pragma unroll
                 for (int m = 0; m < M; ++m)
@@ -444,92 +435,39 @@ __device__ __forceinline__ void linear_segment(const LinearAttnArgs& a) {
         };
         const auto key = [&](int m, int j) { return transposed(lk, 32 * m, spot(16 * j + 4 * (l16 & 3))); };
         constexpr int J = DK < 4 / DV ? DK : 4 / DV; /* tiles side by side: their products do not wait for each other */
-        if constexpr (HALF) {
-            /* scaled by a power of two to fp16's range, for each channel of the values */
-            v8 vp[DV][M][2];
-            float down[DV];
+        /* decayed values as three numbers of bf16, which leave 2^-27 of them; keys' second numbers (fp16) do without the third */
+#pragma unroll
+        for (int j = 0; j < DK; ++j)
+#pragma unroll
+            for (int d = 0; d < DV; ++d) S[j][d] *= keep;
+#pragma unroll
+        for (int m = 0; m < M; ++m) {
+            u4 w[DV][3];
 #pragma unroll
             for (int d = 0; d < DV; ++d) {
-                float x[M][8], most = 0.f, y, z;
+                float x[8];
+                faded(d, m, x);
 #pragma unroll
-                for (int m = 0; m < M; ++m) {
-                    faded(d, m, x[m]);
+                for (int e = 0; e < 4; ++e) {
+                    uint32_t p[3];
+                    parts<3>(x[2 * e], x[2 * e + 1], p);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) most = fmaxf(most, __builtin_fabsf(x[m][e]));
-                }
-                lanes_x16(most, y, z);
-                lanes_x32(fmaxf(y, z), y, z);
-                const float up = part_scale(fmaxf(y, z));
-                down[d] = part_unscale(up);
-#pragma unroll
-                for (int m = 0; m < M; ++m) {
-                    u4 w[2];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        uint32_t p[2];
-                        parts<T, 2>(x[m][2 * e] * up, x[m][2 * e + 1] * up, p);
-                        w[0][e] = p[0];
-                        w[1][e] = p[1];
-                    }
-                    vp[d][m][0] = __builtin_bit_cast(v8, w[0]);
-                    vp[d][m][1] = __builtin_bit_cast(v8, w[1]);
+                    for (int i = 0; i < 3; ++i) w[d][i][e] = p[i];
                 }
             }
 #pragma unroll
             for (int j0 = 0; j0 < DK; j0 += J) {
-                f4 u[J][DV] = {};
+                b8 k[J][IN];
 #pragma unroll
-                for (int m = 0; m < M; ++m) {
-                    v8 k[J];
+                for (int j = 0; j < J; ++j) numbers(key(m, j0 + j), k[j]);
 #pragma unroll
-                    for (int j = 0; j < J; ++j) k[j] = key(m, j0 + j);
+                for (int i = 0; i < 3; ++i)
 #pragma unroll
-                    for (int i = 0; i < 2; ++i)
-#pragma unroll
-                        for (int j = 0; j < J; ++j)
-#pragma unroll
-                            for (int d = 0; d < DV; ++d) u[j][d] = mfma_16x16x32(k[j], vp[d][m][i], u[j][d]);
-                }
-#pragma unroll
-                for (int j = 0; j < J; ++j)
-#pragma unroll
-                    for (int d = 0; d < DV; ++d)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) S[j0 + j][d][e] = __builtin_fmaf(u[j][d][e], down[d], S[j0 + j][d][e] * keep);
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < DK; ++j)
-#pragma unroll
-                for (int d = 0; d < DV; ++d) S[j][d] *= keep;
-#pragma unroll
-            for (int m = 0; m < M; ++m) {
-                u4 w[DV][3];
-#pragma unroll
-                for (int d = 0; d < DV; ++d) {
-                    float x[8];
-                    faded(d, m, x);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        uint32_t p[3];
-                        parts<T, 3>(x[2 * e], x[2 * e + 1], p);
-#pragma unroll
-                        for (int i = 0; i < 3; ++i) w[d][i][e] = p[i];
-                    }
-                }
-#pragma unroll
-                for (int j0 = 0; j0 < DK; j0 += J) {
-                    v8 k[J];
-#pragma unroll
-                    for (int j = 0; j < J; ++j) k[j] = key(m, j0 + j);
-#pragma unroll
-                    for (int i = 0; i < 3; ++i)
+                    for (int x = 0; x < (i < 2 ? IN : 1); ++x)
 #pragma unroll
                         for (int j = 0; j < J; ++j)
 #pragma unroll
-                            for (int d = 0; d < DV; ++d)
-                                S[j0 + j][d] = mfma_16x16x32(k[j], __builtin_bit_cast(v8, w[d][i]), S[j0 + j][d]);
-                }
+                            for (int d = 0; d < DV; ++d) S[j0 + j][d] = mfma_16x16x32(k[j][x], __builtin_bit_cast(b8, w[d][i]), S[j0 + j][d]);
             }
         }
     }

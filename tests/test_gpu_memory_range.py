@@ -55,6 +55,38 @@ def test_linear_one_large_token(engine, dev, dtype, hd, usual, large, lens, quer
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("hd", [16, 32, 64, 128])
+@pytest.mark.parametrize("lens", [[64], [50], [200], [1500, 777]])
+def test_linear_keys_of_zero_after_others(engine, dev, dtype, hd, lens):
+    """Every sequence's last 32 tokens have keys of zero (padding, gates that are closed), and every third channel has a key in
+    one token of 29 alone: states and outputs are sums of values that decayed far below the newest one's."""
+    rng = np.random.default_rng(hd)
+    tokens, heads = sum(lens), 4
+    q, k, v = (rng.standard_normal((tokens, heads, hd)) for _ in "qkv")
+    k[np.arange(tokens) % 29 != 0, :, 0::3] = 0
+    for end in np.cumsum(lens):
+        k[end - 32:end] = 0
+    check_rows(engine, dev, dtype, q, k, v, lens, [0.0, 0.3, 0.7, 1.4])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hd", [16, 32, 64, 128])
+def test_linear_values_of_unlike_sizes(engine, dev, dtype, hd):
+    """Tokens' values from 2^-14 to 2^14 under keys that share no channel with the next token's: a state's rows are of any size
+    beside each other, and queries look at some of them alone."""
+    rng = np.random.default_rng(hd)
+    n, heads = 150, 2
+    q, k = (rng.standard_normal((n, heads, hd)) for _ in "qk")
+    v = rng.standard_normal((n, heads, hd)) * 2.0 ** (14.0 - 28.0 * (np.arange(n) % 2))[:, None, None] / 4
+    k[0::2, :, 0::2] = 0
+    k[1::2, :, 1::2] = 0
+    q[0::3, :, 1::2] = 0
+    q[1::3, :, 0::2] /= 256
+    q /= 16
+    check_rows(engine, dev, dtype, q, k, v, [n], [0.0, 0.2])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hd", [16, 32, 64, 128])
 def test_linear_states_of_unlike_sizes(engine, dev, dtype, hd):
     """A row of the carried state is 2^30 and no query looks at its channel: the others' bits stay."""
     rng = np.random.default_rng(hd)
