@@ -644,13 +644,16 @@ int prism_paged_attn4(prism_ctx* ctx, const prism_paged_attn_push* p, const void
  * last one there in state_out (state_of NULL = s itself). A number out of range, or
  * state_in NULL, starts from zeros; a number out of range is not written, nor
  * anything if state_out is NULL. state_in may be state_out. Two sequences of
- * one number leave it unspecified. A sequence without tokens copies its state.
+ * one number leave it unspecified, and where state_in is state_out their rows
+ * too. A sequence without tokens copies its state.
  * Rows of out outside the sequences stay as they were. scale is finite. Sums and
  * states are fp32 and have to stay in its range; what a matrix product takes of a
  * state or a weight has 16 significant bits or more, what it takes for the next
- * state 21 or more. From its token on, an infinity or NaN in q makes NaN of its row and head, in
- * v of its channel and in k of its whole head, of state_out too; earlier tokens
- * and other sequences do not see it. workspace as in prism_paged_attn. head_dim 16, 32,
+ * state 21 or more. From its token on, an infinity or NaN leaves what is not
+ * finite (either infinity, or NaN): in q, its row and head; in v, its channel and
+ * that column of state_out; in k, its whole head and its channel's row of
+ * state_out. Earlier tokens and other sequences do not see it. workspace as in
+ * prism_paged_attn. head_dim 16, 32,
  * 64 or 128; at most 2^30 rows, token strides at most 2^22. */
 typedef struct prism_linear_attn_push {
     int32_t dtype, n_seqs, n_tokens, n_heads, n_kv_heads, head_dim;

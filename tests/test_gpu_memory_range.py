@@ -1,10 +1,10 @@
-"""Linear attention where rows of one call differ much in size, against memlib.py's definition and bounds."""
+"""Linear attention where rows of one call differ much in size or are not finite, against memlib.py's definition and bounds."""
 import numpy as np
 import pytest
 
 from memlib import linear
-from seqlib import NAN, TYPES, Device, to_bits, values
-from test_gpu_memory import outside, run_linear
+from seqlib import NAN, TYPES, Device, normal, to_bits, values
+from test_gpu_memory import linear_push, outside, run_linear
 
 pytestmark = pytest.mark.gpu
 GUARD = 3
@@ -96,3 +96,33 @@ def test_linear_states_of_unlike_sizes(engine, dev, dtype, hd):
     s0[:, :, hd // 2] = 2.0 ** 30
     q[:, :, hd // 2] = 0
     check_rows(engine, dev, dtype, q, k / 64, v / 64, lens, [0.0, 0.01], s0)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hd", [16, 32, 64, 128])
+@pytest.mark.parametrize("what", [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("which", "qkv")
+@pytest.mark.parametrize("other", [1.0, 0.0])
+def test_linear_step_values_that_are_not_finite(engine, dev, dtype, hd, what, which, other):
+    """They reach their row and head, channel and column, or head and row of the state, also where all that they meet is zero."""
+    rng, n, heads, s, h, c = np.random.default_rng(hd), 3, 2, 1, 1, hd - 3
+    rows = normal(rng, (n, 3 * heads, hd), dtype)
+    s0 = rng.standard_normal((n, heads, hd, hd)).astype(np.float32) * np.float32(other)
+    rows[s, h::heads] = to_bits(values(rows[s, h::heads], dtype) * other, dtype)
+    push = linear_push(dtype, n, n, heads, heads, hd, n, 0.2, 3 * heads * hd)
+
+    def run():
+        x, out, new = dev.put(rows), dev.put(np.full((n, heads, hd), NAN[dtype], np.uint16)), dev.put(np.full(s0.shape, np.nan, np.float32))
+        engine.linear_step(push, x, x + 2 * heads * hd, x + 4 * heads * hd, dev.put(np.array([0.0, 0.1], np.float32)), None, dev.put(s0),
+                           out, new)
+        return dev.get(out, (n, heads, hd)), dev.get(new, s0.shape, np.float32)
+
+    clean, cs = run()
+    rows[s, {"q": 0, "k": heads, "v": 2 * heads}[which] + h, c] = to_bits(np.array(what), dtype)
+    got, gs = run()
+    bad, bad_state = np.zeros(got.shape, bool), np.zeros(gs.shape, bool)
+    bad[s, h, c if which == "v" else slice(None)] = True
+    if which != "q":
+        bad_state[s, h][(slice(None), c) if which == "v" else c] = True
+    assert (~np.isfinite(values(got, dtype)) == bad).all() and (got[~bad] == clean[~bad]).all()
+    assert (~np.isfinite(gs) == bad_state).all() and (gs[~bad_state] == cs[~bad_state]).all()
