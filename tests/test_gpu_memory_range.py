@@ -1,10 +1,11 @@
-"""Linear attention where rows of one call differ much in size or are not finite, against memlib.py's definition and bounds."""
+"""Linear attention where rows of one call differ much in size or are not finite, and calls that take rarer paths, against memlib.py's
+definitions and bounds."""
 import numpy as np
 import pytest
 
 from memlib import linear
 from seqlib import NAN, TYPES, Device, normal, to_bits, values
-from test_gpu_memory import linear_push, outside, run_linear
+from test_gpu_memory import check_linear, check_paged4, linear_push, outside, run_linear
 
 pytestmark = pytest.mark.gpu
 GUARD = 3
@@ -126,3 +127,23 @@ def test_linear_step_values_that_are_not_finite(engine, dev, dtype, hd, what, wh
         bad_state[s, h][(slice(None), c) if which == "v" else c] = True
     assert (~np.isfinite(values(got, dtype)) == bad).all() and (got[~bad] == clean[~bad]).all()
     assert (~np.isfinite(gs) == bad_state).all() and (gs[~bad_state] == cs[~bad_state]).all()
+
+
+# ------------------------------------------------------------- rarer paths
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hd,kv,group", [(32, 2, 1), (32, 1, 2), (64, 1, 1), (128, 1, 4), (128, 2, 4)])
+@pytest.mark.parametrize("lengths,max_len", [([1500, 40], 100), ([6000, 900], 2000)])
+def test_paged4_longer_than_expected(engine, dev, dtype, hd, kv, group, lengths, max_len):
+    """Sequences past max_len, four waves of a workgroup alone or in splits: all keys are seen."""
+    check_paged4(engine, dev, np.random.default_rng(hd), dtype, hd, kv, group, 64, lengths, -1, 0, max_len)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hd", [16, 32, 64, 128])
+@pytest.mark.parametrize("start", ["all", "none"])
+def test_linear_long_without_a_state(engine, dev, dtype, hd, start):
+    """Long sequences in segments, two of which have numbers of states out of range (-1 and as many as there are)."""
+    lens = [900, 1500, 777, 300]
+    assert engine.linear_attn_workspace(linear_push(dtype, len(lens), sum(lens) + 2 * GUARD, 2, 2, hd, 6, 1.0, 6 * hd)) > 0
+    check_linear(engine, dev, np.random.default_rng(hd), dtype, hd, 2, 1, lens, start)

@@ -188,3 +188,24 @@ def test_the_definition_of_a_block(dtype):
     codes, scales = quantise(borders, dtype)
     assert (dequantise(codes, scales) == [6, 0, 1, 1, 2, 2, 4, 4, 0, -1, -1, -2, -2, -4, -4, 0]).all() and scales == 127
     assert codes[-1] >> 4 == 8  # a zero keeps its sign
+
+
+@pytest.mark.parametrize("field", ["q_token_stride", "k_token_stride", "v_token_stride", "out_token_stride"])
+def test_linear_token_strides(rules, field):
+    """Rows of a chunk are addressed with 32 bits: 2^22 elements from one to the next, at most."""
+    for call in (rules.linear_check, rules.linear_step_check):
+        assert call(C.byref(linear(**{field: 2 ** 22}))) == 0
+        assert call(C.byref(linear(**{field: 2 ** 22 + 8}))) == P.ERR_UNSUPPORTED
+        for bad in STRIDES:
+            assert call(C.byref(linear(**{field: bad}))) < 0
+    assert P.lib().prism_linear_attn_workspace(C.byref(linear(**{field: 2 ** 22 + 8}))) == P.ERR_UNSUPPORTED
+
+
+@pytest.mark.parametrize("hd,kv,group,lengths,max_len,splits", [(32, 2, 1, 2, 100, 1), (128, 1, 4, 2, 100, 1), (32, 1, 2, 2, 2000, 5),
+                                                                (64, 1, 1, 2, 2000, 5), (128, 2, 4, 2, 2000, 5)])
+def test_a_wave_of_a_cache_longer_than_expected(rules, hd, kv, group, lengths, max_len, splits):
+    """The calls of test_paged4_longer_than_expected are of four waves, with these splits."""
+    p = P.PagedAttnPush(cache=cache(n_kv_heads=kv, head_dim=hd, page_size=64, n_seqs=lengths, table_pages=97), n_heads=kv * group,
+                        left=-1, max_len=max_len, scale=1.0)
+    many, _, waves, got, _, each, _, _ = numbers(rules.paged4_of, p, 8)
+    assert waves == 4 and got == splits and many == (group > 2 or hd > 32) and 4 * splits * each < 6000
