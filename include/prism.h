@@ -626,7 +626,9 @@ int prism_cache_read(prism_ctx* ctx, const prism_cache_read_push* p, const prism
                      const int32_t* seq_of, const int32_t* pos_of, const int32_t* table, void* k, void* v,
                      void* stream);
 
-/* prism_paged_attn over a cache of PRISM_CACHE_4. */
+/* prism_paged_attn over a cache of PRISM_CACHE_4. Its splits are as long as
+ * max_len asks for: a max_len far above every length costs time (24 streams of
+ * 4,096, 32 heads over 8 x 128: 36 us at 4,096, 75 at 32,768, 183 at 131,072). */
 int64_t prism_paged_attn4_workspace(const prism_paged_attn_push* p);
 int prism_paged_attn4(prism_ctx* ctx, const prism_paged_attn_push* p, const void* q, const prism_cache_pages* pages,
                       const int32_t* table, const int32_t* lengths, void* out, void* workspace,
@@ -649,12 +651,14 @@ int prism_paged_attn4(prism_ctx* ctx, const prism_paged_attn_push* p, const void
  * Rows of out outside the sequences stay as they were. scale is finite. Sums and
  * states are fp32 and have to stay in its range; what a matrix product takes of a
  * state or a weight has 16 significant bits or more, what it takes for the next
- * state 21 or more. From its token on, an infinity or NaN leaves what is not
+ * state 21 or more, each number for itself (fewer below 2^-100, where fp32 ends).
+ * From its token on, an infinity or NaN leaves what is not
  * finite (either infinity, or NaN): in q, its row and head; in v, its channel and
  * that column of state_out; in k, its whole head and its channel's row of
  * state_out. Earlier tokens and other sequences do not see it. workspace as in
- * prism_paged_attn. head_dim 16, 32,
- * 64 or 128; at most 2^30 rows, token strides at most 2^22. */
+ * prism_paged_attn. How the work is split goes by the mean length: one long
+ * sequence beside many short ones is not split, and costs its whole chain. head_dim
+ * 16, 32, 64 or 128; at most 2^30 rows, token strides at most 2^22. */
 typedef struct prism_linear_attn_push {
     int32_t dtype, n_seqs, n_tokens, n_heads, n_kv_heads, head_dim;
     int32_t n_states;

@@ -209,12 +209,15 @@ inline int check_linear_step(const prism_linear_attn_push& p, const char** why) 
  *
  * A workgroup's chunks follow each other, so few sequences are split; each segment but the first then starts from the sum of those
  * before it, which a launch of its own made: its keys and values are read twice. us without, and in segments of 64, 128, 256, 512,
- * 1024, 1536 (heads x channels):
- *   1 x 8,160, 8 x 32    204 | 38 22 21 27 42 59        5 x 4,500, 32 x 32   149 | 217 126 99 90 92 107
- *   1 x 8,160, 8 x 128   598 | 230 86 60 73 118 164     5 x 4,500, 32 x 128  370 | - 689 402 330 339 293
- *   2 x 1,000, 8 x 32    36 | 11 13 17 27               64 x 1,000, 8 x 32   41 | 103 74 65 63
- *   3 x 500, 4 x 64      28 | 13 15 22                  64 x 1,000, 8 x 128  163 | 517 318 247 223
- *   1 x 32,000, 4 x 128  2,317 | - - 162 105 132 173    16 x 500, 8 x 128    48 | 59 45 54 */
+ * 1024, 1536 (heads x channels), bf16:
+ *   1 x 8,160, 8 x 32    206 | 37 22 19 26 43 59        5 x 4,500, 32 x 32   119 | 201 121 95 88 92 92
+ *   1 x 8,160, 8 x 128   569 | 220 81 58 70 114 157     5 x 4,500, 32 x 128  352 | 2,385 632 378 318 325 280
+ *   2 x 1,000, 8 x 32    29 | 10 12 16 24               64 x 1,000, 8 x 32   40 | 102 77 66 64
+ *   3 x 500, 4 x 64      23 | 12 14 19                  64 x 1,000, 8 x 128  160 | 485 312 251 226
+ *   1 x 32,000, 4 x 128  2,195 | - - 148 100 125 167    16 x 500, 8 x 128    45 | 58 44 53
+ * fp16, whose products are more, takes 1.1 to 1.6 times as long and is best at the same lengths (5 x 4,500, 32 x 128: 547 | 2,413 716 494 444
+ * 463 421; 1 x 8,160, 8 x 32: 284 | 39 25 24 33 57 81). Lengths are on the device, so the rule knows their mean alone: 8,160 tokens beside 31 or 63
+ * sequences of one token, 8 x 32, are not split and take 206 us (fp16 285), by themselves 20 (24). */
 struct LinearPlan {
     int32_t segment;
     bool split;
@@ -314,13 +317,14 @@ inline int64_t paged_keys(const prism_paged_attn_push& p) {
  * many there. Splits are as long as those of the longest sequence expected (paged_attn4.hpp), so that of unlike lengths about half
  * have keys: 1,800 workgroups then are as many as the GPU holds at once, and one round of them is fastest. An odd number, so that
  * those that many sequences lack do not fall on the same XCD. us at 1, 5, 8, 9, 15, 16, 25, 63, 95, 191 splits: 24 sequences of 1,000 to
- * 20,001, 32/8 x 128: 249, 103, 101, 73, 81, 103, 83, 117, 138, 223; one of 131,075: 1,398, 291, 188, 167, 109, 101, 70, 46, 43, 47; one of
- * 16,000, 8/1 x 128: 152, 40, 29, 27, 22, 19, 17, 13, 14, 16; 64 of 500 to 4,000, 8 x 128: 59, 53, 64, 55, 68, 76, 82 and more. */
+ * 20,001, 32/8 x 128: 218, 98, 98, 70, 77, 98, 77, 107, 127, 202; one of 131,075: 1,215, 255, 165, 147, 95, 89, 62, 43, 42, 46; one of
+ * 16,000, 8/1 x 128: 134, 36, 26, 23, 19, 16, 15, 12, 13, 15; 64 of 500 to 4,000, 8 x 128: 55, 49, 60, 52, 62, 70, 75 and more. They go by
+ * what is expected, not by the lengths: 24 streams of 4,096 take 36, 38, 75, 183 us where 4,096, 8,192, 32,768, 131,072 are. */
 inline PagedPlan paged4_plan(const prism_paged_attn_push& p) {
     PagedPlan r = paged_plan(p);
     r.many = p.n_heads / p.cache.n_kv_heads > 2 || p.cache.head_dim > 32;
     const int64_t items = std::max<int64_t>((int64_t)p.cache.n_seqs * p.cache.n_kv_heads * r.head_tiles, 1), keys = paged_keys(p);
-    /* waves by themselves: 1,600 items of 300 keys x 64 16.3 us, four a workgroup 19.7; 520 of 1,000 and more 4,000 x 128 60 and 200 */
+    /* us of waves by themselves, and of four a workgroup: 1,600 items of 300 keys x 64 14.7, 17.8; 520 of 1,000 x 128 43, 26; of 1,000 to 4,000 152, 52 */
     r.waves = keys <= 64 || items >= 4096 || (items >= 1024 && keys <= 400) ? 1 : 4;
     r.splits = 1;
     if (r.waves == 4 && keys >= 384 && keys * p.cache.head_dim >= 32 * 1024) {

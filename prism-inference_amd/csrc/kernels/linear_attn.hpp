@@ -88,9 +88,12 @@ __device__ __forceinline__ bool infinite(uint32_t most) { /* bits of magnitudes,
 }
 
 /* What bounds it. Few short sequences: a chain of launch, starts, tokens and products; 9 up to 130, 8 x 16, 8 us. 8,160 tokens,
- * 8 x 32: 16 us behind 5 for the segments' states, of which each chunk is 1 and the rest latency. 23,000 tokens of 5 sequences, 32 x 128:
- * 212 us behind 87 (805 MB: 3.8 TB/s); matrix cores 30 %, vector units 39 % busy. Without any product the kernel still takes 0.8 of
+ * 8 x 32, fp16: 19 us behind 6 for the segments' states, of which each chunk is 1 and the rest latency. 23,000 tokens of 5 sequences, 32 x 128,
+ * bf16: 212 us behind 88 (805 MB: 3.8 TB/s); matrix cores 30 %, vector units 39 % busy. Without any product the kernel still takes 0.8 of
  * that: loads, staging in LDS, barriers and stores, with two workgroups a CU (256 registers, 67 KB of LDS).
+ * fp16's second numbers are products 3 for 2 and 5 for 3, and made anew by each wave from what it reads: 5 x 4,500, 32 x 128 415 us for bf16's 285.
+ * In fp16 with a power of two for each chunk, row of the state or channel it took 297, but numbers far below the largest lost their bits. fp16
+ * keys split once, into LDS, took 409 (of 32 channels 104 for 109) for a barrier more.
  *
  * One segment of one head: its chunks of 64 tokens in turn,
  *   o_i = scale (e^(-r (i+1)) q_i S + sum_{j <= i} e^(-r (i-j)) (q_i k_j) v_j),  S' = e^(-r n) S + sum_j k_j^T e^(-r (n-1-j)) v_j

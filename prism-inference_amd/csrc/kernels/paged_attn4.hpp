@@ -10,9 +10,9 @@
  *                same order. V goes through a wave's own LDS, as 16-bit numbers, for transposed reads.
  *
  * A key and a value are 17/16 of a byte a channel, a quarter of 16-bit ones, so that the vector units come close to memory:
- *   paged4_few   8,160 streams of 52 keys, 8 x 32: 31 us for 117 MB, vector units 96 % busy. One maximum for the wave: 40 us with one a lane,
+ *   paged4_few   8,160 streams of 52 keys, 8 x 32: 32 us for 117 MB, vector units 96 % busy. One maximum for the wave: 40 us with one a lane,
  *                whose sums are scaled once more at the end.
- *   paged4_many  24 streams of 1,000 to 20,001, 32 over 8 x 128: 64 us for 276 MB (4.3 TB/s), its loads alone 53; one of 131,075: 34 for 143 MB.
+ *   paged4_many  24 streams of 1,000 to 20,001, 32 over 8 x 128: 65 us for 276 MB (4.2 TB/s), its loads alone 53; one of 131,075: 34 for 143 MB.
  *                Keys through LDS in whole lines, and the next step's asked for ahead of the softmax, were slower or equal.
  */
 #pragma once
@@ -261,7 +261,8 @@ __device__ __forceinline__ void paged4_many(const PagedAttnArgs& a) {
         const v8 x = ld8<T>(qp + part * QUARTER + 8 * ks);
         q[ks] = HD >= 32 || g < 2 ? x : v8{};
     }
-    /* weights as the sum of two 16-bit numbers, as in paged_attn.hpp */
+    /* Weights as the sum of two 16-bit numbers, as in paged_attn.hpp: what a matrix product takes. bf16's leave 2^-16 of a weight, so that some
+       four outputs of a thousand round to the other side than with fp32 weights; the error against 64 bits is the same, the output's rounding. */
     constexpr bool HALF = __is_same(T, F16);
     constexpr float UP = HALF ? 15.f : 0.f, LEAST = HALF ? 0x1p-24f : 0x1p-133f; /* the type's smallest */
     f4 o[DT] = {};
